@@ -43,7 +43,8 @@ enum {
 enum {
   H3SA_DEVERR_WAIT_TIMEOUT = 1, /* a pipeline wait gave up; outputs are invalid */
   H3SA_DEVERR_BAD_PAGE = 2,     /* page-table entry outside the pool */
-  H3SA_DEVERR_BAD_INDEX = 4     /* row or block index outside its range */
+  H3SA_DEVERR_BAD_INDEX = 4,    /* row or block index outside its range */
+  H3SA_DEVERR_NO_PAGES = 8      /* a pool has too few free pages for the request */
 };
 
 /* One attention problem of a launch: queries [q_lo, q_hi) of the packed query tensor attend
@@ -459,6 +460,82 @@ H3SA_API int h3sa_scatter_qkv_paged(const void* merged, int32_t tokens, int32_t 
                                     const uint64_t* peer_value_pool, int32_t pool_pages,
                                     const int32_t* page_table, int32_t table_blocks,
                                     int32_t dst_start, int32_t* device_error, void* stream);
+
+/* ---- branches: several continuations of one stream over shared pages (no counterpart in the
+ * reference, which holds one clean history per stream).
+ *
+ * A ledger describes the pages of a pool: table int32 [sequences, width] (page of each logical
+ * 128-row block, -1 after the last one held), lengths int32 [sequences] (rows) and refs int32
+ * [pages], the number of table entries that hold each page (0: free). All of it is in device
+ * memory and read there, so no call waits for the host. */
+
+/* Pool tensors that one ledger describes (K and V of every layer): `count` paged pools
+ * [heads, pages * 128, row_bytes], either listed by address or `stride` bytes apart from base. */
+typedef struct h3sa_pools {
+  void* const* list; /* host array of device addresses, or NULL */
+  void* base;        /* used when list is NULL */
+  int64_t stride;
+  int32_t count, heads, pages, row_bytes;
+} h3sa_pools;
+
+/* Bytes of device workspace that h3sa_fork_pages (and, with children = 0, h3sa_compact_pages)
+ * needs; 16-byte aligned, owned by the caller, free again when the call's work is done. */
+H3SA_API int64_t h3sa_pages_workspace(int32_t pages, int32_t children);
+
+/* New branches: child c continues sequence parents[c] (negative: an empty one). It holds the
+ * parent's whole pages with it and a fresh page with a copy of the rows of the parent's last,
+ * partial page; private_copy != 0 gives it fresh copies of all pages instead. Every child also
+ * gets the fresh pages that reserve_rows more rows need. Fresh pages are the lowest free ones, in
+ * child order. Writes child_table [children, width], child_lengths [children] and refs_out
+ * [pages] (which may not overlap refs) and copies rows in all pools. When the pool has too few
+ * free pages (H3SA_DEVERR_NO_PAGES), a child does not fit its table row or a parent or length is
+ * out of range (H3SA_DEVERR_BAD_INDEX) or a parent holds a page that is free or outside the pool
+ * (H3SA_DEVERR_BAD_PAGE), nothing is forked: all children come out empty and refs_out = refs. */
+H3SA_API int h3sa_fork_pages(const h3sa_pools* pools, const int32_t* table, int32_t sequences,
+                             int32_t width, const int32_t* lengths, const int32_t* refs,
+                             const int32_t* parents, int32_t children, int32_t reserve_rows,
+                             int32_t private_copy, int32_t* child_table, int32_t* child_lengths,
+                             int32_t* refs_out, void* workspace, int32_t* device_error,
+                             void* stream);
+
+/* Moves the pages in use to the front of the pool: with n pages in use, the i-th free page below
+ * n receives the i-th page in use at or past n. table_out and refs_out (no overlap with table and
+ * refs) are renumbered, live[0] = n. Entries that name a free page or none of the pool come out
+ * -1 with H3SA_DEVERR_BAD_PAGE. */
+H3SA_API int h3sa_compact_pages(const h3sa_pools* pools, const int32_t* table, int32_t sequences,
+                                int32_t width, const int32_t* refs, int32_t* table_out,
+                                int32_t* refs_out, int32_t* live, void* workspace,
+                                int32_t* device_error, void* stream);
+
+/* Ends the sequences with release[s] != 0: each of their pages loses one reference, their table
+ * rows become -1 and their lengths 0. The outputs may not overlap the inputs. An entry outside
+ * the pool or without a reference left to drop sets H3SA_DEVERR_BAD_PAGE and is skipped. */
+H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t width,
+                             const int32_t* lengths, const int32_t* refs, int32_t pages,
+                             const uint8_t* release, int32_t* table_out, int32_t* lengths_out,
+                             int32_t* refs_out, int32_t* device_error, void* stream);
+
+/* Attention of all branches' new rows, the shared history read once for all of them. query bf16
+ * [batch, rows, heads, 128] with element strides query_strides[3] (multiples of 8); out bf16
+ * [batch, rows, heads, 128] contiguous; lse fp32 [batch, rows, heads] (natural log of the sum of
+ * exponentials, -inf for a row that sees nothing) or NULL. Pools [kv_heads, pool_pages * 128, 128]
+ * bf16, or e4m3 with k_scale / v_scale fp32 [kv_heads]; query head h reads KV head
+ * h / (heads / kv_heads). Row i of sequence b sees the keys j < lengths[b], causal != 0: j <
+ * lengths[b] - (rows - 1 - i), the new rows being the sequence's last ones. The first shared_rows
+ * rows (whole pages) are the same pages in the table rows of all sequences at least that long;
+ * shorter sequences see the first lengths[b] rows of them. Rows that see nothing come out zero.
+ * Rows of a page past a sequence's end are never used, whatever they hold. A length outside
+ * [0, width * 128] is clamped with H3SA_DEVERR_BAD_INDEX; a page outside the pool gives
+ * H3SA_DEVERR_BAD_PAGE and invalid outputs. Results do not depend on timing. */
+H3SA_API int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
+                                              int32_t kv_heads, int32_t shared_rows);
+H3SA_API int h3sa_shared_prefix_attention(
+    const void* query, const int64_t* query_strides, void* out, float* lse, int32_t batch,
+    int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool, const void* value_pool,
+    int32_t pool_pages, int32_t e4m3, const float* k_scale, const float* v_scale,
+    const int32_t* table, int32_t width, const int32_t* lengths, int32_t shared_rows,
+    int32_t causal, float softmax_scale, void* workspace, int64_t workspace_bytes,
+    int32_t* device_error, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,1135 @@
+// Attention of several branches of one stream over their shared history and their own rows.
+//
+// A branch (sequence) b of a paged, head-major KV pool is one row of a page table and a length;
+// the first `shared` pages of every row are the same pages. Row (b, i) of query head h sees the
+// keys j < limit(b, i) = length(b) - (causal ? n - 1 - i : 0) of its own sequence:
+//
+//   x_j = scale * q . k_j,   out = sum_j 2^(x_j' - m) v_j / sum_j 2^(x_j' - m),  x' = x log2 e
+//
+// Work is cut into units of one 128-row KV block of one KV head against one item of up to 256
+// query rows. In the split form an item is either a span of all branches' rows stacked (b, i, and
+// the query heads of the KV head's group) against the shared blocks, which are so read once for
+// all, or the rows of one branch against its own blocks; in the joint form (branches with many
+// rows each) an item is a span of one branch's rows against all its blocks. The units lie in one
+// line (KV head, shared items, own items) that is cut into equal ranges, one per CTA, whatever the
+// lengths are; lengths are read on the device. An item that no cut divides and that nothing else
+// contributes to is written out directly; the pieces of all others go to a workspace as
+// unnormalised fp32 O, running maximum and sum, and branch_merge_kernel joins them in a fixed
+// order, so results do not depend on timing.
+//
+// Warp roles of branch_attn_kernel (one persistent CTA per SM, 384 threads):
+//   warp 0      walks the CTA's units: publishes each item segment in a small descriptor ring and
+//               loads its K and V blocks by TMA into one ring of tiles (K0 V0 K1 V1 ...).
+//   warp 1      issues every MMA (and owns TMEM): S_t = Q_t K^T, then O_t += P_t V, one elected
+//               lane per tcgen05 instruction.
+//   warps 4-7, 8-11: softmax and epilogue of query tile 0 and 1, one thread per TMEM lane.
+// An item of more than 128 rows takes both tiles, each block being used by both; smaller items
+// take one tile per block in turn, so two blocks are in flight. Items of up to 32 (64) rows are
+// held 4 (2) times, once per 32-lane (64-lane) part of the tile: each copy takes the exponentials
+// of its own quarter (half) of the block's columns and writes zeros elsewhere, which spreads the
+// softmax of few rows over all four warps; the copies are joined in the epilogue.
+// TMEM columns: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P of a tile overwrites the
+// first half of its S. One warp issues all MMAs in order, so the barrier of a QK^T also says that
+// the tile's previous P V is complete.
+//
+// e4m3 caches: K and V go to the tensor cores as they are (kind::f8f6f4); each query row, scaled
+// by a power of two to a maximum in [128, 256), and P are both given as a sum of two e4m3 terms,
+// whose products add up in fp32. Two terms keep at least 8 significant bits, as bf16 does, down to
+// 2^-18 of the row's maximum, and K and V need no conversion pass.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <climits>
+#include <cstring>
+#include <mutex>
+
+#include "h3sa_host.h"
+#include "h3sa_ptx.cuh"
+
+namespace h3sa {
+namespace {
+
+constexpr int kD = 128;
+constexpr int kBlk = 128;        // KV rows of a block (a page)
+constexpr int kSpan = 256;       // query rows of an item: two tiles
+constexpr int kBrThreads = 384;
+constexpr int kBrRegsControl = 72;
+constexpr int kBrRegsSoftmax = 216;
+constexpr int kBrRegSplit = 128 * kBrRegsControl + 256 * kBrRegsSoftmax;
+constexpr int kDescRing = 4;
+constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
+// e4m3 P = 2^(x - m + boost) is at most 2^(threshold + boost) = 256 < 448. A fresh maximum sits at
+// 2^6 or above, where the second term still resolves 2^-16 of it.
+constexpr float kBoostF8 = 6.0f;
+constexpr float kThresholdF8 = 2.0f;
+constexpr float kThresholdBf16 = 8.0f;
+
+struct BranchParams {
+  const __nv_bfloat16* q;
+  long long q_sb, q_sn, q_sh;  // element strides of [batch, rows, heads, 128]
+  __nv_bfloat16* out;          // contiguous [batch, rows, heads, 128]
+  float* lse;                  // contiguous [batch, rows, heads] or null
+  const int* table;            // [batch, width]
+  const int* lengths;          // [batch]
+  int width, batch, rows, heads, kv_heads, group;
+  int shared;                  // leading blocks shared by all sequences
+  int causal, joint;
+  int pool_pages;
+  float scale_log2;
+  const float* k_scale;        // e4m3: [kv_heads]
+  const float* v_scale;
+  int shared_tiles;            // items over the shared blocks per KV head (split form)
+  int own_tiles;               // items per KV head and sequence
+  int shared_slot_rows, own_slot_rows;
+  long long own_row0;          // first workspace row of the own items' slots
+  float* part_o;               // [workspace rows, 128]
+  float2* part_ml;             // [workspace rows]: (maximum, sum)
+  int ctas;
+  int* err;
+};
+
+// ------------------------------------------------------------------------------ the schedule
+// Both kernels compute it from the lengths, one warp at a time.
+
+__device__ __forceinline__ int seq_length(const BranchParams& p, int b) {
+  const int n = __ldg(p.lengths + b);
+  return max(0, min(n, p.width * kBlk));
+}
+
+// blocks [lo, hi) that the rows of tile `t` of a sequence of length `len` see outside the shared
+// items
+__device__ __forceinline__ int own_lo(const BranchParams& p) { return p.joint ? 0 : p.shared; }
+__device__ __forceinline__ int own_units(const BranchParams& p, int len, int t) {
+  int limit = len;
+  if (p.causal) {
+    const int last = min((t + 1) * kSpan, p.rows * p.group) - 1;
+    limit -= p.rows - 1 - last / p.group;
+  }
+  return max(0, (limit + kBlk - 1) / kBlk - own_lo(p));
+}
+__device__ __forceinline__ int own_units_all(const BranchParams& p, int len) {
+  if (!p.causal) return own_units(p, len, 0) * p.own_tiles;
+  int n = 0;
+  for (int t = 0; t < p.own_tiles; ++t) n += own_units(p, len, t);
+  return n;
+}
+
+struct Plan {
+  int shared_units;  // blocks of one shared item
+  int head_units;    // units of one KV head
+  int cut;           // units per CTA
+  int longest;       // sequence whose table row gives the shared pages
+  int max_len;
+};
+
+__device__ __forceinline__ Plan make_plan(const BranchParams& p, int lane) {
+  int own = 0, best = -1, at = 0;
+  for (int b = lane; b < p.batch; b += 32) {
+    const int len = seq_length(p, b);
+    own += own_units_all(p, len);
+    if (len > best) {
+      best = len;
+      at = b;
+    }
+  }
+  own = __reduce_add_sync(0xffffffffu, own);
+  const int top = __reduce_max_sync(0xffffffffu, best);
+  at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
+  Plan pl;
+  pl.max_len = top;
+  pl.longest = at;
+  pl.shared_units = p.joint ? 0 : min(p.shared, (top + kBlk - 1) / kBlk);
+  pl.head_units = p.shared_tiles * pl.shared_units + own;
+  const int all = pl.head_units * p.kv_heads;
+  pl.cut = max(1, (all + p.ctas - 1) / p.ctas);
+  return pl;
+}
+
+// One item segment of a CTA, as warp 0 publishes it.
+struct Segment {
+  int live;      // 0: the CTA's last descriptor
+  int head;      // KV head
+  int row0;      // first stacked query row of the item
+  int n_rows;    // rows of the item (1..256)
+  int block0;    // first logical block
+  int blocks;
+  int kv_end;    // rows at or past it hold nothing
+  int direct;    // the segment is its rows' whole result
+  long long slot_row[2];  // workspace row of each tile's partial
+};
+
+template <bool kFp8>
+struct BrCfg {
+  static constexpr int kElem = kFp8 ? 1 : 2;
+  static constexpr int kTile = kBlk * kD * kElem;
+  static constexpr int kStages = kFp8 ? 10 : 5;
+  static constexpr int kSteps = kFp8 ? 4 : 8;      // MMA K steps of a 128-deep product
+  static constexpr int kRowsPerStep = kFp8 ? 32 : 16;
+  static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk, false) : idesc_bf16(kBlk, kBlk, false);
+  static constexpr uint32_t kIdescPV = kFp8 ? idesc_e4m3(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
+};
+
+constexpr int kQBytes = 2 * kAtom;  // a query tile: 128 x 128 bf16, or two e4m3 terms
+
+template <bool kFp8>
+struct alignas(1024) BrSmem {
+  using Cfg = BrCfg<kFp8>;
+  uint8_t q[2][kQBytes];  // also the epilogue's staging
+  uint8_t kv[Cfg::kStages][Cfg::kTile];
+  Segment desc[kDescRing];
+  uint64_t full[Cfg::kStages], empty[Cfg::kStages];
+  uint64_t d_full[kDescRing], d_empty[kDescRing];
+  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], wg[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+template <bool kFp8>
+constexpr size_t br_smem_bytes() {
+  return sizeof(BrSmem<kFp8>) + 1024;
+}
+static_assert(br_smem_bytes<false>() <= 232448 && br_smem_bytes<true>() <= 232448,
+              "branch attention needs more than 227 KB");
+
+__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* s) {
+  uint32_t r[32];
+  tmem_ld32(taddr, r);
+  tmem_wait_ld();
+  reg_fence32(r);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) s[j] = __uint_as_float(r[j]);
+}
+
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3x2_of(uint32_t h2) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h2));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t e) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(e)));
+  return r;
+}
+// Two values below 448 as the sum of two e4m3 terms each, through f16 (11 bits, so nothing that
+// the two 4-bit terms could hold is lost).
+__device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t h = f16x2_of(a, b);
+  hi = e4m3x2_of(h);
+  const uint32_t back = f16x2_of_e4m3x2(hi);
+  uint32_t rest;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(h), "r"(back));
+  lo = e4m3x2_of(rest);
+}
+
+// The address of a stacked row (b, i, g) of KV head `head` in a strided [batch, rows, heads, 128].
+struct RowAt {
+  int b, i, h;
+};
+__device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) {
+  const int bi = r / p.group;
+  RowAt a;
+  a.h = head * p.group + (r - bi * p.group);
+  a.b = bi / p.rows;
+  a.i = bi - a.b * p.rows;
+  return a;
+}
+
+// Softmax of this thread's 32 * kChunks columns of one block: scores from TMEM, P back over them.
+// Returns through m / l the running maximum (log2 units) and sum; O is rescaled here when the
+// maximum grew (lazily: only past the threshold).
+template <bool kFp8, int kChunks>
+__device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0, int limit,
+                                              float sl2, bool first, float& m, float& l) {
+  constexpr int kN = 32 * kChunks;
+  constexpr float kThreshold = kFp8 ? kThresholdF8 : kThresholdBf16;
+  constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
+  float s[kN];
+  {
+    uint32_t r[kChunks][32];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) tmem_ld32(tS + col0 + c * 32, r[c]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      reg_fence32(r[c]);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) s[c * 32 + j] = __uint_as_float(r[c][j]);
+    }
+  }
+  // columns at or past `limit` (relative to the block) are hidden from this row
+  int hide = __any_sync(0xffffffffu, limit < col0 + kN) ? 1 : 0;
+  asm volatile("" : "+r"(hide));  // keeps the compares below out of whole blocks
+  if (hide) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+      if (col0 + j >= limit) s[j] = -INFINITY;
+  }
+  float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
+#pragma unroll
+  for (int j = 4; j < kN; j += 4) {
+    mx0 = fmaxf(mx0, s[j]);
+    mx1 = fmaxf(mx1, s[j + 1]);
+    mx2 = fmaxf(mx2, s[j + 2]);
+    mx3 = fmaxf(mx3, s[j + 3]);
+  }
+  const float mb = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;
+  const bool need = mb > m + kThreshold;
+  const float m_new = need ? mb : m;
+  const float alpha = need ? fast_exp2(m - m_new) : 1.0f;
+  if (!first && __any_sync(0xffffffffu, need)) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tO + c * 32, o);
+      tmem_wait_ld();
+      reg_fence32(o);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+      tmem_st32(tO + c * 32, o);
+    }
+  }
+  l *= alpha;
+  m = m_new;
+  // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
+  const float bias = kBoost - (m == -INFINITY ? 0.0f : m);
+  const uint64_t bias2 = f2_pack(bias, bias), scale2 = f2_pack(sl2, sl2);
+  uint64_t sum2 = f2_pack(0.f, 0.f);
+#pragma unroll
+  for (int j = 0; j < kN; j += 2) {
+    float x0, x1;
+    f2_unpack(f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2), x0, x1);
+    s[j] = fast_exp2(x0);
+    s[j + 1] = fast_exp2(x1);
+    sum2 = f2_add(sum2, f2_pack(s[j], s[j + 1]));
+  }
+  float sa, sb;
+  f2_unpack(sum2, sa, sb);
+  l += sa + sb;
+  // P over the first half of S: bf16, two columns a word; e4m3, four columns a word, the first
+  // terms in words [0, 32) and the second ones in [32, 64). Zeros outside this copy's columns.
+  uint32_t w[32];
+  if constexpr (!kFp8) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {  // words [32 half, 32 half + 32): columns [64 half, ..)
+      const bool mine = kChunks == 4 || (col0 >> 6) == half;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        uint32_t v = 0u;
+        if constexpr (kChunks == 4) v = pack_bf16x2(s[64 * half + 2 * j], s[64 * half + 2 * j + 1]);
+        if constexpr (kChunks == 2) v = mine ? pack_bf16x2(s[2 * j], s[2 * j + 1]) : 0u;
+        if constexpr (kChunks == 1) {
+          const bool here = mine && ((col0 >> 5) & 1) == (j >> 4);
+          v = here ? pack_bf16x2(s[(2 * j) & 31], s[(2 * j + 1) & 31]) : 0u;
+        }
+        w[j] = v;
+      }
+      tmem_st32(tS + 32 * half, w);
+    }
+  } else {
+    uint32_t hi[kN / 4], lo[kN / 4];
+#pragma unroll
+    for (int j = 0; j < kN / 4; ++j) {
+      uint32_t h0, l0, h1, l1;
+      split_e4m3x2(s[4 * j], s[4 * j + 1], h0, l0);
+      split_e4m3x2(s[4 * j + 2], s[4 * j + 3], h1, l1);
+      hi[j] = h0 | (h1 << 16);
+      lo[j] = l0 | (l1 << 16);
+    }
+#pragma unroll
+    for (int term = 0; term < 2; ++term) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const bool here = kChunks == 4 || (col0 >> 2) / (kN / 4) == j / (kN / 4);
+        const uint32_t v = term ? lo[j % (kN / 4)] : hi[j % (kN / 4)];
+        w[j] = here ? v : 0u;
+      }
+      tmem_st32(tS + 32 * term, w);
+    }
+  }
+  tmem_wait_st();
+}
+
+// Loads a query row into the tile buffer (K-major, 128-byte swizzle). bf16: as it is, returns 1.
+// e4m3: as two terms after scaling by a power of two; returns that power's inverse.
+template <bool kFp8>
+__device__ __forceinline__ float load_query_row(uint8_t* tile, int lane_row, const __nv_bfloat16* src) {
+  uint4 v[16];
+#pragma unroll
+  for (int c = 0; c < 16; ++c)
+    v[c] = src ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+  uint8_t* row = tile + lane_row * 128;
+  const int sw = lane_row & 7;
+  if constexpr (!kFp8) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      *reinterpret_cast<uint4*>(row + (c >> 3) * kAtom + (((c & 7) ^ sw) << 4)) = v[c];
+    return 1.0f;
+  } else {
+    float amax = 0.f;
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) {
+      const float a = __uint_as_float(w[i] << 16), b = __uint_as_float(w[i] & 0xffff0000u);
+      amax = fmaxf(amax, fmaxf(fabsf(a), fabsf(b)));
+      bad = bad || !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
+    }
+    // 2^k with amax * 2^k in [128, 256); tiny rows keep their products in fp32's range
+    const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    const int k = max(-120, min(7 - e, 120));
+    const float up = __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {  // 16 columns a chunk
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t h[2], g[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const uint32_t x = w[c * 8 + j * 2 + t];
+          split_e4m3x2(__uint_as_float(x << 16) * up, __uint_as_float(x & 0xffff0000u) * up, h[t], g[t]);
+        }
+        hi[j] = h[0] | (h[1] << 16);
+        lo[j] = g[0] | (g[1] << 16);
+      }
+      const int at = (c ^ sw) << 4;
+      *reinterpret_cast<uint4*>(row + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(row + kAtom + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+    // a row with an infinity or NaN gets NaN scores, as its products have
+    return bad ? __int_as_float(0x7fffffff) : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+  }
+}
+
+template <bool kFp8>
+__global__ void __launch_bounds__(kBrThreads, 1)
+    branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const BranchParams p) {
+  using Cfg = BrCfg<kFp8>;
+  constexpr int kS = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  BrSmem<kFp8>& sm = *reinterpret_cast<BrSmem<kFp8>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  volatile int* abort_flag = &sm.abort_flag;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kS; ++s) {
+      mbar_init(smem_u32(&sm.full[s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 1);
+    }
+    for (int s = 0; s < kDescRing; ++s) {
+      mbar_init(smem_u32(&sm.d_full[s]), 1);
+      mbar_init(smem_u32(&sm.d_empty[s]), 9);  // the MMA warp and eight softmax warps
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(smem_u32(&sm.q_full[t]), 128);
+      mbar_init(smem_u32(&sm.s_full[t]), 1);
+      mbar_init(smem_u32(&sm.p_full[t]), 128);
+      mbar_init(smem_u32(&sm.o_full[t]), 1);
+      mbar_init(smem_u32(&sm.wg[t]), 128);
+    }
+    mbar_init(smem_u32(&sm.drain), 1);
+    sm.abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&sm.tmem_base), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = sm.tmem_base;
+
+  // Cursor of a consumer in the descriptor ring: waits for the next segment, copies it, releases.
+  int d_slot = 0, d_phase = 0;
+  auto next_segment = [&](Segment& g) -> bool {
+    const bool ok = mbar_wait(smem_u32(&sm.d_full[d_slot]), d_phase, abort_flag, p.err);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    g = sm.desc[d_slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sm.d_empty[d_slot]));
+    if (++d_slot == kDescRing) {
+      d_slot = 0;
+      d_phase ^= 1;
+    }
+    return g.live != 0;
+  };
+
+  // every warp of a warpgroup executes the same setmaxnreg at the top of its role
+  if (warp == 0) {
+    // ================================================================ schedule and TMA
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
+    const Plan pl = make_plan(p, lane);
+    if (lane == 0) {
+      tma_prefetch_desc(&tmK);
+      tma_prefetch_desc(&tmV);
+    }
+    for (int b = lane; b < p.batch; b += 32) {
+      const int n = __ldg(p.lengths + b);
+      if ((n < 0 || n > p.width * kBlk) && p.err) atomicOr(p.err, kErrBadIndex);
+    }
+    const int all = pl.head_units * p.kv_heads;
+    int u = min(all, static_cast<int>(blockIdx.x) * pl.cut);
+    const int u_end = min(all, u + pl.cut);
+    const int shared_all = p.shared_tiles * pl.shared_units;
+    // position: head, then a shared tile (b < 0) or (b, t), then the block offset in the item
+    int head = pl.head_units ? u / pl.head_units : 0;
+    int x = u - head * pl.head_units;
+    int b = -1, t = 0, off = 0;
+    if (u < u_end) {
+      if (x < shared_all) {
+        t = x / pl.shared_units;
+        off = x - t * pl.shared_units;
+      } else {
+        x -= shared_all;
+        for (int b0 = 0; b0 < p.batch; b0 += 32) {
+          const int bb = b0 + lane;
+          const int n = bb < p.batch ? own_units_all(p, seq_length(p, bb)) : 0;
+          int cum = n;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, cum, d);
+            if (lane >= d) cum += v;
+          }
+          const uint32_t past = __ballot_sync(0xffffffffu, cum > x);
+          if (past) {
+            const int f = __ffs(past) - 1;
+            b = b0 + f;
+            x -= __shfl_sync(0xffffffffu, cum - n, f);
+            break;
+          }
+          x -= __shfl_sync(0xffffffffu, cum, 31);
+        }
+        const int len = seq_length(p, b);
+        while (x >= own_units(p, len, t)) x -= own_units(p, len, t++);
+        off = x;
+      }
+    }
+    int ring = 0, ring_phase = 0;  // next tile of the K/V ring
+    int issued = 0;
+    int ds = 0, ds_phase = 0;
+    bool ok = true;
+    while (ok) {
+      // ---- the next segment: what is left of the current item within the CTA's range
+      Segment g;
+      memset(&g, 0, sizeof(g));
+      int seq = 0;
+      if (u < u_end) {
+        int units;
+        if (b < 0) {
+          units = pl.shared_units;
+          seq = pl.longest;
+          g.row0 = t * kSpan;
+          g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
+          g.block0 = off;
+          g.kv_end = pl.max_len;
+          for (int k = 0; k < 2; ++k)
+            g.slot_row[k] = (static_cast<long long>(head * p.shared_tiles + t + blockIdx.x) * 2 + k) *
+                            p.shared_slot_rows;
+        } else {
+          const int len = seq_length(p, b);
+          units = own_units(p, len, t);
+          seq = b;
+          g.row0 = b * p.rows * p.group + t * kSpan;
+          g.n_rows = min(kSpan, p.rows * p.group - t * kSpan);
+          g.block0 = own_lo(p) + off;
+          g.kv_end = len;
+          const long long item = (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t;
+          for (int k = 0; k < 2; ++k)
+            g.slot_row[k] = p.own_row0 + ((item + blockIdx.x) * 2 + k) * p.own_slot_rows;
+        }
+        g.live = 1;
+        g.head = head;
+        g.blocks = min(units - off, u_end - u);
+        g.direct = pl.shared_units == 0 && g.blocks == units && (g.n_rows > kBlk || g.blocks == 1);
+        u += g.blocks;
+        off = 0;
+        // ---- step to the next item that has units
+        if (u < u_end) {
+          bool found = false;
+          if (b < 0) {
+            found = ++t < p.shared_tiles && pl.shared_units > 0;
+            if (!found) {
+              b = 0;
+              t = -1;
+            }
+          }
+          while (!found) {
+            if (++t >= p.own_tiles) {
+              t = 0;
+              if (++b >= p.batch) {
+                ++head;
+                b = pl.shared_units > 0 ? -1 : 0;
+              }
+            }
+            found = b < 0 || own_units(p, seq_length(p, b), t) > 0;
+          }
+        }
+      }
+      ok = mbar_wait(smem_u32(&sm.d_empty[ds]), ds_phase ^ 1, abort_flag, p.err);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      if (lane == 0) {
+        sm.desc[ds] = g;
+        mbar_arrive(smem_u32(&sm.d_full[ds]));
+      }
+      if (++ds == kDescRing) {
+        ds = 0;
+        ds_phase ^= 1;
+      }
+      if (!g.live) break;
+      // ---- its blocks
+      for (int j0 = 0; ok && j0 < g.blocks; j0 += 32) {
+        const int n = min(32, g.blocks - j0);
+        int page = 0;
+        if (lane < n) page = __ldg(p.table + static_cast<size_t>(seq) * p.width + g.block0 + j0 + lane);
+        if (__any_sync(0xffffffffu, page < 0 || page >= p.pool_pages)) {
+          if (lane == 0) {
+            if (p.err) atomicOr(p.err, kErrBadPage);
+            *abort_flag = 1;
+          }
+          ok = false;
+          break;
+        }
+        for (int j = 0; ok && j < 2 * n; ++j) {
+          const int pg = __shfl_sync(0xffffffffu, page, j >> 1);
+          ok = mbar_wait(smem_u32(&sm.empty[ring]), ring_phase ^ 1, abort_flag, p.err);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          if (lane == 0) {
+            const uint32_t bar = smem_u32(&sm.full[ring]);
+            mbar_expect_tx(bar, Cfg::kTile);
+            const CUtensorMap* map = (j & 1) ? &tmV : &tmK;
+            for (int a = 0; a < Cfg::kTile / kAtom; ++a)
+              tma_load_3d(smem_u32(sm.kv[ring]) + a * kAtom, map, bar, a * (128 / Cfg::kElem),
+                          pg * kBlk, g.head);
+          }
+          ++issued;
+          if (++ring == kS) {
+            ring = 0;
+            ring_phase ^= 1;
+          }
+        }
+      }
+    }
+    if (!ok) {
+      // leaving early: no copy may still be in flight when the CTA ends
+      for (int i = 0; i < min(issued, kS); ++i) {
+        if (--ring < 0) {
+          ring = kS - 1;
+          ring_phase ^= 1;
+        }
+        const unsigned long long t0 = global_ns();
+        while (!mbar_try_wait(smem_u32(&sm.full[ring]), ring_phase) && global_ns() - t0 < kWaitTimeoutNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ================================================================ MMA issue
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
+    const uint32_t klo0 = sdesc_lo(smem_u32(sm.kv[0]), 16);
+    const uint32_t vlo0 = sdesc_lo(smem_u32(sm.kv[0]), kAtom);
+    constexpr uint32_t kTileDesc = Cfg::kTile >> 4;
+    int ring = 0, ring_phase = 0;  // K tile of the next unit; V follows it
+    int last_tile = 1;
+    uint32_t q_ph[2] = {0u, 0u}, p_ph[2] = {0u, 0u};
+    // the P V of each tile still to be issued
+    bool pend[2] = {}, p_acc[2] = {}, p_last[2] = {}, p_free[2] = {};
+    int p_slot[2] = {}, p_slot_ph[2] = {}, p_bad[2] = {};
+    bool ok = true;
+    auto finish = [&](int t) {  // P V of the tile's pending block
+      bool w = mbar_wait(smem_u32(&sm.full[p_slot[t]]), p_slot_ph[t], abort_flag, p.err);
+      if (w) w = mbar_wait(smem_u32(&sm.p_full[t]), p_ph[t], abort_flag, p.err);
+      p_ph[t] ^= 1u;
+      if (!(ok = __all_sync(0xffffffffu, w))) return;
+      tc_fence_after();
+      if (p_bad[t] < kBlk) {
+        // rows past the sequence's end may hold anything, NaN among it, and the tensor core
+        // multiplies them with P's zeros: clear them (the tile's load has completed)
+        uint8_t* base = sm.kv[p_slot[t]];
+        constexpr int kAtoms = Cfg::kTile / kAtom;
+        for (int i = lane; i < (kBlk - p_bad[t]) * kAtoms * 8; i += 32) {
+          const int row = p_bad[t] + (i >> 3) / kAtoms, a = (i >> 3) % kAtoms;
+          reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+      const uint32_t vlo = vlo0 + static_cast<uint32_t>(p_slot[t]) * kTileDesc;
+      const uint32_t tP = tbase + static_cast<uint32_t>(t) * 128u;
+      const uint32_t tO = tbase + 256u + static_cast<uint32_t>(t) * 128u;
+#pragma unroll
+      for (int kk = 0; kk < Cfg::kSteps; ++kk) {
+        const uint64_t bd = sdesc_join(vlo + ((kk * Cfg::kRowsPerStep * 128) >> 4));
+        const uint32_t acc = (p_acc[t] || kk > 0) ? 1u : 0u;
+        if constexpr (kFp8) {
+          mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, acc);
+          mma_ts_f8(tO, tP + 32 + kk * 8, bd, Cfg::kIdescPV, 1u);
+        } else {
+          mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, acc);
+        }
+      }
+      if (p_free[t]) tc_commit(smem_u32(&sm.empty[p_slot[t]]));
+      if (p_last[t]) tc_commit(smem_u32(&sm.o_full[t]));
+      pend[t] = false;
+    };
+    Segment g;
+    while (ok && next_segment(g)) {
+      const bool pair = g.n_rows > kBlk;
+      bool first[2] = {true, true};
+      for (int j = 0; ok && j < g.blocks; ++j) {
+        const int lo = pair ? 0 : (last_tile ^ 1);
+        const int hi = pair ? 1 : lo;
+        for (int t = lo; ok && t <= hi; ++t) {
+          if (pend[t]) finish(t);
+          if (!ok) break;
+          bool w = true;
+          if (first[t]) {
+            w = mbar_wait(smem_u32(&sm.q_full[t]), q_ph[t], abort_flag, p.err);
+            q_ph[t] ^= 1u;
+          }
+          if (w) w = mbar_wait(smem_u32(&sm.full[ring]), ring_phase, abort_flag, p.err);
+          if (!(ok = __all_sync(0xffffffffu, w))) break;
+          tc_fence_after();
+          const uint32_t klo = klo0 + static_cast<uint32_t>(ring) * kTileDesc;
+          const uint32_t qlo = sdesc_lo(smem_u32(sm.q[t]), 16);
+          const uint32_t tS = tbase + static_cast<uint32_t>(t) * 128u;
+#pragma unroll
+          for (int kk = 0; kk < Cfg::kSteps; ++kk) {
+            const uint32_t step = ((kk * 32 / 128) * kAtom + (kk * 32) % 128) >> 4;
+            if constexpr (kFp8) {
+              mma_ss_f8(tS, sdesc_join(qlo + step), sdesc_join(klo + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
+              mma_ss_f8(tS, sdesc_join(qlo + (kAtom >> 4) + step), sdesc_join(klo + step), Cfg::kIdescQK, 1u);
+            } else {
+              mma_ss(tS, sdesc_join(qlo + step), sdesc_join(klo + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
+            }
+          }
+          tc_commit(smem_u32(&sm.s_full[t]));
+          if (t == hi) tc_commit(smem_u32(&sm.empty[ring]));
+          const int vs = ring + 1 == kS ? 0 : ring + 1;
+          pend[t] = true;
+          p_acc[t] = !first[t];
+          p_last[t] = j >= g.blocks - (pair ? 1 : 2);
+          p_free[t] = t == hi;
+          p_slot[t] = vs;
+          p_slot_ph[t] = vs == 0 ? ring_phase ^ 1 : ring_phase;
+          p_bad[t] = g.kv_end - (g.block0 + j) * kBlk;
+          first[t] = false;
+          last_tile = t;
+        }
+        ring += 2;
+        if (ring >= kS) {
+          ring -= kS;
+          ring_phase ^= 1;
+        }
+      }
+    }
+    // what is still pending, oldest first
+    if (ok && pend[last_tile ^ 1]) finish(last_tile ^ 1);
+    if (ok && pend[last_tile]) finish(last_tile);
+    // leave no tensor-core work in flight past the teardown
+    tc_commit(smem_u32(&sm.drain));
+    const unsigned long long t0 = global_ns();
+    while (!mbar_try_wait(smem_u32(&sm.drain), 0)) {
+      if (global_ns() - t0 > kWaitTimeoutNs) {
+        if (p.err && lane == 0) atomicOr(p.err, kErrWaitTimeout);
+        break;
+      }
+    }
+  } else if (warp >= 4) {
+    // ================================================================ softmax and epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBrRegsSoftmax));
+    const int t = (warp - 4) >> 2;
+    const int quad = warp & 3;
+    const int lr = quad * 32 + lane;  // TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
+    const uint32_t tS = tbase + static_cast<uint32_t>(t) * 128u + lane_off;
+    const uint32_t tO = tbase + 256u + static_cast<uint32_t>(t) * 128u + lane_off;
+    uint32_t s_ph = 0u, o_ph = 0u, wg_ph = 0u;
+    int last_tile = 1;
+    bool ok = true;
+    // all 128 threads of the tile meet (bounded, so a broken pipeline cannot hang it)
+    auto meet = [&]() {
+      mbar_arrive(smem_u32(&sm.wg[t]));
+      ok = mbar_wait(smem_u32(&sm.wg[t]), wg_ph, abort_flag, p.err);
+      wg_ph ^= 1u;
+      ok = __all_sync(0xffffffffu, ok);
+      return ok;
+    };
+    Segment g;
+    while (ok && next_segment(g)) {
+      const bool pair = g.n_rows > kBlk;
+      // blocks of this tile: all, or every other one from the tile whose turn it is
+      const int begin = pair ? 0 : ((last_tile ^ 1) == t ? 0 : 1);
+      const int step = pair ? 1 : 2;
+      const int mine = g.blocks > begin ? (g.blocks - begin + step - 1) / step : 0;
+      last_tile = pair ? 1 : (last_tile ^ (g.blocks & 1));
+      const int r0 = pair ? t * kBlk : 0;
+      const int n_rows = min(kBlk, g.n_rows - r0);  // rows of this tile
+      const int span = n_rows <= 32 ? 32 : n_rows <= 64 ? 64 : 128;
+      const int my = lr & (span - 1);  // this thread's row of the tile
+      const int copy = lr / span;      // and which copy of it
+      const bool live = my < n_rows;
+      const long long ws_row = g.slot_row[t];
+      if (mine == 0) {
+        if (!g.direct && lr < n_rows) p.part_ml[ws_row + lr] = make_float2(-INFINITY, 0.f);
+        continue;
+      }
+      const RowAt at = row_at(p, g.head, g.row0 + r0 + min(my, n_rows - 1));
+      const __nv_bfloat16* src = live ? p.q + at.b * p.q_sb + at.i * p.q_sn + at.h * p.q_sh : nullptr;
+      float sl2 = p.scale_log2 * load_query_row<kFp8>(sm.q[t], lr, src);
+      if constexpr (kFp8) sl2 *= __ldg(p.k_scale + g.head);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(smem_u32(&sm.q_full[t]));
+      const int limit = seq_length(p, at.b) - (p.causal ? p.rows - 1 - at.i : 0);
+      const bool warp_live = quad * 32 % span < n_rows;
+      float m = -INFINITY, l = 0.f;
+      const int col0 = copy * span;
+      for (int j = 0; j < mine; ++j) {
+        const int left = limit - (g.block0 + begin + j * step) * kBlk;
+        ok = mbar_wait(smem_u32(&sm.s_full[t]), s_ph, abort_flag, p.err);
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        s_ph ^= 1u;
+        tc_fence_after();
+        if (warp_live) {
+          if (span == 128) softmax_block<kFp8, 4>(tS, tO, 0, left, sl2, j == 0, m, l);
+          else if (span == 64) softmax_block<kFp8, 2>(tS, tO, col0, left, sl2, j == 0, m, l);
+          else softmax_block<kFp8, 1>(tS, tO, col0, left, sl2, j == 0, m, l);
+        }
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sm.p_full[t]));
+      }
+      if (!ok) break;
+      ok = mbar_wait(smem_u32(&sm.o_full[t]), o_ph, abort_flag, p.err);
+      if (!(ok = __all_sync(0xffffffffu, ok))) break;
+      o_ph ^= 1u;
+      tc_fence_after();
+      // ---- join the copies: weights from their maxima, then O a quarter of the columns at a time
+      // through shared memory (the query tile's buffer: every QK^T of this item is complete)
+      float2* ml = reinterpret_cast<float2*>(sm.q[t] + 128 * 36 * 4);
+      float* stage = reinterpret_cast<float*>(sm.q[t]);
+      ml[lr] = make_float2(m, l);
+      if (!meet()) break;
+      float top = -INFINITY, sum = 0.f;
+      for (int c = 0; c < kBlk / span; ++c) top = fmaxf(top, ml[c * span + my].x);
+      for (int c = 0; c < kBlk / span; ++c) {
+        const float2 v = ml[c * span + my];
+        if (v.x > -INFINITY || v.y != v.y) sum += fast_exp2(v.x - top) * v.y;
+      }
+      // NaN sums must stay NaN; a copy that saw nothing weighs nothing
+      float weight = m > -INFINITY ? fast_exp2(m - top) : (l != l ? l : 0.f);
+      if (g.direct) {
+        weight = sum == 0.f ? 0.f : weight / sum;
+        if constexpr (kFp8) weight *= __ldg(p.v_scale + g.head);
+      }
+      if (live && copy == 0) {
+        const float base = top - (kFp8 ? kBoostF8 : 0.f);
+        if (!g.direct) p.part_ml[ws_row + my] = make_float2(base, sum);
+        else if (p.lse)
+          p.lse[(static_cast<long long>(at.b) * p.rows + at.i) * p.heads + at.h] =
+              sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
+      }
+#pragma unroll 1
+      for (int ch = 0; ok && ch < 4; ++ch) {
+        if (warp_live) {
+          float o[32];
+          tmem_ld_cols(tO + ch * 32, o);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(stage + lr * 36 + j * 4) =
+                weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                              : make_float4(o[4 * j] * weight, o[4 * j + 1] * weight,
+                                            o[4 * j + 2] * weight, o[4 * j + 3] * weight);
+        }
+        if (!meet()) break;
+        for (int i = lr; i < n_rows * 8; i += 128) {
+          const int r = i >> 3, c4 = i & 7;
+          float4 a = *reinterpret_cast<const float4*>(stage + r * 36 + c4 * 4);
+          for (int c = 1; c < kBlk / span; ++c) {
+            const float4 v = *reinterpret_cast<const float4*>(stage + (c * span + r) * 36 + c4 * 4);
+            a.x += v.x;
+            a.y += v.y;
+            a.z += v.z;
+            a.w += v.w;
+          }
+          if (g.direct) {
+            const RowAt ra = row_at(p, g.head, g.row0 + r0 + r);
+            __nv_bfloat16* dst =
+                p.out + ((static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h) * kD;
+            *reinterpret_cast<uint2*>(dst + ch * 32 + c4 * 4) =
+                make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+          } else {
+            *reinterpret_cast<float4*>(p.part_o + (ws_row + r) * kD + ch * 32 + c4 * 4) = a;
+          }
+        }
+        if (!meet()) break;
+      }
+      tc_fence_before();
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tbase, 512);
+  }
+}
+
+// Joins the pieces of every row that more than one segment (or tile) contributed to, in the order
+// of the units, and writes rows that see nothing: one warp per row and query head.
+template <bool kFp8>
+__global__ void __launch_bounds__(256) branch_merge_kernel(const BranchParams p) {
+  const int lane = threadIdx.x & 31;
+  const long long id = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (id >= static_cast<long long>(p.batch) * p.rows * p.heads) return;
+  const int hq = static_cast<int>(id % p.heads);
+  const int bi = static_cast<int>(id / p.heads);
+  const int b = bi / p.rows, i = bi - b * p.rows;
+  const int head = hq / p.group, g = hq - head * p.group;
+  const Plan pl = make_plan(p, lane);
+  int before = 0;  // units of the sequences in front of b
+  for (int k = lane; k < b; k += 32) before += own_units_all(p, seq_length(p, k));
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int len = seq_length(p, b);
+  const int own_row = i * p.group + g;           // row within the sequence's items
+  const int t_own = own_row / kSpan;
+  for (int t = 0; t < t_own; ++t) before += own_units(p, len, t);
+  const int row = b * p.rows * p.group + own_row;  // row of the stacked items
+  const int t_sh = row / kSpan;
+
+  float m = -INFINITY, sum = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  bool done = false;
+  auto pieces = [&](int u0, int units, int n_rows, int r, long long item, long long row0, int slot_rows) {
+    if (units == 0) return;
+    const int c_lo = u0 / pl.cut, c_hi = (u0 + units - 1) / pl.cut;
+    const bool pair = n_rows > kBlk;
+    if (pl.shared_units == 0 && c_lo == c_hi && (pair || units == 1)) {
+      done = true;  // written by the segment itself
+      return;
+    }
+    for (int c = c_lo; c <= c_hi; ++c) {
+      for (int k = pair ? r / kBlk : 0; k <= (pair ? r / kBlk : 1); ++k) {
+        const long long at = row0 + ((item + c) * 2 + k) * slot_rows + (pair ? r % kBlk : r);
+        const float2 ml = __ldcg(p.part_ml + at);
+        if (ml.y == 0.f) continue;  // saw nothing
+        const float top = fmaxf(m, ml.x);
+        const float keep = m > -INFINITY ? fast_exp2(m - top) : (sum != sum ? sum : 0.f);
+        const float w = fast_exp2(ml.x - top);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * kD) + lane);
+        acc = make_float4(acc.x * keep + v.x * w, acc.y * keep + v.y * w, acc.z * keep + v.z * w,
+                          acc.w * keep + v.w * w);
+        sum = sum * keep + ml.y * w;
+        m = top;
+      }
+    }
+  };
+  if (pl.shared_units > 0)
+    pieces(head * pl.head_units + t_sh * pl.shared_units, pl.shared_units,
+           min(kSpan, p.batch * p.rows * p.group - t_sh * kSpan), row - t_sh * kSpan,
+           head * p.shared_tiles + t_sh, 0, p.shared_slot_rows);
+  pieces(head * pl.head_units + p.shared_tiles * pl.shared_units + before, own_units(p, len, t_own),
+         min(kSpan, p.rows * p.group - t_own * kSpan), own_row - t_own * kSpan,
+         (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t_own, p.own_row0, p.own_slot_rows);
+  if (done) return;
+  float scale = sum == 0.f ? 0.f : 1.0f / sum;
+  if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
+  if (sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  reinterpret_cast<uint2*>(p.out + id * kD)[lane] =
+      make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
+  if (p.lse && lane == 0)
+    p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+struct Shape {
+  int shared_tiles, own_tiles, shared_slot_rows, own_slot_rows, joint, ctas;
+  long long own_row0, rows;  // workspace rows
+};
+
+int sm_count() {
+  static int counts[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (counts[dev] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+    counts[dev] = n;
+  }
+  return counts[dev];
+}
+
+// The split form reads the shared blocks once for all branches but merges two partial results per
+// row; with many rows per branch each tile is full within one branch and the joint form has
+// nothing to merge.
+constexpr int kJointRows = 2 * kSpan;
+
+Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
+  Shape s;
+  const long long own = static_cast<long long>(rows) * group;
+  const long long all = own * batch;
+  s.ctas = sm_count();
+  s.joint = own >= kJointRows ? 1 : 0;
+  s.own_tiles = static_cast<int>((own + kSpan - 1) / kSpan);
+  s.shared_tiles = s.joint || shared == 0 ? 0 : static_cast<int>((all + kSpan - 1) / kSpan);
+  s.own_slot_rows = static_cast<int>(own < kBlk ? own : kBlk);
+  s.shared_slot_rows = static_cast<int>(all < kBlk ? all : kBlk);
+  s.own_row0 = s.shared_tiles == 0
+                   ? 0
+                   : (static_cast<long long>(kv_heads) * s.shared_tiles + s.ctas) * 2 * s.shared_slot_rows;
+  s.rows = s.own_row0 +
+           (static_cast<long long>(kv_heads) * batch * s.own_tiles + s.ctas) * 2 * s.own_slot_rows;
+  return s;
+}
+
+template <bool kFp8>
+int configure() {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  if (dev < 64 && done[dev]) return H3SA_OK;
+  const auto kernel = branch_attn_kernel<kFp8>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(br_smem_bytes<kFp8>()));
+  if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch attention)", e);
+  cudaFuncAttributes attr;
+  e = cudaFuncGetAttributes(&attr, kernel);
+  if (e != cudaSuccess) return set_cuda_error("cudaFuncGetAttributes(branch attention)", e);
+  // setmaxnreg.inc waits for registers of the block's launch allocation: refuse a build that
+  // cannot fund the split
+  if (attr.numRegs * kBrThreads < kBrRegSplit)
+    return set_error(H3SA_ERR_UNSUPPORTED, "branch attention build has %d registers per thread; the "
+                     "warp-role register split needs %d", attr.numRegs,
+                     (kBrRegSplit + kBrThreads - 1) / kBrThreads);
+  if (dev < 64) done[dev] = true;
+  return H3SA_OK;
+}
+
+template <bool kFp8>
+int launch(const BranchParams& p, const void* key_pool, const void* value_pool, cudaStream_t stream) {
+  using Cfg = BrCfg<kFp8>;
+  int rc = configure<kFp8>();
+  if (rc) return rc;
+  CUtensorMap tmK, tmV;
+  const CUtensorMapDataType dt = kFp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const uint64_t pool_rows = static_cast<uint64_t>(p.pool_pages) * kBlk;
+  const uint64_t dims[3] = {kD, pool_rows, static_cast<uint64_t>(p.kv_heads)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(kD) * Cfg::kElem, pool_rows * kD * Cfg::kElem};
+  const uint32_t box[3] = {128 / Cfg::kElem, static_cast<uint32_t>(kBlk), 1};
+  if ((rc = encode_tiled_3d(&tmK, dt, key_pool, dims, strides, box))) return rc;
+  if ((rc = encode_tiled_3d(&tmV, dt, value_pool, dims, strides, box))) return rc;
+  branch_attn_kernel<kFp8><<<p.ctas, kBrThreads, br_smem_bytes<kFp8>(), stream>>>(tmK, tmV, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error("branch_attn_kernel launch", e);
+  const long long rows = static_cast<long long>(p.batch) * p.rows * p.heads;
+  branch_merge_kernel<kFp8><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error("branch_merge_kernel launch", e);
+  return H3SA_OK;
+}
+
+bool aligned(const void* q, size_t n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; }
+
+}  // namespace
+}  // namespace h3sa
+
+using namespace h3sa;
+
+extern "C" {
+
+int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+                                     int32_t shared_rows) {
+  if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
+    return 0;
+  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
+  return s.rows * (kD * 4 + 8);
+}
+
+int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides, void* out, float* lse,
+                                 int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+                                 const void* key_pool, const void* value_pool, int32_t pool_pages,
+                                 int32_t e4m3, const float* k_scale, const float* v_scale,
+                                 const int32_t* table, int32_t width, const int32_t* lengths,
+                                 int32_t shared_rows, int32_t causal, float softmax_scale,
+                                 void* workspace, int64_t workspace_bytes, int32_t* device_error,
+                                 void* stream) {
+  if (batch < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads)
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: invalid sizes batch=%d rows=%d heads=%d "
+                     "kv_heads=%d (heads must be a multiple of kv_heads)", batch, rows, heads, kv_heads);
+  if (batch == 0 || rows == 0) return H3SA_OK;
+  if (pool_pages <= 0 || width <= 0 || static_cast<int64_t>(pool_pages) * kBlk > INT32_MAX ||
+      static_cast<int64_t>(width) * kBlk > INT32_MAX)
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: invalid pool of %d pages or table of %d "
+                     "entries a sequence", pool_pages, width);
+  if (shared_rows < 0 || shared_rows % kBlk || shared_rows / kBlk > width)
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: %d shared rows are not whole pages of a "
+                     "table of %d entries", shared_rows, width);
+  if (!query || !query_strides || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
+      (e4m3 && (!k_scale || !v_scale)))
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
+  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f)
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
+  if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
+      !aligned(workspace, 16) || query_strides[0] % 8 || query_strides[1] % 8 || query_strides[2] % 8)
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned");
+  const int group = heads / kv_heads;
+  const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
+  const int64_t tiles = (static_cast<int64_t>(rows) * group + kSpan - 1) / kSpan;
+  if (stacked > INT32_MAX / 2 ||
+      kv_heads * (((stacked + kSpan - 1) / kSpan) * (shared_rows / kBlk) + batch * tiles * width) > INT32_MAX / 2 ||
+      static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
+    return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d over %d "
+                     "pages exceeds the work index", batch, rows, heads, width);
+  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
+  if (workspace_bytes < s.rows * (kD * 4 + 8))
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: workspace of %lld bytes, %lld needed",
+                     static_cast<long long>(workspace_bytes), s.rows * (kD * 4 + 8));
+  BranchParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = static_cast<const __nv_bfloat16*>(query);
+  p.q_sb = query_strides[0];
+  p.q_sn = query_strides[1];
+  p.q_sh = query_strides[2];
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.lse = lse;
+  p.table = table;
+  p.lengths = lengths;
+  p.width = width;
+  p.batch = batch;
+  p.rows = rows;
+  p.heads = heads;
+  p.kv_heads = kv_heads;
+  p.group = group;
+  p.shared = shared_rows / kBlk;
+  p.causal = causal ? 1 : 0;
+  p.joint = s.joint;
+  p.pool_pages = pool_pages;
+  p.scale_log2 = softmax_scale * 1.4426950408889634f;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.shared_tiles = s.shared_tiles;
+  p.own_tiles = s.own_tiles;
+  p.shared_slot_rows = s.shared_slot_rows;
+  p.own_slot_rows = s.own_slot_rows;
+  p.own_row0 = s.own_row0;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + s.rows * kD);
+  p.ctas = s.ctas;
+  p.err = device_error;
+  return e4m3 ? launch<true>(p, key_pool, value_pool, static_cast<cudaStream_t>(stream))
+              : launch<false>(p, key_pool, value_pool, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

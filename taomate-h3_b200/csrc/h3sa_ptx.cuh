@@ -20,6 +20,7 @@ enum DeviceError : int {
   kErrWaitTimeout = 1,      // an mbarrier wait gave up
   kErrBadPage = 2,          // page-table entry outside the pool
   kErrBadIndex = 4,         // row index outside its tensor
+  kErrNoPages = 8,          // a pool has too few free pages
 };
 
 constexpr unsigned long long kWaitTimeoutNs = 2000000000ull;  // 2 s

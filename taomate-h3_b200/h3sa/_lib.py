@@ -22,6 +22,7 @@ H3SA_ERR_CUDA = 3
 DEVERR_WAIT_TIMEOUT = 1
 DEVERR_BAD_PAGE = 2
 DEVERR_BAD_INDEX = 4
+DEVERR_NO_PAGES = 8
 
 MAX_PROBLEMS = 4
 
@@ -62,8 +63,21 @@ class Rows(ctypes.Structure):
     ]
 
 
+class Pools(ctypes.Structure):
+    _fields_ = [
+        ("list", ctypes.c_void_p),
+        ("base", ctypes.c_void_p),
+        ("stride", ctypes.c_int64),
+        ("count", ctypes.c_int32),
+        ("heads", ctypes.c_int32),
+        ("pages", ctypes.c_int32),
+        ("row_bytes", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 _F = ctypes.c_float
 
 # name -> (restype, argtypes)
@@ -137,6 +151,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "h3sa_peer_barrier": (ctypes.c_int, [_P, _I, _I, ctypes.c_uint32, _P, _P]),
     "h3sa_peer_barrier_limit": (ctypes.c_int, [_P, _I, _I, ctypes.c_uint32, ctypes.c_int64, _P,
                                                _P]),
+    "h3sa_pages_workspace": (_L, [_I, _I]),
+    "h3sa_fork_pages": (
+        ctypes.c_int,
+        [ctypes.POINTER(Pools), _P, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "h3sa_compact_pages": (
+        ctypes.c_int, [ctypes.POINTER(Pools), _P, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "h3sa_free_pages": (ctypes.c_int, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
+    "h3sa_shared_prefix_workspace": (_L, [_I, _I, _I, _I, _I]),
+    "h3sa_shared_prefix_attention": (
+        ctypes.c_int,
+        [_P, ctypes.POINTER(_L), _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I,
+         _I, _F, _P, _L, _P, _P]),
     "h3sa_permute_rows": (
         ctypes.c_int,
         [_P, _P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),
