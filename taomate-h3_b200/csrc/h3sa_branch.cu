@@ -20,8 +20,8 @@
 // Warp roles of branch_attn_kernel (one persistent CTA per SM, 384 threads):
 //   warp 0      walks the CTA's units: publishes each item segment in a small descriptor ring and
 //               loads its K and V blocks by TMA into one ring of tiles (K0 V0 K1 V1 ...).
-//   warp 1      issues every MMA (and owns TMEM): S_t = Q_t K^T, then O_t += P_t V, one elected
-//               lane per tcgen05 instruction.
+//   warp 1, 2   issue the MMAs of query tile 0 and 1: S_t = Q_t K^T, then O_t += P_t V, one elected
+//               lane per tcgen05 instruction (warp 1 also owns TMEM).
 //   warps 4-7, 8-11: softmax and epilogue of query tile 0 and 1, one thread per TMEM lane.
 // An item of more than 128 rows takes both tiles, each block being used by both; smaller items
 // take one tile per block in turn, so two blocks are in flight. Items of up to 32 (64) rows are
@@ -29,8 +29,8 @@
 // of its own quarter (half) of the block's columns and writes zeros elsewhere, which spreads the
 // softmax of few rows over all four warps; the copies are joined in the epilogue.
 // TMEM columns: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P of a tile overwrites the
-// first half of its S. One warp issues all MMAs in order, so the barrier of a QK^T also says that
-// the tile's previous P V is complete.
+// first half of its S. A tile's MMAs are issued in order by one warp, so the barrier of a QK^T also
+// says that the tile's previous P V is complete.
 //
 // e4m3 caches: K and V go to the tensor cores as they are (kind::f8f6f4); each query row, scaled
 // by a power of two to a maximum in [128, 256), and P are both given as a sum of two e4m3 terms,
@@ -44,6 +44,7 @@
 #include <climits>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
@@ -168,6 +169,7 @@ struct BrCfg {
   static constexpr int kSteps = kFp8 ? 4 : 8;      // MMA K steps of a 128-deep product
   static constexpr int kRowsPerStep = kFp8 ? 32 : 16;
   static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk, false) : idesc_bf16(kBlk, kBlk, false);
+  static constexpr uint32_t kIdescQKHalf = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
   static constexpr uint32_t kIdescPV = kFp8 ? idesc_e4m3(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
 };
 
@@ -179,10 +181,11 @@ struct alignas(1024) BrSmem {
   uint8_t q[2][kQBytes];  // also the epilogue's staging
   uint8_t kv[Cfg::kStages][Cfg::kTile];
   Segment desc[kDescRing];
-  uint64_t full[Cfg::kStages], empty[Cfg::kStages];
+  uint64_t full[2][Cfg::kStages], empty[Cfg::kStages];
   uint64_t d_full[kDescRing], d_empty[kDescRing];
-  uint64_t q_full[2], s_full[2], p_full[2], o_full[2], wg[2];
-  uint64_t drain;
+  uint64_t q_full[2], o_full[2], pv_done[2], wg[2];
+  uint64_t s_full[2][2], p_full[2][2];  // [tile][half of a block]; whole blocks use the first
+  uint64_t m_sync, drain;
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -241,16 +244,19 @@ __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) 
   return a;
 }
 
-// Softmax of this thread's 32 * kChunks columns of one block: scores from TMEM, P back over them.
-// Returns through m / l the running maximum (log2 units) and sum; O is rescaled here when the
-// maximum grew (lazily: only past the threshold).
-template <bool kFp8, int kChunks>
-__device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0, int limit,
-                                              float sl2, bool first, float& m, float& l) {
-  constexpr int kN = 32 * kChunks;
+// Softmax of kCols score columns of this thread's row: columns [col0, col0 + kCols) of a block, in
+// TMEM at tS + col0. kHalf: they are one half of the block, and P goes over them, dense. Otherwise
+// they are this copy's share of the block, and P goes over the first half of all 128 columns with
+// zeros for the other copies' shares. m / l: running maximum (log2 units) and sum; `pv_done` waits
+// until O holds all earlier blocks, before O is rescaled because the maximum grew (lazily: only
+// past the threshold).
+template <bool kFp8, int kCols, bool kHalf, typename Wait>
+__device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0, int limit, float sl2,
+                                              bool first, float& m, float& l, Wait&& pv_done) {
   constexpr float kThreshold = kFp8 ? kThresholdF8 : kThresholdBf16;
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
-  float s[kN];
+  constexpr int kChunks = kCols / 32;
+  float s[kCols];
   {
     uint32_t r[kChunks][32];
 #pragma unroll
@@ -264,26 +270,50 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
     }
   }
   // columns at or past `limit` (relative to the block) are hidden from this row
-  int hide = __any_sync(0xffffffffu, limit < col0 + kN) ? 1 : 0;
+  int hide = __any_sync(0xffffffffu, limit < col0 + kCols) ? 1 : 0;
   asm volatile("" : "+r"(hide));  // keeps the compares below out of whole blocks
   if (hide) {
 #pragma unroll
-    for (int j = 0; j < kN; ++j)
+    for (int j = 0; j < kCols; ++j)
       if (col0 + j >= limit) s[j] = -INFINITY;
   }
   float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
-  for (int j = 4; j < kN; j += 4) {
-    mx0 = fmaxf(mx0, s[j]);
-    mx1 = fmaxf(mx1, s[j + 1]);
-    mx2 = fmaxf(mx2, s[j + 2]);
-    mx3 = fmaxf(mx3, s[j + 3]);
+  for (int j = 4; j + 4 < kCols; j += 8) {
+    mx0 = fmax3(mx0, s[j], s[j + 4]);
+    mx1 = fmax3(mx1, s[j + 1], s[j + 5]);
+    mx2 = fmax3(mx2, s[j + 2], s[j + 6]);
+    mx3 = fmax3(mx3, s[j + 3], s[j + 7]);
   }
-  const float mb = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sl2;
+  // kCols is a multiple of 8, so four columns are left
+  const float mb = fmax3(fmax3(mx0, mx1, mx2), fmax3(mx3, s[kCols - 4], s[kCols - 3]),
+                         fmaxf(s[kCols - 2], s[kCols - 1])) * sl2;
   const bool need = mb > m + kThreshold;
   const float m_new = need ? mb : m;
   const float alpha = need ? fast_exp2(m - m_new) : 1.0f;
-  if (!first && __any_sync(0xffffffffu, need)) {
+  const bool any_need = !first && __any_sync(0xffffffffu, need);
+  l *= alpha;
+  m = m_new;
+  // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
+  const float bias = kBoost - (m == -INFINITY ? 0.0f : m);
+  const uint64_t bias2 = f2_pack(bias, bias), scale2 = f2_pack(sl2, sl2);
+  uint64_t sum2 = f2_pack(0.f, 0.f);
+  uint32_t pk[kFp8 ? 1 : kCols / 2];
+#pragma unroll
+  for (int j = 0; j < kCols; j += 2) {
+    float x0, x1;
+    f2_unpack(f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2), x0, x1);
+    s[j] = fast_exp2(x0);
+    s[j + 1] = fast_exp2(x1);
+    sum2 = f2_add(sum2, f2_pack(s[j], s[j + 1]));
+    if constexpr (!kFp8) pk[j / 2] = pack_bf16x2(s[j], s[j + 1]);
+  }
+  float sa, sb;
+  f2_unpack(sum2, sa, sb);
+  l += sa + sb;
+  pv_done();
+  if (any_need) {
+    tc_fence_after();
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       uint32_t o[32];
@@ -295,62 +325,50 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
       tmem_st32(tO + c * 32, o);
     }
   }
-  l *= alpha;
-  m = m_new;
-  // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
-  const float bias = kBoost - (m == -INFINITY ? 0.0f : m);
-  const uint64_t bias2 = f2_pack(bias, bias), scale2 = f2_pack(sl2, sl2);
-  uint64_t sum2 = f2_pack(0.f, 0.f);
-#pragma unroll
-  for (int j = 0; j < kN; j += 2) {
-    float x0, x1;
-    f2_unpack(f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2), x0, x1);
-    s[j] = fast_exp2(x0);
-    s[j + 1] = fast_exp2(x1);
-    sum2 = f2_add(sum2, f2_pack(s[j], s[j + 1]));
-  }
-  float sa, sb;
-  f2_unpack(sum2, sa, sb);
-  l += sa + sb;
-  // P over the first half of S: bf16, two columns a word; e4m3, four columns a word, the first
-  // terms in words [0, 32) and the second ones in [32, 64). Zeros outside this copy's columns.
+  // P: bf16, two columns a word; e4m3, four columns a word, the first terms in front of the second
   uint32_t w[32];
   if constexpr (!kFp8) {
+    if constexpr (kHalf) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {  // words [32 half, 32 half + 32): columns [64 half, ..)
-      const bool mine = kChunks == 4 || (col0 >> 6) == half;
+      for (int j = 0; j < 32; ++j) w[j] = pk[j];
+      tmem_st32(tS + col0, w);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        uint32_t v = 0u;
-        if constexpr (kChunks == 4) v = pack_bf16x2(s[64 * half + 2 * j], s[64 * half + 2 * j + 1]);
-        if constexpr (kChunks == 2) v = mine ? pack_bf16x2(s[2 * j], s[2 * j + 1]) : 0u;
-        if constexpr (kChunks == 1) {
-          const bool here = mine && ((col0 >> 5) & 1) == (j >> 4);
-          v = here ? pack_bf16x2(s[(2 * j) & 31], s[(2 * j + 1) & 31]) : 0u;
+      for (int half = 0; half < 2; ++half) {  // words [32 half, 32 half + 32): columns [64 half, ..)
+        const bool mine = (col0 >> 6) == half;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const bool here = mine && (kCols == 64 || ((col0 >> 5) & 1) == (j >> 4));
+          w[j] = here ? pk[j % (kCols / 2)] : 0u;
         }
-        w[j] = v;
+        tmem_st32(tS + 32 * half, w);
       }
-      tmem_st32(tS + 32 * half, w);
     }
   } else {
-    uint32_t hi[kN / 4], lo[kN / 4];
+    constexpr int kW = kCols / 4;
+    uint32_t hi[kW], lo[kW];
 #pragma unroll
-    for (int j = 0; j < kN / 4; ++j) {
+    for (int j = 0; j < kW; ++j) {
       uint32_t h0, l0, h1, l1;
       split_e4m3x2(s[4 * j], s[4 * j + 1], h0, l0);
       split_e4m3x2(s[4 * j + 2], s[4 * j + 3], h1, l1);
       hi[j] = h0 | (h1 << 16);
       lo[j] = l0 | (l1 << 16);
     }
+    if constexpr (kHalf) {
 #pragma unroll
-    for (int term = 0; term < 2; ++term) {
+      for (int j = 0; j < 32; ++j) w[j] = j < 16 ? hi[j % kW] : lo[j % kW];
+      tmem_st32(tS + col0, w);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const bool here = kChunks == 4 || (col0 >> 2) / (kN / 4) == j / (kN / 4);
-        const uint32_t v = term ? lo[j % (kN / 4)] : hi[j % (kN / 4)];
-        w[j] = here ? v : 0u;
+      for (int term = 0; term < 2; ++term) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const bool here = (col0 >> 2) / kW == j / kW;
+          w[j] = here ? (term ? lo[j % kW] : hi[j % kW]) : 0u;
+        }
+        tmem_st32(tS + 32 * term, w);
       }
-      tmem_st32(tS + 32 * term, w);
     }
   }
   tmem_wait_st();
@@ -423,21 +441,26 @@ __global__ void __launch_bounds__(kBrThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kS; ++s) {
-      mbar_init(smem_u32(&sm.full[s]), 1);
-      mbar_init(smem_u32(&sm.empty[s]), 1);
+      mbar_init(smem_u32(&sm.full[0][s]), 1);
+      mbar_init(smem_u32(&sm.full[1][s]), 1);
+      mbar_init(smem_u32(&sm.empty[s]), 2);
     }
     for (int s = 0; s < kDescRing; ++s) {
       mbar_init(smem_u32(&sm.d_full[s]), 1);
-      mbar_init(smem_u32(&sm.d_empty[s]), 9);  // the MMA warp and eight softmax warps
+      mbar_init(smem_u32(&sm.d_empty[s]), 10);  // two MMA warps and eight softmax warps
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&sm.q_full[t]), 128);
-      mbar_init(smem_u32(&sm.s_full[t]), 1);
-      mbar_init(smem_u32(&sm.p_full[t]), 128);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(smem_u32(&sm.s_full[t][h]), 1);
+        mbar_init(smem_u32(&sm.p_full[t][h]), 128);
+      }
+      mbar_init(smem_u32(&sm.pv_done[t]), 1);
       mbar_init(smem_u32(&sm.o_full[t]), 1);
       mbar_init(smem_u32(&sm.wg[t]), 128);
     }
-    mbar_init(smem_u32(&sm.drain), 1);
+    mbar_init(smem_u32(&sm.m_sync), 2);
+    mbar_init(smem_u32(&sm.drain), 2);
     sm.abort_flag = 0;
     fence_mbar_init();
   }
@@ -480,7 +503,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     }
     const int all = pl.head_units * p.kv_heads;
     int u = min(all, static_cast<int>(blockIdx.x) * pl.cut);
-    const int u_end = min(all, u + pl.cut);
+    int u_end = min(all, u + pl.cut);
     const int shared_all = p.shared_tiles * pl.shared_units;
     // position: head, then a shared tile (b < 0) or (b, t), then the block offset in the item
     int head = pl.head_units ? u / pl.head_units : 0;
@@ -515,8 +538,47 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         off = x;
       }
     }
+    const auto step_item = [&]() {  // to the next item that has units
+      bool found = false;
+      if (b < 0) {
+        found = ++t < p.shared_tiles && pl.shared_units > 0;
+        if (!found) {
+          b = 0;
+          t = -1;
+        }
+      }
+      while (!found) {
+        if (++t >= p.own_tiles) {
+          t = 0;
+          if (++b >= p.batch) {
+            ++head;
+            b = pl.shared_units > 0 ? -1 : 0;
+          }
+        }
+        found = b < 0 || own_units(p, seq_length(p, b), t) > 0;
+      }
+    };
+    // A range that starts inside an item and goes on past it takes that rest last. All CTAs then
+    // walk their items from the first block on, and those that read the same keys read them at
+    // about the same time, from L2.
+    int later = 0, later_head = 0, later_b = 0, later_t = 0, later_off = 0;
+    if (u < u_end && off > 0) {
+      const int rest = (b < 0 ? pl.shared_units : own_units(p, seq_length(p, b), t)) - off;
+      if (rest < u_end - u) {
+        later = rest;
+        later_head = head;
+        later_b = b;
+        later_t = t;
+        later_off = off;
+        u += rest;
+        off = 0;
+        step_item();
+      }
+    }
     int ring = 0, ring_phase = 0;  // next tile of the K/V ring
-    int issued = 0;
+    int issued = 0, last_tile = 1;
+    uint32_t on_tile1 = 0u;  // slots whose latest load signals tile 1's barrier
+    uint32_t full_ph[2] = {0u, 0u};
     int ds = 0, ds_phase = 0;
     bool ok = true;
     while (ok) {
@@ -554,26 +616,14 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         g.direct = pl.shared_units == 0 && g.blocks == units && (g.n_rows > kBlk || g.blocks == 1);
         u += g.blocks;
         off = 0;
-        // ---- step to the next item that has units
-        if (u < u_end) {
-          bool found = false;
-          if (b < 0) {
-            found = ++t < p.shared_tiles && pl.shared_units > 0;
-            if (!found) {
-              b = 0;
-              t = -1;
-            }
-          }
-          while (!found) {
-            if (++t >= p.own_tiles) {
-              t = 0;
-              if (++b >= p.batch) {
-                ++head;
-                b = pl.shared_units > 0 ? -1 : 0;
-              }
-            }
-            found = b < 0 || own_units(p, seq_length(p, b), t) > 0;
-          }
+        if (u < u_end) step_item();
+        if (u >= u_end && later > 0) {
+          head = later_head;
+          b = later_b;
+          t = later_t;
+          off = later_off;
+          u_end = u + later;
+          later = 0;
         }
       }
       ok = mbar_wait(smem_u32(&sm.d_empty[ds]), ds_phase ^ 1, abort_flag, p.err);
@@ -588,6 +638,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       }
       if (!g.live) break;
       // ---- its blocks
+      const bool pair = g.n_rows > kBlk;
       for (int j0 = 0; ok && j0 < g.blocks; j0 += 32) {
         const int n = min(32, g.blocks - j0);
         int page = 0;
@@ -604,8 +655,14 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           const int pg = __shfl_sync(0xffffffffu, page, j >> 1);
           ok = mbar_wait(smem_u32(&sm.empty[ring]), ring_phase ^ 1, abort_flag, p.err);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          // a block of one tile signals that tile's barrier, a shared one tile 0's
+          if ((j & 1) == 0) last_tile = pair ? 1 : last_tile ^ 1;
+          const int side = pair ? 0 : last_tile;
+          on_tile1 = (on_tile1 & ~(1u << ring)) | (static_cast<uint32_t>(side) << ring);
+          if (side) full_ph[1] ^= 1u << ring;
+          else full_ph[0] ^= 1u << ring;
           if (lane == 0) {
-            const uint32_t bar = smem_u32(&sm.full[ring]);
+            const uint32_t bar = smem_u32(&sm.full[side][ring]);
             mbar_expect_tx(bar, Cfg::kTile);
             const CUtensorMap* map = (j & 1) ? &tmV : &tmK;
             for (int a = 0; a < Cfg::kTile / kAtom; ++a)
@@ -623,118 +680,192 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     if (!ok) {
       // leaving early: no copy may still be in flight when the CTA ends
       for (int i = 0; i < min(issued, kS); ++i) {
-        if (--ring < 0) {
-          ring = kS - 1;
-          ring_phase ^= 1;
-        }
+        if (--ring < 0) ring = kS - 1;
+        const int side = (on_tile1 >> ring) & 1u;
+        const uint32_t ph = (((side ? full_ph[1] : full_ph[0]) >> ring) & 1u) ^ 1u;
         const unsigned long long t0 = global_ns();
-        while (!mbar_try_wait(smem_u32(&sm.full[ring]), ring_phase) && global_ns() - t0 < kWaitTimeoutNs) {
+        while (!mbar_try_wait(smem_u32(&sm.full[side][ring]), ph) && global_ns() - t0 < kWaitTimeoutNs) {
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || warp == 2) {
     // ================================================================ MMA issue
+    // Warp 1 serves tile 0 and warp 2 tile 1: a warp stays blocked in tcgen05.mma until the tensor
+    // pipe takes the instruction, so one issuer for both tiles left the pipe idle half the time
+    // (2000 cycles a block of one tile, of which 1024 are MMAs).
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
+    const int mt = warp - 1;
     const uint32_t klo0 = sdesc_lo(smem_u32(sm.kv[0]), 16);
     const uint32_t vlo0 = sdesc_lo(smem_u32(sm.kv[0]), kAtom);
     constexpr uint32_t kTileDesc = Cfg::kTile >> 4;
-    int ring = 0, ring_phase = 0;  // K tile of the next unit; V follows it
+    const uint32_t qlo = sdesc_lo(smem_u32(sm.q[mt]), 16);
+    const uint32_t tS = tbase + static_cast<uint32_t>(mt) * 128u;
+    const uint32_t tO = tbase + 256u + static_cast<uint32_t>(mt) * 128u;
+    const uint32_t q_bar = smem_u32(&sm.q_full[mt]), s_bar = smem_u32(&sm.s_full[mt]);
+    const uint32_t p_bar = smem_u32(&sm.p_full[mt]), o_bar = smem_u32(&sm.o_full[mt]);
+    const uint32_t pv_bar = smem_u32(&sm.pv_done[mt]);
+    int ring = 0;  // K tile of the next unit; V follows it
+    // The next phase of each slot's two full barriers, a bit per slot: a tile's own blocks land
+    // on its barrier, blocks of both tiles on that of tile 0. So a warp never waits on a phase
+    // whose predecessor it skipped.
+    uint32_t phase0 = 0u, phase1 = 0u;
+    uint32_t q_ph = 0u, p_ph = 0u, m_ph = 0u;
     int last_tile = 1;
-    uint32_t q_ph[2] = {0u, 0u}, p_ph[2] = {0u, 0u};
-    // the P V of each tile still to be issued
-    bool pend[2] = {}, p_acc[2] = {}, p_last[2] = {}, p_free[2] = {};
-    int p_slot[2] = {}, p_slot_ph[2] = {}, p_bad[2] = {};
-    bool ok = true;
-    auto finish = [&](int t) {  // P V of the tile's pending block
-      bool w = mbar_wait(smem_u32(&sm.full[p_slot[t]]), p_slot_ph[t], abort_flag, p.err);
-      if (w) w = mbar_wait(smem_u32(&sm.p_full[t]), p_ph[t], abort_flag, p.err);
-      p_ph[t] ^= 1u;
+    bool ok = true, was_solo = false;
+    // the P V of this tile's last block, still to be issued
+    bool pend = false, pend_acc = false, pend_pair = false, pend_halves = false;
+    int pend_slot = 0, pend_rows = 0;
+    uint32_t pend_bar = 0u, pend_ph = 0u;
+    // Waits for P and issues the pending P V: of the whole block (half < 0), or of one half of its
+    // rows (P of the first half precedes that of the second).
+    auto finish = [&](int half) {
+      const int which = half < 0 ? 0 : half;
+      const bool w = mbar_wait(p_bar + which * 8, (p_ph >> which) & 1u, abort_flag, p.err);
+      p_ph ^= 1u << which;
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
-      if (p_bad[t] < kBlk) {
+      if (pend_rows < kBlk && half <= 0) {
         // rows past the sequence's end may hold anything, NaN among it, and the tensor core
-        // multiplies them with P's zeros: clear them (the tile's load has completed)
-        uint8_t* base = sm.kv[p_slot[t]];
+        // multiplies them with P's zeros: clear them (the tile's load has completed; both warps
+        // of a shared block write the same zeros)
+        uint8_t* base = sm.kv[pend_slot];
         constexpr int kAtoms = Cfg::kTile / kAtom;
-        for (int i = lane; i < (kBlk - p_bad[t]) * kAtoms * 8; i += 32) {
-          const int row = p_bad[t] + (i >> 3) / kAtoms, a = (i >> 3) % kAtoms;
+        for (int i = lane; i < (kBlk - pend_rows) * kAtoms * 8; i += 32) {
+          const int row = pend_rows + (i >> 3) / kAtoms, a = (i >> 3) % kAtoms;
           reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7] = make_uint4(0u, 0u, 0u, 0u);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      const uint32_t vlo = vlo0 + static_cast<uint32_t>(p_slot[t]) * kTileDesc;
-      const uint32_t tP = tbase + static_cast<uint32_t>(t) * 128u;
-      const uint32_t tO = tbase + 256u + static_cast<uint32_t>(t) * 128u;
+      const uint32_t vlo = vlo0 + static_cast<uint32_t>(pend_slot) * kTileDesc;
+      if (half < 0) {
+        const uint32_t acc = pend_acc ? 1u : 0u;
+#pragma unroll
+        for (int kk = 0; kk < Cfg::kSteps; ++kk) {
+          const uint64_t bd = sdesc_join(vlo + ((kk * Cfg::kRowsPerStep * 128) >> 4));
+          if constexpr (kFp8) {
+            mma_ts_f8(tO, tS + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
+            mma_ts_f8(tO, tS + 32 + kk * 8, bd, Cfg::kIdescPV, 1u);
+          } else {
+            mma_ts(tO, tS + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
+          }
+        }
+      } else {
+        const uint32_t acc = pend_acc || half > 0 ? 1u : 0u;
+        const uint32_t tP = tS + 64u * half, vh = vlo + half * ((64 * 128) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < Cfg::kSteps / 2; ++kk) {
+          const uint64_t bd = sdesc_join(vh + ((kk * Cfg::kRowsPerStep * 128) >> 4));
+          if constexpr (kFp8) {
+            mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
+            mma_ts_f8(tO, tP + 16 + kk * 8, bd, Cfg::kIdescPV, 1u);
+          } else {
+            mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
+          }
+        }
+        tc_commit(pv_bar);
+      }
+    };
+    // Q K^T over a whole K tile (half < 0) or 64 of its rows.
+    auto scores = [&](uint32_t klo, int half) {
+      const uint32_t kh = klo + (half > 0 ? (64 * 128) >> 4 : 0), tD = tS + (half > 0 ? 64u : 0u);
+      const uint32_t idesc = half < 0 ? Cfg::kIdescQK : Cfg::kIdescQKHalf;
 #pragma unroll
       for (int kk = 0; kk < Cfg::kSteps; ++kk) {
-        const uint64_t bd = sdesc_join(vlo + ((kk * Cfg::kRowsPerStep * 128) >> 4));
-        const uint32_t acc = (p_acc[t] || kk > 0) ? 1u : 0u;
+        const uint32_t step = ((kk * 32 / 128) * kAtom + (kk * 32) % 128) >> 4;
         if constexpr (kFp8) {
-          mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, acc);
-          mma_ts_f8(tO, tP + 32 + kk * 8, bd, Cfg::kIdescPV, 1u);
+          mma_ss_f8(tD, sdesc_join(qlo + step), sdesc_join(kh + step), idesc, kk > 0 ? 1u : 0u);
+          mma_ss_f8(tD, sdesc_join(qlo + (kAtom >> 4) + step), sdesc_join(kh + step), idesc, 1u);
         } else {
-          mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, acc);
+          mma_ss(tD, sdesc_join(qlo + step), sdesc_join(kh + step), idesc, kk > 0 ? 1u : 0u);
         }
       }
-      if (p_free[t]) tc_commit(smem_u32(&sm.empty[p_slot[t]]));
-      if (p_last[t]) tc_commit(smem_u32(&sm.o_full[t]));
-      pend[t] = false;
+      tc_commit(s_bar + (half > 0 ? 8u : 0u));
+    };
+    // A slot is free after two arrivals: one per tile of a shared block, both from an only user.
+    auto free_slot = [&](int slot, bool shared) {
+      tc_commit(smem_u32(&sm.empty[slot]));
+      if (!shared) tc_commit(smem_u32(&sm.empty[slot]));
+    };
+    auto wait_v = [&]() { ok = __all_sync(0xffffffffu, mbar_wait(pend_bar, pend_ph, abort_flag, p.err)); };
+    auto finish_item = [&]() {  // the last P V of an item
+      pend = false;
+      wait_v();
+      if (ok) finish(pend_halves ? 0 : -1);
+      if (ok && pend_halves) finish(1);
+      if (!ok) return;
+      tc_commit(o_bar);
+      free_slot(pend_slot, pend_pair);
     };
     Segment g;
     while (ok && next_segment(g)) {
       const bool pair = g.n_rows > kBlk;
-      bool first[2] = {true, true};
+      if (pair && was_solo) {
+        // From here this warp also waits on tile 0's barriers: both warps first see all blocks
+        // they loaded alone.
+        if (pend) finish_item();
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(smem_u32(&sm.m_sync));
+        bool w = mbar_wait(smem_u32(&sm.m_sync), m_ph, abort_flag, p.err);
+        m_ph ^= 1u;
+        if (!(ok = __all_sync(0xffffffffu, w))) break;
+      }
+      was_solo = !pair;
+      const bool halves = g.n_rows > 64;
+      bool first = true;
       for (int j = 0; ok && j < g.blocks; ++j) {
-        const int lo = pair ? 0 : (last_tile ^ 1);
-        const int hi = pair ? 1 : lo;
-        for (int t = lo; ok && t <= hi; ++t) {
-          if (pend[t]) finish(t);
+        const int owner = pair ? mt : last_tile ^ 1;
+        const int vs = ring + 1 == kS ? 0 : ring + 1;
+        const bool second = !pair && owner == 1;
+        if (owner == mt) {
+          const uint32_t phases = second ? phase1 : phase0;
+          if (first) {
+            if (pend) finish_item();
+            if (!ok) break;
+            ok = __all_sync(0xffffffffu, mbar_wait(q_bar, q_ph, abort_flag, p.err));
+            q_ph ^= 1u;
+          } else {
+            wait_v();
+          }
           if (!ok) break;
-          bool w = true;
-          if (first[t]) {
-            w = mbar_wait(smem_u32(&sm.q_full[t]), q_ph[t], abort_flag, p.err);
-            q_ph[t] ^= 1u;
-          }
-          if (w) w = mbar_wait(smem_u32(&sm.full[ring]), ring_phase, abort_flag, p.err);
+          const bool w = mbar_wait(smem_u32(&sm.full[second][ring]), (phases >> ring) & 1u, abort_flag, p.err);
           if (!(ok = __all_sync(0xffffffffu, w))) break;
-          tc_fence_after();
           const uint32_t klo = klo0 + static_cast<uint32_t>(ring) * kTileDesc;
-          const uint32_t qlo = sdesc_lo(smem_u32(sm.q[t]), 16);
-          const uint32_t tS = tbase + static_cast<uint32_t>(t) * 128u;
+          if (!halves) {
+            if (!first) finish(-1);
+            if (!ok) break;
+            tc_fence_after();
+            scores(klo, -1);
+          } else {
 #pragma unroll
-          for (int kk = 0; kk < Cfg::kSteps; ++kk) {
-            const uint32_t step = ((kk * 32 / 128) * kAtom + (kk * 32) % 128) >> 4;
-            if constexpr (kFp8) {
-              mma_ss_f8(tS, sdesc_join(qlo + step), sdesc_join(klo + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
-              mma_ss_f8(tS, sdesc_join(qlo + (kAtom >> 4) + step), sdesc_join(klo + step), Cfg::kIdescQK, 1u);
-            } else {
-              mma_ss(tS, sdesc_join(qlo + step), sdesc_join(klo + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
+            for (int half = 0; half < 2; ++half) {
+              if (!first) finish(half);
+              if (!ok) break;
+              tc_fence_after();
+              scores(klo, half);
             }
+            if (!ok) break;
           }
-          tc_commit(smem_u32(&sm.s_full[t]));
-          if (t == hi) tc_commit(smem_u32(&sm.empty[ring]));
-          const int vs = ring + 1 == kS ? 0 : ring + 1;
-          pend[t] = true;
-          p_acc[t] = !first[t];
-          p_last[t] = j >= g.blocks - (pair ? 1 : 2);
-          p_free[t] = t == hi;
-          p_slot[t] = vs;
-          p_slot_ph[t] = vs == 0 ? ring_phase ^ 1 : ring_phase;
-          p_bad[t] = g.kv_end - (g.block0 + j) * kBlk;
-          first[t] = false;
-          last_tile = t;
+          if (!first) free_slot(pend_slot, pair);
+          free_slot(ring, pair);
+          pend = true;
+          pend_acc = !first;
+          pend_pair = pair;
+          pend_halves = halves;
+          pend_slot = vs;
+          pend_bar = smem_u32(&sm.full[second][vs]);
+          pend_ph = (phases >> vs) & 1u;
+          pend_rows = g.kv_end - (g.block0 + j) * kBlk;
+          first = false;
         }
-        ring += 2;
-        if (ring >= kS) {
-          ring -= kS;
-          ring_phase ^= 1;
-        }
+        const uint32_t bits = (1u << ring) | (1u << vs);
+        if (second) phase1 ^= bits;
+        else phase0 ^= bits;
+        last_tile = pair ? 1 : owner;
+        ring = vs + 1 == kS ? 0 : vs + 1;
       }
     }
-    // what is still pending, oldest first
-    if (ok && pend[last_tile ^ 1]) finish(last_tile ^ 1);
-    if (ok && pend[last_tile]) finish(last_tile);
+    if (ok && pend) finish_item();
     // leave no tensor-core work in flight past the teardown
     tc_commit(smem_u32(&sm.drain));
     const unsigned long long t0 = global_ns();
@@ -753,7 +884,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t tS = tbase + static_cast<uint32_t>(t) * 128u + lane_off;
     const uint32_t tO = tbase + 256u + static_cast<uint32_t>(t) * 128u + lane_off;
-    uint32_t s_ph = 0u, o_ph = 0u, wg_ph = 0u;
+    uint32_t s_ph = 0u, o_ph = 0u, wg_ph = 0u, pv_ph = 0u;
     int last_tile = 1;
     bool ok = true;
     // all 128 threads of the tile meet (bounded, so a broken pipeline cannot hang it)
@@ -774,7 +905,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       last_tile = pair ? 1 : (last_tile ^ (g.blocks & 1));
       const int r0 = pair ? t * kBlk : 0;
       const int n_rows = min(kBlk, g.n_rows - r0);  // rows of this tile
-      const int span = n_rows <= 32 ? 32 : n_rows <= 64 ? 64 : 128;
+      const bool halves = g.n_rows > 64;  // blocks of whole tiles are taken in two halves
+      const int span = halves ? 128 : n_rows <= 32 ? 32 : 64;
       const int my = lr & (span - 1);  // this thread's row of the tile
       const int copy = lr / span;      // and which copy of it
       const bool live = my < n_rows;
@@ -793,20 +925,30 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
       const int col0 = copy * span;
-      for (int j = 0; j < mine; ++j) {
+      for (int j = 0; ok && j < mine; ++j) {
         const int left = limit - (g.block0 + begin + j * step) * kBlk;
-        ok = mbar_wait(smem_u32(&sm.s_full[t]), s_ph, abort_flag, p.err);
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
-        s_ph ^= 1u;
-        tc_fence_after();
-        if (warp_live) {
-          if (span == 128) softmax_block<kFp8, 4>(tS, tO, 0, left, sl2, j == 0, m, l);
-          else if (span == 64) softmax_block<kFp8, 2>(tS, tO, col0, left, sl2, j == 0, m, l);
-          else softmax_block<kFp8, 1>(tS, tO, col0, left, sl2, j == 0, m, l);
+        const int n_steps = halves ? 2 : 1;
+#pragma unroll 1
+        for (int h = 0; h < n_steps; ++h) {
+          ok = mbar_wait(smem_u32(&sm.s_full[t][h]), (s_ph >> h) & 1u, abort_flag, p.err);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          s_ph ^= 1u << h;
+          tc_fence_after();
+          const bool first = j == 0 && h == 0;
+          // whole blocks: the scores' barrier also covers the previous P V
+          const auto pv_done = [&]() {
+            if (halves && !first) ok = mbar_wait(smem_u32(&sm.pv_done[t]), pv_ph ^ 1u, abort_flag, p.err);
+          };
+          if (!warp_live) pv_done();
+          else if (halves) softmax_block<kFp8, 64, true>(tS, tO, 64 * h, left, sl2, first, m, l, pv_done);
+          else if (span == 64) softmax_block<kFp8, 64, false>(tS, tO, col0, left, sl2, first, m, l, pv_done);
+          else softmax_block<kFp8, 32, false>(tS, tO, col0, left, sl2, first, m, l, pv_done);
+          if (halves) pv_ph ^= 1u;
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm.p_full[t][h]));
         }
-        tc_fence_before();
-        mbar_arrive(smem_u32(&sm.p_full[t]));
       }
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       ok = mbar_wait(smem_u32(&sm.o_full[t]), o_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
