@@ -87,6 +87,7 @@ struct BranchParams {
   long long own_row0;          // first workspace row of the own items' slots
   float* part_o;               // [workspace rows, 128]
   float2* part_ml;             // [workspace rows]: (maximum, sum)
+  int* plan;                   // the schedule, for the merge: [3 + batch]
   int ctas;
   int* err;
 };
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
   const int lane = threadIdx.x & 31;
   volatile int* abort_flag = &sm.abort_flag;
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < kS; ++s) {
       mbar_init(smem_u32(&sm.full[0][s]), 1);
@@ -1017,7 +1019,31 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       tc_fence_before();
     }
   } else {
+    // ================================================================ warp 3 of the first CTA
+    // writes the schedule down for the merge: the units of a shared item, of a head and of a CTA,
+    // and the own units in front of each sequence
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
+    if (blockIdx.x == 0) {
+      const Plan pl = make_plan(p, lane);
+      if (lane == 0) {
+        p.plan[0] = pl.shared_units;
+        p.plan[1] = pl.head_units;
+        p.plan[2] = pl.cut;
+      }
+      int before = 0;
+      for (int b0 = 0; b0 < p.batch; b0 += 32) {
+        const int b = b0 + lane;
+        const int n = b < p.batch ? own_units_all(p, seq_length(p, b)) : 0;
+        int cum = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const int v = __shfl_up_sync(0xffffffffu, cum, d);
+          if (lane >= d) cum += v;
+        }
+        if (b < p.batch) p.plan[3 + b] = before + cum - n;
+        before += __shfl_sync(0xffffffffu, cum, 31);
+      }
+    }
   }
 
   tc_fence_before();
@@ -1029,74 +1055,181 @@ __global__ void __launch_bounds__(kBrThreads, 1)
 }
 
 // Joins the pieces of every row that more than one segment (or tile) contributed to, in the order
-// of the units, and writes rows that see nothing: one warp per row and query head.
-template <bool kFp8>
-__global__ void __launch_bounds__(256) branch_merge_kernel(const BranchParams p) {
-  const int lane = threadIdx.x & 31;
-  const long long id = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (id >= static_cast<long long>(p.batch) * p.rows * p.heads) return;
-  const int hq = static_cast<int>(id % p.heads);
-  const int bi = static_cast<int>(id / p.heads);
-  const int b = bi / p.rows, i = bi - b * p.rows;
-  const int head = hq / p.group, g = hq - head * p.group;
-  const Plan pl = make_plan(p, lane);
-  int before = 0;  // units of the sequences in front of b
-  for (int k = lane; k < b; k += 32) before += own_units_all(p, seq_length(p, k));
-  before = __reduce_add_sync(0xffffffffu, before);
-  const int len = seq_length(p, b);
-  const int own_row = i * p.group + g;           // row within the sequence's items
-  const int t_own = own_row / kSpan;
-  for (int t = 0; t < t_own; ++t) before += own_units(p, len, t);
-  const int row = b * p.rows * p.group + own_row;  // row of the stacked items
-  const int t_sh = row / kSpan;
+// of the units, and writes rows that see nothing. A warp takes a row (kTeam warps share one in long
+// shared items) and reads kBatch pieces at a time, maximum, sum and O alike before it needs any of
+// them: what bounds this kernel is the latency of reads from L2, and reading O only after the
+// weights had been found took 21 us instead of 6 for 480 rows of 38 pieces. In the joint form few
+// pieces make a row and a warp takes kRows rows at once instead.
+constexpr int kMergeWarps = 4;
+constexpr int kJointWarpRows = 4;  // joint form: rows of a warp
 
-  float m = -INFINITY, sum = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  bool done = false;
-  auto pieces = [&](int u0, int units, int n_rows, int r, long long item, long long row0, int slot_rows) {
-    if (units == 0) return;
-    const int c_lo = u0 / pl.cut, c_hi = (u0 + units - 1) / pl.cut;
-    const bool pair = n_rows > kBlk;
-    if (pl.shared_units == 0 && c_lo == c_hi && (pair || units == 1)) {
-      done = true;  // written by the segment itself
-      return;
+struct Pieces {  // of one row in one item: workspace rows first + c * stride_c + k * stride_k
+  int n, per;    // all pieces; pieces a CTA (1 or 2)
+  long long first;
+  int stride_c, stride_k;
+};
+__device__ __forceinline__ Pieces pieces_of(int cut, int u0, int units, int n_rows, int r, long long item,
+                                            long long row0, int slot_rows) {
+  if (units == 0) return Pieces{0, 1, 0, 0, 0};
+  Pieces q;
+  const int c_lo = u0 / cut;
+  const bool pair = n_rows > kBlk;
+  q.per = pair ? 1 : 2;
+  q.n = ((u0 + units - 1) / cut - c_lo + 1) * q.per;
+  q.stride_c = 2 * slot_rows;
+  q.stride_k = slot_rows;
+  q.first = row0 + ((item + c_lo) * 2 + (pair ? r / kBlk : 0)) * slot_rows + (pair ? r % kBlk : r);
+  return q;
+}
+__device__ __forceinline__ long long piece_row(const Pieces& q, int j) {
+  const int c = q.per == 1 ? j : j >> 1, k = q.per == 1 ? 0 : j & 1;
+  return q.first + static_cast<long long>(c) * q.stride_c + k * q.stride_k;
+}
+
+template <bool kFp8, bool kJoint, int kTeam>
+__global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const BranchParams p) {
+  constexpr int kTeams = kMergeWarps / kTeam;
+  constexpr int kRows = kJoint ? kJointWarpRows : 1;
+  constexpr int kBatch = kJoint ? 2 : 8;
+  __shared__ float4 sums[kTeam > 1 ? kMergeWarps : 1][32];
+  __shared__ float2 tops[kTeam > 1 ? kMergeWarps : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int team = warp / kTeam, part = warp % kTeam;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int shared_units = kJoint ? 0 : __ldcg(p.plan), head_units = __ldcg(p.plan + 1), cut = __ldcg(p.plan + 2);
+  const int own_all = p.rows * p.group;
+  // split form: stacked rows of all branches, one a team, head by head; joint form: kRows rows of
+  // an item a warp
+  int head, b, t, r;
+  if (!kJoint) {
+    const int stacked = p.batch * own_all;
+    const long long id = static_cast<long long>(blockIdx.x) * kTeams + team;
+    if (id >= static_cast<long long>(stacked) * p.kv_heads) return;  // a whole block if kTeam > 1
+    head = static_cast<int>(id / stacked);
+    const int row = static_cast<int>(id - static_cast<long long>(head) * stacked);
+    b = row / own_all;
+    r = row - b * own_all;
+    t = r / kSpan;
+  } else {
+    constexpr int kGroups = kSpan / (kRows * kMergeWarps);
+    const int item = blockIdx.x / kGroups;
+    t = item % p.own_tiles;
+    b = item / p.own_tiles % p.batch;
+    head = item / p.own_tiles / p.batch;
+    r = t * kSpan + (static_cast<int>(blockIdx.x % kGroups) * kMergeWarps + warp) * kRows;
+    if (r >= min(own_all, (t + 1) * kSpan)) return;
+  }
+  const int len = seq_length(p, b);
+  int u0 = head * head_units + p.shared_tiles * shared_units + __ldcg(p.plan + 3 + b);
+  for (int k = 0; k < t; ++k) u0 += own_units(p, len, k);
+  const int units = own_units(p, len, t);
+  const int n_rows = min(kSpan, own_all - t * kSpan);
+  if (shared_units == 0 && units > 0 && u0 / cut == (u0 + units - 1) / cut && (n_rows > kBlk || units == 1))
+    return;  // written by the segment itself
+  Pieces sh[kRows], own[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    // rows past the item read its last row again and write nothing
+    const int rk = min(r + k, t * kSpan + n_rows - 1);
+    const int row = b * own_all + rk, t_sh = row / kSpan;
+    sh[k] = pieces_of(cut, head * head_units + t_sh * shared_units, shared_units,
+                      min(kSpan, p.batch * own_all - t_sh * kSpan), row % kSpan,
+                      head * p.shared_tiles + t_sh, 0, p.shared_slot_rows);
+    own[k] = pieces_of(cut, u0, units, n_rows, rk - t * kSpan,
+                       (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t, p.own_row0,
+                       p.own_slot_rows);
+  }
+  const int n = sh[0].n + own[0].n;  // the rows of a warp are rows of one item
+  float m[kRows], sum[kRows];
+  float4 acc[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    m[k] = -INFINITY;
+    sum[k] = 0.f;
+    acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i0 = part * kBatch; i0 < n; i0 += kTeam * kBatch) {
+    float2 ml[kRows][kBatch];
+    float4 v[kRows][kBatch];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = min(i0 + j, n - 1);
+        const long long at = i < sh[k].n ? piece_row(sh[k], i) : piece_row(own[k], i - sh[k].n);
+        ml[k][j] = __ldcg(p.part_ml + at);
+        v[k][j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * kD) + lane);
+      }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (i0 + j >= n) ml[k][j] = make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[k][j].x);
+      }
+      // a sum of 0: the piece saw nothing and its O was not written. Sums that are NaN stay so.
+      const float keep = sum[k] != 0.f ? fast_exp2(m[k] - top) : 0.f;
+      sum[k] = sum[k] != 0.f ? sum[k] * keep : 0.f;
+      acc[k] = make_float4(acc[k].x * keep, acc[k].y * keep, acc[k].z * keep, acc[k].w * keep);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        if (ml[k][j].y != 0.f) {
+          const float w = fast_exp2(ml[k][j].x - top);
+          sum[k] += w * ml[k][j].y;
+          acc[k].x += v[k][j].x * w;
+          acc[k].y += v[k][j].y * w;
+          acc[k].z += v[k][j].z * w;
+          acc[k].w += v[k][j].w * w;
+        }
+      }
+      m[k] = top;
     }
-    for (int c = c_lo; c <= c_hi; ++c) {
-      for (int k = pair ? r / kBlk : 0; k <= (pair ? r / kBlk : 1); ++k) {
-        const long long at = row0 + ((item + c) * 2 + k) * slot_rows + (pair ? r % kBlk : r);
-        const float2 ml = __ldcg(p.part_ml + at);
-        if (ml.y == 0.f) continue;  // saw nothing
-        const float top = fmaxf(m, ml.x);
-        const float keep = m > -INFINITY ? fast_exp2(m - top) : (sum != sum ? sum : 0.f);
-        const float w = fast_exp2(ml.x - top);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * kD) + lane);
-        acc = make_float4(acc.x * keep + v.x * w, acc.y * keep + v.y * w, acc.z * keep + v.z * w,
-                          acc.w * keep + v.w * w);
-        sum = sum * keep + ml.y * w;
-        m = top;
+  }
+  if constexpr (kTeam > 1) {  // one row a team, and the teams of a block all get here
+    sums[warp][lane] = acc[0];
+    if (lane == 0) tops[warp] = make_float2(m[0], sum[0]);
+    __syncthreads();
+    if (part != 0) return;
+    float top = m[0];
+#pragma unroll
+    for (int k = 1; k < kTeam; ++k) top = fmaxf(top, tops[warp + k].x);
+    float total = 0.f;
+    float4 all = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kTeam; ++k) {
+      const float2 q = tops[warp + k];
+      if (q.y != 0.f) {
+        const float4 x = sums[warp + k][lane];
+        const float w = fast_exp2(q.x - top);
+        total += q.y * w;
+        all.x += x.x * w;
+        all.y += x.y * w;
+        all.z += x.z * w;
+        all.w += x.w * w;
       }
     }
-  };
-  if (pl.shared_units > 0)
-    pieces(head * pl.head_units + t_sh * pl.shared_units, pl.shared_units,
-           min(kSpan, p.batch * p.rows * p.group - t_sh * kSpan), row - t_sh * kSpan,
-           head * p.shared_tiles + t_sh, 0, p.shared_slot_rows);
-  pieces(head * pl.head_units + p.shared_tiles * pl.shared_units + before, own_units(p, len, t_own),
-         min(kSpan, p.rows * p.group - t_own * kSpan), own_row - t_own * kSpan,
-         (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t_own, p.own_row0, p.own_slot_rows);
-  if (done) return;
-  float scale = sum == 0.f ? 0.f : 1.0f / sum;
-  if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
-  if (sum == 0.f) acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  reinterpret_cast<uint2*>(p.out + id * kD)[lane] =
-      make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
-  if (p.lse && lane == 0)
-    p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+    m[0] = top;
+    sum[0] = total;
+    acc[0] = all;
+  }
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    if (r + k >= t * kSpan + n_rows) break;
+    float scale = sum[k] == 0.f ? 0.f : 1.0f / sum[k];
+    if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
+    const int i = (r + k) / p.group;
+    const long long id = (static_cast<long long>(b) * p.rows + i) * p.heads + head * p.group + r + k - i * p.group;
+    reinterpret_cast<uint2*>(p.out + id * kD)[lane] = make_uint2(
+        pack_bf16x2(acc[k].x * scale, acc[k].y * scale), pack_bf16x2(acc[k].z * scale, acc[k].w * scale));
+    if (p.lse && lane == 0) p.lse[id] = sum[k] == 0.f ? -INFINITY : (m[k] + log2f(sum[k])) * 0.6931471805599453f;
+  }
 }
 
 struct Shape {
   int shared_tiles, own_tiles, shared_slot_rows, own_slot_rows, joint, ctas;
   long long own_row0, rows;  // workspace rows
+  long long bytes;
 };
 
 int sm_count() {
@@ -1131,6 +1264,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
                    : (static_cast<long long>(kv_heads) * s.shared_tiles + s.ctas) * 2 * s.shared_slot_rows;
   s.rows = s.own_row0 +
            (static_cast<long long>(kv_heads) * batch * s.own_tiles + s.ctas) * 2 * s.own_slot_rows;
+  s.bytes = s.rows * (kD * 4 + 8) + (3ll + batch) * 4;
   return s;
 }
 
@@ -1175,9 +1309,28 @@ int launch(const BranchParams& p, const void* key_pool, const void* value_pool, 
   branch_attn_kernel<kFp8><<<p.ctas, kBrThreads, br_smem_bytes<kFp8>(), stream>>>(tmK, tmV, p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error("branch_attn_kernel launch", e);
-  const long long rows = static_cast<long long>(p.batch) * p.rows * p.heads;
-  branch_merge_kernel<kFp8><<<static_cast<unsigned>((rows + 7) / 8), 256, 0, stream>>>(p);
-  e = cudaGetLastError();
+  // The merge is launched along with it and waits on the device for its end.
+  // A row of the split form has about two pieces for each CTA of its shared item: beyond 64 of
+  // them four warps share it.
+  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
+  const bool team = !p.joint && p.shared_tiles > 0 && p.ctas > 32 * p.kv_heads * p.shared_tiles;
+  const long long blocks =
+      p.joint ? static_cast<long long>(p.kv_heads) * p.batch * p.own_tiles * (kSpan / (kJointWarpRows * kMergeWarps))
+      : team  ? stacked
+              : (stacked + kMergeWarps - 1) / kMergeWarps;
+  cudaLaunchConfig_t cfg;
+  memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  e = p.joint ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, true, 1>, p)
+      : team  ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, kMergeWarps>, p)
+              : cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, 1>, p);
   if (e != cudaSuccess) return set_cuda_error("branch_merge_kernel launch", e);
   return H3SA_OK;
 }
@@ -1196,7 +1349,7 @@ int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
   if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
     return 0;
   const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
-  return s.rows * (kD * 4 + 8);
+  return s.bytes;
 }
 
 int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides, void* out, float* lse,
@@ -1235,9 +1388,9 @@ int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d over %d "
                      "pages exceeds the work index", batch, rows, heads, width);
   const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
-  if (workspace_bytes < s.rows * (kD * 4 + 8))
+  if (workspace_bytes < s.bytes)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: workspace of %lld bytes, %lld needed",
-                     static_cast<long long>(workspace_bytes), s.rows * (kD * 4 + 8));
+                     static_cast<long long>(workspace_bytes), s.bytes);
   BranchParams p;
   memset(&p, 0, sizeof(p));
   p.q = static_cast<const __nv_bfloat16*>(query);
@@ -1268,6 +1421,7 @@ int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides
   p.own_row0 = s.own_row0;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + s.rows * kD);
+  p.plan = reinterpret_cast<int*>(p.part_ml + s.rows);
   p.ctas = s.ctas;
   p.err = device_error;
   return e4m3 ? launch<true>(p, key_pool, value_pool, static_cast<cudaStream_t>(stream))
