@@ -1056,41 +1056,83 @@ __global__ void __launch_bounds__(kBrThreads, 1)
 
 // Joins the pieces of every row that more than one segment (or tile) contributed to, in the order
 // of the units, and writes rows that see nothing. A warp takes a row (kTeam warps share one in long
-// shared items) and reads kBatch pieces at a time, maximum, sum and O alike before it needs any of
+// shared items) and reads several pieces at a time, maximum, sum and O alike before it needs any of
 // them: what bounds this kernel is the latency of reads from L2, and reading O only after the
 // weights had been found took 21 us instead of 6 for 480 rows of 38 pieces. In the joint form few
 // pieces make a row and a warp takes kRows rows at once instead.
 constexpr int kMergeWarps = 4;
 constexpr int kJointWarpRows = 4;  // joint form: rows of a warp
 
-struct Pieces {  // of one row in one item: workspace rows first + c * stride_c + k * stride_k
-  int n, per;    // all pieces; pieces a CTA (1 or 2)
+struct Pieces {  // of one row in one item: workspace rows first + j * stride, j < n
+  int n, stride;
   long long first;
-  int stride_c, stride_k;
 };
 __device__ __forceinline__ Pieces pieces_of(int cut, int u0, int units, int n_rows, int r, long long item,
                                             long long row0, int slot_rows) {
-  if (units == 0) return Pieces{0, 1, 0, 0, 0};
-  Pieces q;
-  const int c_lo = u0 / cut;
-  const bool pair = n_rows > kBlk;
-  q.per = pair ? 1 : 2;
-  q.n = ((u0 + units - 1) / cut - c_lo + 1) * q.per;
-  q.stride_c = 2 * slot_rows;
-  q.stride_k = slot_rows;
-  q.first = row0 + ((item + c_lo) * 2 + (pair ? r / kBlk : 0)) * slot_rows + (pair ? r % kBlk : r);
-  return q;
+  if (units == 0) return Pieces{0, 0, 0};
+  const int c_lo = u0 / cut, n_cta = (u0 + units - 1) / cut - c_lo + 1;
+  const long long first = row0 + (item + c_lo) * 2 * slot_rows;
+  // items of both tiles: the slot of the row's tile in each CTA; else the slots of both
+  if (n_rows > kBlk) return Pieces{n_cta, 2 * slot_rows, first + (r / kBlk) * slot_rows + r % kBlk};
+  return Pieces{2 * n_cta, slot_rows, first + r};
 }
-__device__ __forceinline__ long long piece_row(const Pieces& q, int j) {
-  const int c = q.per == 1 ? j : j >> 1, k = q.per == 1 ? 0 : j & 1;
-  return q.first + static_cast<long long>(c) * q.stride_c + k * q.stride_k;
+
+// Adds the pieces of kRows rows, kB at a time and every kTeam-th batch from the part-th on, to their
+// running maxima, sums and O.
+template <int kRows, int kB, int kTeam>
+__device__ __forceinline__ void add_pieces(const BranchParams& p, const Pieces (&q)[kRows], int part, int lane,
+                                         float (&m)[kRows], float (&sum)[kRows], float4 (&acc)[kRows]) {
+  const int n = q[0].n;  // the rows of a warp are rows of one item
+  const float2* ml_at[kRows];
+  const float4* o_at[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) {
+    ml_at[k] = p.part_ml + q[k].first;
+    o_at[k] = reinterpret_cast<const float4*>(p.part_o) + q[k].first * (kD / 4) + lane;
+  }
+  for (int i0 = part * kB; i0 < n; i0 += kTeam * kB) {
+    float2 ml[kRows][kB];
+    float4 v[kRows][kB];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        const long long at = static_cast<long long>(min(i0 + j, n - 1)) * q[k].stride;
+        ml[k][j] = __ldcg(ml_at[k] + at);
+        v[k][j] = __ldcg(o_at[k] + at * (kD / 4));
+      }
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      float top = m[k];
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        if (i0 + j >= n) ml[k][j] = make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[k][j].x);
+      }
+      // a sum of 0: the piece saw nothing and its O was not written. Sums that are NaN stay so.
+      const float keep = sum[k] != 0.f ? fast_exp2(m[k] - top) : 0.f;
+      sum[k] = sum[k] != 0.f ? sum[k] * keep : 0.f;
+      acc[k] = make_float4(acc[k].x * keep, acc[k].y * keep, acc[k].z * keep, acc[k].w * keep);
+#pragma unroll
+      for (int j = 0; j < kB; ++j) {
+        if (ml[k][j].y != 0.f) {
+          const float w = fast_exp2(ml[k][j].x - top);
+          sum[k] += w * ml[k][j].y;
+          acc[k].x += v[k][j].x * w;
+          acc[k].y += v[k][j].y * w;
+          acc[k].z += v[k][j].z * w;
+          acc[k].w += v[k][j].w * w;
+        }
+      }
+      m[k] = top;
+    }
+  }
 }
 
 template <bool kFp8, bool kJoint, int kTeam>
 __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const BranchParams p) {
   constexpr int kTeams = kMergeWarps / kTeam;
   constexpr int kRows = kJoint ? kJointWarpRows : 1;
-  constexpr int kBatch = kJoint ? 2 : 8;
   __shared__ float4 sums[kTeam > 1 ? kMergeWarps : 1][32];
   __shared__ float2 tops[kTeam > 1 ? kMergeWarps : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1139,7 +1181,6 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
                        (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t, p.own_row0,
                        p.own_slot_rows);
   }
-  const int n = sh[0].n + own[0].n;  // the rows of a warp are rows of one item
   float m[kRows], sum[kRows];
   float4 acc[kRows];
 #pragma unroll
@@ -1148,44 +1189,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
     sum[k] = 0.f;
     acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  for (int i0 = part * kBatch; i0 < n; i0 += kTeam * kBatch) {
-    float2 ml[kRows][kBatch];
-    float4 v[kRows][kBatch];
-#pragma unroll
-    for (int k = 0; k < kRows; ++k)
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = min(i0 + j, n - 1);
-        const long long at = i < sh[k].n ? piece_row(sh[k], i) : piece_row(own[k], i - sh[k].n);
-        ml[k][j] = __ldcg(p.part_ml + at);
-        v[k][j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * kD) + lane);
-      }
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      float top = m[k];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (i0 + j >= n) ml[k][j] = make_float2(-INFINITY, 0.f);
-        top = fmaxf(top, ml[k][j].x);
-      }
-      // a sum of 0: the piece saw nothing and its O was not written. Sums that are NaN stay so.
-      const float keep = sum[k] != 0.f ? fast_exp2(m[k] - top) : 0.f;
-      sum[k] = sum[k] != 0.f ? sum[k] * keep : 0.f;
-      acc[k] = make_float4(acc[k].x * keep, acc[k].y * keep, acc[k].z * keep, acc[k].w * keep);
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        if (ml[k][j].y != 0.f) {
-          const float w = fast_exp2(ml[k][j].x - top);
-          sum[k] += w * ml[k][j].y;
-          acc[k].x += v[k][j].x * w;
-          acc[k].y += v[k][j].y * w;
-          acc[k].z += v[k][j].z * w;
-          acc[k].w += v[k][j].w * w;
-        }
-      }
-      m[k] = top;
-    }
-  }
+  if constexpr (!kJoint) add_pieces<kRows, kTeam == 1 ? 8 : 4, kTeam>(p, sh, part, lane, m, sum, acc);
+  add_pieces<kRows, kJoint ? 2 : kTeam == 1 ? 4 : 1, kTeam>(p, own, part, lane, m, sum, acc);
   if constexpr (kTeam > 1) {  // one row a team, and the teams of a block all get here
     sums[warp][lane] = acc[0];
     if (lane == 0) tops[warp] = make_float2(m[0], sum[0]);
@@ -1310,10 +1315,9 @@ int launch(const BranchParams& p, const void* key_pool, const void* value_pool, 
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error("branch_attn_kernel launch", e);
   // The merge is launched along with it and waits on the device for its end.
-  // A row of the split form has about two pieces for each CTA of its shared item: beyond 64 of
-  // them four warps share it.
+  // Four warps share a row where rows are few: its pieces are read one latency after another.
   const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
-  const bool team = !p.joint && p.shared_tiles > 0 && p.ctas > 32 * p.kv_heads * p.shared_tiles;
+  const bool team = !p.joint && p.shared_tiles > 0 && stacked <= 16ll * p.ctas;
   const long long blocks =
       p.joint ? static_cast<long long>(p.kv_heads) * p.batch * p.own_tiles * (kSpan / (kJointWarpRows * kMergeWarps))
       : team  ? stacked
