@@ -19,34 +19,52 @@ stream and has no counterpart.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import Sequence, Union
 
 import torch
 
-from ._lib import LIB, Pools, call, ptr, stream_handle
+from ._lib import LIB, Pools, check
 from .kernels import HEAD_DIM, PAGE_ROWS
 
 PoolTensors = Union[torch.Tensor, Sequence[torch.Tensor]]
 
-
-def _on(stream: torch.cuda.Stream | None):
-    """Results and workspaces are allocated on the stream that uses them."""
-
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
-
-
-def _check(what: str, device: torch.device, dtype: torch.dtype,
-           tensors: Sequence[tuple[str, torch.Tensor, tuple[int, ...]]]) -> None:
-    for name, t, shape in tensors:
-        if t.device != device or t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-            raise RuntimeError(f"{what}: {name} must be contiguous {dtype} {list(shape)} on {device}")
+# A call of a few rows takes the device about ten microseconds, so the host side counts: entry
+# points are bound once, conditions are tested inline and messages built only on failure.
+_FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_free_pages
+_ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
+_PAGES_WORK = LIB.h3sa_pages_workspace
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_Strides = ctypes.c_int64 * 3
 
 
-def _check_error_word(what: str, device: torch.device, word: torch.Tensor | None) -> None:
-    if word is not None and (word.device != device or word.dtype != torch.int32 or word.numel() < 1):
+def _bad(t: torch.Tensor, device: torch.device, dtype: torch.dtype, shape: tuple[int, ...]) -> bool:
+    return t.dtype is not dtype or t.shape != shape or t.device != device or not t.is_contiguous()
+
+
+def _refuse(what: str, name: str, device: torch.device, dtype: torch.dtype, shape: tuple[int, ...]) -> None:
+    raise RuntimeError(f"{what}: {name} must be contiguous {dtype} {list(shape)} on {device}")
+
+
+def _error_word(what: str, device: torch.device, word: torch.Tensor | None) -> int | None:
+    if word is None:
+        return None
+    if word.device != device or word.dtype is not torch.int32 or word.numel() < 1:
         raise RuntimeError(f"{what}: device_error must be an int32 tensor on {device}")
+    return word.data_ptr()
+
+
+def _alloc(stream: torch.cuda.Stream | None, *wanted: tuple[torch.Tensor, tuple[int, ...], torch.dtype]):
+    """Results and workspaces, allocated on the stream that uses them."""
+
+    if stream is None:
+        return [t.new_empty(shape, dtype=dtype) for t, shape, dtype in wanted]
+    with torch.cuda.stream(stream):
+        return [t.new_empty(shape, dtype=dtype) for t, shape, dtype in wanted]
+
+
+def _handle(stream: torch.cuda.Stream | None, device: torch.device) -> int:
+    return _raw_stream(device.index) if stream is None else stream.cuda_stream
 
 
 def _pools(what: str, pools: PoolTensors, pages: int, device: torch.device) -> Pools:
@@ -58,30 +76,30 @@ def _pools(what: str, pools: PoolTensors, pages: int, device: torch.device) -> P
     if isinstance(pools, torch.Tensor):
         if pools.ndim != 4:
             raise RuntimeError(f"{what}: stacked pools must be [count, heads, pages*128, d]")
-        first = pools
-        shape = tuple(pools.shape[1:])
-        p.base, p.count = pools.data_ptr(), pools.shape[0]
-        p.stride = pools.stride(0) * pools.element_size()
-        if pools.device != device or not (pools.is_contiguous() or pools[0].is_contiguous()):
+        p.count, heads, rows, d = pools.shape
+        size = pools.element_size()
+        p.base, p.stride = pools.data_ptr(), pools.stride(0) * size
+        if pools.device != device or not (pools.is_contiguous() or p.count == 0 or pools[0].is_contiguous()):
             raise RuntimeError(f"{what}: pool tensors must be contiguous on {device}")
     else:
         if len(pools) == 0:
             raise RuntimeError(f"{what}: no pool tensors")
         first = pools[0]
-        shape = tuple(first.shape)
-        dtype = first.dtype
+        shape, dtype, size = first.shape, first.dtype, first.element_size()
+        if len(shape) != 3:
+            raise RuntimeError(f"{what}: pool tensors must be [heads, pages*{PAGE_ROWS}, d]")
+        heads, rows, d = shape
         for t in pools:
-            if t.device != device or t.dtype != dtype or t.shape != first.shape or not t.is_contiguous():
+            if t.device != device or t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
                 raise RuntimeError(f"{what}: pool tensors must be contiguous on {device}, of one "
                                    "shape and dtype")
         address = (ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools])
         p.list, p.count = ctypes.addressof(address), len(pools)
         p._address = address
-    if len(shape) != 3 or shape[0] == 0 or shape[1] != pages * PAGE_ROWS:
+    if heads == 0 or rows != pages * PAGE_ROWS:
         raise RuntimeError(f"{what}: pool tensors must be [heads, {pages}*{PAGE_ROWS}, d] for {pages} "
                            "reference counts")
-    p.heads, p.pages = shape[0], pages
-    p.row_bytes = shape[2] * first.element_size()
+    p.heads, p.pages, p.row_bytes = heads, pages, d * size
     return p
 
 
@@ -90,10 +108,12 @@ def _ledger(what: str, table: torch.Tensor, refs: torch.Tensor) -> tuple[torch.d
         raise RuntimeError("h3sa kernels require CUDA tensors")
     if table.ndim != 2 or refs.ndim != 1:
         raise RuntimeError(f"{what}: table must be [sequences, width] and refs [pages]")
-    sequences, width = table.shape
-    _check(what, table.device, torch.int32, (("table", table, (sequences, width)),
-                                             ("refs", refs, (refs.shape[0],))))
-    return table.device, sequences, width, refs.shape[0]
+    device, (sequences, width), (pages,) = table.device, table.shape, refs.shape
+    if _bad(table, device, torch.int32, (sequences, width)):
+        _refuse(what, "table", device, torch.int32, (sequences, width))
+    if _bad(refs, device, torch.int32, (pages,)):
+        _refuse(what, "refs", device, torch.int32, (pages,))
+    return device, sequences, width, pages
 
 
 def fork_pages(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
@@ -111,24 +131,28 @@ def fork_pages(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, r
     fork all of them (``device_error``), every child comes out empty and ``refs`` unchanged.
     """
 
-    device, sequences, width, pages = _ledger("fork_pages", table, refs)
+    what = "fork_pages"
+    device, sequences, width, pages = _ledger(what, table, refs)
     if parents.ndim != 1:
-        raise RuntimeError("fork_pages: parents must be [children]")
+        raise RuntimeError(f"{what}: parents must be [children]")
     children = parents.shape[0]
-    _check("fork_pages", device, torch.int32, (("lengths", lengths, (sequences,)),
-                                               ("parents", parents, (children,))))
-    _check_error_word("fork_pages", device, device_error)
+    if _bad(lengths, device, torch.int32, (sequences,)):
+        _refuse(what, "lengths", device, torch.int32, (sequences,))
+    if _bad(parents, device, torch.int32, (children,)):
+        _refuse(what, "parents", device, torch.int32, (children,))
+    error = _error_word(what, device, device_error)
     if reserve_rows < 0:
-        raise ValueError("fork_pages: reserve_rows must not be negative")
-    p = _pools("fork_pages", pools, pages, device)
-    with _on(stream):
-        child_table = torch.empty((children, width), dtype=torch.int32, device=device)
-        child_lengths = torch.empty(children, dtype=torch.int32, device=device)
-        refs_out = torch.empty_like(refs)
-        work = torch.empty(LIB.h3sa_pages_workspace(pages, children), dtype=torch.uint8, device=device)
-    call("h3sa_fork_pages", p, ptr(table), sequences, width, ptr(lengths), ptr(refs), ptr(parents),
-         children, int(reserve_rows), 1 if private else 0, ptr(child_table), ptr(child_lengths),
-         ptr(refs_out), ptr(work), ptr(device_error), stream_handle(stream))
+        raise ValueError(f"{what}: reserve_rows must not be negative")
+    p = _pools(what, pools, pages, device)
+    child_table, child_lengths, refs_out, work = _alloc(
+        stream, (table, (children, width), torch.int32), (table, (children,), torch.int32),
+        (table, (pages,), torch.int32), (table, (_PAGES_WORK(pages, children),), torch.uint8))
+    code = _FORK(p, table.data_ptr(), sequences, width, lengths.data_ptr(), refs.data_ptr(),
+                 parents.data_ptr(), children, int(reserve_rows), 1 if private else 0,
+                 child_table.data_ptr(), child_lengths.data_ptr(), refs_out.data_ptr(),
+                 work.data_ptr(), error, _handle(stream, device))
+    if code:
+        check("h3sa_fork_pages", code)
     return child_table, child_lengths, refs_out
 
 
@@ -140,15 +164,18 @@ def compact_pages(pools: PoolTensors, table: torch.Tensor, refs: torch.Tensor, *
     i-th page in use at or past n. ``table`` must hold every reference that ``refs`` counts.
     Returns the renumbered ``(table, refs)`` and n as an int32 tensor ``[1]``."""
 
-    device, sequences, width, pages = _ledger("compact_pages", table, refs)
-    _check_error_word("compact_pages", device, device_error)
-    p = _pools("compact_pages", pools, pages, device)
-    with _on(stream):
-        table_out, refs_out = torch.empty_like(table), torch.empty_like(refs)
-        live = torch.empty(1, dtype=torch.int32, device=device)
-        work = torch.empty(LIB.h3sa_pages_workspace(pages, 0), dtype=torch.uint8, device=device)
-    call("h3sa_compact_pages", p, ptr(table), sequences, width, ptr(refs), ptr(table_out),
-         ptr(refs_out), ptr(live), ptr(work), ptr(device_error), stream_handle(stream))
+    what = "compact_pages"
+    device, sequences, width, pages = _ledger(what, table, refs)
+    error = _error_word(what, device, device_error)
+    p = _pools(what, pools, pages, device)
+    table_out, refs_out, live, work = _alloc(
+        stream, (table, (sequences, width), torch.int32), (table, (pages,), torch.int32),
+        (table, (1,), torch.int32), (table, (_PAGES_WORK(pages, 0),), torch.uint8))
+    code = _COMPACT(p, table.data_ptr(), sequences, width, refs.data_ptr(), table_out.data_ptr(),
+                    refs_out.data_ptr(), live.data_ptr(), work.data_ptr(), error,
+                    _handle(stream, device))
+    if code:
+        check("h3sa_compact_pages", code)
     return table_out, refs_out, live
 
 
@@ -159,16 +186,21 @@ def free_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
     """End the sequences with ``release[s]`` (bool ``[sequences]``): their pages lose one reference
     each, their table rows become -1 and their lengths 0. Returns ``(table, lengths, refs)``."""
 
-    device, sequences, width, pages = _ledger("free_pages", table, refs)
-    _check("free_pages", device, torch.int32, (("lengths", lengths, (sequences,)),))
-    _check("free_pages", device, torch.bool, (("release", release, (sequences,)),))
-    _check_error_word("free_pages", device, device_error)
-    with _on(stream):
-        table_out, lengths_out = torch.empty_like(table), torch.empty_like(lengths)
-        refs_out = torch.empty_like(refs)
-    call("h3sa_free_pages", ptr(table), sequences, width, ptr(lengths), ptr(refs), pages,
-         ptr(release), ptr(table_out), ptr(lengths_out), ptr(refs_out), ptr(device_error),
-         stream_handle(stream))
+    what = "free_pages"
+    device, sequences, width, pages = _ledger(what, table, refs)
+    if _bad(lengths, device, torch.int32, (sequences,)):
+        _refuse(what, "lengths", device, torch.int32, (sequences,))
+    if _bad(release, device, torch.bool, (sequences,)):
+        _refuse(what, "release", device, torch.bool, (sequences,))
+    error = _error_word(what, device, device_error)
+    table_out, lengths_out, refs_out = _alloc(
+        stream, (table, (sequences, width), torch.int32), (table, (sequences,), torch.int32),
+        (table, (pages,), torch.int32))
+    code = _FREE(table.data_ptr(), sequences, width, lengths.data_ptr(), refs.data_ptr(), pages,
+                 release.data_ptr(), table_out.data_ptr(), lengths_out.data_ptr(),
+                 refs_out.data_ptr(), error, _handle(stream, device))
+    if code:
+        check("h3sa_free_pages", code)
     return table_out, lengths_out, refs_out
 
 
@@ -197,7 +229,7 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     if not query.is_cuda:
         raise RuntimeError("h3sa kernels require CUDA tensors")
     device = query.device
-    if query.ndim != 4 or query.dtype != torch.bfloat16 or query.shape[3] != HEAD_DIM:
+    if query.ndim != 4 or query.dtype is not torch.bfloat16 or query.shape[3] != HEAD_DIM:
         raise RuntimeError(f"{what}: query must be bf16 [sequences, rows, heads, {HEAD_DIM}]")
     batch, rows, heads, _ = query.shape
     strides = query.stride()
@@ -212,36 +244,41 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     kv_heads, pool_rows, _ = key_pool.shape
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{what}: {heads} query heads are no multiple of {kv_heads} KV heads")
-    e4m3 = key_pool.dtype == torch.float8_e4m3fn
+    e4m3 = key_pool.dtype is torch.float8_e4m3fn
     if e4m3:
         if k_scale is None or v_scale is None:
             raise RuntimeError(f"{what}: e4m3 pools need k_scale and v_scale")
-        _check(what, device, torch.float32, (("k_scale", k_scale, (kv_heads,)),
-                                             ("v_scale", v_scale, (kv_heads,))))
-    elif key_pool.dtype != torch.bfloat16:
+        if _bad(k_scale, device, torch.float32, (kv_heads,)) or _bad(v_scale, device, torch.float32, (kv_heads,)):
+            _refuse(what, "k_scale and v_scale", device, torch.float32, (kv_heads,))
+    elif key_pool.dtype is not torch.bfloat16:
         raise RuntimeError(f"{what}: KV pools must be bf16 or e4m3")
     elif k_scale is not None or v_scale is not None:
         raise RuntimeError(f"{what}: bf16 pools take no scales")
     if table.ndim != 2:
         raise RuntimeError(f"{what}: table must be [sequences, width]")
     width = table.shape[1]
-    _check(what, device, torch.int32, (("table", table, (batch, width)),
-                                       ("lengths", lengths, (batch,))))
-    if out is not None:
-        _check(what, device, torch.bfloat16, (("out", out, (batch, rows, heads, HEAD_DIM)),))
-    if lse is not None:
-        _check(what, device, torch.float32, (("lse", lse, (batch, rows, heads)),))
-    _check_error_word(what, device, device_error)
-    need = LIB.h3sa_shared_prefix_workspace(batch, rows, heads, kv_heads, shared_rows)
-    with _on(stream):
-        if out is None:
-            out = torch.empty((batch, rows, heads, HEAD_DIM), dtype=torch.bfloat16, device=device)
-        work = torch.empty(max(need, 16), dtype=torch.uint8, device=device)
-    call("h3sa_shared_prefix_attention", ptr(query), (ctypes.c_int64 * 3)(*strides[:3]), ptr(out),
-         ptr(lse), batch, rows, heads, kv_heads, ptr(key_pool), ptr(value_pool),
-         pool_rows // PAGE_ROWS, 1 if e4m3 else 0, ptr(k_scale), ptr(v_scale), ptr(table), width,
-         ptr(lengths), int(shared_rows), 1 if causal else 0, float(softmax_scale), ptr(work),
-         work.numel(), ptr(device_error), stream_handle(stream))
+    if _bad(table, device, torch.int32, (batch, width)):
+        _refuse(what, "table", device, torch.int32, (batch, width))
+    if _bad(lengths, device, torch.int32, (batch,)):
+        _refuse(what, "lengths", device, torch.int32, (batch,))
+    if lse is not None and _bad(lse, device, torch.float32, (batch, rows, heads)):
+        _refuse(what, "lse", device, torch.float32, (batch, rows, heads))
+    error = _error_word(what, device, device_error)
+    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows))
+    if out is None:
+        out, work = _alloc(stream, (query, query.shape, torch.bfloat16), (query, (need,), torch.uint8))
+    else:
+        if _bad(out, device, torch.bfloat16, query.shape):
+            _refuse(what, "out", device, torch.bfloat16, query.shape)
+        work, = _alloc(stream, (query, (need,), torch.uint8))
+    code = _ATTEND(query.data_ptr(), _Strides(*strides[:3]), out.data_ptr(),
+                   None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
+                   key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
+                   k_scale.data_ptr() if e4m3 else None, v_scale.data_ptr() if e4m3 else None,
+                   table.data_ptr(), width, lengths.data_ptr(), shared_rows, 1 if causal else 0,
+                   softmax_scale, work.data_ptr(), need, error, _handle(stream, device))
+    if code:
+        check("h3sa_shared_prefix_attention", code)
     return out
 
 
