@@ -56,8 +56,8 @@ constexpr int kD = 128;
 constexpr int kBlk = 128;        // KV rows of a block (a page)
 constexpr int kSpan = 256;       // query rows of an item: two tiles
 constexpr int kBrThreads = 384;
-constexpr int kBrRegsControl = 72;
-constexpr int kBrRegsSoftmax = 216;
+constexpr int kBrRegsControl = 88;
+constexpr int kBrRegsSoftmax = 208;
 constexpr int kBrRegSplit = 128 * kBrRegsControl + 256 * kBrRegsSoftmax;
 constexpr int kDescRing = 4;
 constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
@@ -111,17 +111,21 @@ __device__ __forceinline__ int own_units(const BranchParams& p, int len, int t) 
   }
   return max(0, (limit + kBlk - 1) / kBlk - own_lo(p));
 }
-__device__ __forceinline__ int own_units_all(const BranchParams& p, int len) {
-  if (!p.causal) return own_units(p, len, 0) * p.own_tiles;
+// In the line of units every item with work counts kItemPad more than its blocks: loading its
+// query rows and writing its O out takes about as long.
+constexpr int kItemPad = 2;
+__device__ __forceinline__ int weight_of(int units) { return units > 0 ? units + kItemPad : 0; }
+__device__ __forceinline__ int own_weight_all(const BranchParams& p, int len) {
+  if (!p.causal) return weight_of(own_units(p, len, 0)) * p.own_tiles;
   int n = 0;
-  for (int t = 0; t < p.own_tiles; ++t) n += own_units(p, len, t);
+  for (int t = 0; t < p.own_tiles; ++t) n += weight_of(own_units(p, len, t));
   return n;
 }
 
 struct Plan {
   int shared_units;  // blocks of one shared item
-  int head_units;    // units of one KV head
-  int cut;           // units per CTA
+  int head_weight;   // one KV head's part of the line
+  int cut;           // one CTA's part
   int longest;       // sequence whose table row gives the shared pages
   int max_len;
 };
@@ -130,7 +134,7 @@ __device__ __forceinline__ Plan make_plan(const BranchParams& p, int lane) {
   int own = 0, best = -1, at = 0;
   for (int b = lane; b < p.batch; b += 32) {
     const int len = seq_length(p, b);
-    own += own_units_all(p, len);
+    own += own_weight_all(p, len);
     if (len > best) {
       best = len;
       at = b;
@@ -143,8 +147,8 @@ __device__ __forceinline__ Plan make_plan(const BranchParams& p, int lane) {
   pl.max_len = top;
   pl.longest = at;
   pl.shared_units = p.joint ? 0 : min(p.shared, (top + kBlk - 1) / kBlk);
-  pl.head_units = p.shared_tiles * pl.shared_units + own;
-  const int all = pl.head_units * p.kv_heads;
+  pl.head_weight = p.shared_tiles * weight_of(pl.shared_units) + own;
+  const int all = pl.head_weight * p.kv_heads;
   pl.cut = max(1, (all + p.ctas - 1) / p.ctas);
   return pl;
 }
@@ -375,14 +379,10 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
   tmem_wait_st();
 }
 
-// Loads a query row into the tile buffer (K-major, 128-byte swizzle). bf16: as it is, returns 1.
+// Writes a query row to the tile buffer (K-major, 128-byte swizzle). bf16: as it is, returns 1.
 // e4m3: as two terms after scaling by a power of two; returns that power's inverse.
 template <bool kFp8>
-__device__ __forceinline__ float load_query_row(uint8_t* tile, int lane_row, const __nv_bfloat16* src) {
-  uint4 v[16];
-#pragma unroll
-  for (int c = 0; c < 16; ++c)
-    v[c] = src ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0u, 0u, 0u, 0u);
+__device__ __forceinline__ float store_query_row(uint8_t* tile, int lane_row, const uint4 (&v)[16]) {
   uint8_t* row = tile + lane_row * 128;
   const int sw = lane_row & 7;
   if constexpr (!kFp8) {
@@ -441,7 +441,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
   volatile int* abort_flag = &sm.abort_flag;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) {
+  Plan pl;
+  if (warp == 0) pl = make_plan(p, lane);  // under way while the others set up
+  if (threadIdx.x == 64) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
     for (int s = 0; s < kS; ++s) {
       mbar_init(smem_u32(&sm.full[0][s]), 1);
       mbar_init(smem_u32(&sm.full[1][s]), 1);
@@ -494,32 +498,27 @@ __global__ void __launch_bounds__(kBrThreads, 1)
   if (warp == 0) {
     // ================================================================ schedule and TMA
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
-    const Plan pl = make_plan(p, lane);
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-    }
     for (int b = lane; b < p.batch; b += 32) {
       const int n = __ldg(p.lengths + b);
       if ((n < 0 || n > p.width * kBlk) && p.err) atomicOr(p.err, kErrBadIndex);
     }
-    const int all = pl.head_units * p.kv_heads;
+    const int all = pl.head_weight * p.kv_heads;
     int u = min(all, static_cast<int>(blockIdx.x) * pl.cut);
     int u_end = min(all, u + pl.cut);
-    const int shared_all = p.shared_tiles * pl.shared_units;
-    // position: head, then a shared tile (b < 0) or (b, t), then the block offset in the item
-    int head = pl.head_units ? u / pl.head_units : 0;
-    int x = u - head * pl.head_units;
-    int b = -1, t = 0, off = 0;
+    const int shared_weight = weight_of(pl.shared_units);
+    // position: head, then a shared tile (b < 0) or (b, t), then the offset in the item
+    int head = 0, b = -1, t = 0, off = 0;
     if (u < u_end) {
-      if (x < shared_all) {
-        t = x / pl.shared_units;
-        off = x - t * pl.shared_units;
+      head = u / pl.head_weight;
+      int x = u - head * pl.head_weight;
+      if (x < p.shared_tiles * shared_weight) {
+        t = x / shared_weight;
+        off = x - t * shared_weight;
       } else {
-        x -= shared_all;
+        x -= p.shared_tiles * shared_weight;
         for (int b0 = 0; b0 < p.batch; b0 += 32) {
           const int bb = b0 + lane;
-          const int n = bb < p.batch ? own_units_all(p, seq_length(p, bb)) : 0;
+          const int n = bb < p.batch ? own_weight_all(p, seq_length(p, bb)) : 0;
           int cum = n;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
@@ -536,10 +535,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           x -= __shfl_sync(0xffffffffu, cum, 31);
         }
         const int len = seq_length(p, b);
-        while (x >= own_units(p, len, t)) x -= own_units(p, len, t++);
+        for (int w; x >= (w = weight_of(own_units(p, len, t))); ++t) x -= w;
         off = x;
       }
     }
+    const auto item_units = [&]() { return b < 0 ? pl.shared_units : own_units(p, seq_length(p, b), t); };
     const auto step_item = [&]() {  // to the next item that has units
       bool found = false;
       if (b < 0) {
@@ -565,7 +565,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     // about the same time, from L2.
     int later = 0, later_head = 0, later_b = 0, later_t = 0, later_off = 0;
     if (u < u_end && off > 0) {
-      const int rest = (b < 0 ? pl.shared_units : own_units(p, seq_length(p, b), t)) - off;
+      const int rest = weight_of(item_units()) - off;
       if (rest < u_end - u) {
         later = rest;
         later_head = head;
@@ -588,10 +588,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       Segment g;
       memset(&g, 0, sizeof(g));
       int seq = 0;
-      if (u < u_end) {
-        int units;
+      while (u < u_end && !g.live) {
+        const int units = item_units(), part = min(weight_of(units) - off, u_end - u);
+        const int blocks = min(units, off + part) - off;
+        if (blocks > 0) {
         if (b < 0) {
-          units = pl.shared_units;
           seq = pl.longest;
           g.row0 = t * kSpan;
           g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
@@ -601,22 +602,21 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             g.slot_row[k] = (static_cast<long long>(head * p.shared_tiles + t + blockIdx.x) * 2 + k) *
                             p.shared_slot_rows;
         } else {
-          const int len = seq_length(p, b);
-          units = own_units(p, len, t);
           seq = b;
           g.row0 = b * p.rows * p.group + t * kSpan;
           g.n_rows = min(kSpan, p.rows * p.group - t * kSpan);
           g.block0 = own_lo(p) + off;
-          g.kv_end = len;
+            g.kv_end = seq_length(p, b);
           const long long item = (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t;
           for (int k = 0; k < 2; ++k)
             g.slot_row[k] = p.own_row0 + ((item + blockIdx.x) * 2 + k) * p.own_slot_rows;
         }
         g.live = 1;
         g.head = head;
-        g.blocks = min(units - off, u_end - u);
-        g.direct = pl.shared_units == 0 && g.blocks == units && (g.n_rows > kBlk || g.blocks == 1);
-        u += g.blocks;
+          g.blocks = blocks;
+          g.direct = pl.shared_units == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
+        }
+        u += part;
         off = 0;
         if (u < u_end) step_item();
         if (u >= u_end && later > 0) {
@@ -805,8 +805,6 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (pair && was_solo) {
         // From here this warp also waits on tile 0's barriers: both warps first see all blocks
         // they loaded alone.
-        if (pend) finish_item();
-        if (!ok) break;
         if (lane == 0) mbar_arrive(smem_u32(&sm.m_sync));
         bool w = mbar_wait(smem_u32(&sm.m_sync), m_ph, abort_flag, p.err);
         m_ph ^= 1u;
@@ -822,8 +820,6 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         if (owner == mt) {
           const uint32_t phases = second ? phase1 : phase0;
           if (first) {
-            if (pend) finish_item();
-            if (!ok) break;
             ok = __all_sync(0xffffffffu, mbar_wait(q_bar, q_ph, abort_flag, p.err));
             q_ph ^= 1u;
           } else {
@@ -866,8 +862,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         last_tile = pair ? 1 : owner;
         ring = vs + 1 == kS ? 0 : vs + 1;
       }
-    }
     if (ok && pend) finish_item();
+    }
     // leave no tensor-core work in flight past the teardown
     tc_commit(smem_u32(&sm.drain));
     const unsigned long long t0 = global_ns();
@@ -897,38 +893,62 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       return ok;
     };
+    struct Item {
+      int mine, begin, step;  // blocks of this tile: how many, the first, every step-th
+      int block0, head, row0, n_rows, span;  // of this tile; span: rows a copy has room for
+      int direct;
+      long long ws_row;
+      RowAt at;  // this thread's row
+    };
+    uint4 qv[16];  // and its query
+    // The next segment that this tile has blocks of; starts loading its query rows.
+    auto take = [&](Item& it) -> bool {
     Segment g;
-    while (ok && next_segment(g)) {
+      while (next_segment(g)) {
       const bool pair = g.n_rows > kBlk;
-      // blocks of this tile: all, or every other one from the tile whose turn it is
-      const int begin = pair ? 0 : ((last_tile ^ 1) == t ? 0 : 1);
-      const int step = pair ? 1 : 2;
-      const int mine = g.blocks > begin ? (g.blocks - begin + step - 1) / step : 0;
+        it.begin = pair ? 0 : ((last_tile ^ 1) == t ? 0 : 1);
+        it.step = pair ? 1 : 2;
+        it.mine = g.blocks > it.begin ? (g.blocks - it.begin + it.step - 1) / it.step : 0;
       last_tile = pair ? 1 : (last_tile ^ (g.blocks & 1));
       const int r0 = pair ? t * kBlk : 0;
-      const int n_rows = min(kBlk, g.n_rows - r0);  // rows of this tile
-      const bool halves = g.n_rows > 64;  // blocks of whole tiles are taken in two halves
-      const int span = halves ? 128 : n_rows <= 32 ? 32 : 64;
-      const int my = lr & (span - 1);  // this thread's row of the tile
-      const int copy = lr / span;      // and which copy of it
-      const bool live = my < n_rows;
-      const long long ws_row = g.slot_row[t];
-      if (mine == 0) {
-        if (!g.direct && lr < n_rows) p.part_ml[ws_row + lr] = make_float2(-INFINITY, 0.f);
+        it.n_rows = min(kBlk, g.n_rows - r0);
+        it.ws_row = g.slot_row[t];
+        if (it.mine == 0) {
+          if (!g.direct && lr < it.n_rows) p.part_ml[it.ws_row + lr] = make_float2(-INFINITY, 0.f);
         continue;
       }
-      const RowAt at = row_at(p, g.head, g.row0 + r0 + min(my, n_rows - 1));
-      const __nv_bfloat16* src = live ? p.q + at.b * p.q_sb + at.i * p.q_sn + at.h * p.q_sh : nullptr;
-      float sl2 = p.scale_log2 * load_query_row<kFp8>(sm.q[t], lr, src);
-      if constexpr (kFp8) sl2 *= __ldg(p.k_scale + g.head);
+        it.span = g.n_rows > 64 ? 128 : it.n_rows <= 32 ? 32 : 64;
+        it.block0 = g.block0 + it.begin;
+        it.head = g.head;
+        it.row0 = g.row0 + r0;
+        it.direct = g.direct;
+        const int my = lr & (it.span - 1);
+        it.at = row_at(p, g.head, it.row0 + min(my, it.n_rows - 1));
+        const uint4* src = reinterpret_cast<const uint4*>(p.q + it.at.b * p.q_sb + it.at.i * p.q_sn + it.at.h * p.q_sh);
+#pragma unroll
+        for (int c = 0; c < 16; ++c) qv[c] = my < it.n_rows ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        return true;
+      }
+      return false;
+    };
+    Item next;
+    bool more = take(next);
+    while (more) {
+      const Item it = next;
+      float sl2 = p.scale_log2 * store_query_row<kFp8>(sm.q[t], lr, qv);
+      if constexpr (kFp8) sl2 *= __ldg(p.k_scale + it.head);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const int limit = seq_length(p, at.b) - (p.causal ? p.rows - 1 - at.i : 0);
+      const int span = it.span, n_rows = it.n_rows;
+      const int my = lr & (span - 1);  // this thread's row of the tile
+      const int copy = lr / span;      // and which copy of it
+      const bool halves = span == 128;  // blocks of whole tiles are taken in two halves
+      const int limit = seq_length(p, it.at.b) - (p.causal ? p.rows - 1 - it.at.i : 0);
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
       const int col0 = copy * span;
-      for (int j = 0; ok && j < mine; ++j) {
-        const int left = limit - (g.block0 + begin + j * step) * kBlk;
+      for (int j = 0; ok && j < it.mine; ++j) {
+        const int left = limit - (it.block0 + j * it.step) * kBlk;
         const int n_steps = halves ? 2 : 1;
 #pragma unroll 1
         for (int h = 0; h < n_steps; ++h) {
@@ -952,88 +972,140 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      more = take(next);  // its query rows arrive while this item's O is written
       ok = mbar_wait(smem_u32(&sm.o_full[t]), o_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       o_ph ^= 1u;
       tc_fence_after();
-      // ---- join the copies: weights from their maxima, then O a quarter of the columns at a time
-      // through shared memory (the query tile's buffer: every QK^T of this item is complete)
-      float2* ml = reinterpret_cast<float2*>(sm.q[t] + 128 * 36 * 4);
-      float* stage = reinterpret_cast<float*>(sm.q[t]);
+      // ---- epilogue, through the query tile's buffer (every Q K^T of this item is complete)
+      float* const stage = reinterpret_cast<float*>(sm.q[t]);
+      float top = m, sum = l;
+      const int n_lanes = n_rows * (kBlk / span);  // lanes that hold something
+      if (span < 128) {  // the copies' maxima and sums; kept clear of the rows staged first
+        float2* const ml = reinterpret_cast<float2*>(sm.q[t] + kQBytes - 1024);
       ml[lr] = make_float2(m, l);
       if (!meet()) break;
-      float top = -INFINITY, sum = 0.f;
+        top = -INFINITY;
+        sum = 0.f;
       for (int c = 0; c < kBlk / span; ++c) top = fmaxf(top, ml[c * span + my].x);
       for (int c = 0; c < kBlk / span; ++c) {
         const float2 v = ml[c * span + my];
-        if (v.x > -INFINITY || v.y != v.y) sum += fast_exp2(v.x - top) * v.y;
+          if (v.y != 0.f) sum += fast_exp2(v.x - top) * v.y;
       }
-      // NaN sums must stay NaN; a copy that saw nothing weighs nothing
-      float weight = m > -INFINITY ? fast_exp2(m - top) : (l != l ? l : 0.f);
-      if (g.direct) {
+        if (n_lanes > 124 && !meet()) break;
+      }
+      // A copy that saw nothing weighs nothing; sums that are NaN stay so.
+      float weight = l == 0.f ? 0.f : fast_exp2(m - top);
+      if (it.direct) {
         weight = sum == 0.f ? 0.f : weight / sum;
-        if constexpr (kFp8) weight *= __ldg(p.v_scale + g.head);
+        if constexpr (kFp8) weight *= __ldg(p.v_scale + it.head);
       }
-      if (live && copy == 0) {
+      if (my < n_rows && copy == 0) {
         const float base = top - (kFp8 ? kBoostF8 : 0.f);
-        if (!g.direct) p.part_ml[ws_row + my] = make_float2(base, sum);
+        if (!it.direct) p.part_ml[it.ws_row + my] = make_float2(base, sum);
         else if (p.lse)
-          p.lse[(static_cast<long long>(at.b) * p.rows + at.i) * p.heads + at.h] =
+          p.lse[(static_cast<long long>(it.at.b) * p.rows + it.at.i) * p.heads + it.at.h] =
               sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
       }
+      const auto scaled = [&](const float* o, int j) {
+        return weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                             : make_float4(o[4 * j] * weight, o[4 * j + 1] * weight, o[4 * j + 2] * weight,
+                                           o[4 * j + 3] * weight);
+      };
+      const long long own_dst = ((static_cast<long long>(it.at.b) * p.rows + it.at.i) * p.heads + it.at.h) * kD;
+      if (span == 128) {
+        // a warp turns its 32 rows around by itself, 64 columns at a time, and writes whole lines
+        float* const mine = stage + quad * (32 * 64);
 #pragma unroll 1
-      for (int ch = 0; ok && ch < 4; ++ch) {
-        if (warp_live) {
+        for (int half = 0; warp_live && half < 2; ++half) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
           float o[32];
-          tmem_ld_cols(tO + ch * 32, o);
+            tmem_ld_cols(tO + half * 64 + c * 32, o);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(stage + lr * 36 + j * 4) =
-                weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                              : make_float4(o[4 * j] * weight, o[4 * j + 1] * weight,
-                                            o[4 * j + 2] * weight, o[4 * j + 3] * weight);
+              *reinterpret_cast<float4*>(mine + lane * 64 + (((c * 8 + j) ^ (lane & 7)) << 2)) = scaled(o, j);
+          }
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            const int r = i * 2 + (lane >> 4), c4 = lane & 15;
+            const float4 a = *reinterpret_cast<const float4*>(mine + r * 64 + ((c4 ^ (r & 7)) << 2));
+            const int lo = __shfl_sync(0xffffffffu, static_cast<int>(own_dst), r);
+            const int hi = __shfl_sync(0xffffffffu, static_cast<int>(own_dst >> 32), r);
+            if (quad * 32 + r >= n_rows) continue;
+            if (it.direct) {
+              const long long dst = static_cast<long long>(static_cast<uint32_t>(lo)) | (static_cast<long long>(hi) << 32);
+              *reinterpret_cast<uint2*>(p.out + dst + half * 64 + c4 * 4) =
+                  make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+            } else {
+              *reinterpret_cast<float4*>(p.part_o + (it.ws_row + quad * 32 + r) * kD + half * 64 + c4 * 4) = a;
+            }
+          }
+          __syncwarp();
+        }
+        ok = meet();
+      } else {
+        // the copies' rows side by side, all columns at once where they fit, then their sums
+        const int shift = n_lanes <= 60 ? 5 : 4;  // float4s of a staged row
+        const int slot = copy * n_rows + my;
+#pragma unroll 1
+        for (int c0 = 0; ok && c0 < 32; c0 += 1 << shift) {
+          if (warp_live) {
+#pragma unroll 1
+            for (int c = 0; c < 1 << shift; c += 8) {
+              float o[32];
+              tmem_ld_cols(tO + (c0 + c) * 4, o);
+              if (my < n_rows) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                  *reinterpret_cast<float4*>(stage + (((slot << shift) + ((c + j) ^ (slot & 7))) << 2)) = scaled(o, j);
+              }
+            }
         }
         if (!meet()) break;
-        for (int i = lr; i < n_rows * 8; i += 128) {
-          const int r = i >> 3, c4 = i & 7;
-          float4 a = *reinterpret_cast<const float4*>(stage + r * 36 + c4 * 4);
-          for (int c = 1; c < kBlk / span; ++c) {
-            const float4 v = *reinterpret_cast<const float4*>(stage + (c * span + r) * 36 + c4 * 4);
+          for (int i = lr; i < n_rows << shift; i += 128) {
+            const int r = i >> shift, c4 = i & ((1 << shift) - 1);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < kBlk / span; ++c) {
+              const int from = c * n_rows + r;
+              const float4 v = *reinterpret_cast<const float4*>(stage + (((from << shift) + (c4 ^ (from & 7))) << 2));
             a.x += v.x;
             a.y += v.y;
             a.z += v.z;
             a.w += v.w;
           }
-          if (g.direct) {
-            const RowAt ra = row_at(p, g.head, g.row0 + r0 + r);
+            if (it.direct) {
+              const RowAt ra = row_at(p, it.head, it.row0 + r);
             __nv_bfloat16* dst =
                 p.out + ((static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h) * kD;
-            *reinterpret_cast<uint2*>(dst + ch * 32 + c4 * 4) =
-                make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
+              *reinterpret_cast<uint2*>(dst + (c0 + c4) * 4) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
           } else {
-            *reinterpret_cast<float4*>(p.part_o + (ws_row + r) * kD + ch * 32 + c4 * 4) = a;
+              *reinterpret_cast<float4*>(p.part_o + (it.ws_row + r) * kD + (c0 + c4) * 4) = a;
           }
         }
         if (!meet()) break;
       }
+      }
       tc_fence_before();
+      if (!ok) break;
     }
   } else {
     // ================================================================ warp 3 of the first CTA
-    // writes the schedule down for the merge: the units of a shared item, of a head and of a CTA,
-    // and the own units in front of each sequence
+    // writes the schedule down for the merge: the units of a shared item, a head's and a CTA's part
+    // of the line, and what lies in front of each sequence's own items
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
     if (blockIdx.x == 0) {
-      const Plan pl = make_plan(p, lane);
+      pl = make_plan(p, lane);
       if (lane == 0) {
         p.plan[0] = pl.shared_units;
-        p.plan[1] = pl.head_units;
+        p.plan[1] = pl.head_weight;
         p.plan[2] = pl.cut;
       }
       int before = 0;
       for (int b0 = 0; b0 < p.batch; b0 += 32) {
         const int b = b0 + lane;
-        const int n = b < p.batch ? own_units_all(p, seq_length(p, b)) : 0;
+        const int n = b < p.batch ? own_weight_all(p, seq_length(p, b)) : 0;
         int cum = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -1138,7 +1210,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int team = warp / kTeam, part = warp % kTeam;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int shared_units = kJoint ? 0 : __ldcg(p.plan), head_units = __ldcg(p.plan + 1), cut = __ldcg(p.plan + 2);
+  const int shared_units = kJoint ? 0 : __ldcg(p.plan), head_weight = __ldcg(p.plan + 1), cut = __ldcg(p.plan + 2);
+  const int shared_weight = weight_of(shared_units);
   const int own_all = p.rows * p.group;
   // split form: stacked rows of all branches, one a team, head by head; joint form: kRows rows of
   // an item a warp
@@ -1162,8 +1235,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
     if (r >= min(own_all, (t + 1) * kSpan)) return;
   }
   const int len = seq_length(p, b);
-  int u0 = head * head_units + p.shared_tiles * shared_units + __ldcg(p.plan + 3 + b);
-  for (int k = 0; k < t; ++k) u0 += own_units(p, len, k);
+  int u0 = head * head_weight + p.shared_tiles * shared_weight + __ldcg(p.plan + 3 + b);
+  for (int k = 0; k < t; ++k) u0 += weight_of(own_units(p, len, k));
   const int units = own_units(p, len, t);
   const int n_rows = min(kSpan, own_all - t * kSpan);
   if (shared_units == 0 && units > 0 && u0 / cut == (u0 + units - 1) / cut && (n_rows > kBlk || units == 1))
@@ -1174,7 +1247,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
     // rows past the item read its last row again and write nothing
     const int rk = min(r + k, t * kSpan + n_rows - 1);
     const int row = b * own_all + rk, t_sh = row / kSpan;
-    sh[k] = pieces_of(cut, head * head_units + t_sh * shared_units, shared_units,
+    sh[k] = pieces_of(cut, head * head_weight + t_sh * shared_weight, shared_units,
                       min(kSpan, p.batch * own_all - t_sh * kSpan), row % kSpan,
                       head * p.shared_tiles + t_sh, 0, p.shared_slot_rows);
     own[k] = pieces_of(cut, u0, units, n_rows, rk - t * kSpan,
@@ -1387,7 +1460,8 @@ int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides
   const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
   const int64_t tiles = (static_cast<int64_t>(rows) * group + kSpan - 1) / kSpan;
   if (stacked > INT32_MAX / 2 ||
-      kv_heads * (((stacked + kSpan - 1) / kSpan) * (shared_rows / kBlk) + batch * tiles * width) > INT32_MAX / 2 ||
+      kv_heads * (((stacked + kSpan - 1) / kSpan) * (shared_rows / kBlk + kItemPad) +
+                  batch * tiles * (width + kItemPad)) > INT32_MAX / 2 ||
       static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d over %d "
                      "pages exceeds the work index", batch, rows, heads, width);
