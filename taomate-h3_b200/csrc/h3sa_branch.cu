@@ -1429,8 +1429,8 @@ int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
   return s.bytes;
 }
 
-int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides, void* out, float* lse,
-                                 int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int64_t stride_row,
+                                 int64_t stride_head, void* out, float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
                                  const void* key_pool, const void* value_pool, int32_t pool_pages,
                                  int32_t e4m3, const float* k_scale, const float* v_scale,
                                  const int32_t* table, int32_t width, const int32_t* lengths,
@@ -1448,13 +1448,13 @@ int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides
   if (shared_rows < 0 || shared_rows % kBlk || shared_rows / kBlk > width)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: %d shared rows are not whole pages of a "
                      "table of %d entries", shared_rows, width);
-  if (!query || !query_strides || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
+  if (!query || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
       (e4m3 && (!k_scale || !v_scale)))
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
   if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
   if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
-      !aligned(workspace, 16) || query_strides[0] % 8 || query_strides[1] % 8 || query_strides[2] % 8)
+      !aligned(workspace, 16) || stride_sequence % 8 || stride_row % 8 || stride_head % 8)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned");
   const int group = heads / kv_heads;
   const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
@@ -1472,9 +1472,9 @@ int h3sa_shared_prefix_attention(const void* query, const int64_t* query_strides
   BranchParams p;
   memset(&p, 0, sizeof(p));
   p.q = static_cast<const __nv_bfloat16*>(query);
-  p.q_sb = query_strides[0];
-  p.q_sn = query_strides[1];
-  p.q_sh = query_strides[2];
+  p.q_sb = stride_sequence;
+  p.q_sn = stride_row;
+  p.q_sh = stride_head;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.lse = lse;
   p.table = table;

@@ -161,8 +161,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "h3sa_shared_prefix_workspace": (_L, [_I, _I, _I, _I, _I]),
     "h3sa_shared_prefix_attention": (
         ctypes.c_int,
-        [_P, ctypes.POINTER(_L), _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I,
-         _I, _F, _P, _L, _P, _P]),
+        [_P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _F,
+         _P, _L, _P, _P]),
     "h3sa_permute_rows": (
         ctypes.c_int,
         [_P, _P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),

@@ -35,7 +35,8 @@ _FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_f
 _ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
 _PAGES_WORK = LIB.h3sa_pages_workspace
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_Strides = ctypes.c_int64 * 3
+_I32, _U8, _F32, _BF16, _E4M3 = torch.int32, torch.uint8, torch.float32, torch.bfloat16, torch.float8_e4m3fn
+_empty, _empty_like = torch.empty, torch.empty_like
 
 
 def _bad(t: torch.Tensor, device: torch.device, dtype: torch.dtype, shape: tuple[int, ...]) -> bool:
@@ -49,18 +50,28 @@ def _refuse(what: str, name: str, device: torch.device, dtype: torch.dtype, shap
 def _error_word(what: str, device: torch.device, word: torch.Tensor | None) -> int | None:
     if word is None:
         return None
-    if word.device != device or word.dtype is not torch.int32 or word.numel() < 1:
+    if word.device != device or word.dtype is not _I32 or word.numel() < 1:
         raise RuntimeError(f"{what}: device_error must be an int32 tensor on {device}")
     return word.data_ptr()
 
 
-def _alloc(stream: torch.cuda.Stream | None, *wanted: tuple[torch.Tensor, tuple[int, ...], torch.dtype]):
-    """Results and workspaces, allocated on the stream that uses them."""
+class _Current:
+    """The current stream: nothing to switch."""
 
-    if stream is None:
-        return [t.new_empty(shape, dtype=dtype) for t, shape, dtype in wanted]
-    with torch.cuda.stream(stream):
-        return [t.new_empty(shape, dtype=dtype) for t, shape, dtype in wanted]
+    def __enter__(self) -> None:
+        return None
+
+    def __exit__(self, *exc: object) -> None:
+        return None
+
+
+_CURRENT = _Current()
+
+
+def _on(stream: torch.cuda.Stream | None):
+    """Results and workspaces are allocated on the stream that uses them."""
+
+    return _CURRENT if stream is None else torch.cuda.stream(stream)
 
 
 def _handle(stream: torch.cuda.Stream | None, device: torch.device) -> int:
@@ -109,10 +120,10 @@ def _ledger(what: str, table: torch.Tensor, refs: torch.Tensor) -> tuple[torch.d
     if table.ndim != 2 or refs.ndim != 1:
         raise RuntimeError(f"{what}: table must be [sequences, width] and refs [pages]")
     device, (sequences, width), (pages,) = table.device, table.shape, refs.shape
-    if _bad(table, device, torch.int32, (sequences, width)):
-        _refuse(what, "table", device, torch.int32, (sequences, width))
-    if _bad(refs, device, torch.int32, (pages,)):
-        _refuse(what, "refs", device, torch.int32, (pages,))
+    if _bad(table, device, _I32, (sequences, width)):
+        _refuse(what, "table", device, _I32, (sequences, width))
+    if _bad(refs, device, _I32, (pages,)):
+        _refuse(what, "refs", device, _I32, (pages,))
     return device, sequences, width, pages
 
 
@@ -136,17 +147,19 @@ def fork_pages(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, r
     if parents.ndim != 1:
         raise RuntimeError(f"{what}: parents must be [children]")
     children = parents.shape[0]
-    if _bad(lengths, device, torch.int32, (sequences,)):
-        _refuse(what, "lengths", device, torch.int32, (sequences,))
-    if _bad(parents, device, torch.int32, (children,)):
-        _refuse(what, "parents", device, torch.int32, (children,))
+    if _bad(lengths, device, _I32, (sequences,)):
+        _refuse(what, "lengths", device, _I32, (sequences,))
+    if _bad(parents, device, _I32, (children,)):
+        _refuse(what, "parents", device, _I32, (children,))
     error = _error_word(what, device, device_error)
     if reserve_rows < 0:
         raise ValueError(f"{what}: reserve_rows must not be negative")
     p = _pools(what, pools, pages, device)
-    child_table, child_lengths, refs_out, work = _alloc(
-        stream, (table, (children, width), torch.int32), (table, (children,), torch.int32),
-        (table, (pages,), torch.int32), (table, (_PAGES_WORK(pages, children),), torch.uint8))
+    with _on(stream):
+        child_table = _empty((children, width), dtype=_I32, device=device)
+        child_lengths = _empty_like(parents)
+        refs_out = _empty_like(refs)
+        work = _empty(_PAGES_WORK(pages, children), dtype=_U8, device=device)
     code = _FORK(p, table.data_ptr(), sequences, width, lengths.data_ptr(), refs.data_ptr(),
                  parents.data_ptr(), children, int(reserve_rows), 1 if private else 0,
                  child_table.data_ptr(), child_lengths.data_ptr(), refs_out.data_ptr(),
@@ -168,9 +181,10 @@ def compact_pages(pools: PoolTensors, table: torch.Tensor, refs: torch.Tensor, *
     device, sequences, width, pages = _ledger(what, table, refs)
     error = _error_word(what, device, device_error)
     p = _pools(what, pools, pages, device)
-    table_out, refs_out, live, work = _alloc(
-        stream, (table, (sequences, width), torch.int32), (table, (pages,), torch.int32),
-        (table, (1,), torch.int32), (table, (_PAGES_WORK(pages, 0),), torch.uint8))
+    with _on(stream):
+        table_out, refs_out = _empty_like(table), _empty_like(refs)
+        live = _empty(1, dtype=_I32, device=device)
+        work = _empty(_PAGES_WORK(pages, 0), dtype=_U8, device=device)
     code = _COMPACT(p, table.data_ptr(), sequences, width, refs.data_ptr(), table_out.data_ptr(),
                     refs_out.data_ptr(), live.data_ptr(), work.data_ptr(), error,
                     _handle(stream, device))
@@ -188,14 +202,13 @@ def free_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
 
     what = "free_pages"
     device, sequences, width, pages = _ledger(what, table, refs)
-    if _bad(lengths, device, torch.int32, (sequences,)):
-        _refuse(what, "lengths", device, torch.int32, (sequences,))
+    if _bad(lengths, device, _I32, (sequences,)):
+        _refuse(what, "lengths", device, _I32, (sequences,))
     if _bad(release, device, torch.bool, (sequences,)):
         _refuse(what, "release", device, torch.bool, (sequences,))
     error = _error_word(what, device, device_error)
-    table_out, lengths_out, refs_out = _alloc(
-        stream, (table, (sequences, width), torch.int32), (table, (sequences,), torch.int32),
-        (table, (pages,), torch.int32))
+    with _on(stream):
+        table_out, lengths_out, refs_out = _empty_like(table), _empty_like(lengths), _empty_like(refs)
     code = _FREE(table.data_ptr(), sequences, width, lengths.data_ptr(), refs.data_ptr(), pages,
                  release.data_ptr(), table_out.data_ptr(), lengths_out.data_ptr(),
                  refs_out.data_ptr(), error, _handle(stream, device))
@@ -228,50 +241,50 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     what = "shared_prefix_attention"
     if not query.is_cuda:
         raise RuntimeError("h3sa kernels require CUDA tensors")
-    device = query.device
-    if query.ndim != 4 or query.dtype is not torch.bfloat16 or query.shape[3] != HEAD_DIM:
+    device, shape, pool = query.device, query.shape, key_pool.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or query.dtype is not _BF16:
         raise RuntimeError(f"{what}: query must be bf16 [sequences, rows, heads, {HEAD_DIM}]")
-    batch, rows, heads, _ = query.shape
+    batch, rows, heads, _ = shape
     strides = query.stride()
-    if strides[3] != 1 or strides[0] % 8 or strides[1] % 8 or strides[2] % 8 or query.data_ptr() % 16:
+    if strides[3] != 1 or (strides[0] | strides[1] | strides[2]) % 8 or query.data_ptr() % 16:
         raise RuntimeError(f"{what}: query rows must be contiguous and 16-byte aligned")
-    if (key_pool.ndim != 3 or key_pool.shape != value_pool.shape or key_pool.shape[2] != HEAD_DIM
-            or key_pool.shape[1] % PAGE_ROWS or key_pool.dtype != value_pool.dtype
-            or not key_pool.is_contiguous() or not value_pool.is_contiguous()
-            or key_pool.device != device or value_pool.device != device):
+    kind = key_pool.dtype
+    if (len(pool) != 3 or pool[1] % PAGE_ROWS or pool[2] != HEAD_DIM or _bad(key_pool, device, kind, pool)
+            or _bad(value_pool, device, kind, pool)):
         raise RuntimeError(f"{what}: KV pools must be contiguous [kv_heads, pages*{PAGE_ROWS}, "
                            f"{HEAD_DIM}] of one dtype on {device}")
-    kv_heads, pool_rows, _ = key_pool.shape
+    kv_heads, pool_rows, _ = pool
     if kv_heads == 0 or heads == 0 or heads % kv_heads:
         raise RuntimeError(f"{what}: {heads} query heads are no multiple of {kv_heads} KV heads")
-    e4m3 = key_pool.dtype is torch.float8_e4m3fn
+    e4m3 = kind is _E4M3
     if e4m3:
         if k_scale is None or v_scale is None:
             raise RuntimeError(f"{what}: e4m3 pools need k_scale and v_scale")
-        if _bad(k_scale, device, torch.float32, (kv_heads,)) or _bad(v_scale, device, torch.float32, (kv_heads,)):
-            _refuse(what, "k_scale and v_scale", device, torch.float32, (kv_heads,))
-    elif key_pool.dtype is not torch.bfloat16:
+        if _bad(k_scale, device, _F32, (kv_heads,)) or _bad(v_scale, device, _F32, (kv_heads,)):
+            _refuse(what, "k_scale and v_scale", device, _F32, (kv_heads,))
+    elif kind is not _BF16:
         raise RuntimeError(f"{what}: KV pools must be bf16 or e4m3")
     elif k_scale is not None or v_scale is not None:
         raise RuntimeError(f"{what}: bf16 pools take no scales")
     if table.ndim != 2:
         raise RuntimeError(f"{what}: table must be [sequences, width]")
     width = table.shape[1]
-    if _bad(table, device, torch.int32, (batch, width)):
-        _refuse(what, "table", device, torch.int32, (batch, width))
-    if _bad(lengths, device, torch.int32, (batch,)):
-        _refuse(what, "lengths", device, torch.int32, (batch,))
-    if lse is not None and _bad(lse, device, torch.float32, (batch, rows, heads)):
-        _refuse(what, "lse", device, torch.float32, (batch, rows, heads))
+    if _bad(table, device, _I32, (batch, width)):
+        _refuse(what, "table", device, _I32, (batch, width))
+    if _bad(lengths, device, _I32, (batch,)):
+        _refuse(what, "lengths", device, _I32, (batch,))
+    if lse is not None and _bad(lse, device, _F32, (batch, rows, heads)):
+        _refuse(what, "lse", device, _F32, (batch, rows, heads))
     error = _error_word(what, device, device_error)
     need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows))
-    if out is None:
-        out, work = _alloc(stream, (query, query.shape, torch.bfloat16), (query, (need,), torch.uint8))
-    else:
-        if _bad(out, device, torch.bfloat16, query.shape):
-            _refuse(what, "out", device, torch.bfloat16, query.shape)
-        work, = _alloc(stream, (query, (need,), torch.uint8))
-    code = _ATTEND(query.data_ptr(), _Strides(*strides[:3]), out.data_ptr(),
+    if out is not None and _bad(out, device, _BF16, query.shape):
+        _refuse(what, "out", device, _BF16, query.shape)
+    with _on(stream):
+        if out is None:
+            out = (_empty_like(query) if query.is_contiguous() else
+                   _empty(query.shape, dtype=_BF16, device=device))
+        work = _empty(need, dtype=_U8, device=device)
+    code = _ATTEND(query.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(),
                    None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
                    key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
                    k_scale.data_ptr() if e4m3 else None, v_scale.data_ptr() if e4m3 else None,
