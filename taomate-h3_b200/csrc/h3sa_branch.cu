@@ -592,27 +592,27 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         const int units = item_units(), part = min(weight_of(units) - off, u_end - u);
         const int blocks = min(units, off + part) - off;
         if (blocks > 0) {
-        if (b < 0) {
-          seq = pl.longest;
-          g.row0 = t * kSpan;
-          g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
-          g.block0 = off;
-          g.kv_end = pl.max_len;
-          for (int k = 0; k < 2; ++k)
+          if (b < 0) {
+            seq = pl.longest;
+            g.row0 = t * kSpan;
+            g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
+            g.block0 = off;
+            g.kv_end = pl.max_len;
+            for (int k = 0; k < 2; ++k)
             g.slot_row[k] = (static_cast<long long>(head * p.shared_tiles + t + blockIdx.x) * 2 + k) *
                             p.shared_slot_rows;
-        } else {
-          seq = b;
-          g.row0 = b * p.rows * p.group + t * kSpan;
-          g.n_rows = min(kSpan, p.rows * p.group - t * kSpan);
-          g.block0 = own_lo(p) + off;
+          } else {
+            seq = b;
+            g.row0 = b * p.rows * p.group + t * kSpan;
+            g.n_rows = min(kSpan, p.rows * p.group - t * kSpan);
+            g.block0 = own_lo(p) + off;
             g.kv_end = seq_length(p, b);
-          const long long item = (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t;
-          for (int k = 0; k < 2; ++k)
+            const long long item = (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t;
+            for (int k = 0; k < 2; ++k)
             g.slot_row[k] = p.own_row0 + ((item + blockIdx.x) * 2 + k) * p.own_slot_rows;
-        }
-        g.live = 1;
-        g.head = head;
+          }
+          g.live = 1;
+          g.head = head;
           g.blocks = blocks;
           g.direct = pl.shared_units == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
         }
@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         last_tile = pair ? 1 : owner;
         ring = vs + 1 == kS ? 0 : vs + 1;
       }
-    if (ok && pend) finish_item();
+      if (ok && pend) finish_item();
     }
     // leave no tensor-core work in flight past the teardown
     tc_commit(smem_u32(&sm.drain));
@@ -903,20 +903,20 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     uint4 qv[16];  // and its query
     // The next segment that this tile has blocks of; starts loading its query rows.
     auto take = [&](Item& it) -> bool {
-    Segment g;
+      Segment g;
       while (next_segment(g)) {
-      const bool pair = g.n_rows > kBlk;
+        const bool pair = g.n_rows > kBlk;
         it.begin = pair ? 0 : ((last_tile ^ 1) == t ? 0 : 1);
         it.step = pair ? 1 : 2;
         it.mine = g.blocks > it.begin ? (g.blocks - it.begin + it.step - 1) / it.step : 0;
-      last_tile = pair ? 1 : (last_tile ^ (g.blocks & 1));
-      const int r0 = pair ? t * kBlk : 0;
+        last_tile = pair ? 1 : (last_tile ^ (g.blocks & 1));
+        const int r0 = pair ? t * kBlk : 0;
         it.n_rows = min(kBlk, g.n_rows - r0);
         it.ws_row = g.slot_row[t];
         if (it.mine == 0) {
           if (!g.direct && lr < it.n_rows) p.part_ml[it.ws_row + lr] = make_float2(-INFINITY, 0.f);
-        continue;
-      }
+          continue;
+        }
         it.span = g.n_rows > 64 ? 128 : it.n_rows <= 32 ? 32 : 64;
         it.block0 = g.block0 + it.begin;
         it.head = g.head;
@@ -983,15 +983,15 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       const int n_lanes = n_rows * (kBlk / span);  // lanes that hold something
       if (span < 128) {  // the copies' maxima and sums; kept clear of the rows staged first
         float2* const ml = reinterpret_cast<float2*>(sm.q[t] + kQBytes - 1024);
-      ml[lr] = make_float2(m, l);
-      if (!meet()) break;
+        ml[lr] = make_float2(m, l);
+        if (!meet()) break;
         top = -INFINITY;
         sum = 0.f;
-      for (int c = 0; c < kBlk / span; ++c) top = fmaxf(top, ml[c * span + my].x);
-      for (int c = 0; c < kBlk / span; ++c) {
-        const float2 v = ml[c * span + my];
+        for (int c = 0; c < kBlk / span; ++c) top = fmaxf(top, ml[c * span + my].x);
+        for (int c = 0; c < kBlk / span; ++c) {
+          const float2 v = ml[c * span + my];
           if (v.y != 0.f) sum += fast_exp2(v.x - top) * v.y;
-      }
+        }
         if (n_lanes > 124 && !meet()) break;
       }
       // A copy that saw nothing weighs nothing; sums that are NaN stay so.
@@ -1020,10 +1020,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         for (int half = 0; warp_live && half < 2; ++half) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-          float o[32];
+            float o[32];
             tmem_ld_cols(tO + half * 64 + c * 32, o);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 8; ++j)
               *reinterpret_cast<float4*>(mine + lane * 64 + (((c * 8 + j) ^ (lane & 7)) << 2)) = scaled(o, j);
           }
           __syncwarp();
@@ -1062,30 +1062,30 @@ __global__ void __launch_bounds__(kBrThreads, 1)
                   *reinterpret_cast<float4*>(stage + (((slot << shift) + ((c + j) ^ (slot & 7))) << 2)) = scaled(o, j);
               }
             }
-        }
-        if (!meet()) break;
+          }
+          if (!meet()) break;
           for (int i = lr; i < n_rows << shift; i += 128) {
             const int r = i >> shift, c4 = i & ((1 << shift) - 1);
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int c = 0; c < kBlk / span; ++c) {
               const int from = c * n_rows + r;
               const float4 v = *reinterpret_cast<const float4*>(stage + (((from << shift) + (c4 ^ (from & 7))) << 2));
-            a.x += v.x;
-            a.y += v.y;
-            a.z += v.z;
-            a.w += v.w;
-          }
+              a.x += v.x;
+              a.y += v.y;
+              a.z += v.z;
+              a.w += v.w;
+            }
             if (it.direct) {
               const RowAt ra = row_at(p, it.head, it.row0 + r);
-            __nv_bfloat16* dst =
+              __nv_bfloat16* dst =
                 p.out + ((static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h) * kD;
               *reinterpret_cast<uint2*>(dst + (c0 + c4) * 4) = make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
-          } else {
+            } else {
               *reinterpret_cast<float4*>(p.part_o + (it.ws_row + r) * kD + (c0 + c4) * 4) = a;
+            }
           }
+          if (!meet()) break;
         }
-        if (!meet()) break;
-      }
       }
       tc_fence_before();
       if (!ok) break;
