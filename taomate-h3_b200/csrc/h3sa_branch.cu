@@ -201,15 +201,6 @@ constexpr size_t br_smem_bytes() {
 static_assert(br_smem_bytes<false>() <= 232448 && br_smem_bytes<true>() <= 232448,
               "branch attention needs more than 227 KB");
 
-__device__ __forceinline__ void tmem_ld_cols(uint32_t taddr, float* s) {
-  uint32_t r[32];
-  tmem_ld32(taddr, r);
-  tmem_wait_ld();
-  reg_fence32(r);
-#pragma unroll
-  for (int j = 0; j < 32; ++j) s[j] = __uint_as_float(r[j]);
-}
-
 __device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -379,33 +370,35 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
   tmem_wait_st();
 }
 
-// Writes a query row to the tile buffer (K-major, 128-byte swizzle). bf16: as it is, returns 1.
-// e4m3: as two terms after scaling by a power of two; returns that power's inverse.
+// Writes query row `my` of a tile that holds `copies` of each row, span rows apart (K-major, 128-byte
+// swizzle); `copy` says which of them this thread stands for. bf16: its own copy, as it is; returns
+// 1. e4m3: as two terms after scaling by a power of two; returns that power's inverse. The splits
+// are some ten instructions an element, so the threads of a row's copies share them out and each
+// writes its columns to all copies.
 template <bool kFp8>
-__device__ __forceinline__ float store_query_row(uint8_t* tile, int lane_row, const uint4 (&v)[16]) {
-  uint8_t* row = tile + lane_row * 128;
-  const int sw = lane_row & 7;
+__device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy, int copies, int span,
+                                                 const uint4 (&v)[16]) {
+  const int sw = my & 7;  // the same for all copies: span is a multiple of 8
   if constexpr (!kFp8) {
+    uint8_t* row = tile + (copy * span + my) * 128;
 #pragma unroll
     for (int c = 0; c < 16; ++c)
       *reinterpret_cast<uint4*>(row + (c >> 3) * kAtom + (((c & 7) ^ sw) << 4)) = v[c];
     return 1.0f;
   } else {
-    float amax = 0.f;
+    // the largest magnitude as bits: those of an infinity or NaN are larger than any number's
     const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
-    bool bad = false;
+    uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) {
-      const float a = __uint_as_float(w[i] << 16), b = __uint_as_float(w[i] & 0xffff0000u);
-      amax = fmaxf(amax, fmaxf(fabsf(a), fabsf(b)));
-      bad = bad || !(fabsf(a) < INFINITY) || !(fabsf(b) < INFINITY);
-    }
-    // 2^k with amax * 2^k in [128, 256); tiny rows keep their products in fp32's range
-    const int e = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    for (int i = 0; i < 64; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+    top = max(top >> 16, top & 0xffffu);
+    // 2^k with the largest * 2^k in [128, 256); tiny rows keep their products in fp32's range
+    const int e = static_cast<int>(top >> 7) - 127;
     const int k = max(-120, min(7 - e, 120));
     const float up = __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {  // 16 columns a chunk
+      if ((c & (copies - 1)) != copy) continue;
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -418,12 +411,14 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int lane_row, co
         hi[j] = h[0] | (h[1] << 16);
         lo[j] = g[0] | (g[1] << 16);
       }
-      const int at = (c ^ sw) << 4;
-      *reinterpret_cast<uint4*>(row + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(row + kAtom + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      for (int r = my; r < kBlk; r += span) {
+        uint8_t* at = tile + r * 128 + ((c ^ sw) << 4);
+        *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(at + kAtom) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
     }
     // a row with an infinity or NaN gets NaN scores, as its products have
-    return bad ? __int_as_float(0x7fffffff) : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    return top >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
   }
 }
 
@@ -935,13 +930,13 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     bool more = take(next);
     while (more) {
       const Item it = next;
-      float sl2 = p.scale_log2 * store_query_row<kFp8>(sm.q[t], lr, qv);
+      const int span = it.span, n_rows = it.n_rows, copies = kBlk / span;
+      const int my = lr & (span - 1);  // this thread's row of the tile
+      const int copy = lr / span;      // and which copy of it
+      float sl2 = p.scale_log2 * store_query_row<kFp8>(sm.q[t], my, copy, copies, span, qv);
       if constexpr (kFp8) sl2 *= __ldg(p.k_scale + it.head);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const int span = it.span, n_rows = it.n_rows;
-      const int my = lr & (span - 1);  // this thread's row of the tile
-      const int copy = lr / span;      // and which copy of it
       const bool halves = span == 128;  // blocks of whole tiles are taken in two halves
       const int limit = seq_length(p, it.at.b) - (p.causal ? p.rows - 1 - it.at.i : 0);
       const bool warp_live = quad * 32 % span < n_rows;
@@ -980,18 +975,18 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       // ---- epilogue, through the query tile's buffer (every Q K^T of this item is complete)
       float* const stage = reinterpret_cast<float*>(sm.q[t]);
       float top = m, sum = l;
-      const int n_lanes = n_rows * (kBlk / span);  // lanes that hold something
+      const int n_lanes = n_rows * copies;  // lanes that hold something
       if (span < 128) {  // the copies' maxima and sums; kept clear of the rows staged first
         float2* const ml = reinterpret_cast<float2*>(sm.q[t] + kQBytes - 1024);
         ml[lr] = make_float2(m, l);
         if (!meet()) break;
-        top = -INFINITY;
+        float2 v[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) v[c] = c < copies ? ml[c * span + my] : make_float2(-INFINITY, 0.f);
+        top = fmax3(fmaxf(v[0].x, v[1].x), v[2].x, v[3].x);
         sum = 0.f;
-        for (int c = 0; c < kBlk / span; ++c) top = fmaxf(top, ml[c * span + my].x);
-        for (int c = 0; c < kBlk / span; ++c) {
-          const float2 v = ml[c * span + my];
-          if (v.y != 0.f) sum += fast_exp2(v.x - top) * v.y;
-        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum += v[c].y != 0.f ? fast_exp2(v[c].x - top) * v[c].y : 0.f;
         if (n_lanes > 124 && !meet()) break;
       }
       // A copy that saw nothing weighs nothing; sums that are NaN stay so.
@@ -1007,10 +1002,15 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           p.lse[(static_cast<long long>(it.at.b) * p.rows + it.at.i) * p.heads + it.at.h] =
               sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
       }
-      const auto scaled = [&](const float* o, int j) {
-        return weight == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                             : make_float4(o[4 * j] * weight, o[4 * j + 1] * weight, o[4 * j + 2] * weight,
-                                           o[4 * j + 3] * weight);
+      // Four columns of O times the weight. O of a copy that weighs nothing may hold NaN (a hidden
+      // infinity of V times P's zeros): it counts as zero.
+      const auto scaled = [&](const uint32_t (&o)[32], int j) {
+        float4 a;
+        a.x = weight == 0.f ? 0.f : __uint_as_float(o[4 * j]) * weight;
+        a.y = weight == 0.f ? 0.f : __uint_as_float(o[4 * j + 1]) * weight;
+        a.z = weight == 0.f ? 0.f : __uint_as_float(o[4 * j + 2]) * weight;
+        a.w = weight == 0.f ? 0.f : __uint_as_float(o[4 * j + 3]) * weight;
+        return a;
       };
       const long long own_dst = ((static_cast<long long>(it.at.b) * p.rows + it.at.i) * p.heads + it.at.h) * kD;
       if (span == 128) {
@@ -1018,13 +1018,16 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         float* const mine = stage + quad * (32 * 64);
 #pragma unroll 1
         for (int half = 0; warp_live && half < 2; ++half) {
+          uint32_t o[2][32];
+          tmem_ld32(tO + half * 64, o[0]);
+          tmem_ld32(tO + half * 64 + 32, o[1]);
+          tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float o[32];
-            tmem_ld_cols(tO + half * 64 + c * 32, o);
+            reg_fence32(o[c]);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              *reinterpret_cast<float4*>(mine + lane * 64 + (((c * 8 + j) ^ (lane & 7)) << 2)) = scaled(o, j);
+              *reinterpret_cast<float4*>(mine + lane * 64 + (((c * 8 + j) ^ (lane & 7)) << 2)) = scaled(o[c], j);
           }
           __syncwarp();
 #pragma unroll 4
@@ -1053,13 +1056,19 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         for (int c0 = 0; ok && c0 < 32; c0 += 1 << shift) {
           if (warp_live) {
 #pragma unroll 1
-            for (int c = 0; c < 1 << shift; c += 8) {
-              float o[32];
-              tmem_ld_cols(tO + (c0 + c) * 4, o);
-              if (my < n_rows) {
+            for (int c = 0; c < 1 << shift; c += 16) {
+              uint32_t o[2][32];
+              tmem_ld32(tO + (c0 + c) * 4, o[0]);
+              tmem_ld32(tO + (c0 + c) * 4 + 32, o[1]);
+              tmem_wait_ld();
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                reg_fence32(o[half]);
+                if (my >= n_rows) continue;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                  *reinterpret_cast<float4*>(stage + (((slot << shift) + ((c + j) ^ (slot & 7))) << 2)) = scaled(o, j);
+                  *reinterpret_cast<float4*>(stage + (((slot << shift) + ((c + half * 8 + j) ^ (slot & 7))) << 2)) =
+                      scaled(o[half], j);
               }
             }
           }
@@ -1067,7 +1076,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           for (int i = lr; i < n_rows << shift; i += 128) {
             const int r = i >> shift, c4 = i & ((1 << shift) - 1);
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c = 0; c < kBlk / span; ++c) {
+            for (int c = 0; c < copies; ++c) {
               const int from = c * n_rows + r;
               const float4 v = *reinterpret_cast<const float4*>(stage + (((from << shift) + (c4 ^ (from & 7))) << 2));
               a.x += v.x;
