@@ -173,8 +173,7 @@ struct BrCfg {
   static constexpr int kStages = kFp8 ? 10 : 5;
   static constexpr int kSteps = kFp8 ? 4 : 8;      // MMA K steps of a 128-deep product
   static constexpr int kRowsPerStep = kFp8 ? 32 : 16;
-  static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk, false) : idesc_bf16(kBlk, kBlk, false);
-  static constexpr uint32_t kIdescQKHalf = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
+  static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
   static constexpr uint32_t kIdescPV = kFp8 ? idesc_e4m3(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
 };
 
@@ -240,30 +239,46 @@ __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) 
   return a;
 }
 
-// Softmax of kCols score columns of this thread's row: columns [col0, col0 + kCols) of a block, in
-// TMEM at tS + col0. kHalf: they are one half of the block, and P goes over them, dense. Otherwise
-// they are this copy's share of the block, and P goes over the first half of all 128 columns with
-// zeros for the other copies' shares. m / l: running maximum (log2 units) and sum; `pv_done` waits
-// until O holds all earlier blocks, before O is rescaled because the maximum grew (lazily: only
-// past the threshold).
-template <bool kFp8, int kCols, bool kHalf, typename Wait>
-__device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0, int limit, float sl2,
-                                              bool first, float& m, float& l, Wait&& pv_done) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// Softmax of kCols score columns of this thread's row, its copy's share of one half of a block:
+// columns [col0, col0 + kCols) of the block, col0 = 64 half + copy * kCols, in TMEM at tS + col0.
+// P goes over the half's scores, zeros in the other copies' shares. m / l: running maximum (log2
+// units) and sum; `pv_done` waits until O holds all earlier halves, before O is rescaled because
+// the maximum grew (lazily: only past the threshold).
+template <bool kFp8, int kCols, typename Wait>
+__device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half, int copy, int limit, float sl2,
+                                             bool first, float& m, float& l, Wait&& pv_done) {
   constexpr float kThreshold = kFp8 ? kThresholdF8 : kThresholdBf16;
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
-  constexpr int kChunks = kCols / 32;
+  const int col0 = 64 * half + copy * kCols;
   float s[kCols];
-  {
-    uint32_t r[kChunks][32];
+  if constexpr (kCols >= 32) {
+    uint32_t r[kCols / 32][32];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) tmem_ld32(tS + col0 + c * 32, r[c]);
+    for (int c = 0; c < kCols / 32; ++c) tmem_ld32(tS + col0 + c * 32, r[c]);
     tmem_wait_ld();
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
+    for (int c = 0; c < kCols / 32; ++c) {
       reg_fence32(r[c]);
 #pragma unroll
       for (int j = 0; j < 32; ++j) s[c * 32 + j] = __uint_as_float(r[c][j]);
     }
+  } else {
+    uint32_t r[16];
+    tmem_ld16(tS + col0, r);
+    tmem_wait_ld();
+    asm volatile("" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(r[j]);
   }
   // columns at or past `limit` (relative to the block) are hidden from this row
   int hide = __any_sync(0xffffffffu, limit < col0 + kCols) ? 1 : 0;
@@ -307,39 +322,11 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
   float sa, sb;
   f2_unpack(sum2, sa, sb);
   l += sa + sb;
-  pv_done();
-  if (any_need) {
-    tc_fence_after();
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t o[32];
-      tmem_ld32(tO + c * 32, o);
-      tmem_wait_ld();
-      reg_fence32(o);
-#pragma unroll
-      for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-      tmem_st32(tO + c * 32, o);
-    }
-  }
   // P: bf16, two columns a word; e4m3, four columns a word, the first terms in front of the second
   uint32_t w[32];
   if constexpr (!kFp8) {
-    if constexpr (kHalf) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) w[j] = pk[j];
-      tmem_st32(tS + col0, w);
-    } else {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {  // words [32 half, 32 half + 32): columns [64 half, ..)
-        const bool mine = (col0 >> 6) == half;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const bool here = mine && (kCols == 64 || ((col0 >> 5) & 1) == (j >> 4));
-          w[j] = here ? pk[j % (kCols / 2)] : 0u;
-        }
-        tmem_st32(tS + 32 * half, w);
-      }
-    }
+    for (int j = 0; j < 32; ++j) w[j] = kCols == 64 || j / (kCols / 2) == copy ? pk[j % (kCols / 2)] : 0u;
   } else {
     constexpr int kW = kCols / 4;
     uint32_t hi[kW], lo[kW];
@@ -351,22 +338,28 @@ __device__ __forceinline__ void softmax_block(uint32_t tS, uint32_t tO, int col0
       hi[j] = h0 | (h1 << 16);
       lo[j] = l0 | (l1 << 16);
     }
-    if constexpr (kHalf) {
 #pragma unroll
-      for (int j = 0; j < 32; ++j) w[j] = j < 16 ? hi[j % kW] : lo[j % kW];
-      tmem_st32(tS + col0, w);
-    } else {
-#pragma unroll
-      for (int term = 0; term < 2; ++term) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const bool here = (col0 >> 2) / kW == j / kW;
-          w[j] = here ? (term ? lo[j % kW] : hi[j % kW]) : 0u;
-        }
-        tmem_st32(tS + 32 * term, w);
-      }
+    for (int j = 0; j < 16; ++j) {
+      const bool mine = kCols == 64 || j / kW == copy;
+      w[j] = mine ? hi[j % kW] : 0u;
+      w[16 + j] = mine ? lo[j % kW] : 0u;
     }
   }
+  pv_done();
+  if (any_need) {
+    tc_fence_after();
+#pragma unroll 1
+    for (int c = 0; c < 4; ++c) {
+      uint32_t o[32];
+      tmem_ld32(tO + c * 32, o);
+      tmem_wait_ld();
+      reg_fence32(o);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+      tmem_st32(tO + c * 32, o);
+    }
+  }
+  tmem_st32(tS + 64 * half, w);
   tmem_wait_st();
 }
 
@@ -710,18 +703,15 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     int last_tile = 1;
     bool ok = true, was_solo = false;
     // the P V of this tile's last block, still to be issued
-    bool pend = false, pend_acc = false, pend_pair = false, pend_halves = false;
+    bool pend = false, pend_acc = false, pend_pair = false;
     int pend_slot = 0, pend_rows = 0;
     uint32_t pend_bar = 0u, pend_ph = 0u;
-    // Waits for P and issues the pending P V: of the whole block (half < 0), or of one half of its
-    // rows (P of the first half precedes that of the second).
+    // Waits for P of one half of the pending block and issues its P V.
     auto finish = [&](int half) {
-      const int which = half < 0 ? 0 : half;
-      const bool w = mbar_wait(p_bar + which * 8, (p_ph >> which) & 1u, abort_flag, p.err);
-      p_ph ^= 1u << which;
+      const bool w = mbar_wait(p_bar + half * 8, p_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
-      if (pend_rows < kBlk && half <= 0) {
+      if (pend_rows < kBlk && half == 0) {
         // rows past the sequence's end may hold anything, NaN among it, and the tensor core
         // multiplies them with P's zeros: clear them (the tile's load has completed; both warps
         // of a shared block write the same zeros)
@@ -734,50 +724,36 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      const uint32_t vlo = vlo0 + static_cast<uint32_t>(pend_slot) * kTileDesc;
-      if (half < 0) {
-        const uint32_t acc = pend_acc ? 1u : 0u;
+      const uint32_t vh = vlo0 + static_cast<uint32_t>(pend_slot) * kTileDesc + half * ((64 * 128) >> 4);
+      const uint32_t acc = pend_acc || half > 0 ? 1u : 0u;
+      const uint32_t tP = tS + 64u * half;
 #pragma unroll
-        for (int kk = 0; kk < Cfg::kSteps; ++kk) {
-          const uint64_t bd = sdesc_join(vlo + ((kk * Cfg::kRowsPerStep * 128) >> 4));
-          if constexpr (kFp8) {
-            mma_ts_f8(tO, tS + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-            mma_ts_f8(tO, tS + 32 + kk * 8, bd, Cfg::kIdescPV, 1u);
-          } else {
-            mma_ts(tO, tS + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-          }
+      for (int kk = 0; kk < Cfg::kSteps / 2; ++kk) {
+        const uint64_t bd = sdesc_join(vh + ((kk * Cfg::kRowsPerStep * 128) >> 4));
+        if constexpr (kFp8) {
+          mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
+          mma_ts_f8(tO, tP + 16 + kk * 8, bd, Cfg::kIdescPV, 1u);
+        } else {
+          mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
         }
-      } else {
-        const uint32_t acc = pend_acc || half > 0 ? 1u : 0u;
-        const uint32_t tP = tS + 64u * half, vh = vlo + half * ((64 * 128) >> 4);
-#pragma unroll
-        for (int kk = 0; kk < Cfg::kSteps / 2; ++kk) {
-          const uint64_t bd = sdesc_join(vh + ((kk * Cfg::kRowsPerStep * 128) >> 4));
-          if constexpr (kFp8) {
-            mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-            mma_ts_f8(tO, tP + 16 + kk * 8, bd, Cfg::kIdescPV, 1u);
-          } else {
-            mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-          }
-        }
-        tc_commit(pv_bar);
       }
+      tc_commit(pv_bar);
+      if (half == 1) p_ph ^= 1u;
     };
-    // Q K^T over a whole K tile (half < 0) or 64 of its rows.
+    // Q K^T over 64 rows of a K tile.
     auto scores = [&](uint32_t klo, int half) {
-      const uint32_t kh = klo + (half > 0 ? (64 * 128) >> 4 : 0), tD = tS + (half > 0 ? 64u : 0u);
-      const uint32_t idesc = half < 0 ? Cfg::kIdescQK : Cfg::kIdescQKHalf;
+      const uint32_t kh = klo + half * ((64 * 128) >> 4), tD = tS + 64u * half;
 #pragma unroll
       for (int kk = 0; kk < Cfg::kSteps; ++kk) {
         const uint32_t step = ((kk * 32 / 128) * kAtom + (kk * 32) % 128) >> 4;
         if constexpr (kFp8) {
-          mma_ss_f8(tD, sdesc_join(qlo + step), sdesc_join(kh + step), idesc, kk > 0 ? 1u : 0u);
-          mma_ss_f8(tD, sdesc_join(qlo + (kAtom >> 4) + step), sdesc_join(kh + step), idesc, 1u);
+          mma_ss_f8(tD, sdesc_join(qlo + step), sdesc_join(kh + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
+          mma_ss_f8(tD, sdesc_join(qlo + (kAtom >> 4) + step), sdesc_join(kh + step), Cfg::kIdescQK, 1u);
         } else {
-          mma_ss(tD, sdesc_join(qlo + step), sdesc_join(kh + step), idesc, kk > 0 ? 1u : 0u);
+          mma_ss(tD, sdesc_join(qlo + step), sdesc_join(kh + step), Cfg::kIdescQK, kk > 0 ? 1u : 0u);
         }
       }
-      tc_commit(s_bar + (half > 0 ? 8u : 0u));
+      tc_commit(s_bar + half * 8u);
     };
     // A slot is free after two arrivals: one per tile of a shared block, both from an only user.
     auto free_slot = [&](int slot, bool shared) {
@@ -788,8 +764,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     auto finish_item = [&]() {  // the last P V of an item
       pend = false;
       wait_v();
-      if (ok) finish(pend_halves ? 0 : -1);
-      if (ok && pend_halves) finish(1);
+      if (ok) finish(0);
+      if (ok) finish(1);
       if (!ok) return;
       tc_commit(o_bar);
       free_slot(pend_slot, pend_pair);
@@ -806,7 +782,6 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         if (!(ok = __all_sync(0xffffffffu, w))) break;
       }
       was_solo = !pair;
-      const bool halves = g.n_rows > 64;
       bool first = true;
       for (int j = 0; ok && j < g.blocks; ++j) {
         const int owner = pair ? mt : last_tile ^ 1;
@@ -824,27 +799,19 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           const bool w = mbar_wait(smem_u32(&sm.full[second][ring]), (phases >> ring) & 1u, abort_flag, p.err);
           if (!(ok = __all_sync(0xffffffffu, w))) break;
           const uint32_t klo = klo0 + static_cast<uint32_t>(ring) * kTileDesc;
-          if (!halves) {
-            if (!first) finish(-1);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            if (!first) finish(half);
             if (!ok) break;
             tc_fence_after();
-            scores(klo, -1);
-          } else {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              if (!first) finish(half);
-              if (!ok) break;
-              tc_fence_after();
-              scores(klo, half);
-            }
-            if (!ok) break;
+            scores(klo, half);
           }
+          if (!ok) break;
           if (!first) free_slot(pend_slot, pair);
           free_slot(ring, pair);
           pend = true;
           pend_acc = !first;
           pend_pair = pair;
-          pend_halves = halves;
           pend_slot = vs;
           pend_bar = smem_u32(&sm.full[second][vs]);
           pend_ph = (phases >> vs) & 1u;
@@ -877,7 +844,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t tS = tbase + static_cast<uint32_t>(t) * 128u + lane_off;
     const uint32_t tO = tbase + 256u + static_cast<uint32_t>(t) * 128u + lane_off;
-    uint32_t s_ph = 0u, o_ph = 0u, wg_ph = 0u, pv_ph = 0u;
+    uint32_t s_ph = 0u, o_ph = 0u, wg_ph = 0u;
     int last_tile = 1;
     bool ok = true;
     // all 128 threads of the tile meet (bounded, so a broken pipeline cannot hang it)
@@ -937,33 +904,28 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if constexpr (kFp8) sl2 *= __ldg(p.k_scale + it.head);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const bool halves = span == 128;  // blocks of whole tiles are taken in two halves
       const int limit = seq_length(p, it.at.b) - (p.causal ? p.rows - 1 - it.at.i : 0);
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
-      const int col0 = copy * span;
       for (int j = 0; ok && j < it.mine; ++j) {
         const int left = limit - (it.block0 + j * it.step) * kBlk;
-        const int n_steps = halves ? 2 : 1;
 #pragma unroll 1
-        for (int h = 0; h < n_steps; ++h) {
-          ok = mbar_wait(smem_u32(&sm.s_full[t][h]), (s_ph >> h) & 1u, abort_flag, p.err);
+        for (int h = 0; h < 2; ++h) {
+          ok = mbar_wait(smem_u32(&sm.s_full[t][h]), s_ph, abort_flag, p.err);
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
-          s_ph ^= 1u << h;
           tc_fence_after();
           const bool first = j == 0 && h == 0;
-          // whole blocks: the scores' barrier also covers the previous P V
           const auto pv_done = [&]() {
-            if (halves && !first) ok = mbar_wait(smem_u32(&sm.pv_done[t]), pv_ph ^ 1u, abort_flag, p.err);
+            if (!first) ok = mbar_wait(smem_u32(&sm.pv_done[t]), h ^ 1, abort_flag, p.err);
           };
           if (!warp_live) pv_done();
-          else if (halves) softmax_block<kFp8, 64, true>(tS, tO, 64 * h, left, sl2, first, m, l, pv_done);
-          else if (span == 64) softmax_block<kFp8, 64, false>(tS, tO, col0, left, sl2, first, m, l, pv_done);
-          else softmax_block<kFp8, 32, false>(tS, tO, col0, left, sl2, first, m, l, pv_done);
-          if (halves) pv_ph ^= 1u;
+          else if (span == 128) softmax_half<kFp8, 64>(tS, tO, h, 0, left, sl2, first, m, l, pv_done);
+          else if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, left, sl2, first, m, l, pv_done);
+          else softmax_half<kFp8, 16>(tS, tO, h, copy, left, sl2, first, m, l, pv_done);
           tc_fence_before();
           mbar_arrive(smem_u32(&sm.p_full[t][h]));
         }
+        s_ph ^= 1u;
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
