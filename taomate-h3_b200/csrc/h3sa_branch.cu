@@ -185,7 +185,7 @@ struct alignas(1024) BrSmem {
   uint8_t q[2][kQBytes];  // also the epilogue's staging
   uint8_t kv[Cfg::kStages][Cfg::kTile];
   Segment desc[kDescRing];
-  uint64_t full[2][Cfg::kStages], empty[Cfg::kStages];
+  uint64_t full[2][Cfg::kStages], empty[2][Cfg::kStages];  // [tile]; see the MMA warps
   uint64_t d_full[kDescRing], d_empty[kDescRing];
   uint64_t q_full[2], o_full[2], pv_done[2], wg[2];
   uint64_t s_full[2][2], p_full[2][2];  // [tile][half of a block]; whole blocks use the first
@@ -437,7 +437,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     for (int s = 0; s < kS; ++s) {
       mbar_init(smem_u32(&sm.full[0][s]), 1);
       mbar_init(smem_u32(&sm.full[1][s]), 1);
-      mbar_init(smem_u32(&sm.empty[s]), 2);
+      mbar_init(smem_u32(&sm.empty[0][s]), 1);
+      mbar_init(smem_u32(&sm.empty[1][s]), 1);
     }
     for (int s = 0; s < kDescRing; ++s) {
       mbar_init(smem_u32(&sm.d_full[s]), 1);
@@ -565,10 +566,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         step_item();
       }
     }
-    int ring = 0, ring_phase = 0;  // next tile of the K/V ring
+    int ring = 0;  // next tile of the K/V ring
     int issued = 0, last_tile = 1;
-    uint32_t on_tile1 = 0u;  // slots whose latest load signals tile 1's barrier
-    uint32_t full_ph[2] = {0u, 0u};
+    // A bit per slot: which tiles read its latest load (each releases it on a barrier of its own),
+    // the parities of those releases, whose full barrier it signals and that one's parity.
+    uint32_t used0 = 0u, used1 = 0u, free0 = 0u, free1 = 0u, on_tile1 = 0u, full0 = 0u, full1 = 0u;
     int ds = 0, ds_phase = 0;
     bool ok = true;
     while (ok) {
@@ -643,14 +645,24 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         }
         for (int j = 0; ok && j < 2 * n; ++j) {
           const int pg = __shfl_sync(0xffffffffu, page, j >> 1);
-          ok = mbar_wait(smem_u32(&sm.empty[ring]), ring_phase ^ 1, abort_flag, p.err);
+          const uint32_t bit = 1u << ring;
+          if (used0 & bit) {
+            ok = mbar_wait(smem_u32(&sm.empty[0][ring]), (free0 >> ring) & 1u, abort_flag, p.err);
+            free0 ^= bit;
+          }
+          if (ok && (used1 & bit)) {
+            ok = mbar_wait(smem_u32(&sm.empty[1][ring]), (free1 >> ring) & 1u, abort_flag, p.err);
+            free1 ^= bit;
+          }
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           // a block of one tile signals that tile's barrier, a shared one tile 0's
           if ((j & 1) == 0) last_tile = pair ? 1 : last_tile ^ 1;
           const int side = pair ? 0 : last_tile;
-          on_tile1 = (on_tile1 & ~(1u << ring)) | (static_cast<uint32_t>(side) << ring);
-          if (side) full_ph[1] ^= 1u << ring;
-          else full_ph[0] ^= 1u << ring;
+          used0 = pair || side == 0 ? used0 | bit : used0 & ~bit;
+          used1 = pair || side == 1 ? used1 | bit : used1 & ~bit;
+          on_tile1 = side ? on_tile1 | bit : on_tile1 & ~bit;
+          if (side) full1 ^= bit;
+          else full0 ^= bit;
           if (lane == 0) {
             const uint32_t bar = smem_u32(&sm.full[side][ring]);
             mbar_expect_tx(bar, Cfg::kTile);
@@ -660,10 +672,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
                           pg * kBlk, g.head);
           }
           ++issued;
-          if (++ring == kS) {
-            ring = 0;
-            ring_phase ^= 1;
-          }
+          if (++ring == kS) ring = 0;
         }
       }
     }
@@ -672,7 +681,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       for (int i = 0; i < min(issued, kS); ++i) {
         if (--ring < 0) ring = kS - 1;
         const int side = (on_tile1 >> ring) & 1u;
-        const uint32_t ph = (((side ? full_ph[1] : full_ph[0]) >> ring) & 1u) ^ 1u;
+        const uint32_t ph = (((side ? full1 : full0) >> ring) & 1u) ^ 1u;
         const unsigned long long t0 = global_ns();
         while (!mbar_try_wait(smem_u32(&sm.full[side][ring]), ph) && global_ns() - t0 < kWaitTimeoutNs) {
         }
@@ -703,7 +712,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     int last_tile = 1;
     bool ok = true, was_solo = false;
     // the P V of this tile's last block, still to be issued
-    bool pend = false, pend_acc = false, pend_pair = false;
+    bool pend = false, pend_acc = false;
     int pend_slot = 0, pend_rows = 0;
     uint32_t pend_bar = 0u, pend_ph = 0u;
     // Waits for P of one half of the pending block and issues its P V.
@@ -755,11 +764,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       }
       tc_commit(s_bar + half * 8u);
     };
-    // A slot is free after two arrivals: one per tile of a shared block, both from an only user.
-    auto free_slot = [&](int slot, bool shared) {
-      tc_commit(smem_u32(&sm.empty[slot]));
-      if (!shared) tc_commit(smem_u32(&sm.empty[slot]));
-    };
+    const auto free_slot = [&](int slot) { tc_commit(smem_u32(&sm.empty[mt][slot])); };
     auto wait_v = [&]() { ok = __all_sync(0xffffffffu, mbar_wait(pend_bar, pend_ph, abort_flag, p.err)); };
     auto finish_item = [&]() {  // the last P V of an item
       pend = false;
@@ -768,7 +773,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (ok) finish(1);
       if (!ok) return;
       tc_commit(o_bar);
-      free_slot(pend_slot, pend_pair);
+      free_slot(pend_slot);
     };
     Segment g;
     while (ok && next_segment(g)) {
@@ -796,22 +801,23 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             wait_v();
           }
           if (!ok) break;
-          const bool w = mbar_wait(smem_u32(&sm.full[second][ring]), (phases >> ring) & 1u, abort_flag, p.err);
-          if (!(ok = __all_sync(0xffffffffu, w))) break;
           const uint32_t klo = klo0 + static_cast<uint32_t>(ring) * kTileDesc;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             if (!first) finish(half);
             if (!ok) break;
+            if (half == 0) {
+              const bool w = mbar_wait(smem_u32(&sm.full[second][ring]), (phases >> ring) & 1u, abort_flag, p.err);
+              if (!(ok = __all_sync(0xffffffffu, w))) break;
+            }
             tc_fence_after();
             scores(klo, half);
           }
           if (!ok) break;
-          if (!first) free_slot(pend_slot, pair);
-          free_slot(ring, pair);
+          if (!first) free_slot(pend_slot);
+          free_slot(ring);
           pend = true;
           pend_acc = !first;
-          pend_pair = pair;
           pend_slot = vs;
           pend_bar = smem_u32(&sm.full[second][vs]);
           pend_ph = (phases >> vs) & 1u;
