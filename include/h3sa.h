@@ -518,8 +518,8 @@ H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t wi
 /* Attention of all branches' new rows, the shared history read once for all of them. query bf16
  * [batch, rows, heads, 128] with the given element strides (multiples of 8); out bf16
  * [batch, rows, heads, 128] contiguous; lse fp32 [batch, rows, heads] (natural log of the sum of
- * exponentials, -inf for a row that sees nothing) or NULL. Pools [kv_heads, pool_pages * 128, 128]
- * bf16, or e4m3 with k_scale / v_scale fp32 [kv_heads]; query head h reads KV head
+ * exponentials, -inf for a row that sees nothing) or NULL. Pools [kv_heads, pool_pages * 128, 128],
+ * 32-byte aligned, bf16, or e4m3 with k_scale / v_scale fp32 [kv_heads]; query head h reads KV head
  * h / (heads / kv_heads). Row i of sequence b sees the keys j < lengths[b], causal != 0: j <
  * lengths[b] - (rows - 1 - i), the new rows being the sequence's last ones. The first shared_rows
  * rows (whole pages) are the same pages in the table rows of all sequences at least that long;

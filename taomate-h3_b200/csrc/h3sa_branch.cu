@@ -41,20 +41,14 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <climits>
 #include <cstring>
 #include <mutex>
-#include <type_traits>
 
-#include "h3sa_host.h"
-#include "h3sa_ptx.cuh"
+#include "h3sa_branch.cuh"
 
 namespace h3sa {
 namespace {
 
-constexpr int kD = 128;
-constexpr int kBlk = 128;        // KV rows of a block (a page)
-constexpr int kSpan = 256;       // query rows of an item: two tiles
 constexpr int kBrThreads = 384;
 constexpr int kBrRegsControl = 88;
 constexpr int kBrRegsSoftmax = 208;
@@ -66,92 +60,6 @@ constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
 constexpr float kBoostF8 = 6.0f;
 constexpr float kThresholdF8 = 2.0f;
 constexpr float kThresholdBf16 = 8.0f;
-
-struct BranchParams {
-  const __nv_bfloat16* q;
-  long long q_sb, q_sn, q_sh;  // element strides of [batch, rows, heads, 128]
-  __nv_bfloat16* out;          // contiguous [batch, rows, heads, 128]
-  float* lse;                  // contiguous [batch, rows, heads] or null
-  const int* table;            // [batch, width]
-  const int* lengths;          // [batch]
-  int width, batch, rows, heads, kv_heads, group;
-  int shared;                  // leading blocks shared by all sequences
-  int causal, joint;
-  int pool_pages;
-  float scale_log2;
-  const float* k_scale;        // e4m3: [kv_heads]
-  const float* v_scale;
-  int shared_tiles;            // items over the shared blocks per KV head (split form)
-  int own_tiles;               // items per KV head and sequence
-  int shared_slot_rows, own_slot_rows;
-  long long own_row0;          // first workspace row of the own items' slots
-  float* part_o;               // [workspace rows, 128]
-  float2* part_ml;             // [workspace rows]: (maximum, sum)
-  int* plan;                   // the schedule, for the merge: [3 + batch]
-  int ctas;
-  int* err;
-};
-
-// ------------------------------------------------------------------------------ the schedule
-// Both kernels compute it from the lengths, one warp at a time.
-
-__device__ __forceinline__ int seq_length(const BranchParams& p, int b) {
-  const int n = __ldg(p.lengths + b);
-  return max(0, min(n, p.width * kBlk));
-}
-
-// blocks [lo, hi) that the rows of tile `t` of a sequence of length `len` see outside the shared
-// items
-__device__ __forceinline__ int own_lo(const BranchParams& p) { return p.joint ? 0 : p.shared; }
-__device__ __forceinline__ int own_units(const BranchParams& p, int len, int t) {
-  int limit = len;
-  if (p.causal) {
-    const int last = min((t + 1) * kSpan, p.rows * p.group) - 1;
-    limit -= p.rows - 1 - last / p.group;
-  }
-  return max(0, (limit + kBlk - 1) / kBlk - own_lo(p));
-}
-// In the line of units every item with work counts kItemPad more than its blocks: loading its
-// query rows and writing its O out takes about as long.
-constexpr int kItemPad = 2;
-__device__ __forceinline__ int weight_of(int units) { return units > 0 ? units + kItemPad : 0; }
-__device__ __forceinline__ int own_weight_all(const BranchParams& p, int len) {
-  if (!p.causal) return weight_of(own_units(p, len, 0)) * p.own_tiles;
-  int n = 0;
-  for (int t = 0; t < p.own_tiles; ++t) n += weight_of(own_units(p, len, t));
-  return n;
-}
-
-struct Plan {
-  int shared_units;  // blocks of one shared item
-  int head_weight;   // one KV head's part of the line
-  int cut;           // one CTA's part
-  int longest;       // sequence whose table row gives the shared pages
-  int max_len;
-};
-
-__device__ __forceinline__ Plan make_plan(const BranchParams& p, int lane) {
-  int own = 0, best = -1, at = 0;
-  for (int b = lane; b < p.batch; b += 32) {
-    const int len = seq_length(p, b);
-    own += own_weight_all(p, len);
-    if (len > best) {
-      best = len;
-      at = b;
-    }
-  }
-  own = __reduce_add_sync(0xffffffffu, own);
-  const int top = __reduce_max_sync(0xffffffffu, best);
-  at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
-  Plan pl;
-  pl.max_len = top;
-  pl.longest = at;
-  pl.shared_units = p.joint ? 0 : min(p.shared, (top + kBlk - 1) / kBlk);
-  pl.head_weight = p.shared_tiles * weight_of(pl.shared_units) + own;
-  const int all = pl.head_weight * p.kv_heads;
-  pl.cut = max(1, (all + p.ctas - 1) / p.ctas);
-  return pl;
-}
 
 // One item segment of a CTA, as warp 0 publishes it.
 struct Segment {
@@ -200,19 +108,9 @@ constexpr size_t br_smem_bytes() {
 static_assert(br_smem_bytes<false>() <= 232448 && br_smem_bytes<true>() <= 232448,
               "branch attention needs more than 227 KB");
 
-__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
 __device__ __forceinline__ uint32_t e4m3x2_of(uint32_t h2) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h2));
-  return r;
-}
-__device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t e) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(static_cast<uint16_t>(e)));
   return r;
 }
 // Two values below 448 as the sum of two e4m3 terms each, through f16 (11 bits, so nothing that
@@ -224,19 +122,6 @@ __device__ __forceinline__ void split_e4m3x2(float a, float b, uint32_t& hi, uin
   uint32_t rest;
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(h), "r"(back));
   lo = e4m3x2_of(rest);
-}
-
-// The address of a stacked row (b, i, g) of KV head `head` in a strided [batch, rows, heads, 128].
-struct RowAt {
-  int b, i, h;
-};
-__device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) {
-  const int bi = r / p.group;
-  RowAt a;
-  a.h = head * p.group + (r - bi * p.group);
-  a.b = bi / p.rows;
-  a.i = bi - a.b * p.rows;
-  return a;
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -385,10 +270,8 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
 #pragma unroll
     for (int i = 0; i < 64; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
     top = max(top >> 16, top & 0xffffu);
-    // 2^k with the largest * 2^k in [128, 256); tiny rows keep their products in fp32's range
-    const int e = static_cast<int>(top >> 7) - 127;
-    const int k = max(-120, min(7 - e, 120));
-    const float up = __uint_as_float(static_cast<uint32_t>(k + 127) << 23);
+    const int k = row_exponent(top);
+    const float up = exp2_int(k);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {  // 16 columns a chunk
       if ((c & (copies - 1)) != copy) continue;
@@ -411,7 +294,7 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
       }
     }
     // a row with an infinity or NaN gets NaN scores, as its products have
-    return top >= 0x7f80u ? __int_as_float(0x7fffffff) : __uint_as_float(static_cast<uint32_t>(127 - k) << 23);
+    return top >= 0x7f80u ? __int_as_float(0x7fffffff) : exp2_int(-k);
   }
 }
 
@@ -430,7 +313,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Plan pl;
-  if (warp == 0) pl = make_plan(p, lane);  // under way while the others set up
+  const Line& ln = p.tensor;
+  if (warp == 0) pl = make_plan(p, ln, lane);  // under way while the others set up
   if (threadIdx.x == 64) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -487,83 +371,23 @@ __global__ void __launch_bounds__(kBrThreads, 1)
   if (warp == 0) {
     // ================================================================ schedule and TMA
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
-    for (int b = lane; b < p.batch; b += 32) {
-      const int n = __ldg(p.lengths + b);
-      if ((n < 0 || n > p.width * kBlk) && p.err) atomicOr(p.err, kErrBadIndex);
-    }
+    flag_lengths(p, lane);
     const int all = pl.head_weight * p.kv_heads;
     int u = min(all, static_cast<int>(blockIdx.x) * pl.cut);
     int u_end = min(all, u + pl.cut);
-    const int shared_weight = weight_of(pl.shared_units);
-    // position: head, then a shared tile (b < 0) or (b, t), then the offset in the item
-    int head = 0, b = -1, t = 0, off = 0;
-    if (u < u_end) {
-      head = u / pl.head_weight;
-      int x = u - head * pl.head_weight;
-      if (x < p.shared_tiles * shared_weight) {
-        t = x / shared_weight;
-        off = x - t * shared_weight;
-      } else {
-        x -= p.shared_tiles * shared_weight;
-        for (int b0 = 0; b0 < p.batch; b0 += 32) {
-          const int bb = b0 + lane;
-          const int n = bb < p.batch ? own_weight_all(p, seq_length(p, bb)) : 0;
-          int cum = n;
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, cum, d);
-            if (lane >= d) cum += v;
-          }
-          const uint32_t past = __ballot_sync(0xffffffffu, cum > x);
-          if (past) {
-            const int f = __ffs(past) - 1;
-            b = b0 + f;
-            x -= __shfl_sync(0xffffffffu, cum - n, f);
-            break;
-          }
-          x -= __shfl_sync(0xffffffffu, cum, 31);
-        }
-        const int len = seq_length(p, b);
-        for (int w; x >= (w = weight_of(own_units(p, len, t))); ++t) x -= w;
-        off = x;
-      }
-    }
-    const auto item_units = [&]() { return b < 0 ? pl.shared_units : own_units(p, seq_length(p, b), t); };
-    const auto step_item = [&]() {  // to the next item that has units
-      bool found = false;
-      if (b < 0) {
-        found = ++t < p.shared_tiles && pl.shared_units > 0;
-        if (!found) {
-          b = 0;
-          t = -1;
-        }
-      }
-      while (!found) {
-        if (++t >= p.own_tiles) {
-          t = 0;
-          if (++b >= p.batch) {
-            ++head;
-            b = pl.shared_units > 0 ? -1 : 0;
-          }
-        }
-        found = b < 0 || own_units(p, seq_length(p, b), t) > 0;
-      }
-    };
+    Place at = {0, -1, 0, 0};
+    if (u < u_end) at = locate(p, ln, pl, u, lane);
     // A range that starts inside an item and goes on past it takes that rest last. All CTAs then
     // walk their items from the first block on, and those that read the same keys read them at
     // about the same time, from L2.
-    int later = 0, later_head = 0, later_b = 0, later_t = 0, later_off = 0;
-    if (u < u_end && off > 0) {
-      const int rest = weight_of(item_units()) - off;
+    int later = 0;
+    Place later_at = at;
+    if (u < u_end && at.off > 0) {
+      const int rest = weight_of(ln, place_units(p, ln, pl, at)) - at.off;
       if (rest < u_end - u) {
         later = rest;
-        later_head = head;
-        later_b = b;
-        later_t = t;
-        later_off = off;
         u += rest;
-        off = 0;
-        step_item();
+        step_item(p, ln, pl, at);
       }
     }
     int ring = 0;  // next tile of the K/V ring
@@ -579,41 +403,41 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       memset(&g, 0, sizeof(g));
       int seq = 0;
       while (u < u_end && !g.live) {
-        const int units = item_units(), part = min(weight_of(units) - off, u_end - u);
-        const int blocks = min(units, off + part) - off;
+        const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
+        const int blocks = min(units, at.off + part) - at.off;
         if (blocks > 0) {
-          if (b < 0) {
+          long long item, row0;
+          int slot_rows;
+          if (at.b < 0) {
             seq = pl.longest;
-            g.row0 = t * kSpan;
+            g.row0 = at.t * kSpan;
             g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
-            g.block0 = off;
+            g.block0 = at.off;
             g.kv_end = pl.max_len;
-            for (int k = 0; k < 2; ++k)
-            g.slot_row[k] = (static_cast<long long>(head * p.shared_tiles + t + blockIdx.x) * 2 + k) *
-                            p.shared_slot_rows;
+            item = at.head * ln.shared_tiles + at.t;
+            row0 = 0;
+            slot_rows = p.shared_slot_rows;
           } else {
-            seq = b;
-            g.row0 = b * p.rows * p.group + t * kSpan;
-            g.n_rows = min(kSpan, p.rows * p.group - t * kSpan);
-            g.block0 = own_lo(p) + off;
-            g.kv_end = seq_length(p, b);
-            const long long item = (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t;
-            for (int k = 0; k < 2; ++k)
-            g.slot_row[k] = p.own_row0 + ((item + blockIdx.x) * 2 + k) * p.own_slot_rows;
+            seq = at.b;
+            g.row0 = at.b * p.rows * p.group + at.t * kSpan;
+            g.n_rows = min(kSpan, p.rows * p.group - at.t * kSpan);
+            g.block0 = own_lo(p) / kBlk + at.off;
+            g.kv_end = seq_length(p, at.b);
+            item = (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
+            row0 = p.own_row0;
+            slot_rows = p.own_slot_rows;
           }
+          for (int k = 0; k < 2; ++k) g.slot_row[k] = row0 + ((item + blockIdx.x) * 2 + k) * slot_rows;
           g.live = 1;
-          g.head = head;
+          g.head = at.head;
           g.blocks = blocks;
-          g.direct = pl.shared_units == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
+          g.direct = pl.shared_blocks == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
         }
         u += part;
-        off = 0;
-        if (u < u_end) step_item();
-        if (u >= u_end && later > 0) {
-          head = later_head;
-          b = later_b;
-          t = later_t;
-          off = later_off;
+        if (u < u_end) {
+          step_item(p, ln, pl, at);
+        } else if (later > 0) {
+          at = later_at;
           u_end = u + later;
           later = 0;
         }
@@ -1069,30 +893,14 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     }
   } else {
     // ================================================================ warp 3 of the first CTA
-    // writes the schedule down for the merge: the units of a shared item, a head's and a CTA's part
-    // of the line, and what lies in front of each sequence's own items
+    // writes the schedule down for the merge
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
     if (blockIdx.x == 0) {
-      pl = make_plan(p, lane);
-      if (lane == 0) {
-        p.plan[0] = pl.shared_units;
-        p.plan[1] = pl.head_weight;
-        p.plan[2] = pl.cut;
-      }
-      int before = 0;
-      for (int b0 = 0; b0 < p.batch; b0 += 32) {
-        const int b = b0 + lane;
-        const int n = b < p.batch ? own_weight_all(p, seq_length(p, b)) : 0;
-        int cum = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, cum, d);
-          if (lane >= d) cum += v;
-        }
-        if (b < p.batch) p.plan[3 + b] = before + cum - n;
-        before += __shfl_sync(0xffffffffu, cum, 31);
-      }
+      pl = make_plan(p, ln, lane);
+      write_plan(p, ln, pl, p.plan, lane);
     }
+    // The warp line's kernel may still be running: what follows this one needs both.
+    if (p.warp.own_tiles > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   }
 
   tc_fence_before();
@@ -1117,9 +925,10 @@ struct Pieces {  // of one row in one item: workspace rows first + j * stride, j
   long long first;
 };
 __device__ __forceinline__ Pieces pieces_of(int cut, int u0, int units, int n_rows, int r, long long item,
-                                            long long row0, int slot_rows) {
+                                            long long row0, int slot_rows, bool warps) {
   if (units == 0) return Pieces{0, 0, 0};
   const int c_lo = u0 / cut, n_cta = (u0 + units - 1) / cut - c_lo + 1;
+  if (warps) return Pieces{n_cta, slot_rows, row0 + (item + c_lo) * slot_rows + r};
   const long long first = row0 + (item + c_lo) * 2 * slot_rows;
   // items of both tiles: the slot of the row's tile in each CTA; else the slots of both
   if (n_rows > kBlk) return Pieces{n_cta, 2 * slot_rows, first + (r / kBlk) * slot_rows + r % kBlk};
@@ -1187,8 +996,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int team = warp / kTeam, part = warp % kTeam;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int shared_units = kJoint ? 0 : __ldcg(p.plan), head_weight = __ldcg(p.plan + 1), cut = __ldcg(p.plan + 2);
-  const int shared_weight = weight_of(shared_units);
+  // what each line wrote down; own items and shared items each belong to one of them
+  const bool shared_by_warps = p.warp.shared_tiles > 0, own_by_warps = !kJoint && p.warp.own_tiles > 0;
+  const Line& ls = shared_by_warps ? p.warp : p.tensor;
+  const Line& lo = own_by_warps ? p.warp : p.tensor;
+  const int* const ps = p.plan + (shared_by_warps ? 3 + p.batch : 0);
+  const int* const po = p.plan + (own_by_warps ? 3 + p.batch : 0);
+  const int shared_blocks = kJoint ? 0 : __ldcg(po);
+  const int cut_s = __ldcg(ps + 2), cut_o = __ldcg(po + 2);
+  const int shared_units = shared_blocks * (kBlk / ls.unit), shared_weight = weight_of(ls, shared_units);
   const int own_all = p.rows * p.group;
   // split form: stacked rows of all branches, one a team, head by head; joint form: kRows rows of
   // an item a warp
@@ -1201,35 +1017,36 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
     const int row = static_cast<int>(id - static_cast<long long>(head) * stacked);
     b = row / own_all;
     r = row - b * own_all;
-    t = r / kSpan;
+    t = r / lo.span;
   } else {
     constexpr int kGroups = kSpan / (kRows * kMergeWarps);
     const int item = blockIdx.x / kGroups;
-    t = item % p.own_tiles;
-    b = item / p.own_tiles % p.batch;
-    head = item / p.own_tiles / p.batch;
+    t = item % lo.own_tiles;
+    b = item / lo.own_tiles % p.batch;
+    head = item / lo.own_tiles / p.batch;
     r = t * kSpan + (static_cast<int>(blockIdx.x % kGroups) * kMergeWarps + warp) * kRows;
     if (r >= min(own_all, (t + 1) * kSpan)) return;
   }
   const int len = seq_length(p, b);
-  int u0 = head * head_weight + p.shared_tiles * shared_weight + __ldcg(p.plan + 3 + b);
-  for (int k = 0; k < t; ++k) u0 += weight_of(own_units(p, len, k));
-  const int units = own_units(p, len, t);
-  const int n_rows = min(kSpan, own_all - t * kSpan);
-  if (shared_units == 0 && units > 0 && u0 / cut == (u0 + units - 1) / cut && (n_rows > kBlk || units == 1))
+  int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * (kBlk / lo.unit)) + __ldcg(po + 3 + b);
+  for (int k = 0; k < t; ++k) u0 += weight_of(lo, own_units(p, lo, len, k));
+  const int units = own_units(p, lo, len, t);
+  const int n_rows = min(lo.span, own_all - t * lo.span);
+  if (shared_blocks == 0 && units > 0 && u0 / cut_o == (u0 + units - 1) / cut_o &&
+      (own_by_warps || n_rows > kBlk || units == 1))
     return;  // written by the segment itself
   Pieces sh[kRows], own[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
     // rows past the item read its last row again and write nothing
-    const int rk = min(r + k, t * kSpan + n_rows - 1);
-    const int row = b * own_all + rk, t_sh = row / kSpan;
-    sh[k] = pieces_of(cut, head * head_weight + t_sh * shared_weight, shared_units,
-                      min(kSpan, p.batch * own_all - t_sh * kSpan), row % kSpan,
-                      head * p.shared_tiles + t_sh, 0, p.shared_slot_rows);
-    own[k] = pieces_of(cut, u0, units, n_rows, rk - t * kSpan,
-                       (static_cast<long long>(head) * p.batch + b) * p.own_tiles + t, p.own_row0,
-                       p.own_slot_rows);
+    const int rk = min(r + k, t * lo.span + n_rows - 1);
+    const int row = b * own_all + rk, t_sh = row / ls.span;
+    sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, shared_units,
+                      min(ls.span, p.batch * own_all - t_sh * ls.span), row % ls.span,
+                      head * ls.shared_tiles + t_sh, 0, p.shared_slot_rows, shared_by_warps);
+    own[k] = pieces_of(cut_o, u0, units, n_rows, rk - t * lo.span,
+                       (static_cast<long long>(head) * p.batch + b) * lo.own_tiles + t, p.own_row0,
+                       p.own_slot_rows, own_by_warps);
   }
   float m[kRows], sum[kRows];
   float4 acc[kRows];
@@ -1270,7 +1087,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
   }
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    if (r + k >= t * kSpan + n_rows) break;
+    if (r + k >= t * lo.span + n_rows) break;
     float scale = sum[k] == 0.f ? 0.f : 1.0f / sum[k];
     if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
     const int i = (r + k) / p.group;
@@ -1282,7 +1099,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
 }
 
 struct Shape {
-  int shared_tiles, own_tiles, shared_slot_rows, own_slot_rows, joint, ctas;
+  Line tensor, warp;
+  int shared_slot_rows, own_slot_rows, joint;
   long long own_row0, rows;  // workspace rows
   long long bytes;
 };
@@ -1304,22 +1122,36 @@ int sm_count() {
 // nothing to merge.
 constexpr int kJointRows = 2 * kSpan;
 
+// Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
+// tensor line passes a dozen barriers; what it costs is that more rows mean reading K and V again.
+constexpr int kWarpOwnRows = 64;
+constexpr int kWarpSharedRows = 16;
+
 Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   Shape s;
+  memset(&s, 0, sizeof(s));
   const long long own = static_cast<long long>(rows) * group;
   const long long all = own * batch;
-  s.ctas = sm_count();
+  const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
   s.joint = own >= kJointRows ? 1 : 0;
-  s.own_tiles = static_cast<int>((own + kSpan - 1) / kSpan);
-  s.shared_tiles = s.joint || shared == 0 ? 0 : static_cast<int>((all + kSpan - 1) / kSpan);
-  s.own_slot_rows = static_cast<int>(own < kBlk ? own : kBlk);
-  s.shared_slot_rows = static_cast<int>(all < kBlk ? all : kBlk);
-  s.own_row0 = s.shared_tiles == 0
-                   ? 0
-                   : (static_cast<long long>(kv_heads) * s.shared_tiles + s.ctas) * 2 * s.shared_slot_rows;
+  s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count()};
+  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * 8};
+  Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;
+  lo.own_tiles = tiles(own, lo.span);
+  s.own_slot_rows = static_cast<int>(own < lo.span ? own : lo.span);
+  if (&lo == &s.tensor && own > kBlk) s.own_slot_rows = kBlk;
+  const int own_slots = &lo == &s.warp ? 1 : 2;
+  if (!s.joint && shared > 0) {
+    Line& ls = all <= kWarpSharedRows ? s.warp : s.tensor;
+    ls.shared_tiles = tiles(all, ls.span);
+    s.shared_slot_rows = static_cast<int>(all < ls.span ? all : ls.span);
+    if (&ls == &s.tensor && all > kBlk) s.shared_slot_rows = kBlk;
+    s.own_row0 = (static_cast<long long>(kv_heads) * ls.shared_tiles + ls.workers) * (&ls == &s.warp ? 1 : 2) *
+                 s.shared_slot_rows;
+  }
   s.rows = s.own_row0 +
-           (static_cast<long long>(kv_heads) * batch * s.own_tiles + s.ctas) * 2 * s.own_slot_rows;
-  s.bytes = s.rows * (kD * 4 + 8) + (3ll + batch) * 4;
+           (static_cast<long long>(kv_heads) * batch * lo.own_tiles + lo.workers) * own_slots * s.own_slot_rows;
+  s.bytes = s.rows * (kD * 4 + 8) + 2 * (3ll + batch) * 4;
   return s;
 }
 
@@ -1349,7 +1181,7 @@ int configure() {
 }
 
 template <bool kFp8>
-int launch(const BranchParams& p, const void* key_pool, const void* value_pool, cudaStream_t stream) {
+int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg, bool along) {
   using Cfg = BrCfg<kFp8>;
   int rc = configure<kFp8>();
   if (rc) return rc;
@@ -1359,28 +1191,46 @@ int launch(const BranchParams& p, const void* key_pool, const void* value_pool, 
   const uint64_t dims[3] = {kD, pool_rows, static_cast<uint64_t>(p.kv_heads)};
   const uint64_t strides[2] = {static_cast<uint64_t>(kD) * Cfg::kElem, pool_rows * kD * Cfg::kElem};
   const uint32_t box[3] = {128 / Cfg::kElem, static_cast<uint32_t>(kBlk), 1};
-  if ((rc = encode_tiled_3d(&tmK, dt, key_pool, dims, strides, box))) return rc;
-  if ((rc = encode_tiled_3d(&tmV, dt, value_pool, dims, strides, box))) return rc;
-  branch_attn_kernel<kFp8><<<p.ctas, kBrThreads, br_smem_bytes<kFp8>(), stream>>>(tmK, tmV, p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error("branch_attn_kernel launch", e);
-  // The merge is launched along with it and waits on the device for its end.
-  // Four warps share a row where rows are few: its pieces are read one latency after another.
-  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
-  const bool team = !p.joint && p.shared_tiles > 0 && stacked <= 16ll * p.ctas;
-  const long long blocks =
-      p.joint ? static_cast<long long>(p.kv_heads) * p.batch * p.own_tiles * (kSpan / (kJointWarpRows * kMergeWarps))
-      : team  ? stacked
-              : (stacked + kMergeWarps - 1) / kMergeWarps;
+  if ((rc = encode_tiled_3d(&tmK, dt, p.key_pool, dims, strides, box))) return rc;
+  if ((rc = encode_tiled_3d(&tmV, dt, p.value_pool, dims, strides, box))) return rc;
+  cfg.gridDim = dim3(p.tensor.workers);
+  cfg.blockDim = dim3(kBrThreads);
+  cfg.dynamicSmemBytes = br_smem_bytes<kFp8>();
+  cfg.numAttrs = along ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_attn_kernel<kFp8>, tmK, tmV, p);
+  return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_attn_kernel launch", e);
+}
+
+template <bool kFp8>
+int launch(const BranchParams& p, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = stream;
+  // Each kernel is launched along with the one before it and waits for it on the device.
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
+  const bool by_warps = p.warp.own_tiles > 0;
+  if (by_warps) {
+    e = launch_branch_rows(p, kFp8, stream);
+    if (e != cudaSuccess) return set_cuda_error("branch_rows_kernel launch", e);
+  }
+  if (p.tensor.own_tiles > 0 || p.tensor.shared_tiles > 0) {
+    const int rc = launch_tensor<kFp8>(p, cfg, by_warps);
+    if (rc) return rc;
+  }
+  // Four warps share a row where rows are few: its pieces are read one latency after another.
+  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
+  const bool team = !p.joint && p.shared > 0 && stacked <= 16ll * p.tensor.workers;
+  const long long blocks =
+      p.joint ? static_cast<long long>(p.kv_heads) * p.batch * p.tensor.own_tiles * (kSpan / (kJointWarpRows * kMergeWarps))
+      : team  ? stacked
+              : (stacked + kMergeWarps - 1) / kMergeWarps;
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(32 * kMergeWarps);
+  cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
   e = p.joint ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, true, 1>, p)
       : team  ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, kMergeWarps>, p)
@@ -1430,19 +1280,23 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
   if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
-  if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
+  if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 32) || !aligned(value_pool, 32) ||
       !aligned(workspace, 16) || stride_sequence % 8 || stride_row % 8 || stride_head % 8)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned");
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned, pools 32-byte");
   const int group = heads / kv_heads;
   const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
-  const int64_t tiles = (static_cast<int64_t>(rows) * group + kSpan - 1) / kSpan;
-  if (stacked > INT32_MAX / 2 ||
-      kv_heads * (((stacked + kSpan - 1) / kSpan) * (shared_rows / kBlk + kItemPad) +
-                  batch * tiles * (width + kItemPad)) > INT32_MAX / 2 ||
-      static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
+  if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
+    return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d is too large",
+                     batch, rows, heads);
+  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
+  const auto line_units = [&](const Line& ln) {
+    const int64_t blocks = kBlk / ln.unit;
+    return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks + ln.pad) +
+                       static_cast<int64_t>(batch) * ln.own_tiles * (width * blocks + ln.pad));
+  };
+  if (line_units(s.tensor) > INT32_MAX / 2 || line_units(s.warp) > INT32_MAX / 2)
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d over %d "
                      "pages exceeds the work index", batch, rows, heads, width);
-  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
   if (workspace_bytes < s.bytes)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: workspace of %lld bytes, %lld needed",
                      static_cast<long long>(workspace_bytes), s.bytes);
@@ -1469,18 +1323,19 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.k_scale = k_scale;
   p.v_scale = v_scale;
-  p.shared_tiles = s.shared_tiles;
-  p.own_tiles = s.own_tiles;
+  p.key_pool = key_pool;
+  p.value_pool = value_pool;
+  p.tensor = s.tensor;
+  p.warp = s.warp;
   p.shared_slot_rows = s.shared_slot_rows;
   p.own_slot_rows = s.own_slot_rows;
   p.own_row0 = s.own_row0;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + s.rows * kD);
   p.plan = reinterpret_cast<int*>(p.part_ml + s.rows);
-  p.ctas = s.ctas;
   p.err = device_error;
-  return e4m3 ? launch<true>(p, key_pool, value_pool, static_cast<cudaStream_t>(stream))
-              : launch<false>(p, key_pool, value_pool, static_cast<cudaStream_t>(stream));
+  return e4m3 ? launch<true>(p, static_cast<cudaStream_t>(stream))
+              : launch<false>(p, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
