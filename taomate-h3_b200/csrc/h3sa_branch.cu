@@ -298,6 +298,16 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
   }
 }
 
+// A tile load that marks its lines as the first to go from L2.
+__device__ __forceinline__ void tma_load_3d_once(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
+                                                 int c2, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+      : "memory");
+}
+
 template <bool kFp8>
 __global__ void __launch_bounds__(kBrThreads, 1)
     branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -390,6 +400,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         step_item(p, ln, pl, at);
       }
     }
+    // Keys that one item alone reads would push everything else out of L2, the kernel's own code
+    // and queries among it, whose next reads then queue behind them for memory.
+    const bool once = ln.shared_tiles <= 1 && ln.own_tiles <= 1;
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
     int ring = 0;  // next tile of the K/V ring
     int issued = 0, last_tile = 1;
     // A bit per slot: which tiles read its latest load (each releases it on a barrier of its own),
@@ -491,9 +506,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             const uint32_t bar = smem_u32(&sm.full[side][ring]);
             mbar_expect_tx(bar, Cfg::kTile);
             const CUtensorMap* map = (j & 1) ? &tmV : &tmK;
-            for (int a = 0; a < Cfg::kTile / kAtom; ++a)
-              tma_load_3d(smem_u32(sm.kv[ring]) + a * kAtom, map, bar, a * (128 / Cfg::kElem),
-                          pg * kBlk, g.head);
+            for (int a = 0; a < Cfg::kTile / kAtom; ++a) {
+              const uint32_t dst = smem_u32(sm.kv[ring]) + a * kAtom;
+              if (once) tma_load_3d_once(dst, map, bar, a * (128 / Cfg::kElem), pg * kBlk, g.head, policy);
+              else tma_load_3d(dst, map, bar, a * (128 / Cfg::kElem), pg * kBlk, g.head);
+            }
           }
           ++issued;
           if (++ring == kS) ring = 0;
