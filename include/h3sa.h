@@ -528,7 +528,7 @@ H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t wi
  * [0, width * 128] is clamped with H3SA_DEVERR_BAD_INDEX; a page outside the pool gives
  * H3SA_DEVERR_BAD_PAGE and invalid outputs. Results do not depend on timing. */
 H3SA_API int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
-                                              int32_t kv_heads, int32_t shared_rows);
+                                              int32_t kv_heads, int32_t shared_rows, int32_t e4m3);
 H3SA_API int h3sa_shared_prefix_attention(
     const void* query, int64_t stride_sequence, int64_t stride_row, int64_t stride_head, void* out,
     float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool, const void* value_pool,

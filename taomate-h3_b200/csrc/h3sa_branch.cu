@@ -916,8 +916,6 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       pl = make_plan(p, ln, lane);
       write_plan(p, ln, pl, p.plan, lane);
     }
-    // The warp line's kernel may still be running: what follows this one needs both.
-    if (p.warp.own_tiles > 0) asm volatile("griddepcontrol.wait;" ::: "memory");
   }
 
   tc_fence_before();
@@ -1140,26 +1138,32 @@ int sm_count() {
 constexpr int kJointRows = 2 * kSpan;
 
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
-// tensor line passes a dozen barriers; what it costs is that more rows mean reading K and V again.
+// tensor line passes a dozen barriers; what it costs is that every 16 rows read K and V again.
+// Measured with 8 KV heads, both lines (us, tensor / warp): bf16, 60 rows, 4096 shared keys 34 / 24,
+// 16384 keys 49 / 51, 65536 keys 86 / 180; 32 rows, 16384 keys 43 / 37, 65536 keys 78 / 98; 16 rows,
+// 65536 keys 76 / 66; e4m3, 60 rows, 16384 keys 54 / 37, 65536 keys 82 / 102; 32 rows 74 / 62.
+constexpr int kWarpLeast = 4;  // a piece costs the merge as much as some more keys cost the warp
 constexpr int kWarpOwnRows = 64;
-constexpr int kWarpSharedRows = 16;
+constexpr long long kWarpSharedWork = 500000, kWarpSharedWorkF8 = 1200000;  // KV heads x keys x 16-row tiles
 
-Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
+Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4m3) {
   Shape s;
   memset(&s, 0, sizeof(s));
   const long long own = static_cast<long long>(rows) * group;
   const long long all = own * batch;
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
   s.joint = own >= kJointRows ? 1 : 0;
-  s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count()};
-  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * 8};
+  s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
+  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * 8, kWarpLeast};
   Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;
   lo.own_tiles = tiles(own, lo.span);
   s.own_slot_rows = static_cast<int>(own < lo.span ? own : lo.span);
   if (&lo == &s.tensor && own > kBlk) s.own_slot_rows = kBlk;
   const int own_slots = &lo == &s.warp ? 1 : 2;
   if (!s.joint && shared > 0) {
-    Line& ls = all <= kWarpSharedRows ? s.warp : s.tensor;
+    const long long work = static_cast<long long>(kv_heads) * shared * kBlk * tiles(all, kRowSpan);
+    const bool few = &lo == &s.warp && (all <= kRowSpan || work <= (e4m3 ? kWarpSharedWorkF8 : kWarpSharedWork));
+    Line& ls = few ? s.warp : s.tensor;
     ls.shared_tiles = tiles(all, ls.span);
     s.shared_slot_rows = static_cast<int>(all < ls.span ? all : ls.span);
     if (&ls == &s.tensor && all > kBlk) s.shared_slot_rows = kBlk;
@@ -1198,7 +1202,7 @@ int configure() {
 }
 
 template <bool kFp8>
-int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg, bool along) {
+int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg) {
   using Cfg = BrCfg<kFp8>;
   int rc = configure<kFp8>();
   if (rc) return rc;
@@ -1213,7 +1217,7 @@ int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg, bool along) {
   cfg.gridDim = dim3(p.tensor.workers);
   cfg.blockDim = dim3(kBrThreads);
   cfg.dynamicSmemBytes = br_smem_bytes<kFp8>();
-  cfg.numAttrs = along ? 1 : 0;
+  cfg.numAttrs = 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_attn_kernel<kFp8>, tmK, tmV, p);
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_attn_kernel launch", e);
 }
@@ -1229,14 +1233,15 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &early;
-  const bool by_warps = p.warp.own_tiles > 0;
-  if (by_warps) {
-    e = launch_branch_rows(p, kFp8, stream);
-    if (e != cudaSuccess) return set_cuda_error("branch_rows_kernel launch", e);
-  }
-  if (p.tensor.own_tiles > 0 || p.tensor.shared_tiles > 0) {
-    const int rc = launch_tensor<kFp8>(p, cfg, by_warps);
+  const bool tensor = p.tensor.own_tiles > 0 || p.tensor.shared_tiles > 0;
+  if (tensor) {
+    const int rc = launch_tensor<kFp8>(p, cfg);
     if (rc) return rc;
+  }
+  if (p.warp.own_tiles > 0) {  // takes the SMs that the other line is done with
+    cfg.numAttrs = tensor ? 1 : 0;
+    e = launch_branch_rows(p, kFp8, tensor, cfg);
+    if (e != cudaSuccess) return set_cuda_error("branch_rows_kernel launch", e);
   }
   // Four warps share a row where rows are few: its pieces are read one latency after another.
   const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
@@ -1266,10 +1271,10 @@ using namespace h3sa;
 extern "C" {
 
 int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
-                                     int32_t shared_rows) {
+                                     int32_t shared_rows, int32_t e4m3) {
   if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
     return 0;
-  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
+  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk, e4m3 != 0);
   return s.bytes;
 }
 
@@ -1305,7 +1310,7 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d is too large",
                      batch, rows, heads);
-  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
+  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk, e4m3 != 0);
   const auto line_units = [&](const Line& ln) {
     const int64_t blocks = kBlk / ln.unit;
     return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks + ln.pad) +

@@ -27,6 +27,7 @@ struct Line {
   int shared_tiles;  // items per KV head against the shared blocks (0: the other line has them)
   int own_tiles;     // items per KV head and branch against its own (0: the other line has them)
   int workers;
+  int least;  // a worker's part is at least this
 };
 
 struct BranchParams {
@@ -107,7 +108,7 @@ __device__ __forceinline__ Plan make_plan(const BranchParams& p, const Line& ln,
   pl.shared_units = pl.shared_blocks * (kBlk / ln.unit);
   pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units) + own;
   const int all = pl.head_weight * p.kv_heads;
-  pl.cut = max(1, (all + ln.workers - 1) / ln.workers);
+  pl.cut = max(ln.least, (all + ln.workers - 1) / ln.workers);
   return pl;
 }
 
@@ -241,7 +242,8 @@ __device__ __forceinline__ int row_exponent(uint32_t top) {
 }
 __device__ __forceinline__ float exp2_int(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
 
-// Launches the warp line's kernel (h3sa_branch_rows.cu).
-cudaError_t launch_branch_rows(const BranchParams& p, bool e4m3, cudaStream_t stream);
+// Launches the warp line's kernel (h3sa_branch_rows.cu); `after`: along with another kernel, whose end
+// the line then waits for as well.
+cudaError_t launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg);
 
 }  // namespace h3sa

@@ -64,7 +64,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 
 template <bool kFp8>
-__global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const BranchParams p) {
+__global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const BranchParams p, const bool after) {
   constexpr int kElem = kFp8 ? 1 : 2;
   constexpr int kRowBytes = kD * kElem;
   constexpr int kKWords = kRowBytes / 16;  // a lane's quarter of a key row
@@ -320,15 +320,18 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const Br
     flag_lengths(p, lane);
     write_plan(p, ln, pl, p.plan + 3 + p.batch, lane);
   }
+  // what follows this kernel needs the other line's too
+  if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 }  // namespace
 
-cudaError_t launch_branch_rows(const BranchParams& p, bool e4m3, cudaStream_t stream) {
-  const int blocks = p.warp.workers / kRowWarps;
-  if (e4m3) branch_rows_kernel<true><<<blocks, 32 * kRowWarps, 0, stream>>>(p);
-  else branch_rows_kernel<false><<<blocks, 32 * kRowWarps, 0, stream>>>(p);
-  return cudaGetLastError();
+cudaError_t launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
+  cfg.gridDim = dim3(p.warp.workers / kRowWarps);
+  cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.dynamicSmemBytes = 0;
+  return e4m3 ? cudaLaunchKernelEx(&cfg, branch_rows_kernel<true>, p, after)
+              : cudaLaunchKernelEx(&cfg, branch_rows_kernel<false>, p, after);
 }
 
 }  // namespace h3sa
