@@ -298,16 +298,6 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
   }
 }
 
-// A tile load that marks its lines as the first to go from L2.
-__device__ __forceinline__ void tma_load_3d_once(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
-                                                 int c2, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
-      : "memory");
-}
-
 template <bool kFp8>
 __global__ void __launch_bounds__(kBrThreads, 1)
     branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -1154,7 +1144,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
   s.joint = own >= kJointRows ? 1 : 0;
   s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
-  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * 8, kWarpLeast};
+  s.warp = Line{kRowSpan, e4m3 ? kRowUnitF8 : kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
   Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;
   lo.own_tiles = tiles(own, lo.span);
   s.own_slot_rows = static_cast<int>(own < lo.span ? own : lo.span);
@@ -1203,17 +1193,11 @@ int configure() {
 
 template <bool kFp8>
 int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg) {
-  using Cfg = BrCfg<kFp8>;
   int rc = configure<kFp8>();
   if (rc) return rc;
   CUtensorMap tmK, tmV;
-  const CUtensorMapDataType dt = kFp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const uint64_t pool_rows = static_cast<uint64_t>(p.pool_pages) * kBlk;
-  const uint64_t dims[3] = {kD, pool_rows, static_cast<uint64_t>(p.kv_heads)};
-  const uint64_t strides[2] = {static_cast<uint64_t>(kD) * Cfg::kElem, pool_rows * kD * Cfg::kElem};
-  const uint32_t box[3] = {128 / Cfg::kElem, static_cast<uint32_t>(kBlk), 1};
-  if ((rc = encode_tiled_3d(&tmK, dt, p.key_pool, dims, strides, box))) return rc;
-  if ((rc = encode_tiled_3d(&tmV, dt, p.value_pool, dims, strides, box))) return rc;
+  if ((rc = encode_pool(&tmK, p, p.key_pool, kFp8, kBlk))) return rc;
+  if ((rc = encode_pool(&tmV, p, p.value_pool, kFp8, kBlk))) return rc;
   cfg.gridDim = dim3(p.tensor.workers);
   cfg.blockDim = dim3(kBrThreads);
   cfg.dynamicSmemBytes = br_smem_bytes<kFp8>();
@@ -1240,8 +1224,8 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   }
   if (p.warp.own_tiles > 0) {  // takes the SMs that the other line is done with
     cfg.numAttrs = tensor ? 1 : 0;
-    e = launch_branch_rows(p, kFp8, tensor, cfg);
-    if (e != cudaSuccess) return set_cuda_error("branch_rows_kernel launch", e);
+    const int rc = launch_branch_rows(p, kFp8, tensor, cfg);
+    if (rc) return rc;
   }
   // Four warps share a row where rows are few: its pieces are read one latency after another.
   const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;

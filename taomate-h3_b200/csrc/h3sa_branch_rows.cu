@@ -4,42 +4,46 @@
 //   x_j = scale * q . k_j,   O = sum_j 2^(x_j' - m) v_j,   l = sum_j 2^(x_j' - m),   x' = x log2 e
 //
 // Sixteen rows use a key 2 * 16 * 2 * 128 flops for its 512 bytes: the kernel is bound by reading K
-// and V, and for a branch's own few blocks by latency. So a warp works alone: it takes 32 keys at a
-// time straight from global memory into registers in the order the tensor instruction wants them,
-// with the next 32 keys of K (then of V) in flight, and passes no barrier and no shared memory
-// but its own query's.
+// and V, and for a branch's own few blocks by latency. So a warp works alone, without a barrier
+// but that of its own copies: it keeps three 16 KB units of keys and values (32 keys, 64 in e4m3)
+// on their way from memory by TMA, across the ends of its items, and four warps an SM have 192 KB
+// in flight. Reading straight into registers, which hold one unit, took 1.6 us a unit and warp.
 //
 // mma.m16n8k16 leaves the order of the contracted index open as long as both operands agree, and so
-// the column order of the result:
-//   S = Q K^T: lane 4r + c holds key r of each group of eight and contracts d = 32c + 4s .. + 3 in step
-//      s, a quarter of the key's row that it reads in one piece.
-//   O += P V: lane 4r + c holds keys 2c, 2c + 1, 2c + 8, 2c + 9 of sixteen and the columns 16r .. + 15 of
-//      each, so a row's 256 (128) bytes are read by eight lanes side by side; two keys' words are
-//      woven into the operand's pairs by byte permutes. Lane 4r + c ends up with columns 32c ..
-//      32c + 31 of rows r and r + 8.
-// e4m3 caches become f16 pairs, exactly, on the way; the query row is scaled by a power of two and
-// taken as f16 (11 bits to bf16's 8), and P is f16 too.
-#include <cstring>
+// the column order of the result, and the orders are chosen for the 128-byte swizzle of the tiles:
+//   S = Q K^T: lane 4r + c takes, of key r of each group of eight, 32 bytes (two 16-byte chunks) of every
+//      128; step s contracts four elements of them;
+//   O += P V: lane 4r + c takes keys 2c, 2c + 1, 2c + 8, 2c + 9 of sixteen and chunk r of every 128 bytes of
+//      each; two keys' words are woven into the operand's pairs by byte permutes.
+// Either way the eight lanes of a phase read eight different chunks: no bank conflicts. e4m3 caches
+// become f16 pairs, exactly, on the way; the query row is scaled by a power of two and taken as
+// f16 (11 bits to bf16's 8), and P is f16 too.
+#include <mutex>
 
 #include "h3sa_branch.cuh"
 
 namespace h3sa {
 namespace {
 
-constexpr int kRowWarps = 8;
+constexpr int kRowWarps = kRowWarpsPerBlock;
+constexpr int kRowStages = 3;
+constexpr int kTileBytes = 8192;  // K or V of a unit: 32 rows of 256 bytes, or 64 of 128
+constexpr int kStageBytes = 2 * kTileBytes;
+constexpr size_t kRowSmem = static_cast<size_t>(kRowWarps) * kRowStages * kStageBytes + 1024;
 // P is at most 2^threshold; f16 and bf16 both hold it, and O is rescaled only past it.
 constexpr float kThreshold = 8.0f;
 
-// 32 bytes of read-once data.
-__device__ __forceinline__ void load32(const void* at, uint32_t* r) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "l"(at));
-}
 __device__ __forceinline__ void load16(const void* at, uint32_t* r) {
-  asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "l"(at));
+  const uint4 v = __ldg(static_cast<const uint4*>(at));
+  r[0] = v.x;
+  r[1] = v.y;
+  r[2] = v.z;
+  r[3] = v.w;
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
 }
 
 template <bool kF16>
@@ -63,144 +67,198 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 
+// What a warp knows of a segment: rows row0 .. of KV head `head` against `units` units of keys from key0.
+struct RowSegment {
+  int units, head, seq, shared, row0, n_rows, key0, kv_end, direct;
+  long long slot;
+};
+
 template <bool kFp8>
-__global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const BranchParams p, const bool after) {
-  constexpr int kElem = kFp8 ? 1 : 2;
-  constexpr int kRowBytes = kD * kElem;
-  constexpr int kKWords = kRowBytes / 16;  // a lane's quarter of a key row
-  constexpr int kVWords = kRowBytes / 32;  // a lane's sixteen columns of a value row
-  __shared__ uint4 q_frag[kRowWarps][8][32];
+__global__ void __launch_bounds__(32 * kRowWarps, 1)
+    branch_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                       const BranchParams p, const bool after) {
+  constexpr int kUnit = kFp8 ? kRowUnitF8 : kRowUnit;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[kRowWarps][kRowStages];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * (kRowStages * kStageBytes);
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kRowWarps; ++w)
+      for (int s = 0; s < kRowStages; ++s) mbar_init(smem_u32(&full[w][s]), 1);
+    abort_word = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 32) {
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
   const Line& ln = p.warp;
   const int worker = blockIdx.x * kRowWarps + warp;
   const Plan pl = make_plan(p, ln, lane);
-  const int all = pl.head_weight * p.kv_heads;
+  const int all = pl.head_weight * p.kv_heads, own_all = p.rows * p.group;
   int u = min(all, worker * pl.cut);
   const int u_end = min(all, u + pl.cut);
   Place at = {0, -1, 0, 0};
   if (u < u_end) at = locate(p, ln, pl, u, lane);
-  while (u < u_end) {
-    const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
-    const int n_units = min(units, at.off + part) - at.off;
-    if (n_units > 0) {
-      // ---- a segment: rows row0 .. of KV head `head` against keys [key0, key0 + 32 n_units)
-      const int head = at.head, seq = at.b < 0 ? pl.longest : at.b;
-      const int own_all = p.rows * p.group;
-      const int row0 = (at.b < 0 ? 0 : at.b * own_all) + at.t * kRowSpan;
-      const int n_rows = min(kRowSpan, (at.b < 0 ? p.batch * own_all : (at.b + 1) * own_all) - row0);
-      const int key0 = (at.b < 0 ? 0 : own_lo(p)) + at.off * kRowUnit;
-      const int kv_end = at.b < 0 ? pl.max_len : seq_length(p, at.b);
-      const bool direct = pl.shared_blocks == 0 && n_units == units;
-      // this lane's rows, r and r + 8 of the item
-      const RowAt at0 = row_at(p, head, row0 + min(r, n_rows - 1)), at1 = row_at(p, head, row0 + min(r + 8, n_rows - 1));
-      const int hide0 = p.causal ? p.rows - 1 - at0.i : 0, hide1 = p.causal ? p.rows - 1 - at1.i : 0;
-      const int lim0 = seq_length(p, at0.b) - hide0, lim1 = seq_length(p, at1.b) - hide1;
-      float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
-      if constexpr (kFp8) sl2 = sl2b = p.scale_log2 * __ldg(p.k_scale + head);
-      {
-        uint32_t a[16], b[16];
-        const __nv_bfloat16* qa = p.q + at0.b * p.q_sb + at0.i * p.q_sn + at0.h * p.q_sh + 32 * c;
-        const __nv_bfloat16* qb = p.q + at1.b * p.q_sb + at1.i * p.q_sn + at1.h * p.q_sh + 32 * c;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          load16(qa + 8 * k, a + 4 * k);
-          load16(qb + 8 * k, b + 4 * k);
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          if (r >= n_rows) a[k] = 0u;
-          if (r + 8 >= n_rows) b[k] = 0u;
-        }
-        if constexpr (kFp8) {
-          uint32_t ta = 0u, tb = 0u;
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            ta = __vmaxu2(ta, a[k] & 0x7fff7fffu);
-            tb = __vmaxu2(tb, b[k] & 0x7fff7fffu);
-          }
-          ta = max(ta >> 16, ta & 0xffffu);
-          tb = max(tb >> 16, tb & 0xffffu);
-          for (int d = 1; d < 4; d <<= 1) {
-            ta = max(ta, __shfl_xor_sync(0xffffffffu, ta, d));
-            tb = max(tb, __shfl_xor_sync(0xffffffffu, tb, d));
-          }
-          const int ka = row_exponent(ta), kb = row_exponent(tb);
-          const float ua = exp2_int(ka), ub = exp2_int(kb);
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            a[k] = f16x2_of(__uint_as_float(a[k] << 16) * ua, __uint_as_float(a[k] & 0xffff0000u) * ua);
-            b[k] = f16x2_of(__uint_as_float(b[k] << 16) * ub, __uint_as_float(b[k] & 0xffff0000u) * ub);
-          }
-          // infinities and NaN stay what they are in f16
-          sl2 *= exp2_int(-ka);
-          sl2b *= exp2_int(-kb);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int s = 0; s < 8; ++s) q_frag[warp][s][lane] = make_uint4(a[2 * s], b[2 * s], a[2 * s + 1], b[2 * s + 1]);
-        __syncwarp();
-      }
+  __syncthreads();
 
-      const int* pages = p.table + static_cast<size_t>(seq) * p.width;
-      const size_t plane = static_cast<size_t>(head) * p.pool_pages * kBlk;
-      // the pool row of key `key`; a page outside the pool is flagged and read as page 0
-      const auto row_of = [&](int key) -> size_t {
-        int page = __ldg(pages + (key >> 7));
-        if (page < 0 || page >= p.pool_pages) {
-          if (p.err && lane == 0) atomicOr(p.err, kErrBadPage);
-          page = 0;
+  // The next segment of this warp's part (units 0: there is none).
+  const auto next_segment = [&]() {
+    RowSegment g;
+    g.units = 0;
+    while (u < u_end && g.units == 0) {
+      const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
+      const int n = min(units, at.off + part) - at.off;
+      if (n > 0) {
+        g.units = n;
+        g.head = at.head;
+        g.shared = at.b < 0;
+        g.seq = g.shared ? pl.longest : at.b;
+        g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
+        g.n_rows = min(kRowSpan, (g.shared ? p.batch * own_all : (at.b + 1) * own_all) - g.row0);
+        g.key0 = (g.shared ? 0 : own_lo(p)) + at.off * kUnit;
+        g.kv_end = g.shared ? pl.max_len : seq_length(p, at.b);
+        g.direct = pl.shared_blocks == 0 && n == units;
+        const long long item = g.shared ? static_cast<long long>(at.head) * ln.shared_tiles + at.t
+                                        : (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
+        g.slot = (g.shared ? 0 : p.own_row0) + (item + worker) * (g.shared ? p.shared_slot_rows : p.own_slot_rows);
+      }
+      u += part;
+      if (u < u_end) step_item(p, ln, pl, at);
+    }
+    return g;
+  };
+  // The pages of a segment's keys from block `first` (of the segment) on, one a lane.
+  const auto pages_of = [&](const RowSegment& g, int first) {
+    const int block = (g.key0 >> 7) + first + lane, last = (g.key0 + g.units * kUnit - 1) >> 7;
+    int page = block <= last ? __ldg(p.table + static_cast<size_t>(g.seq) * p.width + block) : 0;
+    if (page < 0 || page >= p.pool_pages) {  // flagged, and read as page 0
+      if (p.err) atomicOr(p.err, kErrBadPage);
+      page = 0;
+    }
+    return page;
+  };
+  int issued = 0, used = 0;  // units whose copies were started, and that were waited for
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  const bool once = ln.shared_tiles <= 1 && ln.own_tiles <= 1;  // keys that only one warp reads
+  const auto issue = [&](const RowSegment& g, int i, int page) {
+    if (lane == 0) {
+      const int s = issued % kRowStages, row = page * kBlk + ((g.key0 + i * kUnit) & (kBlk - 1));
+      const uint32_t bar = smem_u32(&full[warp][s]);
+      mbar_expect_tx(bar, kStageBytes);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
+          const uint32_t dst = ring + s * kStageBytes + kv * kTileBytes + a * (kTileBytes / 2);
+          if (once) tma_load_3d_once(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head, policy);
+          else tma_load_3d(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head);
         }
-        return plane + static_cast<size_t>(page) * kBlk + (key & (kBlk - 1));
-      };
-      uint32_t kr[4][kKWords], vr[2][4][kVWords];
-      const auto load_k = [&](size_t row) {
-        const char* base = static_cast<const char*>(p.key_pool) + (row + r) * kRowBytes + c * (kKWords * 4);
+    }
+    ++issued;
+  };
+
+  RowSegment g = next_segment();
+  int pages = g.units > 0 ? pages_of(g, 0) : 0, ahead = 0;  // units of g that were started
+  for (; ahead < min(kRowStages, g.units); ++ahead)
+    issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7)));
+  bool ok = true;
+  while (ok && g.units > 0) {
+    // this lane's rows, r and r + 8 of the item
+    const RowAt at0 = row_at(p, g.head, g.row0 + min(r, g.n_rows - 1));
+    const RowAt at1 = row_at(p, g.head, g.row0 + min(r + 8, g.n_rows - 1));
+    uint32_t qa[16], qb[16];
+    {
+      const __nv_bfloat16* a = p.q + at0.b * p.q_sb + at0.i * p.q_sn + at0.h * p.q_sh;
+      const __nv_bfloat16* b = p.q + at1.b * p.q_sb + at1.i * p.q_sn + at1.h * p.q_sh;
+      // the elements that this lane's chunks of a key hold
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int k = 0; k < 4; ++k) {
+        const int from = kFp8 ? 32 * c + 8 * k : 64 * (k >> 1) + 16 * c + 8 * (k & 1);
+        load16(a + from, qa + 4 * k);
+        load16(b + from, qb + 4 * k);
+      }
+    }
+    const RowSegment next = next_segment();
+    int next_pages = next.units > 0 ? pages_of(next, 0) : 0, next_ahead = 0;
+    const int lim0 = seq_length(p, at0.b) - (p.causal ? p.rows - 1 - at0.i : 0);
+    const int lim1 = seq_length(p, at1.b) - (p.causal ? p.rows - 1 - at1.i : 0);
+    float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
 #pragma unroll
-          for (int k = 0; k < kKWords; k += 8) load32(base + j * 8 * kRowBytes + k * 4, kr[j] + k);
-      };
-      const auto load_v = [&](size_t row) {
-        const char* base = static_cast<const char*>(p.value_pool) + (row + 2 * c) * kRowBytes + r * (kVWords * 4);
+    for (int k = 0; k < 16; ++k) {
+      if (r >= g.n_rows) qa[k] = 0u;
+      if (r + 8 >= g.n_rows) qb[k] = 0u;
+    }
+    if constexpr (kFp8) {
+      sl2 = sl2b = p.scale_log2 * __ldg(p.k_scale + g.head);
+      uint32_t ta = 0u, tb = 0u;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+      for (int k = 0; k < 16; ++k) {
+        ta = __vmaxu2(ta, qa[k] & 0x7fff7fffu);
+        tb = __vmaxu2(tb, qb[k] & 0x7fff7fffu);
+      }
+      ta = max(ta >> 16, ta & 0xffffu);
+      tb = max(tb >> 16, tb & 0xffffu);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const char* from = base + (g * 16 + (k >> 1) * 8 + (k & 1)) * kRowBytes;
-            if constexpr (kFp8) load16(from, vr[g][k]);
-            else load32(from, vr[g][k]);
-          }
-      };
-      float o[16][4];
+      for (int d = 1; d < 4; d <<= 1) {
+        ta = max(ta, __shfl_xor_sync(0xffffffffu, ta, d));
+        tb = max(tb, __shfl_xor_sync(0xffffffffu, tb, d));
+      }
+      const int ka = row_exponent(ta), kb = row_exponent(tb);
+      const float ua = exp2_int(ka), ub = exp2_int(kb);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-      size_t row = row_of(key0);
-      load_k(row);
-      load_v(row);
+      for (int k = 0; k < 16; ++k) {  // infinities and NaN stay what they are
+        qa[k] = f16x2_of(__uint_as_float(qa[k] << 16) * ua, __uint_as_float(qa[k] & 0xffff0000u) * ua);
+        qb[k] = f16x2_of(__uint_as_float(qb[k] << 16) * ub, __uint_as_float(qb[k] & 0xffff0000u) * ub);
+      }
+      sl2 *= exp2_int(-ka);
+      sl2b *= exp2_int(-kb);
+    }
+    float o[16][4];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    int pages_from = 0;  // the block (of the segment) whose page lane 0 holds
 #pragma unroll 1
-      for (int i = 0; i < n_units; ++i) {
-        const int key = key0 + i * kRowUnit;
+    for (int i = 0; i < g.units; ++i) {
+      const int st = used % kRowStages;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[warp][st]), (used / kRowStages) & 1, abort_flag, p.err));
+      if (!ok) break;
+      ++used;
+      const uint32_t kt = ring + st * kStageBytes, vt = kt + kTileBytes;
+#pragma unroll 1
+      for (int sub = 0; sub < kUnit / 32; ++sub) {
+        const int key = g.key0 + i * kUnit + sub * 32;
+        if (sub > 0 && key >= g.kv_end) break;
         float s[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int j = 0; j < 4; ++j) {
+          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+          const uint32_t row = kt + (sub * 32 + 8 * j + r) * 128;
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          const uint4 a = q_frag[warp][st][lane];
+          for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
+            const uint4 x = lds16(row + a * (kTileBytes / 2) + (((2 * c) ^ r) << 4));
+            const uint4 y = lds16(row + a * (kTileBytes / 2) + (((2 * c + 1) ^ r) << 4));
+            const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            if constexpr (kFp8) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if constexpr (kFp8) mma16<true>(s[j], a, f16x2_of_e4m3x2(kr[j][st]), f16x2_of_e4m3x2(kr[j][st] >> 16));
-            else mma16<false>(s[j], a, kr[j][2 * st], kr[j][2 * st + 1]);
+              for (int k = 0; k < 8; ++k)
+                mma16<true>(s[j], make_uint4(qa[2 * k], qb[2 * k], qa[2 * k + 1], qb[2 * k + 1]), f16x2_of_e4m3x2(w[k]),
+                            f16x2_of_e4m3x2(w[k] >> 16));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                mma16<false>(s[j], make_uint4(qa[8 * a + 2 * k], qb[8 * a + 2 * k], qa[8 * a + 2 * k + 1], qb[8 * a + 2 * k + 1]),
+                             w[2 * k], w[2 * k + 1]);
+            }
           }
         }
-        size_t next_row = row;
-        if (i + 1 < n_units) {
-          next_row = (key + kRowUnit) & (kBlk - 1) ? row + kRowUnit : row_of(key + kRowUnit);
-          load_k(next_row);
-        }
         // keys at or past a row's limit are hidden from it
-        if (__any_sync(0xffffffffu, key + kRowUnit > min(lim0, lim1))) {
+        if (__any_sync(0xffffffffu, key + 32 > min(lim0, lim1))) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -240,81 +298,108 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const Br
           l0 += s[j][0] + s[j][1];
           l1 += s[j][2] + s[j][3];
         }
-        // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
-        if (key + kRowUnit > kv_end) {
+        const bool tail = key + 32 > g.kv_end;
 #pragma unroll
-          for (int g = 0; g < 2; ++g)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              if (key + g * 16 + 2 * c + (k >> 1) * 8 + (k & 1) >= kv_end)
-#pragma unroll
-                for (int w = 0; w < kVWords; ++w) vr[g][k][w] = 0u;
-        }
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
+        for (int h = 0; h < 2; ++h) {  // sixteen keys
           uint4 a;
           if constexpr (kFp8)
-            a = make_uint4(f16x2_of(s[2 * g][0], s[2 * g][1]), f16x2_of(s[2 * g][2], s[2 * g][3]),
-                           f16x2_of(s[2 * g + 1][0], s[2 * g + 1][1]), f16x2_of(s[2 * g + 1][2], s[2 * g + 1][3]));
+            a = make_uint4(f16x2_of(s[2 * h][0], s[2 * h][1]), f16x2_of(s[2 * h][2], s[2 * h][3]),
+                           f16x2_of(s[2 * h + 1][0], s[2 * h + 1][1]), f16x2_of(s[2 * h + 1][2], s[2 * h + 1][3]));
           else
-            a = make_uint4(pack_bf16x2(s[2 * g][0], s[2 * g][1]), pack_bf16x2(s[2 * g][2], s[2 * g][3]),
-                           pack_bf16x2(s[2 * g + 1][0], s[2 * g + 1][1]), pack_bf16x2(s[2 * g + 1][2], s[2 * g + 1][3]));
+            a = make_uint4(pack_bf16x2(s[2 * h][0], s[2 * h][1]), pack_bf16x2(s[2 * h][2], s[2 * h][3]),
+                           pack_bf16x2(s[2 * h + 1][0], s[2 * h + 1][1]), pack_bf16x2(s[2 * h + 1][2], s[2 * h + 1][3]));
 #pragma unroll
-          for (int w = 0; w < kVWords; ++w) {
-            const uint32_t x = vr[g][0][w], y = vr[g][1][w], z = vr[g][2][w], v = vr[g][3][w];
-            if constexpr (kFp8) {  // four columns a word
-              const uint32_t xy = __byte_perm(x, y, 0x5140), zv = __byte_perm(z, v, 0x5140);
-              const uint32_t xy2 = __byte_perm(x, y, 0x7362), zv2 = __byte_perm(z, v, 0x7362);
-              mma16<true>(o[4 * w], a, f16x2_of_e4m3x2(xy), f16x2_of_e4m3x2(zv));
-              mma16<true>(o[4 * w + 1], a, f16x2_of_e4m3x2(xy >> 16), f16x2_of_e4m3x2(zv >> 16));
-              mma16<true>(o[4 * w + 2], a, f16x2_of_e4m3x2(xy2), f16x2_of_e4m3x2(zv2));
-              mma16<true>(o[4 * w + 3], a, f16x2_of_e4m3x2(xy2 >> 16), f16x2_of_e4m3x2(zv2 >> 16));
-            } else {  // two
-              mma16<false>(o[2 * w], a, __byte_perm(x, y, 0x5410), __byte_perm(z, v, 0x5410));
-              mma16<false>(o[2 * w + 1], a, __byte_perm(x, y, 0x7632), __byte_perm(z, v, 0x7632));
+          for (int atom = 0; atom < (kFp8 ? 1 : 2); ++atom) {
+            uint4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = sub * 32 + h * 16 + 2 * c + (k >> 1) * 8 + (k & 1);
+              v[k] = lds16(vt + atom * (kTileBytes / 2) + row * 128 + ((r ^ (row & 7)) << 4));
+              // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
+              if (tail && key - sub * 32 + row >= g.kv_end) v[k] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, y[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+            const uint32_t z[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, t[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if constexpr (kFp8) {  // four columns a word
+                const uint32_t xy = __byte_perm(x[w], y[w], 0x5140), zt = __byte_perm(z[w], t[w], 0x5140);
+                const uint32_t xy2 = __byte_perm(x[w], y[w], 0x7362), zt2 = __byte_perm(z[w], t[w], 0x7362);
+                mma16<true>(o[4 * w], a, f16x2_of_e4m3x2(xy), f16x2_of_e4m3x2(zt));
+                mma16<true>(o[4 * w + 1], a, f16x2_of_e4m3x2(xy >> 16), f16x2_of_e4m3x2(zt >> 16));
+                mma16<true>(o[4 * w + 2], a, f16x2_of_e4m3x2(xy2), f16x2_of_e4m3x2(zt2));
+                mma16<true>(o[4 * w + 3], a, f16x2_of_e4m3x2(xy2 >> 16), f16x2_of_e4m3x2(zt2 >> 16));
+              } else {  // two
+                const int n = 8 * atom + 2 * w;
+                mma16<false>(o[n], a, __byte_perm(x[w], y[w], 0x5410), __byte_perm(z[w], t[w], 0x5410));
+                mma16<false>(o[n + 1], a, __byte_perm(x[w], y[w], 0x7632), __byte_perm(z[w], t[w], 0x7632));
+              }
             }
           }
         }
-        if (i + 1 < n_units) load_v(next_row);
-        row = next_row;
       }
-      l0 = quad_sum(l0);
-      l1 = quad_sum(l1);
-      // ---- columns 32c .. + 31 of rows r and r + 8: o[j][0 / 2] is column j, o[j][1 / 3] column 16 + j
-      const long long item = at.b < 0 ? static_cast<long long>(head) * ln.shared_tiles + at.t
-                                      : (static_cast<long long>(head) * p.batch + at.b) * ln.own_tiles + at.t;
-      const long long slot = (at.b < 0 ? 0 : p.own_row0) + (item + worker) * (at.b < 0 ? p.shared_slot_rows : p.own_slot_rows);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int row_in = r + 8 * half;
-        if (row_in >= n_rows) continue;
-        const float l = half ? l1 : l0, m = half ? m1 : m0;
-        if (direct) {
-          float w = l == 0.f ? 0.f : 1.0f / l;
-          if constexpr (kFp8) w *= __ldg(p.v_scale + head);
-          const RowAt& ra = half ? at1 : at0;
-          const long long id = (static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h;
-          uint4* dst = reinterpret_cast<uint4*>(p.out + id * kD + 32 * c);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int j = (k & 1) * 8, e = 2 * half + (k >> 1);
-            dst[k] = make_uint4(pack_bf16x2(o[j][e] * w, o[j + 1][e] * w), pack_bf16x2(o[j + 2][e] * w, o[j + 3][e] * w),
-                                pack_bf16x2(o[j + 4][e] * w, o[j + 5][e] * w), pack_bf16x2(o[j + 6][e] * w, o[j + 7][e] * w));
-          }
-          if (p.lse && c == 0) p.lse[id] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-        } else {
-          if (c == 0) p.part_ml[slot + row_in] = make_float2(m, l);
-          float4* dst = reinterpret_cast<float4*>(p.part_o + (slot + row_in) * kD + 32 * c);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int j = (k & 3) * 4, e = 2 * half + (k >> 2);
-            dst[k] = make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
-          }
+      __syncwarp();  // every lane has read the stage: the next unit may go there
+      if (ahead < g.units) {
+        const int block = ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7);
+        if (block - pages_from >= 32) {
+          pages_from = block;
+          pages = pages_of(g, block);
         }
+        issue(g, ahead, __shfl_sync(0xffffffffu, pages, block - pages_from));
+        ++ahead;
+      } else if (next_ahead < next.units) {
+        issue(next, next_ahead,
+              __shfl_sync(0xffffffffu, next_pages, ((next.key0 + next_ahead * kUnit) >> 7) - (next.key0 >> 7)));
+        ++next_ahead;
       }
     }
-    u += part;
-    if (u < u_end) step_item(p, ln, pl, at);
+    if (!ok) break;
+    l0 = quad_sum(l0);
+    l1 = quad_sum(l1);
+    // ---- this lane's columns: e4m3 32c .. + 31, bf16 16c .. + 15 and 64 + 16c .. + 15; eight at a time
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int row_in = r + 8 * half;
+      if (row_in >= g.n_rows) continue;
+      const float l = half ? l1 : l0, m = half ? m1 : m0;
+      const RowAt& ra = half ? at1 : at0;
+      const long long id = (static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h;
+      float w = l == 0.f ? 0.f : 1.0f / l;
+      if constexpr (kFp8) w *= __ldg(p.v_scale + g.head);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // o[j][e], o[j + 1][e] ..: eight neighbouring columns from `col` on
+        const int j = kFp8 ? (k & 1) * 8 : (k >> 1) * 8, e = 2 * half + (kFp8 ? k >> 1 : k & 1);
+        const int col = kFp8 ? 32 * c + 8 * k : 64 * (k >> 1) + 16 * c + 8 * (k & 1);
+        if (g.direct) {
+          *reinterpret_cast<uint4*>(p.out + id * kD + col) =
+              make_uint4(pack_bf16x2(o[j][e] * w, o[j + 1][e] * w), pack_bf16x2(o[j + 2][e] * w, o[j + 3][e] * w),
+                         pack_bf16x2(o[j + 4][e] * w, o[j + 5][e] * w), pack_bf16x2(o[j + 6][e] * w, o[j + 7][e] * w));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part_o + (g.slot + row_in) * kD + col);
+          dst[0] = make_float4(o[j][e], o[j + 1][e], o[j + 2][e], o[j + 3][e]);
+          dst[1] = make_float4(o[j + 4][e], o[j + 5][e], o[j + 6][e], o[j + 7][e]);
+        }
+      }
+      if (c == 0) {
+        if (!g.direct) p.part_ml[g.slot + row_in] = make_float2(m, l);
+        else if (p.lse) p.lse[id] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      }
+    }
+    g = next;
+    pages = next_pages;
+    ahead = next_ahead;
+    for (; ahead < min(kRowStages, g.units); ++ahead)  // what the last segment left no time for
+      issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7)));
+  }
+  if (!ok) {
+    // leaving early: no copy may still be in flight when the block ends
+    for (; used < issued; ++used) {
+      const unsigned long long t0 = global_ns();
+      while (!mbar_try_wait(smem_u32(&full[warp][used % kRowStages]), (used / kRowStages) & 1) &&
+             global_ns() - t0 < kWaitTimeoutNs) {
+      }
+    }
   }
   if (worker == 0) {
     flag_lengths(p, lane);
@@ -324,14 +409,45 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) branch_rows_kernel(const Br
   if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-}  // namespace
-
-cudaError_t launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
+template <bool kFp8>
+int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
+  static std::mutex mu;
+  static bool done[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (dev >= 64 || !done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(kRowSmem));
+      if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch rows)", e);
+      if (dev < 64) done[dev] = true;
+    }
+  }
+  CUtensorMap tmK, tmV;
+  int rc = encode_pool(&tmK, p, p.key_pool, kFp8, kFp8 ? kRowUnitF8 : kRowUnit);
+  if (!rc) rc = encode_pool(&tmV, p, p.value_pool, kFp8, kFp8 ? kRowUnitF8 : kRowUnit);
+  if (rc) return rc;
   cfg.gridDim = dim3(p.warp.workers / kRowWarps);
   cfg.blockDim = dim3(32 * kRowWarps);
-  cfg.dynamicSmemBytes = 0;
-  return e4m3 ? cudaLaunchKernelEx(&cfg, branch_rows_kernel<true>, p, after)
-              : cudaLaunchKernelEx(&cfg, branch_rows_kernel<false>, p, after);
+  cfg.dynamicSmemBytes = kRowSmem;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8>, tmK, tmV, p, after);
+  return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_rows_kernel launch", e);
+}
+
+}  // namespace
+
+int launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
+  return e4m3 ? launch_rows<true>(p, after, cfg) : launch_rows<false>(p, after, cfg);
+}
+
+int encode_pool(CUtensorMap* map, const BranchParams& p, const void* pool, bool e4m3, int rows) {
+  const uint64_t pool_rows = static_cast<uint64_t>(p.pool_pages) * kBlk, row_bytes = kD * (e4m3 ? 1 : 2);
+  const uint64_t dims[3] = {kD, pool_rows, static_cast<uint64_t>(p.kv_heads)};
+  const uint64_t strides[2] = {row_bytes, pool_rows * row_bytes};
+  const uint32_t box[3] = {e4m3 ? 128u : 64u, static_cast<uint32_t>(rows), 1};
+  return encode_tiled_3d(map, e4m3 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, pool, dims,
+                         strides, box);
 }
 
 }  // namespace h3sa
