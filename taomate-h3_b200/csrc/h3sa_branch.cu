@@ -1132,7 +1132,7 @@ constexpr int kJointRows = 2 * kSpan;
 // Measured with 8 KV heads, both lines (us, tensor / warp): bf16, 60 rows, 4096 shared keys 34 / 24,
 // 16384 keys 49 / 51, 65536 keys 86 / 180; 32 rows, 16384 keys 43 / 37, 65536 keys 78 / 98; 16 rows,
 // 65536 keys 76 / 66; e4m3, 60 rows, 16384 keys 54 / 37, 65536 keys 82 / 102; 32 rows 74 / 62.
-constexpr int kWarpLeast = 4;  // a piece costs the merge as much as some more keys cost the warp
+constexpr int kWarpLeast = 4, kWarpLeastBeside = 8;
 constexpr int kWarpOwnRows = 64;
 constexpr long long kWarpSharedWork = 500000, kWarpSharedWorkF8 = 1200000;  // KV heads x keys x 16-row tiles
 
@@ -1144,7 +1144,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
   s.joint = own >= kJointRows ? 1 : 0;
   s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
-  s.warp = Line{kRowSpan, e4m3 ? kRowUnitF8 : kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
+  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
   Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;
   lo.own_tiles = tiles(own, lo.span);
   s.own_slot_rows = static_cast<int>(own < lo.span ? own : lo.span);
@@ -1154,6 +1154,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4
     const long long work = static_cast<long long>(kv_heads) * shared * kBlk * tiles(all, kRowSpan);
     const bool few = &lo == &s.warp && (all <= kRowSpan || work <= (e4m3 ? kWarpSharedWorkF8 : kWarpSharedWork));
     Line& ls = few ? s.warp : s.tensor;
+    if (!few) s.warp.least = kWarpLeastBeside;
     ls.shared_tiles = tiles(all, ls.span);
     s.shared_slot_rows = static_cast<int>(all < ls.span ? all : ls.span);
     if (&ls == &s.tensor && all > kBlk) s.shared_slot_rows = kBlk;

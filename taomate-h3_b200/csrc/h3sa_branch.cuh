@@ -17,7 +17,7 @@ constexpr int kD = 128;    // head dimension
 constexpr int kBlk = 128;  // KV rows of a block (a page)
 constexpr int kSpan = 256;     // query rows of an item of the tensor line: two tiles
 constexpr int kRowSpan = 16;   // query rows of an item of the warp line
-constexpr int kRowUnit = 32, kRowUnitF8 = 64;  // keys of a unit of the warp line: 16 KB of K and V
+constexpr int kRowUnit = 32;   // keys of a unit of the warp line
 constexpr int kRowWarpsPerBlock = 4;
 
 // A line: items of up to `span` query rows, first those against the shared blocks and then those

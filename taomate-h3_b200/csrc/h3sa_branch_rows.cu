@@ -5,7 +5,7 @@
 //
 // Sixteen rows use a key 2 * 16 * 2 * 128 flops for its 512 bytes: the kernel is bound by reading K
 // and V, and for a branch's own few blocks by latency. So a warp works alone, without a barrier
-// but that of its own copies: it keeps three 16 KB units of keys and values (32 keys, 64 in e4m3)
+// but that of its own copies: it keeps 48 KB of keys and values, three units of 32 keys or six in e4m3,
 // on their way from memory by TMA, across the ends of its items, and four warps an SM have 192 KB
 // in flight. Reading straight into registers, which hold one unit, took 1.6 us a unit and warp.
 //
@@ -26,10 +26,15 @@ namespace h3sa {
 namespace {
 
 constexpr int kRowWarps = kRowWarpsPerBlock;
-constexpr int kRowStages = 3;
-constexpr int kTileBytes = 8192;  // K or V of a unit: 32 rows of 256 bytes, or 64 of 128
-constexpr int kStageBytes = 2 * kTileBytes;
-constexpr size_t kRowSmem = static_cast<size_t>(kRowWarps) * kRowStages * kStageBytes + 1024;
+constexpr int kRowRing = 48 * 1024;  // bytes a warp
+constexpr int kMaxRowStages = 6;
+template <bool kFp8>
+struct RowCfg {
+  static constexpr int kTileBytes = kRowUnit * kD * (kFp8 ? 1 : 2);  // K or V of a unit
+  static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = kRowRing / kStageBytes;  // 3, and 6 for e4m3
+};
+constexpr size_t kRowSmem = static_cast<size_t>(kRowWarps) * kRowRing + 1024;
 // P is at most 2^threshold; f16 and bf16 both hold it, and O is rescaled only past it.
 constexpr float kThreshold = 8.0f;
 
@@ -77,14 +82,15 @@ template <bool kFp8>
 __global__ void __launch_bounds__(32 * kRowWarps, 1)
     branch_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const BranchParams p, const bool after) {
-  constexpr int kUnit = kFp8 ? kRowUnitF8 : kRowUnit;
+  constexpr int kTileBytes = RowCfg<kFp8>::kTileBytes, kStageBytes = RowCfg<kFp8>::kStageBytes;
+  constexpr int kRowStages = RowCfg<kFp8>::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kRowWarps][kRowStages];
+  __shared__ uint64_t full[kRowWarps][kMaxRowStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * (kRowStages * kStageBytes);
+  const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * kRowRing;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kRowWarps; ++w)
       for (int s = 0; s < kRowStages; ++s) mbar_init(smem_u32(&full[w][s]), 1);
@@ -119,7 +125,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
         g.n_rows = min(kRowSpan, (g.shared ? p.batch * own_all : (at.b + 1) * own_all) - g.row0);
-        g.key0 = (g.shared ? 0 : own_lo(p)) + at.off * kUnit;
+        g.key0 = (g.shared ? 0 : own_lo(p)) + at.off * kRowUnit;
         g.kv_end = g.shared ? pl.max_len : seq_length(p, at.b);
         g.direct = pl.shared_blocks == 0 && n == units;
         const long long item = g.shared ? static_cast<long long>(at.head) * ln.shared_tiles + at.t
@@ -133,7 +139,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
   };
   // The pages of a segment's keys from block `first` (of the segment) on, one a lane.
   const auto pages_of = [&](const RowSegment& g, int first) {
-    const int block = (g.key0 >> 7) + first + lane, last = (g.key0 + g.units * kUnit - 1) >> 7;
+    const int block = (g.key0 >> 7) + first + lane, last = (g.key0 + g.units * kRowUnit - 1) >> 7;
     int page = block <= last ? __ldg(p.table + static_cast<size_t>(g.seq) * p.width + block) : 0;
     if (page < 0 || page >= p.pool_pages) {  // flagged, and read as page 0
       if (p.err) atomicOr(p.err, kErrBadPage);
@@ -147,7 +153,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
   const bool once = ln.shared_tiles <= 1 && ln.own_tiles <= 1;  // keys that only one warp reads
   const auto issue = [&](const RowSegment& g, int i, int page) {
     if (lane == 0) {
-      const int s = issued % kRowStages, row = page * kBlk + ((g.key0 + i * kUnit) & (kBlk - 1));
+      const int s = issued % kRowStages, row = page * kBlk + ((g.key0 + i * kRowUnit) & (kBlk - 1));
       const uint32_t bar = smem_u32(&full[warp][s]);
       mbar_expect_tx(bar, kStageBytes);
 #pragma unroll
@@ -165,7 +171,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
   RowSegment g = next_segment();
   int pages = g.units > 0 ? pages_of(g, 0) : 0, ahead = 0;  // units of g that were started
   for (; ahead < min(kRowStages, g.units); ++ahead)
-    issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7)));
+    issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7)));
   bool ok = true;
   while (ok && g.units > 0) {
     // this lane's rows, r and r + 8 of the item
@@ -230,117 +236,113 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
       if (!ok) break;
       ++used;
       const uint32_t kt = ring + st * kStageBytes, vt = kt + kTileBytes;
-#pragma unroll 1
-      for (int sub = 0; sub < kUnit / 32; ++sub) {
-        const int key = g.key0 + i * kUnit + sub * 32;
-        if (sub > 0 && key >= g.kv_end) break;
-        float s[4][4];
+      const int key = g.key0 + i * kRowUnit;
+      float s[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-          const uint32_t row = kt + (sub * 32 + 8 * j + r) * 128;
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        const uint32_t row = kt + (8 * j + r) * 128;
 #pragma unroll
-          for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
-            const uint4 x = lds16(row + a * (kTileBytes / 2) + (((2 * c) ^ r) << 4));
-            const uint4 y = lds16(row + a * (kTileBytes / 2) + (((2 * c + 1) ^ r) << 4));
-            const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            if constexpr (kFp8) {
+        for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
+          const uint4 x = lds16(row + a * (kTileBytes / 2) + (((2 * c) ^ r) << 4));
+          const uint4 y = lds16(row + a * (kTileBytes / 2) + (((2 * c + 1) ^ r) << 4));
+          const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          if constexpr (kFp8) {
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                mma16<true>(s[j], make_uint4(qa[2 * k], qb[2 * k], qa[2 * k + 1], qb[2 * k + 1]), f16x2_of_e4m3x2(w[k]),
-                            f16x2_of_e4m3x2(w[k] >> 16));
-            } else {
+            for (int k = 0; k < 8; ++k)
+              mma16<true>(s[j], make_uint4(qa[2 * k], qb[2 * k], qa[2 * k + 1], qb[2 * k + 1]), f16x2_of_e4m3x2(w[k]),
+                          f16x2_of_e4m3x2(w[k] >> 16));
+          } else {
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                mma16<false>(s[j], make_uint4(qa[8 * a + 2 * k], qb[8 * a + 2 * k], qa[8 * a + 2 * k + 1], qb[8 * a + 2 * k + 1]),
-                             w[2 * k], w[2 * k + 1]);
-            }
+            for (int k = 0; k < 4; ++k)
+              mma16<false>(s[j], make_uint4(qa[8 * a + 2 * k], qb[8 * a + 2 * k], qa[8 * a + 2 * k + 1], qb[8 * a + 2 * k + 1]),
+                           w[2 * k], w[2 * k + 1]);
           }
         }
-        // keys at or past a row's limit are hidden from it
-        if (__any_sync(0xffffffffu, key + 32 > min(lim0, lim1))) {
+      }
+      // keys at or past a row's limit are hidden from it
+      if (__any_sync(0xffffffffu, key + 32 > min(lim0, lim1))) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int at_key = key + 8 * j + 2 * c + k;
-              if (at_key >= lim0) s[j][k] = -INFINITY;
-              if (at_key >= lim1) s[j][2 + k] = -INFINITY;
-            }
-        }
-        float t0 = fmaxf(fmax3(fmaxf(s[0][0], s[0][1]), s[1][0], s[1][1]), fmax3(fmaxf(s[2][0], s[2][1]), s[3][0], s[3][1]));
-        float t1 = fmaxf(fmax3(fmaxf(s[0][2], s[0][3]), s[1][2], s[1][3]), fmax3(fmaxf(s[2][2], s[2][3]), s[3][2], s[3][3]));
-        t0 = quad_max(t0) * sl2;
-        t1 = quad_max(t1) * sl2b;
-        const bool need0 = t0 > m0 + kThreshold, need1 = t1 > m1 + kThreshold;
-        if (__any_sync(0xffffffffu, need0 || need1)) {
-          const float a0 = need0 ? fast_exp2(m0 - t0) : 1.f, a1 = need1 ? fast_exp2(m1 - t1) : 1.f;
-          m0 = need0 ? t0 : m0;
-          m1 = need1 ? t1 : m1;
-          l0 *= a0;
-          l1 *= a1;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            o[j][0] *= a0;
-            o[j][1] *= a0;
-            o[j][2] *= a1;
-            o[j][3] *= a1;
+          for (int k = 0; k < 2; ++k) {
+            const int at_key = key + 8 * j + 2 * c + k;
+            if (at_key >= lim0) s[j][k] = -INFINITY;
+            if (at_key >= lim1) s[j][2 + k] = -INFINITY;
           }
+      }
+      float t0 = fmaxf(fmax3(fmaxf(s[0][0], s[0][1]), s[1][0], s[1][1]), fmax3(fmaxf(s[2][0], s[2][1]), s[3][0], s[3][1]));
+      float t1 = fmaxf(fmax3(fmaxf(s[0][2], s[0][3]), s[1][2], s[1][3]), fmax3(fmaxf(s[2][2], s[2][3]), s[3][2], s[3][3]));
+      t0 = quad_max(t0) * sl2;
+      t1 = quad_max(t1) * sl2b;
+      const bool need0 = t0 > m0 + kThreshold, need1 = t1 > m1 + kThreshold;
+      if (__any_sync(0xffffffffu, need0 || need1)) {
+        const float a0 = need0 ? fast_exp2(m0 - t0) : 1.f, a1 = need1 ? fast_exp2(m1 - t1) : 1.f;
+        m0 = need0 ? t0 : m0;
+        m1 = need1 ? t1 : m1;
+        l0 *= a0;
+        l1 *= a1;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          o[j][0] *= a0;
+          o[j][1] *= a0;
+          o[j][2] *= a1;
+          o[j][3] *= a1;
         }
-        // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
-        const float b0 = m0 == -INFINITY ? 0.f : -m0, b1 = m1 == -INFINITY ? 0.f : -m1;
+      }
+      // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
+      const float b0 = m0 == -INFINITY ? 0.f : -m0, b1 = m1 == -INFINITY ? 0.f : -m1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          s[j][0] = fast_exp2(fmaf(s[j][0], sl2, b0));
-          s[j][1] = fast_exp2(fmaf(s[j][1], sl2, b0));
-          s[j][2] = fast_exp2(fmaf(s[j][2], sl2b, b1));
-          s[j][3] = fast_exp2(fmaf(s[j][3], sl2b, b1));
-          l0 += s[j][0] + s[j][1];
-          l1 += s[j][2] + s[j][3];
-        }
-        const bool tail = key + 32 > g.kv_end;
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = fast_exp2(fmaf(s[j][0], sl2, b0));
+        s[j][1] = fast_exp2(fmaf(s[j][1], sl2, b0));
+        s[j][2] = fast_exp2(fmaf(s[j][2], sl2b, b1));
+        s[j][3] = fast_exp2(fmaf(s[j][3], sl2b, b1));
+        l0 += s[j][0] + s[j][1];
+        l1 += s[j][2] + s[j][3];
+      }
+      const bool tail = key + 32 > g.kv_end;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {  // sixteen keys
-          uint4 a;
-          if constexpr (kFp8)
-            a = make_uint4(f16x2_of(s[2 * h][0], s[2 * h][1]), f16x2_of(s[2 * h][2], s[2 * h][3]),
-                           f16x2_of(s[2 * h + 1][0], s[2 * h + 1][1]), f16x2_of(s[2 * h + 1][2], s[2 * h + 1][3]));
-          else
-            a = make_uint4(pack_bf16x2(s[2 * h][0], s[2 * h][1]), pack_bf16x2(s[2 * h][2], s[2 * h][3]),
-                           pack_bf16x2(s[2 * h + 1][0], s[2 * h + 1][1]), pack_bf16x2(s[2 * h + 1][2], s[2 * h + 1][3]));
+      for (int h = 0; h < 2; ++h) {  // sixteen keys
+        uint4 a;
+        if constexpr (kFp8)
+          a = make_uint4(f16x2_of(s[2 * h][0], s[2 * h][1]), f16x2_of(s[2 * h][2], s[2 * h][3]),
+                         f16x2_of(s[2 * h + 1][0], s[2 * h + 1][1]), f16x2_of(s[2 * h + 1][2], s[2 * h + 1][3]));
+        else
+          a = make_uint4(pack_bf16x2(s[2 * h][0], s[2 * h][1]), pack_bf16x2(s[2 * h][2], s[2 * h][3]),
+                         pack_bf16x2(s[2 * h + 1][0], s[2 * h + 1][1]), pack_bf16x2(s[2 * h + 1][2], s[2 * h + 1][3]));
 #pragma unroll
-          for (int atom = 0; atom < (kFp8 ? 1 : 2); ++atom) {
-            uint4 v[4];
+        for (int atom = 0; atom < (kFp8 ? 1 : 2); ++atom) {
+          uint4 v[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = sub * 32 + h * 16 + 2 * c + (k >> 1) * 8 + (k & 1);
-              v[k] = lds16(vt + atom * (kTileBytes / 2) + row * 128 + ((r ^ (row & 7)) << 4));
-              // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
-              if (tail && key - sub * 32 + row >= g.kv_end) v[k] = make_uint4(0u, 0u, 0u, 0u);
-            }
-            const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, y[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
-            const uint32_t z[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, t[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
+          for (int k = 0; k < 4; ++k) {
+            const int row = h * 16 + 2 * c + (k >> 1) * 8 + (k & 1);
+            v[k] = lds16(vt + atom * (kTileBytes / 2) + row * 128 + ((r ^ (row & 7)) << 4));
+            // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
+            if (tail && key + row >= g.kv_end) v[k] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, y[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+          const uint32_t z[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, t[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if constexpr (kFp8) {  // four columns a word
-                const uint32_t xy = __byte_perm(x[w], y[w], 0x5140), zt = __byte_perm(z[w], t[w], 0x5140);
-                const uint32_t xy2 = __byte_perm(x[w], y[w], 0x7362), zt2 = __byte_perm(z[w], t[w], 0x7362);
-                mma16<true>(o[4 * w], a, f16x2_of_e4m3x2(xy), f16x2_of_e4m3x2(zt));
-                mma16<true>(o[4 * w + 1], a, f16x2_of_e4m3x2(xy >> 16), f16x2_of_e4m3x2(zt >> 16));
-                mma16<true>(o[4 * w + 2], a, f16x2_of_e4m3x2(xy2), f16x2_of_e4m3x2(zt2));
-                mma16<true>(o[4 * w + 3], a, f16x2_of_e4m3x2(xy2 >> 16), f16x2_of_e4m3x2(zt2 >> 16));
-              } else {  // two
-                const int n = 8 * atom + 2 * w;
-                mma16<false>(o[n], a, __byte_perm(x[w], y[w], 0x5410), __byte_perm(z[w], t[w], 0x5410));
-                mma16<false>(o[n + 1], a, __byte_perm(x[w], y[w], 0x7632), __byte_perm(z[w], t[w], 0x7632));
-              }
+          for (int w = 0; w < 4; ++w) {
+            if constexpr (kFp8) {  // four columns a word
+              const uint32_t xy = __byte_perm(x[w], y[w], 0x5140), zt = __byte_perm(z[w], t[w], 0x5140);
+              const uint32_t xy2 = __byte_perm(x[w], y[w], 0x7362), zt2 = __byte_perm(z[w], t[w], 0x7362);
+              mma16<true>(o[4 * w], a, f16x2_of_e4m3x2(xy), f16x2_of_e4m3x2(zt));
+              mma16<true>(o[4 * w + 1], a, f16x2_of_e4m3x2(xy >> 16), f16x2_of_e4m3x2(zt >> 16));
+              mma16<true>(o[4 * w + 2], a, f16x2_of_e4m3x2(xy2), f16x2_of_e4m3x2(zt2));
+              mma16<true>(o[4 * w + 3], a, f16x2_of_e4m3x2(xy2 >> 16), f16x2_of_e4m3x2(zt2 >> 16));
+            } else {  // two
+              const int n = 8 * atom + 2 * w;
+              mma16<false>(o[n], a, __byte_perm(x[w], y[w], 0x5410), __byte_perm(z[w], t[w], 0x5410));
+              mma16<false>(o[n + 1], a, __byte_perm(x[w], y[w], 0x7632), __byte_perm(z[w], t[w], 0x7632));
             }
           }
         }
       }
       __syncwarp();  // every lane has read the stage: the next unit may go there
       if (ahead < g.units) {
-        const int block = ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7);
+        const int block = ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7);
         if (block - pages_from >= 32) {
           pages_from = block;
           pages = pages_of(g, block);
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
         ++ahead;
       } else if (next_ahead < next.units) {
         issue(next, next_ahead,
-              __shfl_sync(0xffffffffu, next_pages, ((next.key0 + next_ahead * kUnit) >> 7) - (next.key0 >> 7)));
+              __shfl_sync(0xffffffffu, next_pages, ((next.key0 + next_ahead * kRowUnit) >> 7) - (next.key0 >> 7)));
         ++next_ahead;
       }
     }
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
     pages = next_pages;
     ahead = next_ahead;
     for (; ahead < min(kRowStages, g.units); ++ahead)  // what the last segment left no time for
-      issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kUnit) >> 7) - (g.key0 >> 7)));
+      issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7)));
   }
   if (!ok) {
     // leaving early: no copy may still be in flight when the block ends
@@ -425,8 +427,8 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
     }
   }
   CUtensorMap tmK, tmV;
-  int rc = encode_pool(&tmK, p, p.key_pool, kFp8, kFp8 ? kRowUnitF8 : kRowUnit);
-  if (!rc) rc = encode_pool(&tmV, p, p.value_pool, kFp8, kFp8 ? kRowUnitF8 : kRowUnit);
+  int rc = encode_pool(&tmK, p, p.key_pool, kFp8, kRowUnit);
+  if (!rc) rc = encode_pool(&tmV, p, p.value_pool, kFp8, kRowUnit);
   if (rc) return rc;
   cfg.gridDim = dim3(p.warp.workers / kRowWarps);
   cfg.blockDim = dim3(32 * kRowWarps);
