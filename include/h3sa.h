@@ -519,7 +519,7 @@ H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t wi
  * [batch, rows, heads, 128] with the given element strides (multiples of 8); out bf16
  * [batch, rows, heads, 128] contiguous; lse fp32 [batch, rows, heads] (natural log of the sum of
  * exponentials, -inf for a row that sees nothing) or NULL. Pools [kv_heads, pool_pages * 128, 128],
- * 32-byte aligned, bf16, or e4m3 with k_scale / v_scale fp32 [kv_heads]; query head h reads KV head
+ * 16-byte aligned, bf16, or e4m3 with k_scale / v_scale fp32 [kv_heads]; query head h reads KV head
  * h / (heads / kv_heads). Row i of sequence b sees the keys j < lengths[b], causal != 0: j <
  * lengths[b] - (rows - 1 - i), the new rows being the sequence's last ones. The first shared_rows
  * rows (whole pages) are the same pages in the table rows of all sequences at least that long;
@@ -528,10 +528,11 @@ H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t wi
  * [0, width * 128] is clamped with H3SA_DEVERR_BAD_INDEX; a page outside the pool gives
  * H3SA_DEVERR_BAD_PAGE and invalid outputs. Results do not depend on timing. */
 H3SA_API int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
-                                              int32_t kv_heads, int32_t shared_rows, int32_t e4m3);
+                                              int32_t kv_heads, int32_t shared_rows);
 H3SA_API int h3sa_shared_prefix_attention(
     const void* query, int64_t stride_sequence, int64_t stride_row, int64_t stride_head, void* out,
-    float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool, const void* value_pool,
+    float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool,
+    const void* value_pool,
     int32_t pool_pages, int32_t e4m3, const float* k_scale, const float* v_scale,
     const int32_t* table, int32_t width, const int32_t* lengths, int32_t shared_rows,
     int32_t causal, float softmax_scale, void* workspace, int64_t workspace_bytes,

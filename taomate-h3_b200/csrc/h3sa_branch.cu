@@ -6,16 +6,17 @@
 //
 //   x_j = scale * q . k_j,   out = sum_j 2^(x_j' - m) v_j / sum_j 2^(x_j' - m),  x' = x log2 e
 //
-// Work is cut into units of one 128-row KV block of one KV head against one item of up to 256
-// query rows. In the split form an item is either a span of all branches' rows stacked (b, i, and
-// the query heads of the KV head's group) against the shared blocks, which are so read once for
-// all, or the rows of one branch against its own blocks; in the joint form (branches with many
-// rows each) an item is a span of one branch's rows against all its blocks. The units lie in one
-// line (KV head, shared items, own items) that is cut into equal ranges, one per CTA, whatever the
-// lengths are; lengths are read on the device. An item that no cut divides and that nothing else
-// contributes to is written out directly; the pieces of all others go to a workspace as
-// unnormalised fp32 O, running maximum and sum, and branch_merge_kernel joins them in a fixed
-// order, so results do not depend on timing.
+// In the split form an item is either a span of all branches' rows stacked (b, i, and the query
+// heads of the KV head's group) against the shared blocks, which are so read once for all, or the
+// rows of one branch against its own blocks; in the joint form (branches with many rows each) an
+// item is a span of one branch's rows against all its blocks. There are two kernels for them, the
+// tensor line here (items of up to 256 rows, tcgen05) and the warp line in h3sa_branch_rows.cu
+// (items of 16 rows, each warp by itself); shape_of says which takes what. Either one's units,
+// a step of keys of one KV head against one item, lie in one line (KV head, shared items, own items)
+// that is cut into equal ranges, one per CTA or warp, whatever the lengths are; lengths are read on
+// the device. An item that no cut divides and that nothing else contributes to is written out
+// directly; the pieces of all others go to a workspace as unnormalised fp32 O, running maximum and
+// sum, and branch_merge_kernel joins them in a fixed order, so results do not depend on timing.
 //
 // Warp roles of branch_attn_kernel (one persistent CTA per SM, 384 threads):
 //   warp 0      walks the CTA's units: publishes each item segment in a small descriptor ring and
@@ -920,7 +921,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
 // of the units, and writes rows that see nothing. A warp takes a row (kTeam warps share one in long
 // shared items) and reads several pieces at a time, maximum, sum and O alike before it needs any of
 // them: what bounds this kernel is the latency of reads from L2, and reading O only after the
-// weights had been found took 21 us instead of 6 for 480 rows of 38 pieces. In the joint form few
+// weights had been found took 18 us instead of 8.5 for 480 rows of 38 pieces. In the joint form few
 // pieces make a row and a warp takes kRows rows at once instead.
 constexpr int kMergeWarps = 4;
 constexpr int kJointWarpRows = 4;  // joint form: rows of a warp
@@ -1129,14 +1130,20 @@ constexpr int kJointRows = 2 * kSpan;
 
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
 // tensor line passes a dozen barriers; what it costs is that every 16 rows read K and V again.
-// Measured with 8 KV heads, both lines (us, tensor / warp): bf16, 60 rows, 4096 shared keys 34 / 24,
-// 16384 keys 49 / 51, 65536 keys 86 / 180; 32 rows, 16384 keys 43 / 37, 65536 keys 78 / 98; 16 rows,
-// 65536 keys 76 / 66; e4m3, 60 rows, 16384 keys 54 / 37, 65536 keys 82 / 102; 32 rows 74 / 62.
-constexpr int kWarpLeast = 4, kWarpLeastBeside = 8;
+// Shared blocks under 8 KV heads, both lines, with merge and own parts (us, warp / tensor): bf16,
+// 60 rows, 1024 keys 17 / 27, 4096 keys 22 / 29, 16384 keys 46 / 43, 65536 keys 156 / 82; 240 rows,
+// 4096 keys 48 / 43; 32 rows, 16384 keys 31 / 38, 65536 keys 97 / 78; 16 rows, 65536 keys 57 / 75.
+// e4m3, 60 rows, 16384 keys 43 / 47, 65536 keys 128 / 75; 32 rows, 65536 keys 72 / 65; 16 rows 47 / 61.
+// So: always up to one tile of rows, else up to the product where the two meet.
 constexpr int kWarpOwnRows = 64;
-constexpr long long kWarpSharedWork = 500000, kWarpSharedWorkF8 = 1200000;  // KV heads x keys x 16-row tiles
+constexpr long long kWarpSharedWork = 500000;  // KV heads x keys x 16-row tiles
+// The least part of a worker, in units: a piece costs the merge as much as some more keys cost the
+// warp, and more so beside the tensor line, whose time hides the warps'. 24 branches of 4 x 32 rows,
+// 8192 shared keys, own lengths to 700 (us): 8 units 50.9, 4 units 55.6, 12 units 53.9; alone, 24 KV
+// heads over 1024 keys: 4 units 12.6, 8 units 16.3, 2 units 13.8.
+constexpr int kWarpLeast = 4, kWarpLeastBeside = 8;
 
-Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4m3) {
+Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   Shape s;
   memset(&s, 0, sizeof(s));
   const long long own = static_cast<long long>(rows) * group;
@@ -1152,7 +1159,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, bool e4
   const int own_slots = &lo == &s.warp ? 1 : 2;
   if (!s.joint && shared > 0) {
     const long long work = static_cast<long long>(kv_heads) * shared * kBlk * tiles(all, kRowSpan);
-    const bool few = &lo == &s.warp && (all <= kRowSpan || work <= (e4m3 ? kWarpSharedWorkF8 : kWarpSharedWork));
+    const bool few = &lo == &s.warp && (all <= kRowSpan || work <= kWarpSharedWork);
     Line& ls = few ? s.warp : s.tensor;
     if (!few) s.warp.least = kWarpLeastBeside;
     ls.shared_tiles = tiles(all, ls.span);
@@ -1256,15 +1263,16 @@ using namespace h3sa;
 extern "C" {
 
 int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
-                                     int32_t shared_rows, int32_t e4m3) {
+                                     int32_t shared_rows) {
   if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
     return 0;
-  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk, e4m3 != 0);
+  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
   return s.bytes;
 }
 
 int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int64_t stride_row,
-                                 int64_t stride_head, void* out, float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+                                 int64_t stride_head, void* out, float* lse, int32_t batch,
+                                 int32_t rows, int32_t heads, int32_t kv_heads,
                                  const void* key_pool, const void* value_pool, int32_t pool_pages,
                                  int32_t e4m3, const float* k_scale, const float* v_scale,
                                  const int32_t* table, int32_t width, const int32_t* lengths,
@@ -1287,15 +1295,15 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
   if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
-  if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 32) || !aligned(value_pool, 32) ||
+  if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
       !aligned(workspace, 16) || stride_sequence % 8 || stride_row % 8 || stride_head % 8)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned, pools 32-byte");
+    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned");
   const int group = heads / kv_heads;
   const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
   if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d is too large",
                      batch, rows, heads);
-  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk, e4m3 != 0);
+  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
   const auto line_units = [&](const Line& ln) {
     const int64_t blocks = kBlk / ln.unit;
     return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks + ln.pad) +

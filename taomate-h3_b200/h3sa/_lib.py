@@ -158,7 +158,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "h3sa_compact_pages": (
         ctypes.c_int, [ctypes.POINTER(Pools), _P, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
     "h3sa_free_pages": (ctypes.c_int, [_P, _I, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P]),
-    "h3sa_shared_prefix_workspace": (_L, [_I, _I, _I, _I, _I, _I]),
+    "h3sa_shared_prefix_workspace": (_L, [_I, _I, _I, _I, _I]),
     "h3sa_shared_prefix_attention": (
         ctypes.c_int,
         [_P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _F,

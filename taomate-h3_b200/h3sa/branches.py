@@ -276,7 +276,7 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     if lse is not None and _bad(lse, device, _F32, (batch, rows, heads)):
         _refuse(what, "lse", device, _F32, (batch, rows, heads))
     error = _error_word(what, device, device_error)
-    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows, 1 if e4m3 else 0))
+    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows))
     if out is not None and _bad(out, device, _BF16, query.shape):
         _refuse(what, "out", device, _BF16, query.shape)
     with _on(stream):
