@@ -1293,7 +1293,7 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   if (!query || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
       (e4m3 && (!k_scale || !v_scale)))
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
-  if (!(softmax_scale > 0.f) || softmax_scale > 3.0e38f)
+  if (!(softmax_scale > 0.f) || softmax_scale > 2.0e38f)
     return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
   if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
       !aligned(workspace, 16) || stride_sequence % 8 || stride_row % 8 || stride_head % 8)

@@ -235,7 +235,8 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     ``shared_rows`` rows (a multiple of 128) are the same pages in the table rows of all
     sequences that reach that far, as ``fork_pages`` leaves them. Rows that see nothing come out
     zero. ``out``: optional contiguous bf16 result tensor; ``lse``: optional fp32
-    ``[sequences, rows, heads]`` that receives the log-sum-exp (-inf for such rows).
+    ``[sequences, rows, heads]`` that receives the log-sum-exp (-inf for such rows). Neither may
+    overlap ``query``.
     """
 
     what = "shared_prefix_attention"
