@@ -134,6 +134,29 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
+// 2^x of a pair, x below 128, on the multiply-add pipe: x = i + f with |f| <= 1/2, 2^f as a polynomial
+// (least maximum relative error of its degree with 2^0 = 1 exactly: 2^-18.4), i added to the exponent.
+// From x = -127 down the result is 0; NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
+  float x0, x1, r0, r1, t0, t1;
+  f2_unpack(x2, x0, x1);
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-127.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-127.0f));
+  x2 = f2_pack(x0, x1);
+  const auto both = [](float c) { return f2_pack(c, c); };
+  const uint64_t t2 = f2_add(x2, both(12582912.0f));  // 1.5 * 2^23: i in the last bits
+  const uint64_t f2 = f2_fma(f2_add(t2, both(-12582912.0f)), both(-1.0f), x2);
+  uint64_t r2 = f2_fma(both(0.009585382416844368f), f2, both(0.05590662732720375f));
+  r2 = f2_fma(r2, f2, both(0.24024038016796112f));
+  r2 = f2_fma(r2, f2, both(0.6931241750717163f));
+  r2 = f2_fma(r2, f2, both(1.0f));
+  f2_unpack(t2, t0, t1);
+  f2_unpack(r2, r0, r1);
+  r0 = __int_as_float(__float_as_int(r0) + (__float_as_int(t0) << 23));
+  r1 = __int_as_float(__float_as_int(r1) + (__float_as_int(t1) << 23));
+  return f2_fma(x2, both(0.0f), f2_pack(r0, r1));
+}
+
 // Softmax of kCols score columns of this thread's row, its copy's share of one half of a block:
 // columns [col0, col0 + kCols) of the block, col0 = 64 half + copy * kCols, in TMEM at tS + col0.
 // P goes over the half's scores, zeros in the other copies' shares. m / l: running maximum (log2
@@ -198,10 +221,15 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
   uint32_t pk[kFp8 ? 1 : kCols / 2];
 #pragma unroll
   for (int j = 0; j < kCols; j += 2) {
-    float x0, x1;
-    f2_unpack(f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2), x0, x1);
-    s[j] = fast_exp2(x0);
-    s[j + 1] = fast_exp2(x1);
+    const uint64_t x2 = f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2);
+    if (kCols == 64 && (j & 7) == 6) {
+      f2_unpack(exp2_pair(x2), s[j], s[j + 1]);
+    } else {
+      float x0, x1;
+      f2_unpack(x2, x0, x1);
+      s[j] = fast_exp2(x0);
+      s[j + 1] = fast_exp2(x1);
+    }
     sum2 = f2_add(sum2, f2_pack(s[j], s[j + 1]));
     if constexpr (!kFp8) pk[j / 2] = pack_bf16x2(s[j], s[j + 1]);
   }
