@@ -19,6 +19,7 @@ stream and has no counterpart.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Sequence, Union
 
@@ -35,8 +36,8 @@ _FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_f
 _ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
 _PAGES_WORK = LIB.h3sa_pages_workspace
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_I32, _U8, _F32, _BF16, _E4M3 = torch.int32, torch.uint8, torch.float32, torch.bfloat16, torch.float8_e4m3fn
-_empty, _empty_like = torch.empty, torch.empty_like
+_I32, _F32, _BF16, _E4M3 = torch.int32, torch.float32, torch.bfloat16, torch.float8_e4m3fn
+_empty_like = torch.empty_like
 
 
 def _bad(t: torch.Tensor, device: torch.device, dtype: torch.dtype, shape: tuple[int, ...]) -> bool:
@@ -55,21 +56,11 @@ def _error_word(what: str, device: torch.device, word: torch.Tensor | None) -> i
     return word.data_ptr()
 
 
-class _Current:
-    """The current stream: nothing to switch."""
-
-    def __enter__(self) -> None:
-        return None
-
-    def __exit__(self, *exc: object) -> None:
-        return None
-
-
-_CURRENT = _Current()
+_CURRENT = contextlib.nullcontext()
 
 
 def _on(stream: torch.cuda.Stream | None):
-    """Results and workspaces are allocated on the stream that uses them."""
+    """Results and workspaces are allocated on the stream that uses them; the current one needs no switch."""
 
     return _CURRENT if stream is None else torch.cuda.stream(stream)
 
@@ -156,10 +147,10 @@ def fork_pages(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, r
         raise ValueError(f"{what}: reserve_rows must not be negative")
     p = _pools(what, pools, pages, device)
     with _on(stream):
-        child_table = _empty((children, width), dtype=_I32, device=device)
+        child_table = table.new_empty((children, width))
         child_lengths = _empty_like(parents)
         refs_out = _empty_like(refs)
-        work = _empty(_PAGES_WORK(pages, children), dtype=_U8, device=device)
+        work = refs.new_empty(_PAGES_WORK(pages, children) // 4)
     code = _FORK(p, table.data_ptr(), sequences, width, lengths.data_ptr(), refs.data_ptr(),
                  parents.data_ptr(), children, int(reserve_rows), 1 if private else 0,
                  child_table.data_ptr(), child_lengths.data_ptr(), refs_out.data_ptr(),
@@ -183,8 +174,8 @@ def compact_pages(pools: PoolTensors, table: torch.Tensor, refs: torch.Tensor, *
     p = _pools(what, pools, pages, device)
     with _on(stream):
         table_out, refs_out = _empty_like(table), _empty_like(refs)
-        live = _empty(1, dtype=_I32, device=device)
-        work = _empty(_PAGES_WORK(pages, 0), dtype=_U8, device=device)
+        live = refs.new_empty(1)
+        work = refs.new_empty(_PAGES_WORK(pages, 0) // 4)
     code = _COMPACT(p, table.data_ptr(), sequences, width, refs.data_ptr(), table_out.data_ptr(),
                     refs_out.data_ptr(), live.data_ptr(), work.data_ptr(), error,
                     _handle(stream, device))
@@ -283,8 +274,8 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     with _on(stream):
         if out is None:
             out = (_empty_like(query) if query.is_contiguous() else
-                   _empty(query.shape, dtype=_BF16, device=device))
-        work = _empty(need, dtype=_U8, device=device)
+                   query.new_empty(shape))
+        work = lengths.new_empty(need // 4)
     code = _ATTEND(query.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(),
                    None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
                    key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
