@@ -8,7 +8,7 @@
 //
 // In the split form an item is either a span of all branches' rows stacked (b, i, and the query
 // heads of the KV head's group) against the shared blocks, which are so read once for all, or the
-// rows of one branch against its own blocks; in the joint form (branches with many rows each) an
+// rows of one branch against its own blocks; in the joint form (see joint_form) an
 // item is a span of one branch's rows against all its blocks. There are two kernels for them, the
 // tensor line here (items of up to 256 rows, tcgen05) and the warp line in h3sa_branch_rows.cu
 // (items of 16 rows, each warp by itself); shape_of says which takes what. Either one's units,
@@ -37,6 +37,12 @@
 // by a power of two to a maximum in [128, 256), and P are both given as a sum of two e4m3 terms,
 // whose products add up in fp32. Two terms keep at least 8 significant bits, as bf16 does, down to
 // 2^-18 of the row's maximum, and K and V need no conversion pass.
+//
+// Measured: 3 branches of 1211 rows, 24 heads, to 15.7 K keys, bf16, joint: 640 to 750 us (0.86 to
+// 1.0 PFLOP/s, by power), the tensor pipe 53 % active; what bounds it is the softmax's latency, 2000 cycles
+// a half block of both tiles in step, 1024 of them 2^x. 60 stacked rows of 8 KV heads over 98304 e4m3 keys:
+// 80 us (2.5 TB/s), bound by the round trips of half blocks; 9 us go by before the first scores (all
+// CTAs' first loads and queries at once) and 5 in the epilogue.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -134,7 +140,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// 2^x of a pair, x below 128, on the multiply-add pipe: x = i + f with |f| <= 1/2, 2^f as a polynomial
+// 2^x of a pair, x below 128, on the multiply-add pipe, which takes over a quarter of full tiles' (joint
+// chunks 684 -> 640 us; an eighth 660, three eighths 670, half 716): x = i + f with |f| <= 1/2, 2^f as a polynomial
 // (least maximum relative error of its degree with 2^0 = 1 exactly: 2^-18.4), i added to the exponent.
 // From x = -127 down the result is 0; NaN stays NaN.
 __device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
@@ -1151,10 +1158,19 @@ int sm_count() {
   return counts[dev];
 }
 
-// The split form reads the shared blocks once for all branches but merges two partial results per
-// row; with many rows per branch each tile is full within one branch and the joint form has
-// nothing to merge.
-constexpr int kJointRows = 2 * kSpan;
+// The split form reads the shared blocks once for all branches, but every row has partial results to
+// merge; in the joint form an item that no CTA shares is written out as it is. So branches of more
+// than a tile take the joint form if it makes items enough, or takes hardly more of them than the
+// stacked rows do, and not so few that many CTAs share each. 8 KV heads, own lengths to 700, bf16,
+// joint / split (us): 24 branches of 200 rows, 2048 shared keys 86 / 135, 8192 keys 203 / 267 (192 items);
+// 40 of 130, 112 / 154 and 287 / 290 (320); 8 of 180, 42 / 57 and 82 / 95 (64); 3 of 300, 46 / 46 and
+// 109 / 96 at 13312 keys (48); 3 of 200, 33 / 38 and 68 / 75 (24, as stacked); 3 of 150, 31 / 30 and
+// 51 / 48 (24, stacked 16); 2 of 200, 31 / 30 and 46 / 48 (16); 1 of 300, 36 / 30 and 49 / 46 (16).
+bool joint_form(long long own, int batch, int kv_heads) {
+  const auto spans = [](long long n) { return (n + kSpan - 1) / kSpan; };
+  const long long each = batch * spans(own), items = each * kv_heads, workers = sm_count();
+  return own > kBlk && (5 * items >= 2 * workers || (8 * items >= workers && 4 * each <= 5 * spans(own * batch)));
+}
 
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
 // tensor line passes a dozen barriers; what it costs is that every 16 rows read K and V again.
@@ -1163,6 +1179,8 @@ constexpr int kJointRows = 2 * kSpan;
 // 4096 keys 48 / 43; 32 rows, 16384 keys 31 / 38, 65536 keys 97 / 78; 16 rows, 65536 keys 57 / 75.
 // e4m3, 60 rows, 16384 keys 43 / 47, 65536 keys 128 / 75; 32 rows, 65536 keys 72 / 65; 16 rows 47 / 61.
 // So: always up to one tile of rows, else up to the product where the two meet.
+// A branch's own rows, 2 KV heads over 1024 shared keys: 8 branches, own lengths to 2000, warp / tensor:
+// 32 rows 18 / 23, 64 rows 23 / 27, 128 rows 33 / 31; 40 branches, to 1000: 28 / 34, 45 / 40, 61 / 49.
 constexpr int kWarpOwnRows = 64;
 constexpr long long kWarpSharedWork = 500000;  // KV heads x keys x 16-row tiles
 // The least part of a worker, in units: a piece costs the merge as much as some more keys cost the
@@ -1177,7 +1195,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   const long long own = static_cast<long long>(rows) * group;
   const long long all = own * batch;
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
-  s.joint = own >= kJointRows ? 1 : 0;
+  s.joint = joint_form(own, batch, kv_heads) ? 1 : 0;
   s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
   s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
   Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;

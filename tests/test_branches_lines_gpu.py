@@ -129,8 +129,13 @@ def test_oracles_agree() -> None:
     ([900, 1300], 2, 100, 4, 2),                               # 200: both tiles
     ([1000, 1400], 2, 75, 8, 2),                               # 300: a span, then two copies of 44
     ([2000, 1400], 2, 69, 8, 2),                               # 276: a span, then four copies of 20
-    ([5000, 3000], 3, 512, 3, 3),                              # joint: every row by itself
-    ([2100, 2600], 3, 900, 2, 1),                              # joint, ragged
+    ([5000, 3000], 3, 512, 3, 3),                              # few items of many rows
+    ([2100, 2600], 3, 900, 2, 1),                              # the same, ragged
+    ([1000 + 64 * b for b in range(9)], 2, 130, 8, 8),         # joint: a tile and two rows
+    ([2100, 0, 2600, 700], 3, 515, 8, 8),                      # joint: two spans and three rows; an idle one
+    ([900, 1300, 641, 5000], 5, 300, 16, 8),                   # joint: the last span has 88 rows
+    ([700, 1300], 1, 257, 24, 24),                             # joint: one row in the last span
+    ([3000, 2000, 1000], 7, 250, 6, 6),                        # joint, no more items than the stacked rows make
 ])
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_of_many_rows(lengths, shared, rows, heads, kv, kind, causal) -> None:
