@@ -1281,9 +1281,12 @@ int launch(const BranchParams& p, cudaStream_t stream) {
     const int rc = launch_branch_rows(p, kFp8, tensor, cfg);
     if (rc) return rc;
   }
-  // Four warps share a row where rows are few: its pieces are read one latency after another.
+  // Four warps share a row where rows are few, or not too many and in as many pieces as the tensor line
+  // cuts a shared item into: its pieces are read one latency after another. One warp / four (us of the
+  // whole call): 126 rows 13.8 / 12.8; 256 rows of 4096 shared keys (warp line) 19.8 / 17.1; 480 rows of
+  // 1024 (warp line) 14.6 / 18.0, of 98304 (tensor line) 105.6 / 103.6; 2400 rows 57.4 / 58.5.
   const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
-  const bool team = !p.joint && p.shared > 0 && stacked <= 16ll * p.tensor.workers;
+  const bool team = !p.joint && stacked <= (p.tensor.shared_tiles > 0 ? 4ll : 2ll) * p.tensor.workers;
   const long long blocks =
       p.joint ? static_cast<long long>(p.kv_heads) * p.batch * p.tensor.own_tiles * (kSpan / (kJointWarpRows * kMergeWarps))
       : team  ? stacked
