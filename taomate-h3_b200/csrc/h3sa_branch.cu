@@ -1158,18 +1158,24 @@ int sm_count() {
   return counts[dev];
 }
 
-// The split form reads the shared blocks once for all branches, but every row has partial results to
-// merge; in the joint form an item that no CTA shares is written out as it is. So branches of more
-// than a tile take the joint form if it makes items enough, or takes hardly more of them than the
-// stacked rows do, and not so few that many CTAs share each. 8 KV heads, own lengths to 700, bf16,
-// joint / split (us): 24 branches of 200 rows, 2048 shared keys 86 / 135, 8192 keys 203 / 267 (192 items);
-// 40 of 130, 112 / 154 and 287 / 290 (320); 8 of 180, 42 / 57 and 82 / 95 (64); 3 of 300, 46 / 46 and
-// 109 / 96 at 13312 keys (48); 3 of 200, 33 / 38 and 68 / 75 (24, as stacked); 3 of 150, 31 / 30 and
-// 51 / 48 (24, stacked 16); 2 of 200, 31 / 30 and 46 / 48 (16); 1 of 300, 36 / 30 and 49 / 46 (16).
-bool joint_form(long long own, int batch, int kv_heads) {
-  const auto spans = [](long long n) { return (n + kSpan - 1) / kSpan; };
-  const long long each = batch * spans(own), items = each * kv_heads, workers = sm_count();
-  return own > kBlk && (5 * items >= 2 * workers || (8 * items >= workers && 4 * each <= 5 * spans(own * batch)));
+// Branches of up to this many rows have them on the warp line. 2 KV heads over 1024 shared keys, warp /
+// tensor (us): 8 branches, own lengths to 2000: 32 rows 18 / 23, 64 rows 23 / 27, 128 rows 33 / 31; 40
+// branches, to 1000: 28 / 34, 45 / 40, 61 / 49.
+constexpr int kWarpOwnRows = 64;
+
+// The split form reads the shared blocks once for all branches and packs their rows into full tiles, but
+// every row has partial results to merge; in the joint form an item that no CTA shares is written out
+// as it is. So the joint form is taken where items are enough, and where the rows that its last tiles
+// lack, times the shared blocks, stay below some blocks a row. 8 KV heads, own lengths to 700, bf16, joint /
+// split (us) by branches x rows: 24 x 200, 2048 shared keys 86 / 135, 8192 keys 203 / 267; 8 x 180, 42 / 57
+// and 82 / 95; 40 x 130, 112 / 154 and 287 / 290; 3 x 200, 33 / 38 and (13312 keys) 68 / 75; 3 x 300, 46 / 46
+// and (13312) 109 / 96; 24 x 128, 1024 keys 58 / 85, 8192 keys 161 / 169; 24 x 100, 55 / 75 and 156 / 143; 40 x
+// 70, 77 / 94 and 228 / 177. Few items: 2 x 200, 2048 keys 31 / 30; 1 x 300, 36 / 30; 1 x 100, 35 / 25.
+bool joint_form(long long own, int batch, int kv_heads, int shared) {
+  const long long workers = sm_count(), items = static_cast<long long>(kv_heads) * batch * ((own + kSpan - 1) / kSpan);
+  const long long lack = (kBlk - own % kBlk) % kBlk;
+  if (own <= kWarpOwnRows) return false;
+  return own > kBlk ? 8 * items >= workers && lack * shared <= 28 * own : 5 * items >= 2 * workers && lack * shared <= 12 * own;
 }
 
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
@@ -1179,9 +1185,6 @@ bool joint_form(long long own, int batch, int kv_heads) {
 // 4096 keys 48 / 43; 32 rows, 16384 keys 31 / 38, 65536 keys 97 / 78; 16 rows, 65536 keys 57 / 75.
 // e4m3, 60 rows, 16384 keys 43 / 47, 65536 keys 128 / 75; 32 rows, 65536 keys 72 / 65; 16 rows 47 / 61.
 // So: always up to one tile of rows, else up to the product where the two meet.
-// A branch's own rows, 2 KV heads over 1024 shared keys: 8 branches, own lengths to 2000, warp / tensor:
-// 32 rows 18 / 23, 64 rows 23 / 27, 128 rows 33 / 31; 40 branches, to 1000: 28 / 34, 45 / 40, 61 / 49.
-constexpr int kWarpOwnRows = 64;
 constexpr long long kWarpSharedWork = 500000;  // KV heads x keys x 16-row tiles
 // The least part of a worker, in units: a piece costs the merge as much as some more keys cost the
 // warp, and more so beside the tensor line, whose time hides the warps'. 24 branches of 4 x 32 rows,
@@ -1195,7 +1198,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   const long long own = static_cast<long long>(rows) * group;
   const long long all = own * batch;
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
-  s.joint = joint_form(own, batch, kv_heads) ? 1 : 0;
+  s.joint = joint_form(own, batch, kv_heads, shared) ? 1 : 0;
   s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
   s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
   Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;

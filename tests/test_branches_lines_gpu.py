@@ -135,6 +135,8 @@ def test_oracles_agree() -> None:
     ([2100, 0, 2600, 700], 3, 515, 8, 8),                      # joint: two spans and three rows; an idle one
     ([900, 1300, 641, 5000], 5, 300, 16, 8),                   # joint: the last span has 88 rows
     ([700, 1300], 1, 257, 24, 24),                             # joint: one row in the last span
+    ([900 + 40 * b for b in range(11)], 4, 100, 6, 6),         # joint: a tile each, not full
+    ([700 + 90 * b for b in range(8)], 0, 33, 24, 8),          # the same with nothing shared, three heads a KV head
     ([3000, 2000, 1000], 7, 250, 6, 6),                        # joint, no more items than the stacked rows make
 ])
 @pytest.mark.parametrize("causal", [False, True])
