@@ -1178,6 +1178,16 @@ bool joint_form(long long own, int batch, int kv_heads, int shared) {
   return own > kBlk ? 8 * items >= workers && lack * shared <= 28 * own : 5 * items >= 2 * workers && lack * shared <= 12 * own;
 }
 
+// Short tables on the warp line: a warp takes a branch's rows against all its keys, shared ones too, and
+// there is nothing to merge. 0.6 us a 32-key unit and warp then stand against the merge's launch and the
+// better spread. Whole / split (us), 3, 5 and 9 blocks a branch: 6 items 10.1 / 10.5, 15.0 / 10.1, 24.8 / 10.1; 96
+// items 10.5 / 11.8, 15.5 / 12.2, 25.5 / 13.5; 128 items 10.6 / 16.4, 15.6 / 17.3, 25.6 / 20.7; 512 items 11.3 /
+// 21.3, 16.5 / 23.5, 27.2 / 29.1; 1600 items 28.3 / 36.3, 44.4 / 38.7, 75.7 / 48.2.
+bool whole_form(int width, int kv_heads, int batch, const Line& warp) {
+  const long long items = static_cast<long long>(kv_heads) * batch * warp.own_tiles;
+  return items > 0 && width <= (5 * items < warp.workers ? 3 : items <= warp.workers ? 6 : 4);
+}
+
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
 // tensor line passes a dozen barriers; what it costs is that every 16 rows read K and V again.
 // Shared blocks under 8 KV heads, both lines, with merge and own parts (us, warp / tensor): bf16,
@@ -1282,7 +1292,7 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   if (p.warp.own_tiles > 0) {  // takes the SMs that the other line is done with
     cfg.numAttrs = tensor ? 1 : 0;
     const int rc = launch_branch_rows(p, kFp8, tensor, cfg);
-    if (rc) return rc;
+    if (rc || p.whole) return rc;
   }
   // Four warps share a row where rows are few, or not too many and in as many pieces as the tensor line
   // cuts a shared item into: its pieces are read one latency after another. One warp / four (us of the
@@ -1355,7 +1365,7 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
     return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d is too large",
                      batch, rows, heads);
-  const Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
+  Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
   const auto line_units = [&](const Line& ln) {
     const int64_t blocks = kBlk / ln.unit;
     return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks + ln.pad) +
@@ -1386,6 +1396,10 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   p.shared = shared_rows / kBlk;
   p.causal = causal ? 1 : 0;
   p.joint = s.joint;
+  if (whole_form(width, kv_heads, batch, s.warp)) {
+    p.whole = p.joint = 1;
+    s.tensor.shared_tiles = s.warp.shared_tiles = 0;
+  }
   p.pool_pages = pool_pages;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.k_scale = k_scale;

@@ -41,6 +41,7 @@ struct BranchParams {
   int width, batch, rows, heads, kv_heads, group;
   int shared;                  // leading blocks shared by all sequences
   int causal, joint;
+  int whole;                   // the warp line takes whole items
   int pool_pages;
   float scale_log2;
   const float* k_scale;        // e4m3: [kv_heads]

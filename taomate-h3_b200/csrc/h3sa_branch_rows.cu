@@ -4,10 +4,10 @@
 //   x_j = scale * q . k_j,   O = sum_j 2^(x_j' - m) v_j,   l = sum_j 2^(x_j' - m),   x' = x log2 e
 //
 // Sixteen rows use a key 2 * 16 * 2 * 128 flops for its 512 bytes: the kernel is bound by reading K
-// and V, and for a branch's own few blocks by latency. So a warp works alone, without a barrier
-// but that of its own copies: it keeps 48 KB of keys and values, three units of 32 keys or six in e4m3,
-// on their way from memory by TMA, across the ends of its items, and four warps an SM have 192 KB
-// in flight. Reading straight into registers, which hold one unit, took 40.1 us where this takes
+// and V, and for a branch's own few blocks by latency. So a warp works alone, with
+// another that starts its copies: 48 KB of keys and values, three units of 32 keys or six in e4m3,
+// are on their way from memory by TMA, across the ends of its items, and the four pairs of an SM have
+// 192 KB in flight. Starting the copies itself cost a warp 600 of 1800 cycles a unit. Reading straight into registers, which hold one unit, took 40.1 us where this takes
 // 35.0 (60 rows of 8 KV heads over 4096 shared keys and up to 1000 of their own), 44.3 against 41.2
 // for one row of 24 heads over 16384 keys: 201 MB, 0.75 of the measured copy rate with launch and merge.
 //
@@ -80,22 +80,28 @@ struct RowSegment {
   long long slot;
 };
 
-template <bool kFp8>
-__global__ void __launch_bounds__(32 * kRowWarps, 1)
+// kWhole: no line; a warp takes whole items, a branch's rows against all its keys, and nothing is left
+// to merge.
+template <bool kFp8, bool kWhole>
+__global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     branch_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const BranchParams p, const bool after) {
   constexpr int kTileBytes = RowCfg<kFp8>::kTileBytes, kStageBytes = RowCfg<kFp8>::kStageBytes;
   constexpr int kRowStages = RowCfg<kFp8>::kStages;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t full[kRowWarps][kMaxRowStages];
+  __shared__ uint64_t full[kRowWarps][kMaxRowStages], empty[kRowWarps][kMaxRowStages];
   __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const int warp = (threadIdx.x >> 5) & (kRowWarps - 1), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+  const bool loader = threadIdx.x >= 32 * kRowWarps;
   const uint32_t ring = ((smem_u32(smem_raw) + 1023u) & ~1023u) + warp * kRowRing;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kRowWarps; ++w)
-      for (int s = 0; s < kRowStages; ++s) mbar_init(smem_u32(&full[w][s]), 1);
+      for (int s = 0; s < kRowStages; ++s) {
+        mbar_init(smem_u32(&full[w][s]), 1);
+        mbar_init(smem_u32(&empty[w][s]), 1);
+      }
     abort_word = 0;
     fence_mbar_init();
   }
@@ -105,18 +111,49 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
   }
   const Line& ln = p.warp;
   const int worker = blockIdx.x * kRowWarps + warp;
-  const Plan pl = make_plan(p, ln, lane);
-  const int all = pl.head_weight * p.kv_heads, own_all = p.rows * p.group;
-  int u = min(all, worker * pl.cut);
-  const int u_end = min(all, u + pl.cut);
+  const int own_all = p.rows * p.group;
+  Plan pl;
+  int u, u_end;  // this warp's part of the line; kWhole: its next item, and how many there are
   Place at = {0, -1, 0, 0};
-  if (u < u_end) at = locate(p, ln, pl, u, lane);
+  if constexpr (kWhole) {
+    u = warp * gridDim.x + blockIdx.x;  // few items: one an SM
+    u_end = p.kv_heads * p.batch * ln.own_tiles;
+  } else {
+    pl = make_plan(p, ln, lane);
+    const int all = pl.head_weight * p.kv_heads;
+    u = min(all, worker * pl.cut);
+    u_end = min(all, u + pl.cut);
+    if (u < u_end) at = locate(p, ln, pl, u, lane);
+  }
   __syncthreads();
 
-  // The next segment of this warp's part (units 0: there is none).
+  // The next segment of this pair of warps' part (units 0: there is none).
   const auto next_segment = [&]() {
     RowSegment g;
     g.units = 0;
+    if constexpr (kWhole) {
+      for (; u < u_end && g.units == 0; u += gridDim.x * kRowWarps) {
+        const int bh = u / ln.own_tiles, t = u - bh * ln.own_tiles;
+        g.head = bh / p.batch;
+        g.seq = bh - g.head * p.batch;
+        g.shared = 0;
+        g.row0 = g.seq * own_all + t * kRowSpan;
+        g.n_rows = min(kRowSpan, own_all - t * kRowSpan);
+        g.key0 = 0;
+        g.kv_end = seq_length(p, g.seq);
+        g.direct = 1;
+        g.slot = 0;
+        g.units = own_units(p, ln, g.kv_end, t);
+        if (g.units > 0) continue;
+        for (int i = lane; !loader && i < g.n_rows * 16; i += 32) {  // rows that see nothing
+          const RowAt ra = row_at(p, g.head, g.row0 + (i >> 4));
+          const long long id = (static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h;
+          reinterpret_cast<uint4*>(p.out + id * kD)[i & 15] = make_uint4(0u, 0u, 0u, 0u);
+          if (p.lse && (i & 15) == 0) p.lse[id] = -INFINITY;
+        }
+      }
+      return g;
+    }
     while (u < u_end && g.units == 0) {
       const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
       const int n = min(units, at.off + part) - at.off;
@@ -149,33 +186,63 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
     }
     return page;
   };
-  int issued = 0, used = 0;  // units whose copies were started, and that were waited for
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  const bool once = ln.shared_tiles <= 1 && ln.own_tiles <= 1;  // keys that only one warp reads
-  const auto issue = [&](const RowSegment& g, int i, int page) {
-    if (lane == 0) {
-      const int s = issued % kRowStages, row = page * kBlk + ((g.key0 + i * kRowUnit) & (kBlk - 1));
-      const uint32_t bar = smem_u32(&full[warp][s]);
-      mbar_expect_tx(bar, kStageBytes);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-        for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
-          const uint32_t dst = ring + s * kStageBytes + kv * kTileBytes + a * (kTileBytes / 2);
-          if (once) tma_load_3d_once(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head, policy);
-          else tma_load_3d(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head);
-        }
-    }
-    ++issued;
-  };
-
-  RowSegment g = next_segment();
-  int pages = g.units > 0 ? pages_of(g, 0) : 0, ahead = 0;  // units of g that were started
-  for (; ahead < min(kRowStages, g.units); ++ahead)
-    issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7)));
   bool ok = true;
-  while (ok && g.units > 0) {
+  int stage = 0, phase = 0;
+  const auto advance = [&]() {
+    if (++stage == kRowStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  };
+  if (loader) {
+    // ================================================================ copies
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    const bool once = !kWhole && ln.shared_tiles <= 1 && ln.own_tiles <= 1;  // keys that only one warp reads
+    int issued = 0;
+    for (RowSegment g = next_segment(); ok && g.units > 0; g = next_segment()) {
+      int pages = 0, pages_from = -32;  // the block (of the segment) whose page lane 0 holds
+      for (int i = 0; i < g.units; ++i) {
+        const int key = g.key0 + i * kRowUnit, block = (key >> 7) - (g.key0 >> 7);
+        if (block - pages_from >= 32) {
+          pages_from = block;
+          pages = pages_of(g, block);
+        }
+        const int row = __shfl_sync(0xffffffffu, pages, block - pages_from) * kBlk + (key & (kBlk - 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[warp][stage]), phase ^ 1, abort_flag, p.err));
+        if (!ok) break;
+        if (lane == 0) {
+          const uint32_t bar = smem_u32(&full[warp][stage]);
+          mbar_expect_tx(bar, kStageBytes);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int a = 0; a < (kFp8 ? 1 : 2); ++a) {
+              const uint32_t dst = ring + stage * kStageBytes + kv * kTileBytes + a * (kTileBytes / 2);
+              if (once) tma_load_3d_once(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head, policy);
+              else tma_load_3d(dst, kv ? &tmV : &tmK, bar, a * 64, row, g.head);
+            }
+        }
+        ++issued;
+        advance();
+      }
+    }
+    if (!ok) {
+      // leaving early: no copy may still be in flight when the block ends
+      for (int k = min(issued, kRowStages); k > 0; --k) {
+        if (--stage < 0) {
+          stage = kRowStages - 1;
+          phase ^= 1;
+        }
+        const unsigned long long t0 = global_ns();
+        while (!mbar_try_wait(smem_u32(&full[warp][stage]), phase) && global_ns() - t0 < kWaitTimeoutNs) {
+        }
+      }
+    }
+    return;
+  }
+  // ================================================================ products and softmax
+  for (RowSegment g = next_segment(); g.units > 0; g = next_segment()) {
     // this lane's rows, r and r + 8 of the item
     const RowAt at0 = row_at(p, g.head, g.row0 + min(r, g.n_rows - 1));
     const RowAt at1 = row_at(p, g.head, g.row0 + min(r + 8, g.n_rows - 1));
@@ -191,8 +258,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
         load16(b + from, qb + 4 * k);
       }
     }
-    const RowSegment next = next_segment();
-    int next_pages = next.units > 0 ? pages_of(next, 0) : 0, next_ahead = 0;
     const int lim0 = seq_length(p, at0.b) - (p.causal ? p.rows - 1 - at0.i : 0);
     const int lim1 = seq_length(p, at1.b) - (p.causal ? p.rows - 1 - at1.i : 0);
     float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
@@ -230,14 +295,11 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    int pages_from = 0;  // the block (of the segment) whose page lane 0 holds
 #pragma unroll 1
     for (int i = 0; i < g.units; ++i) {
-      const int st = used % kRowStages;
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[warp][st]), (used / kRowStages) & 1, abort_flag, p.err));
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[warp][stage]), phase, abort_flag, p.err));
       if (!ok) break;
-      ++used;
-      const uint32_t kt = ring + st * kStageBytes, vt = kt + kTileBytes;
+      const uint32_t kt = ring + stage * kStageBytes, vt = kt + kTileBytes;
       const int key = g.key0 + i * kRowUnit;
       float s[4][4];
 #pragma unroll
@@ -342,20 +404,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
           }
         }
       }
-      __syncwarp();  // every lane has read the stage: the next unit may go there
-      if (ahead < g.units) {
-        const int block = ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7);
-        if (block - pages_from >= 32) {
-          pages_from = block;
-          pages = pages_of(g, block);
-        }
-        issue(g, ahead, __shfl_sync(0xffffffffu, pages, block - pages_from));
-        ++ahead;
-      } else if (next_ahead < next.units) {
-        issue(next, next_ahead,
-              __shfl_sync(0xffffffffu, next_pages, ((next.key0 + next_ahead * kRowUnit) >> 7) - (next.key0 >> 7)));
-        ++next_ahead;
-      }
+      __syncwarp();  // every lane has read the stage
+      if (lane == 0) mbar_arrive(smem_u32(&empty[warp][stage]));
+      advance();
     }
     if (!ok) break;
     l0 = quad_sum(l0);
@@ -390,30 +441,17 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1)
         else if (p.lse) p.lse[id] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       }
     }
-    g = next;
-    pages = next_pages;
-    ahead = next_ahead;
-    for (; ahead < min(kRowStages, g.units); ++ahead)  // what the last segment left no time for
-      issue(g, ahead, __shfl_sync(0xffffffffu, pages, ((g.key0 + ahead * kRowUnit) >> 7) - (g.key0 >> 7)));
-  }
-  if (!ok) {
-    // leaving early: no copy may still be in flight when the block ends
-    for (; used < issued; ++used) {
-      const unsigned long long t0 = global_ns();
-      while (!mbar_try_wait(smem_u32(&full[warp][used % kRowStages]), (used / kRowStages) & 1) &&
-             global_ns() - t0 < kWaitTimeoutNs) {
-      }
-    }
   }
   if (worker == 0) {
     flag_lengths(p, lane);
-    write_plan(p, ln, pl, p.plan + 3 + p.batch, lane);
+    if constexpr (!kWhole) write_plan(p, ln, pl, p.plan + 3 + p.batch, lane);
   }
-  // what follows this kernel needs the other line's too
-  if (after) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // what follows this kernel needs the other line's too; one block's wait holds it, and the others make
+  // room for it
+  if (after && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <bool kFp8>
+template <bool kFp8, bool kWhole>
 int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   static std::mutex mu;
   static bool done[64] = {};
@@ -422,7 +460,7 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(kRowSmem));
       if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch rows)", e);
       if (dev < 64) done[dev] = true;
@@ -432,17 +470,19 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   int rc = encode_pool(&tmK, p, p.key_pool, kFp8, kRowUnit);
   if (!rc) rc = encode_pool(&tmV, p, p.value_pool, kFp8, kRowUnit);
   if (rc) return rc;
-  cfg.gridDim = dim3(p.warp.workers / kRowWarps);
-  cfg.blockDim = dim3(32 * kRowWarps);
+  const int sms = p.warp.workers / kRowWarps;
+  cfg.gridDim = dim3(kWhole ? min(sms, p.kv_heads * p.batch * p.warp.own_tiles) : sms);
+  cfg.blockDim = dim3(2 * 32 * kRowWarps);
   cfg.dynamicSmemBytes = kRowSmem;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8>, tmK, tmV, p, after);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8, kWhole>, tmK, tmV, p, after);
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_rows_kernel launch", e);
 }
 
 }  // namespace
 
 int launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
-  return e4m3 ? launch_rows<true>(p, after, cfg) : launch_rows<false>(p, after, cfg);
+  if (p.whole) return e4m3 ? launch_rows<true, true>(p, after, cfg) : launch_rows<false, true>(p, after, cfg);
+  return e4m3 ? launch_rows<true, false>(p, after, cfg) : launch_rows<false, false>(p, after, cfg);
 }
 
 int encode_pool(CUtensorMap* map, const BranchParams& p, const void* pool, bool e4m3, int rows) {
