@@ -1159,8 +1159,8 @@ int sm_count() {
 }
 
 // Branches of up to this many rows have them on the warp line. 2 KV heads over 1024 shared keys, warp /
-// tensor (us): 8 branches, own lengths to 2000: 32 rows 18 / 23, 64 rows 23 / 27, 128 rows 33 / 31; 40
-// branches, to 1000: 28 / 34, 45 / 40, 61 / 49.
+// tensor (us): 8 branches, own lengths to 2000: 32 rows 16 / 24, 64 rows 19 / 25; 40 branches, to 1000: 25 /
+// 34, 39 / 40; over 8192 shared keys and up to 300 59 / 60, e4m3 69 / 67.
 constexpr int kWarpOwnRows = 64;
 
 // The split form reads the shared blocks once for all branches and packs their rows into full tiles, but
@@ -1190,17 +1190,17 @@ bool whole_form(int width, int kv_heads, int batch, const Line& warp) {
 
 // Few rows go to the warp line: a warp takes 16 rows and needs none but itself, where an item of the
 // tensor line passes a dozen barriers; what it costs is that every 16 rows read K and V again.
-// Shared blocks under 8 KV heads, both lines, with merge and own parts (us, warp / tensor): bf16,
-// 60 rows, 1024 keys 17 / 27, 4096 keys 22 / 29, 16384 keys 46 / 43, 65536 keys 156 / 82; 240 rows,
-// 4096 keys 48 / 43; 32 rows, 16384 keys 31 / 38, 65536 keys 97 / 78; 16 rows, 65536 keys 57 / 75.
-// e4m3, 60 rows, 16384 keys 43 / 47, 65536 keys 128 / 75; 32 rows, 65536 keys 72 / 65; 16 rows 47 / 61.
+// Shared blocks under 8 KV heads, with merge and own parts (us, warp / tensor): bf16, 60 rows, 1024
+// keys 13 / 25, 4096 keys 20 / 27, 16384 keys 42 / 45, 65536 keys 153 / 83; 240 rows, 4096 keys 35 / 40, 16384
+// keys 100 / 50; 32 rows, 16384 keys 27 / 39, 65536 keys 94 / 78; 16 rows, 65536 keys 55 / 75. e4m3, 60 rows,
+// 16384 keys 39 / 49, 65536 keys 110 / 75; 32 rows, 65536 keys 66 / 66; 16 rows 44 / 61.
 // So: always up to one tile of rows, else up to the product where the two meet.
-constexpr long long kWarpSharedWork = 500000;  // KV heads x keys x 16-row tiles
+constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 // The least part of a worker, in units: a piece costs the merge as much as some more keys cost the
 // warp, and more so beside the tensor line, whose time hides the warps'. 24 branches of 4 x 32 rows,
-// 8192 shared keys, own lengths to 700 (us): 8 units 50.9, 4 units 55.6, 12 units 53.9; alone, 24 KV
-// heads over 1024 keys: 4 units 12.6, 8 units 16.3, 2 units 13.8.
-constexpr int kWarpLeast = 4, kWarpLeastBeside = 8;
+// 8192 shared keys, own lengths to 700 (us): 8 units 50.4, 4 units 53.0, 12 units 52.8; alone, 24 KV
+// heads over 1024 keys: 2 units 11.3, 4 units 12.2, 6 units 13.2.
+constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 
 Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   Shape s;

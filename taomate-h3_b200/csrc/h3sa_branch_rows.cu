@@ -4,12 +4,13 @@
 //   x_j = scale * q . k_j,   O = sum_j 2^(x_j' - m) v_j,   l = sum_j 2^(x_j' - m),   x' = x log2 e
 //
 // Sixteen rows use a key 2 * 16 * 2 * 128 flops for its 512 bytes: the kernel is bound by reading K
-// and V, and for a branch's own few blocks by latency. So a warp works alone, with
-// another that starts its copies: 48 KB of keys and values, three units of 32 keys or six in e4m3,
-// are on their way from memory by TMA, across the ends of its items, and the four pairs of an SM have
-// 192 KB in flight. Starting the copies itself cost a warp 600 of 1800 cycles a unit. Reading straight into registers, which hold one unit, took 40.1 us where this takes
-// 35.0 (60 rows of 8 KV heads over 4096 shared keys and up to 1000 of their own), 44.3 against 41.2
-// for one row of 24 heads over 16384 keys: 201 MB, 0.75 of the measured copy rate with launch and merge.
+// and V, and for a branch's own few blocks by latency. So a warp works alone, with another that
+// starts its copies: 48 KB of keys and values, three units of 32 keys or six in e4m3, are on their
+// way from memory by TMA, across the ends of its items, and the four pairs of an SM have 192 KB in
+// flight. A unit takes a warp 1200 cycles, 350 for S, 360 for the softmax and 440 for P V; when it
+// started its copies itself, 1800. Reading straight into registers, which hold one unit, took 40.1 us
+// where this takes 32.4 (60 rows of 8 KV heads over 4096 shared keys and up to 1000 of their own). One
+// row of 24 heads over 16384 keys, 201 MB: 41.2 us, 0.75 of the measured copy rate with launch and merge.
 //
 // mma.m16n8k16 leaves the order of the contracted index open as long as both operands agree, and so
 // the column order of the result, and the orders are chosen for the 128-byte swizzle of the tiles:
