@@ -1179,10 +1179,11 @@ bool joint_form(long long own, int batch, int kv_heads, int shared) {
 }
 
 // Short tables on the warp line: a warp takes a branch's rows against all its keys, shared ones too, and
-// there is nothing to merge. 0.6 us a 32-key unit and warp then stand against the merge's launch and the
-// better spread. Whole / split (us), 3, 5 and 9 blocks a branch: 6 items 10.1 / 10.5, 15.0 / 10.1, 24.8 / 10.1; 96
-// items 10.5 / 11.8, 15.5 / 12.2, 25.5 / 13.5; 128 items 10.6 / 16.4, 15.6 / 17.3, 25.6 / 20.7; 512 items 11.3 /
-// 21.3, 16.5 / 23.5, 27.2 / 29.1; 1600 items 28.3 / 36.3, 44.4 / 38.7, 75.7 / 48.2.
+// there is nothing to merge. 0.8 us a 32-key unit and warp (P in two terms) then stand against the merge,
+// its launch and the better spread. Whole / split (us), 1, 3 and 5 blocks a branch: 6 items 6.2 / 9.9, 12.5 / 10.5
+// (the call 27.8 / 33, for its launch), 19 / 10.1; 96 items 6.3 / 10.7, 12.8 / 11.8, 19 / 12.2; 128 items 6.4 /
+// 14.0, 12.8 / 16.4, 19.2 / 17.3; 512 items 6.9 / 15.2, 13.5 / 21.3, 20.1 / 23.5; 1600 items 14 / 25, 34 / 36,
+// 54 / 39; e4m3 512 items 6.6 / 16.6, 12.4 / 23.7, 18.2 / 26.4.
 bool whole_form(int width, int kv_heads, int batch, const Line& warp) {
   const long long items = static_cast<long long>(kv_heads) * batch * warp.own_tiles;
   return items > 0 && width <= (5 * items < warp.workers ? 3 : items <= warp.workers ? 6 : 4);

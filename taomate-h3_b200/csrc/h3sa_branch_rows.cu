@@ -75,6 +75,18 @@ __device__ __forceinline__ float quad_sum(float x) {
   return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 
+// P of two groups of eight keys as operands of bf16 and of what that leaves off, 16 bits in all. P in
+// bf16 adds as much to the error as the output's own rounding (0.0024 against 0.0017 relative). The
+// second product is taken where it costs least, for few rows (6 over 1152 keys 9.9 -> 10.0 us, 126 rows
+// 11.0 -> 11.5) and short tables (384 keys 10.4 -> 12.5); 2400 rows over 4096 keys would take 22.0 for 20.7.
+__device__ __forceinline__ void split_bf16(const float (&p)[4], const float (&q)[4], uint4& hi, uint4& lo) {
+  const auto rest = [](uint32_t h, float a, float b) {
+    return pack_bf16x2(a - __uint_as_float(h << 16), b - __uint_as_float(h & 0xffff0000u));
+  };
+  hi = make_uint4(pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3]), pack_bf16x2(q[0], q[1]), pack_bf16x2(q[2], q[3]));
+  lo = make_uint4(rest(hi.x, p[0], p[1]), rest(hi.y, p[2], p[3]), rest(hi.z, q[0], q[1]), rest(hi.w, q[2], q[3]));
+}
+
 // What a warp knows of a segment: rows row0 .. of KV head `head` against `units` units of keys from key0.
 struct RowSegment {
   int units, head, seq, shared, row0, n_rows, key0, kv_end, direct;
@@ -82,8 +94,8 @@ struct RowSegment {
 };
 
 // kWhole: no line; a warp takes whole items, a branch's rows against all its keys, and nothing is left
-// to merge.
-template <bool kFp8, bool kWhole>
+// to merge. kFine: bf16 P in two terms.
+template <bool kFp8, bool kWhole, bool kFine>
 __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     branch_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                        const BranchParams p, const bool after) {
@@ -369,13 +381,12 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       const bool tail = key + 32 > g.kv_end;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // sixteen keys
-        uint4 a;
+        uint4 a, rest;
         if constexpr (kFp8)
           a = make_uint4(f16x2_of(s[2 * h][0], s[2 * h][1]), f16x2_of(s[2 * h][2], s[2 * h][3]),
                          f16x2_of(s[2 * h + 1][0], s[2 * h + 1][1]), f16x2_of(s[2 * h + 1][2], s[2 * h + 1][3]));
         else
-          a = make_uint4(pack_bf16x2(s[2 * h][0], s[2 * h][1]), pack_bf16x2(s[2 * h][2], s[2 * h][3]),
-                         pack_bf16x2(s[2 * h + 1][0], s[2 * h + 1][1]), pack_bf16x2(s[2 * h + 1][2], s[2 * h + 1][3]));
+          split_bf16(s[2 * h], s[2 * h + 1], a, rest);
 #pragma unroll
         for (int atom = 0; atom < (kFp8 ? 1 : 2); ++atom) {
           uint4 v[4];
@@ -399,8 +410,14 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
               mma16<true>(o[4 * w + 3], a, f16x2_of_e4m3x2(xy2 >> 16), f16x2_of_e4m3x2(zt2 >> 16));
             } else {  // two
               const int n = 8 * atom + 2 * w;
-              mma16<false>(o[n], a, __byte_perm(x[w], y[w], 0x5410), __byte_perm(z[w], t[w], 0x5410));
-              mma16<false>(o[n + 1], a, __byte_perm(x[w], y[w], 0x7632), __byte_perm(z[w], t[w], 0x7632));
+              const uint32_t b0 = __byte_perm(x[w], y[w], 0x5410), b1 = __byte_perm(z[w], t[w], 0x5410);
+              const uint32_t b2 = __byte_perm(x[w], y[w], 0x7632), b3 = __byte_perm(z[w], t[w], 0x7632);
+              mma16<false>(o[n], a, b0, b1);
+              mma16<false>(o[n + 1], a, b2, b3);
+              if constexpr (kFine) {
+                mma16<false>(o[n], rest, b0, b1);
+                mma16<false>(o[n + 1], rest, b2, b3);
+              }
             }
           }
         }
@@ -452,7 +469,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
   if (after && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <bool kFp8, bool kWhole>
+template <bool kFp8, bool kWhole, bool kFine>
 int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   static std::mutex mu;
   static bool done[64] = {};
@@ -461,7 +478,7 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8, kWhole>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8, kWhole, kFine>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(kRowSmem));
       if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch rows)", e);
       if (dev < 64) done[dev] = true;
@@ -475,15 +492,18 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   cfg.gridDim = dim3(kWhole ? min(sms, p.kv_heads * p.batch * p.warp.own_tiles) : sms);
   cfg.blockDim = dim3(2 * 32 * kRowWarps);
   cfg.dynamicSmemBytes = kRowSmem;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8, kWhole>, tmK, tmV, p, after);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8, kWhole, kFine>, tmK, tmV, p, after);
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_rows_kernel launch", e);
 }
 
 }  // namespace
 
 int launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
-  if (p.whole) return e4m3 ? launch_rows<true, true>(p, after, cfg) : launch_rows<false, true>(p, after, cfg);
-  return e4m3 ? launch_rows<true, false>(p, after, cfg) : launch_rows<false, false>(p, after, cfg);
+  if (e4m3) return p.whole ? launch_rows<true, true, false>(p, after, cfg) : launch_rows<true, false, false>(p, after, cfg);
+  if (p.whole) return launch_rows<false, true, true>(p, after, cfg);
+  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
+  return kRowWarps * stacked <= p.warp.workers ? launch_rows<false, false, true>(p, after, cfg)
+                                               : launch_rows<false, false, false>(p, after, cfg);
 }
 
 int encode_pool(CUtensorMap* map, const BranchParams& p, const void* pool, bool e4m3, int rows) {
