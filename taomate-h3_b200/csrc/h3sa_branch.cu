@@ -23,6 +23,7 @@
 //               loads its K and V blocks by TMA into one ring of tiles (K0 V0 K1 V1 ...).
 //   warp 1, 2   issue the MMAs of query tile 0 and 1: S_t = Q_t K^T, then O_t += P_t V, one elected
 //               lane per tcgen05 instruction (warp 1 also owns TMEM).
+//   warp 3      e4m3: widens V to f16.
 //   warps 4-7, 8-11: softmax and epilogue of query tile 0 and 1, one thread per TMEM lane.
 // An item of more than 128 rows takes both tiles, each block being used by both; smaller items
 // take one tile per block in turn, so two blocks are in flight. Items of up to 32 (64) rows are
@@ -33,15 +34,22 @@
 // first half of its S. A tile's MMAs are issued in order by one warp, so the barrier of a QK^T also
 // says that the tile's previous P V is complete.
 //
-// e4m3 caches: K and V go to the tensor cores as they are (kind::f8f6f4); each query row, scaled
-// by a power of two to a maximum in [128, 256), and P are both given as a sum of two e4m3 terms,
-// whose products add up in fp32. Two terms keep at least 8 significant bits, as bf16 does, down to
-// 2^-18 of the row's maximum, and K and V need no conversion pass.
+// e4m3 caches: K goes to the tensor cores as it is (kind::f8f6f4), and each query row, scaled by a
+// power of two to a maximum in [128, 256), as a sum of two e4m3 terms, whose products add up in fp32. Two
+// terms hold a bf16 number exactly from 2^-2 on, and a smaller one to within 2^-10, 2^-17 of the row's
+// maximum. P cannot go that way: the terms' last step would be 2^-15 of the largest weight, and the tail
+// behind a key that dominates, thousands of keys each below that, would count in the sum and not in O. So P
+// is f16 (11 bits down to 2^-21 of a fresh maximum, steps of 2^-31 of it below), and warp 3 widens each
+// V block to f16 in shared memory, where kind::f16 takes it: one f16 product costs what two of e4m3 do, and
+// the softmax has no terms to split. Against two e4m3 terms (us): 3 x 1211 rows of 24 heads to 15.7 K keys 721 /
+// 821, 60 stacked rows of 8 KV heads over 98304 keys 97.6 / 92.2: a block's 1850 cycles in warp 3 take issue
+// slots from the softmax warps beside it.
+// P of bf16 caches is bf16, 8 bits of each weight however small, as the output has.
 //
 // Measured: 3 branches of 1211 rows, 24 heads, to 15.7 K keys, bf16, joint: 640 to 750 us (0.86 to
 // 1.0 PFLOP/s, by power), the tensor pipe 53 % active; what bounds it is the softmax's latency, 2000 cycles
 // a half block of both tiles in step, 1024 of them 2^x. 60 stacked rows of 8 KV heads over 98304 e4m3 keys:
-// 80 us (2.5 TB/s), bound by the round trips of half blocks; 9 us go by before the first scores (all
+// 87 us (2.3 TB/s), bound by the round trips of half blocks; 9 us go by before the first scores (all
 // CTAs' first loads and queries at once) and 5 in the epilogue.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -62,11 +70,6 @@ constexpr int kBrRegsSoftmax = 208;
 constexpr int kBrRegSplit = 128 * kBrRegsControl + 256 * kBrRegsSoftmax;
 constexpr int kDescRing = 4;
 constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
-// e4m3 P = 2^(x - m + boost) is at most 2^(threshold + boost) = 256 < 448. A fresh maximum sits at
-// 2^6 or above, where the second term still resolves 2^-16 of it.
-constexpr float kBoostF8 = 6.0f;
-constexpr float kThresholdF8 = 2.0f;
-constexpr float kThresholdBf16 = 8.0f;
 
 // One item segment of a CTA, as warp 0 publishes it.
 struct Segment {
@@ -85,20 +88,33 @@ template <bool kFp8>
 struct BrCfg {
   static constexpr int kElem = kFp8 ? 1 : 2;
   static constexpr int kTile = kBlk * kD * kElem;
-  static constexpr int kStages = kFp8 ? 10 : 5;
-  static constexpr int kSteps = kFp8 ? 4 : 8;      // MMA K steps of a 128-deep product
-  static constexpr int kRowsPerStep = kFp8 ? 32 : 16;
+  static constexpr int kStages = kFp8 ? 6 : 5;  // even for e4m3: K in the even slots, V in the odd ones
+  static constexpr int kSteps = kFp8 ? 4 : 8;   // MMA K steps of S
   static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
-  static constexpr uint32_t kIdescPV = kFp8 ? idesc_e4m3(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
+  static constexpr uint32_t kIdescPV = kFp8 ? idesc_f16(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
 };
 
 constexpr int kQBytes = 2 * kAtom;  // a query tile: 128 x 128 bf16, or two e4m3 terms
+
+// V of e4m3 caches in f16, blocks in turn, and the barriers between the warp that widens them and the
+// MMA warps: [tile][buffer], of the tiles as those of the ring. With a third buffer for two slots of the ring
+// 60 rows over 98304 keys take 100.7 us instead of 97.6.
+constexpr int kWide = 2;
+constexpr int kWideTile = 2 * kAtom;
+template <bool kFp8>
+struct BrWide {};
+template <>
+struct alignas(1024) BrWide<true> {
+  uint8_t v[kWide][kWideTile];
+  uint64_t full[2][kWide], empty[2][kWide];
+};
 
 template <bool kFp8>
 struct alignas(1024) BrSmem {
   using Cfg = BrCfg<kFp8>;
   uint8_t q[2][kQBytes];  // also the epilogue's staging
   uint8_t kv[Cfg::kStages][Cfg::kTile];
+  BrWide<kFp8> wide;
   Segment desc[kDescRing];
   uint64_t full[2][Cfg::kStages], empty[2][Cfg::kStages];  // [tile]; see the MMA warps
   uint64_t d_full[kDescRing], d_empty[kDescRing];
@@ -172,7 +188,6 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
 template <bool kFp8, int kCols, typename Wait>
 __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half, int copy, int limit, float sl2,
                                              bool first, float& m, float& l, Wait&& pv_done) {
-  constexpr float kThreshold = kFp8 ? kThresholdF8 : kThresholdBf16;
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
   const int col0 = 64 * half + copy * kCols;
   float s[kCols];
@@ -215,7 +230,7 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
   // kCols is a multiple of 8, so four columns are left
   const float mb = fmax3(fmax3(mx0, mx1, mx2), fmax3(mx3, s[kCols - 4], s[kCols - 3]),
                          fmaxf(s[kCols - 2], s[kCols - 1])) * sl2;
-  const bool need = mb > m + kThreshold;
+  const bool need = mb > m + kGrowth;
   const float m_new = need ? mb : m;
   const float alpha = need ? fast_exp2(m - m_new) : 1.0f;
   const bool any_need = !first && __any_sync(0xffffffffu, need);
@@ -225,7 +240,7 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
   const float bias = kBoost - (m == -INFINITY ? 0.0f : m);
   const uint64_t bias2 = f2_pack(bias, bias), scale2 = f2_pack(sl2, sl2);
   uint64_t sum2 = f2_pack(0.f, 0.f);
-  uint32_t pk[kFp8 ? 1 : kCols / 2];
+  uint32_t pk[kCols / 2];
 #pragma unroll
   for (int j = 0; j < kCols; j += 2) {
     const uint64_t x2 = f2_fma(f2_pack(s[j], s[j + 1]), scale2, bias2);
@@ -238,34 +253,14 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
       s[j + 1] = fast_exp2(x1);
     }
     sum2 = f2_add(sum2, f2_pack(s[j], s[j + 1]));
-    if constexpr (!kFp8) pk[j / 2] = pack_bf16x2(s[j], s[j + 1]);
+    pk[j / 2] = kFp8 ? f16x2_of(s[j], s[j + 1]) : pack_bf16x2(s[j], s[j + 1]);
   }
   float sa, sb;
   f2_unpack(sum2, sa, sb);
   l += sa + sb;
-  // P: bf16, two columns a word; e4m3, four columns a word, the first terms in front of the second
   uint32_t w[32];
-  if constexpr (!kFp8) {
 #pragma unroll
-    for (int j = 0; j < 32; ++j) w[j] = kCols == 64 || j / (kCols / 2) == copy ? pk[j % (kCols / 2)] : 0u;
-  } else {
-    constexpr int kW = kCols / 4;
-    uint32_t hi[kW], lo[kW];
-#pragma unroll
-    for (int j = 0; j < kW; ++j) {
-      uint32_t h0, l0, h1, l1;
-      split_e4m3x2(s[4 * j], s[4 * j + 1], h0, l0);
-      split_e4m3x2(s[4 * j + 2], s[4 * j + 3], h1, l1);
-      hi[j] = h0 | (h1 << 16);
-      lo[j] = l0 | (l1 << 16);
-    }
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const bool mine = kCols == 64 || j / kW == copy;
-      w[j] = mine ? hi[j % kW] : 0u;
-      w[16 + j] = mine ? lo[j % kW] : 0u;
-    }
-  }
+  for (int j = 0; j < 32; ++j) w[j] = kCols == 64 || j / (kCols / 2) == copy ? pk[j % (kCols / 2)] : 0u;
   pv_done();
   if (any_need) {
     tc_fence_after();
@@ -334,6 +329,43 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
   }
 }
 
+// A V block (128 rows of 128 bytes, 128-byte swizzle) from e4m3 to f16 as a bf16 block lies (two atoms of 64
+// columns), by a warp; kTail: rows at or past `rows` become zeros. A lane takes a 16-byte chunk of a row at a
+// time, eight rows in two steps, and all its offsets but two are constants. Lanes of the second atom take
+// the halves of their chunk the other way round: the eight of a phase write eight different chunks.
+template <bool kTail>
+__device__ __forceinline__ void widen_block(uint32_t from, uint32_t to, int rows, int lane) {
+  const int c = lane & 7, h = c >> 2, at = 2 * (c & 3);
+  const int r = (lane >> 4) + ((lane >> 1) & 4);  // rows r and r ^ 2 of eight; those of a half warp differ by 4
+#pragma unroll
+  for (int step = 0; step < 2; ++step) {
+    const int row = r ^ (2 * step);
+    const uint32_t src = from + row * 128 + ((c ^ row) << 4) + 8 * h;
+    const uint32_t dst = to + h * kAtom + row * 128 + (((at + h) ^ row) << 4);
+#pragma unroll 1
+    for (int i0 = 0; i0 < kBlk / 8; i0 += 8) {
+      uint2 x[8][2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];"
+                       : "=r"(x[i][k].x), "=r"(x[i][k].y)
+                       : "r"((src ^ (8 * k)) + (i0 + i) * 1024));
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (kTail && (i0 + i) * 8 + row >= rows) x[i][k] = make_uint2(0u, 0u);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((dst ^ (16 * k)) + (i0 + i) * 1024),
+                       "r"(f16x2_of_e4m3x2(x[i][k].x)), "r"(f16x2_of_e4m3x2(x[i][k].x >> 16)),
+                       "r"(f16x2_of_e4m3x2(x[i][k].y)), "r"(f16x2_of_e4m3x2(x[i][k].y >> 16))
+                       : "memory");
+        }
+    }
+  }
+}
+
 template <bool kFp8>
 __global__ void __launch_bounds__(kBrThreads, 1)
     branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -362,7 +394,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     }
     for (int s = 0; s < kDescRing; ++s) {
       mbar_init(smem_u32(&sm.d_full[s]), 1);
-      mbar_init(smem_u32(&sm.d_empty[s]), 10);  // two MMA warps and eight softmax warps
+      mbar_init(smem_u32(&sm.d_empty[s]), kFp8 ? 11 : 10);  // MMA, softmax and (e4m3) widening warps
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(smem_u32(&sm.q_full[t]), 128);
@@ -373,6 +405,13 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       mbar_init(smem_u32(&sm.pv_done[t]), 1);
       mbar_init(smem_u32(&sm.o_full[t]), 1);
       mbar_init(smem_u32(&sm.wg[t]), 128);
+    }
+    if constexpr (kFp8) {
+      for (int t = 0; t < 2; ++t)
+        for (int k = 0; k < kWide; ++k) {
+          mbar_init(smem_u32(&sm.wide.full[t][k]), 1);
+          mbar_init(smem_u32(&sm.wide.empty[t][k]), 1);
+        }
     }
     mbar_init(smem_u32(&sm.m_sync), 2);
     mbar_init(smem_u32(&sm.drain), 2);
@@ -523,8 +562,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           // a block of one tile signals that tile's barrier, a shared one tile 0's
           if ((j & 1) == 0) last_tile = pair ? 1 : last_tile ^ 1;
           const int side = pair ? 0 : last_tile;
-          used0 = pair || side == 0 ? used0 | bit : used0 & ~bit;
-          used1 = pair || side == 1 ? used1 | bit : used1 & ~bit;
+          const bool widened = kFp8 && (j & 1);  // warp 3 alone reads it, and releases it on tile 0's
+          used0 = pair || side == 0 || widened ? used0 | bit : used0 & ~bit;
+          used1 = (pair || side == 1) && !widened ? used1 | bit : used1 & ~bit;
           on_tile1 = side ? on_tile1 | bit : on_tile1 & ~bit;
           if (side) full1 ^= bit;
           else full0 ^= bit;
@@ -562,8 +602,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
     const int mt = warp - 1;
     const uint32_t klo0 = sdesc_lo(smem_u32(sm.kv[0]), 16);
-    const uint32_t vlo0 = sdesc_lo(smem_u32(sm.kv[0]), kAtom);
     constexpr uint32_t kTileDesc = Cfg::kTile >> 4;
+    uint32_t vlo0;  // V: a slot of the ring, or a widened block
+    if constexpr (kFp8) vlo0 = sdesc_lo(smem_u32(sm.wide.v[0]), kAtom);
+    else vlo0 = sdesc_lo(smem_u32(sm.kv[0]), kAtom);
     const uint32_t qlo = sdesc_lo(smem_u32(sm.q[mt]), 16);
     const uint32_t tS = tbase + static_cast<uint32_t>(mt) * 128u;
     const uint32_t tO = tbase + 256u + static_cast<uint32_t>(mt) * 128u;
@@ -571,10 +613,12 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     const uint32_t p_bar = smem_u32(&sm.p_full[mt]), o_bar = smem_u32(&sm.o_full[mt]);
     const uint32_t pv_bar = smem_u32(&sm.pv_done[mt]);
     int ring = 0;  // K tile of the next unit; V follows it
+    int wide = 0;  // e4m3: the next widened block
     // The next phase of each slot's two full barriers, a bit per slot: a tile's own blocks land
     // on its barrier, blocks of both tiles on that of tile 0. So a warp never waits on a phase
     // whose predecessor it skipped.
     uint32_t phase0 = 0u, phase1 = 0u;
+    uint32_t wide0 = 0u, wide1 = 0u;  // and those of the widened blocks' barriers
     uint32_t q_ph = 0u, p_ph = 0u, m_ph = 0u;
     int last_tile = 1;
     bool ok = true, was_solo = false;
@@ -587,10 +631,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       const bool w = mbar_wait(p_bar + half * 8, p_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
-      if (pend_rows < kBlk && half == 0) {
+      if (!kFp8 && pend_rows < kBlk && half == 0) {
         // rows past the sequence's end may hold anything, NaN among it, and the tensor core
         // multiplies them with P's zeros: clear them (the tile's load has completed; both warps
-        // of a shared block write the same zeros)
+        // of a shared block write the same zeros; e4m3: done when widened)
         uint8_t* base = sm.kv[pend_slot];
         constexpr int kAtoms = Cfg::kTile / kAtom;
         for (int i = lane; i < (kBlk - pend_rows) * kAtoms * 8; i += 32) {
@@ -600,19 +644,12 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      const uint32_t vh = vlo0 + static_cast<uint32_t>(pend_slot) * kTileDesc + half * ((64 * 128) >> 4);
+      const uint32_t vh = vlo0 + static_cast<uint32_t>(pend_slot) * (2 * kAtom >> 4) + half * ((64 * 128) >> 4);
       const uint32_t acc = pend_acc || half > 0 ? 1u : 0u;
       const uint32_t tP = tS + 64u * half;
 #pragma unroll
-      for (int kk = 0; kk < Cfg::kSteps / 2; ++kk) {
-        const uint64_t bd = sdesc_join(vh + ((kk * Cfg::kRowsPerStep * 128) >> 4));
-        if constexpr (kFp8) {
-          mma_ts_f8(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-          mma_ts_f8(tO, tP + 16 + kk * 8, bd, Cfg::kIdescPV, 1u);
-        } else {
-          mma_ts(tO, tP + kk * 8, bd, Cfg::kIdescPV, kk > 0 ? 1u : acc);
-        }
-      }
+      for (int kk = 0; kk < 4; ++kk)
+        mma_ts(tO, tP + kk * 8, sdesc_join(vh + ((kk * 16 * 128) >> 4)), Cfg::kIdescPV, kk > 0 ? 1u : acc);
       tc_commit(pv_bar);
       if (half == 1) p_ph ^= 1u;
     };
@@ -632,6 +669,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       tc_commit(s_bar + half * 8u);
     };
     const auto free_slot = [&](int slot) { tc_commit(smem_u32(&sm.empty[mt][slot])); };
+    const auto free_v = [&]() {
+      if constexpr (kFp8) tc_commit(smem_u32(&sm.wide.empty[mt][pend_slot]));
+      else free_slot(pend_slot);
+    };
     auto wait_v = [&]() { ok = __all_sync(0xffffffffu, mbar_wait(pend_bar, pend_ph, abort_flag, p.err)); };
     auto finish_item = [&]() {  // the last P V of an item
       pend = false;
@@ -640,7 +681,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (ok) finish(1);
       if (!ok) return;
       tc_commit(o_bar);
-      free_slot(pend_slot);
+      free_v();
     };
     Segment g;
     while (ok && next_segment(g)) {
@@ -681,19 +722,30 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             scores(klo, half);
           }
           if (!ok) break;
-          if (!first) free_slot(pend_slot);
+          if (!first) free_v();
           free_slot(ring);
           pend = true;
           pend_acc = !first;
-          pend_slot = vs;
-          pend_bar = smem_u32(&sm.full[second][vs]);
-          pend_ph = (phases >> vs) & 1u;
+          if constexpr (kFp8) {
+            pend_slot = wide;
+            pend_bar = smem_u32(&sm.wide.full[second][wide]);
+            pend_ph = ((second ? wide1 : wide0) >> wide) & 1u;
+          } else {
+            pend_slot = vs;
+            pend_bar = smem_u32(&sm.full[second][vs]);
+            pend_ph = (phases >> vs) & 1u;
+          }
           pend_rows = g.kv_end - (g.block0 + j) * kBlk;
           first = false;
         }
         const uint32_t bits = (1u << ring) | (1u << vs);
         if (second) phase1 ^= bits;
         else phase0 ^= bits;
+        if constexpr (kFp8) {
+          if (second) wide1 ^= 1u << wide;
+          else wide0 ^= 1u << wide;
+          if (++wide == kWide) wide = 0;
+        }
         last_tile = pair ? 1 : owner;
         ring = vs + 1 == kS ? 0 : vs + 1;
       }
@@ -935,12 +987,54 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (!ok) break;
     }
   } else {
-    // ================================================================ warp 3 of the first CTA
-    // writes the schedule down for the merge
+    // ================================================================ warp 3
+    // of the first CTA writes the schedule down for the merge
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBrRegsControl));
     if (blockIdx.x == 0) {
       pl = make_plan(p, ln, lane);
       write_plan(p, ln, pl, p.plan, lane);
+    }
+    if constexpr (kFp8) {
+      // Widens V, rows past the sequence's end as zeros.
+      int ring = 1, wide = 0, last_tile = 1;
+      // a bit per slot of the ring: parities of the two full barriers; a bit per widened block: which
+      // tiles read its latest content, and the parities of their releases
+      uint32_t phase0 = 0u, phase1 = 0u, used0 = 0u, used1 = 0u, free0 = 0u, free1 = 0u;
+      bool ok = true;
+      Segment g;
+      while (ok && next_segment(g)) {
+        const bool pair = g.n_rows > kBlk;
+        for (int j = 0; j < g.blocks; ++j) {
+          const int side = pair ? 0 : last_tile ^ 1;
+          const uint32_t bit = 1u << wide, slot_bit = 1u << ring;
+          if (used0 & bit) {
+            ok = mbar_wait(smem_u32(&sm.wide.empty[0][wide]), (free0 >> wide) & 1u, abort_flag, p.err);
+            free0 ^= bit;
+          }
+          if (ok && (used1 & bit)) {
+            ok = mbar_wait(smem_u32(&sm.wide.empty[1][wide]), (free1 >> wide) & 1u, abort_flag, p.err);
+            free1 ^= bit;
+          }
+          if (ok) ok = mbar_wait(smem_u32(&sm.full[side][ring]), ((side ? phase1 : phase0) >> ring) & 1u, abort_flag, p.err);
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          if (side) phase1 ^= slot_bit;
+          else phase0 ^= slot_bit;
+          const int rows = g.kv_end - (g.block0 + j) * kBlk;  // that hold anything
+          if (rows >= kBlk) widen_block<false>(smem_u32(sm.kv[ring]), smem_u32(sm.wide.v[wide]), kBlk, lane);
+          else widen_block<true>(smem_u32(sm.kv[ring]), smem_u32(sm.wide.v[wide]), rows, lane);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&sm.empty[0][ring]));
+            mbar_arrive(smem_u32(&sm.wide.full[side][wide]));
+          }
+          used0 = pair || side == 0 ? used0 | bit : used0 & ~bit;
+          used1 = pair || side == 1 ? used1 | bit : used1 & ~bit;
+          last_tile = pair ? 1 : side;
+          ring = ring + 2 > kS ? 1 : ring + 2;
+          if (++wide == kWide) wide = 0;
+        }
+      }
     }
   }
 

@@ -19,6 +19,12 @@ constexpr int kSpan = 256;     // query rows of an item of the tensor line: two 
 constexpr int kRowSpan = 16;   // query rows of an item of the warp line
 constexpr int kRowUnit = 32;   // keys of a unit of the warp line
 constexpr int kRowWarpsPerBlock = 4;
+// P = 2^(x - m + boost). m follows a row's maximum only when that grows past it by more than kGrowth, so P is
+// at most 2^(kGrowth + boost) and O is seldom rescaled. bf16 caches take P in bf16, which holds any of these,
+// with no boost; e4m3 caches take it in f16, 11 bits from 2^-14 to 2^16: the boost puts a fresh maximum at
+// 2^7, so that weights of 2^-21 of it have all bits and the last step is 2^-31 of it.
+constexpr float kGrowth = 8.0f;
+constexpr float kBoostF8 = 7.0f;
 
 // A line: items of up to `span` query rows, first those against the shared blocks and then those
 // of each branch against its own, KV head by KV head; an item has a unit for every `unit` keys and

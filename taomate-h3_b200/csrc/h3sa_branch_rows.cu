@@ -38,8 +38,6 @@ struct RowCfg {
   static constexpr int kStages = kRowRing / kStageBytes;  // 3, and 6 for e4m3
 };
 constexpr size_t kRowSmem = static_cast<size_t>(kRowWarps) * kRowRing + 1024;
-// P is at most 2^threshold; f16 and bf16 both hold it, and O is rescaled only past it.
-constexpr float kThreshold = 8.0f;
 
 __device__ __forceinline__ void load16(const void* at, uint32_t* r) {
   const uint4 v = __ldg(static_cast<const uint4*>(at));
@@ -101,6 +99,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
                        const BranchParams p, const bool after) {
   constexpr int kTileBytes = RowCfg<kFp8>::kTileBytes, kStageBytes = RowCfg<kFp8>::kStageBytes;
   constexpr int kRowStages = RowCfg<kFp8>::kStages;
+  constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kRowWarps][kMaxRowStages], empty[kRowWarps][kMaxRowStages];
   __shared__ int abort_word;
@@ -352,7 +351,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       float t1 = fmaxf(fmax3(fmaxf(s[0][2], s[0][3]), s[1][2], s[1][3]), fmax3(fmaxf(s[2][2], s[2][3]), s[3][2], s[3][3]));
       t0 = quad_max(t0) * sl2;
       t1 = quad_max(t1) * sl2b;
-      const bool need0 = t0 > m0 + kThreshold, need1 = t1 > m1 + kThreshold;
+      const bool need0 = t0 > m0 + kGrowth, need1 = t1 > m1 + kGrowth;
       if (__any_sync(0xffffffffu, need0 || need1)) {
         const float a0 = need0 ? fast_exp2(m0 - t0) : 1.f, a1 = need1 ? fast_exp2(m1 - t1) : 1.f;
         m0 = need0 ? t0 : m0;
@@ -368,7 +367,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         }
       }
       // a row that has seen nothing yet keeps m = -inf: x - m would be NaN
-      const float b0 = m0 == -INFINITY ? 0.f : -m0, b1 = m1 == -INFINITY ? 0.f : -m1;
+      const float b0 = kBoost - (m0 == -INFINITY ? 0.f : m0), b1 = kBoost - (m1 == -INFINITY ? 0.f : m1);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         s[j][0] = fast_exp2(fmaf(s[j][0], sl2, b0));
@@ -434,7 +433,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     for (int half = 0; half < 2; ++half) {
       const int row_in = r + 8 * half;
       if (row_in >= g.n_rows) continue;
-      const float l = half ? l1 : l0, m = half ? m1 : m0;
+      const float l = half ? l1 : l0, m = (half ? m1 : m0) - kBoost;
       const RowAt& ra = half ? at1 : at0;
       const long long id = (static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h;
       float w = l == 0.f ? 0.f : 1.0f / l;
