@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       const int my = lr & (span - 1);  // this thread's row of the tile
       const int copy = lr / span;      // and which copy of it
       float sl2 = p.scale_log2 * store_query_row<kFp8>(sm.q[t], my, copy, copies, span, qv);
-      if constexpr (kFp8) sl2 *= __ldg(p.k_scale + it.head);
+      if constexpr (kFp8) sl2 = score_factor(sl2 * __ldg(p.k_scale + it.head));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
       const int limit = seq_length(p, it.at.b) - (p.causal ? p.rows - 1 - it.at.i : 0);

@@ -244,10 +244,14 @@ __device__ __forceinline__ uint32_t f16x2_of_e4m3x2(uint32_t e) {
 }
 
 // The power of two that brings a bf16 row's largest magnitude (given as its bits) into [128, 256),
-// as an exponent; rows of tiny numbers keep their products within fp32.
+// as an exponent; rows of tiny numbers keep their products within fp32, rows of zeros are left alone.
 __device__ __forceinline__ int row_exponent(uint32_t top) {
-  return max(-120, min(7 - (static_cast<int>(top >> 7) - 127), 120));
+  return top == 0u ? 0 : max(-120, min(7 - (static_cast<int>(top >> 7) - 127), 120));
 }
+// The factor of e4m3 scores. Hidden ones are -inf before they are scaled, and -inf times a factor that is
+// zero (a k_scale of zero) or came out as zero (tiny queries over tiny keys) would be NaN. With the
+// smallest normal number instead, visible scores, at most 2^24, still come out as nothing.
+__device__ __forceinline__ float score_factor(float f) { return f == 0.f ? 1.17549435e-38f : f; }
 __device__ __forceinline__ float exp2_int(int k) { return __uint_as_float(static_cast<uint32_t>(k + 127) << 23); }
 
 // A tile load that marks its lines as the first to go from L2. Keys that one worker alone reads would

@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         qa[k] = f16x2_of(__uint_as_float(qa[k] << 16) * ua, __uint_as_float(qa[k] & 0xffff0000u) * ua);
         qb[k] = f16x2_of(__uint_as_float(qb[k] << 16) * ub, __uint_as_float(qb[k] & 0xffff0000u) * ub);
       }
-      sl2 *= exp2_int(-ka);
-      sl2b *= exp2_int(-kb);
+      sl2 = score_factor(sl2 * exp2_int(-ka));
+      sl2b = score_factor(sl2b * exp2_int(-kb));
     }
     float o[16][4];
 #pragma unroll
