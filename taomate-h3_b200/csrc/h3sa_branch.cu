@@ -302,7 +302,9 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
     for (int i = 0; i < 64; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
     top = max(top >> 16, top & 0xffffu);
     const int k = row_exponent(top);
-    const float up = exp2_int(k);
+    // a row with an infinity or NaN becomes NaN, as its products are; its factor stays finite, so that
+    // keys hidden from it stay hidden
+    const float up = top >= 0x7f80u ? __int_as_float(0x7fffffff) : exp2_int(k);
 #pragma unroll
     for (int c = 0; c < 8; ++c) {  // 16 columns a chunk
       if ((c & (copies - 1)) != copy) continue;
@@ -324,8 +326,7 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
         *reinterpret_cast<uint4*>(at + kAtom) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
-    // a row with an infinity or NaN gets NaN scores, as its products have
-    return top >= 0x7f80u ? __int_as_float(0x7fffffff) : exp2_int(-k);
+    return exp2_int(-k);
   }
 }
 
