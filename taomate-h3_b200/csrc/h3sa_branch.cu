@@ -73,7 +73,7 @@ constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
 
 // One item segment of a CTA, as warp 0 publishes it.
 struct Segment {
-  int live;      // 0: the CTA's last descriptor
+  int live;      // 0: the CTA's last descriptor; 2: against the shared blocks
   int head;      // KV head
   int row0;      // first stacked query row of the item
   int n_rows;    // rows of the item (1..256)
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             g.row0 = at.t * kSpan;
             g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
             g.block0 = at.off;
-            g.kv_end = pl.max_len;
+            g.kv_end = pl.shared_blocks * kBlk;
             item = at.head * ln.shared_tiles + at.t;
             row0 = 0;
             slot_rows = p.shared_slot_rows;
@@ -502,14 +502,14 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             seq = at.b;
             g.row0 = at.b * p.rows * p.group + at.t * kSpan;
             g.n_rows = min(kSpan, p.rows * p.group - at.t * kSpan);
-            g.block0 = own_lo(p) / kBlk + at.off;
             g.kv_end = seq_length(p, at.b);
+            g.block0 = own_lo(p, g.kv_end) / kBlk + at.off;
             item = (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
             row0 = p.own_row0;
             slot_rows = p.own_slot_rows;
           }
           for (int k = 0; k < 2; ++k) g.slot_row[k] = row0 + ((item + blockIdx.x) * 2 + k) * slot_rows;
-          g.live = 1;
+          g.live = at.b < 0 ? 2 : 1;
           g.head = at.head;
           g.blocks = blocks;
           g.direct = pl.shared_blocks == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
@@ -784,7 +784,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     struct Item {
       int mine, begin, step;  // blocks of this tile: how many, the first, every step-th
       int block0, head, row0, n_rows, span;  // of this tile; span: rows a copy has room for
-      int direct;
+      int direct, shared;
       long long ws_row;
       RowAt at;  // this thread's row
     };
@@ -810,6 +810,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         it.head = g.head;
         it.row0 = g.row0 + r0;
         it.direct = g.direct;
+        it.shared = g.live == 2;
         const int my = lr & (it.span - 1);
         it.at = row_at(p, g.head, it.row0 + min(my, it.n_rows - 1));
         const uint4* src = reinterpret_cast<const uint4*>(p.q + it.at.b * p.q_sb + it.at.i * p.q_sn + it.at.h * p.q_sh);
@@ -830,7 +831,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if constexpr (kFp8) sl2 = score_factor(sl2 * __ldg(p.k_scale + it.head));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const int limit = seq_length(p, it.at.b) - (p.causal ? p.rows - 1 - it.at.i : 0);
+      const int len = seq_length(p, it.at.b);
+      const int limit = it.shared && !takes_shared(p, len) ? 0 : len - (p.causal ? p.rows - 1 - it.at.i : 0);
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; ok && j < it.mine; ++j) {
@@ -1489,13 +1491,13 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   p.heads = heads;
   p.kv_heads = kv_heads;
   p.group = group;
-  p.shared = shared_rows / kBlk;
   p.causal = causal ? 1 : 0;
   p.joint = s.joint;
   if (whole_form(width, kv_heads, batch, s.warp)) {
     p.whole = p.joint = 1;
     s.tensor.shared_tiles = s.warp.shared_tiles = 0;
   }
+  p.shared_keys = p.joint ? 0 : shared_rows;
   p.pool_pages = pool_pages;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.k_scale = k_scale;

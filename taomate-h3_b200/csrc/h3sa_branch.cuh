@@ -45,7 +45,7 @@ struct BranchParams {
   const int* table;            // [batch, width]
   const int* lengths;          // [batch]
   int width, batch, rows, heads, kv_heads, group;
-  int shared;                  // leading blocks shared by all sequences
+  int shared_keys;             // leading keys of the shared items (0: there are none), whole blocks
   int causal, joint;
   int whole;                   // the warp line takes whole items
   int pool_pages;
@@ -68,16 +68,20 @@ __device__ __forceinline__ int seq_length(const BranchParams& p, int b) {
   return max(0, min(n, p.width * kBlk));
 }
 
+// A sequence that ends inside the shared blocks has no part in their items, where rows behind its end that
+// others see would meet its zeros of P, and NaN or infinities among them its output: its own items
+// have all its keys.
+__device__ __forceinline__ bool takes_shared(const BranchParams& p, int len) { return len >= p.shared_keys; }
 // The first key outside the shared items, and the units behind it of the rows of tile t of a
 // sequence of length `len`.
-__device__ __forceinline__ int own_lo(const BranchParams& p) { return p.joint ? 0 : p.shared * kBlk; }
+__device__ __forceinline__ int own_lo(const BranchParams& p, int len) { return takes_shared(p, len) ? p.shared_keys : 0; }
 __device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, int len, int t) {
   if (!p.causal) return len;
   const int last = min((t + 1) * ln.span, p.rows * p.group) - 1;
   return len - (p.rows - 1 - last / p.group);
 }
 __device__ __forceinline__ int own_units(const BranchParams& p, const Line& ln, int len, int t) {
-  return max(0, own_limit(p, ln, len, t) - own_lo(p) + ln.unit - 1) / ln.unit;
+  return max(0, own_limit(p, ln, len, t) - own_lo(p, len) + ln.unit - 1) / ln.unit;
 }
 __device__ __forceinline__ int weight_of(const Line& ln, int units) { return units > 0 ? units + ln.pad : 0; }
 __device__ __forceinline__ int own_weight_all(const BranchParams& p, const Line& ln, int len) {
@@ -88,12 +92,11 @@ __device__ __forceinline__ int own_weight_all(const BranchParams& p, const Line&
 }
 
 struct Plan {
-  int shared_blocks;  // shared blocks that hold anything
+  int shared_blocks;  // of the shared items: 0 if no sequence has all of them
   int shared_units;   // units of one shared item
   int head_weight;    // one KV head's part of the line
   int cut;            // one worker's part
   int longest;        // sequence whose table row gives the shared pages
-  int max_len;
 };
 
 __device__ __forceinline__ Plan make_plan(const BranchParams& p, const Line& ln, int lane) {
@@ -110,9 +113,8 @@ __device__ __forceinline__ Plan make_plan(const BranchParams& p, const Line& ln,
   const int top = __reduce_max_sync(0xffffffffu, best);
   at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
   Plan pl;
-  pl.max_len = top;
   pl.longest = at;
-  pl.shared_blocks = p.joint ? 0 : min(p.shared, (top + kBlk - 1) / kBlk);
+  pl.shared_blocks = own_lo(p, top) / kBlk;
   pl.shared_units = pl.shared_blocks * (kBlk / ln.unit);
   pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units) + own;
   const int all = pl.head_weight * p.kv_heads;

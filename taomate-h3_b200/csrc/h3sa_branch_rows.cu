@@ -176,8 +176,9 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
         g.n_rows = min(kRowSpan, (g.shared ? p.batch * own_all : (at.b + 1) * own_all) - g.row0);
-        g.key0 = (g.shared ? 0 : own_lo(p)) + at.off * kRowUnit;
-        g.kv_end = g.shared ? pl.max_len : seq_length(p, at.b);
+        const int len = seq_length(p, g.seq);
+        g.key0 = (g.shared ? 0 : own_lo(p, len)) + at.off * kRowUnit;
+        g.kv_end = len;
         g.direct = pl.shared_blocks == 0 && n == units;
         const long long item = g.shared ? static_cast<long long>(at.head) * ln.shared_tiles + at.t
                                         : (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
@@ -270,8 +271,11 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         load16(b + from, qb + 4 * k);
       }
     }
-    const int lim0 = seq_length(p, at0.b) - (p.causal ? p.rows - 1 - at0.i : 0);
-    const int lim1 = seq_length(p, at1.b) - (p.causal ? p.rows - 1 - at1.i : 0);
+    const auto limit_of = [&](const RowAt& ra) {
+      const int len = seq_length(p, ra.b);
+      return g.shared && !takes_shared(p, len) ? 0 : len - (p.causal ? p.rows - 1 - ra.i : 0);
+    };
+    const int lim0 = limit_of(at0), lim1 = limit_of(at1);
     float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
 #pragma unroll
     for (int k = 0; k < 16; ++k) {

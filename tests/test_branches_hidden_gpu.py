@@ -1,4 +1,5 @@
-"""NaN and infinities where a row does not look: queries of rows that see nothing."""
+"""NaN and infinities where a row does not look: queries of rows that see nothing, and values of shared
+pages behind the end of a sequence that is shorter than the prefix."""
 
 from __future__ import annotations
 
@@ -62,3 +63,47 @@ def test_a_query_that_is_nan_reaches_its_own_row_only(rows, heads, kv, kind) -> 
     assert torch.isnan(out[1, rows // 3, heads - 1]).all() and torch.isnan(lse[1, rows // 3, heads - 1])
     out[1, rows // 3, heads - 1] = want[1, rows // 3, heads - 1]
     assert torch.equal(out, want) and int(torch.isnan(lse).sum()) == 1
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths,shared,rows,heads,kv", [
+    ([100, 1000, 130, 0], 6, 1, 4, 2),             # few rows
+    ([300, 2000], 12, 1, 4, 4),
+    ([500, 1100, 513, 0], 5, 100, 4, 2),           # tensor cores, both lines' items
+    ([9000, 200] + [16500] * 8, 128, 1, 64, 8),    # shared keys on the tensor cores, own ones not
+    ([900, 100], 6, 300, 40, 40),                  # joint
+    ([200, 100], 4, 3, 2, 2),                      # all of them shorter than the prefix
+])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_rows_of_shared_pages_behind_a_short_sequence(lengths, shared, rows, heads, kv, kind, causal, bad) -> None:
+    from h3sa.branches import shared_prefix_attention
+
+    rng = np.random.default_rng(41)
+    gen = torch.Generator(device="cuda").manual_seed(41)
+    width = max([shared] + [ob.pages_of(n) for n in lengths])
+    pages = shared + sum(max(0, ob.pages_of(n) - shared) for n in lengths) + 1
+    ids, at = rng.permutation(pages), shared
+    table = np.full((len(lengths), width), -1, np.int64)
+    for b, n in enumerate(lengths):
+        held = ob.pages_of(n)
+        table[b, :min(held, shared)] = ids[:min(held, shared)]
+        for j in range(shared, held):
+            table[b, j] = ids[at]
+            at += 1
+    k, v, scales = _pools(kv, pages, kind, gen)
+    q = torch.randn(len(lengths), rows, heads, 128, generator=gen, device="cuda").bfloat16()
+    args = (_i32(table), _i32(lengths), shared * 128, SCALE)
+    want = shared_prefix_attention(q, k, v, *args, causal=causal, **scales)
+    short = [b for b, n in enumerate(lengths) if n < shared * 128]
+    first = max(lengths[b] for b in short)  # the first row that no short sequence has
+    rows_of = np.concatenate([np.arange(max(first, j * 128), (j + 1) * 128) - j * 128 + ids[j] * 128
+                              for j in range(first // 128, shared)])
+    hidden = torch.from_numpy(rows_of).cuda()
+    if kind == "bf16":
+        v[:, hidden] = bad
+    else:
+        v.view(torch.uint8)[:, hidden] = 0x7f  # NaN, the only one of the two that e4m3 has
+    out = shared_prefix_attention(q, k, v, *args, causal=causal, **scales)
+    for b in short:
+        assert torch.equal(out[b], want[b])
