@@ -400,8 +400,10 @@ bool sizes_ok(int32_t sequences, int32_t width) {
 }
 
 int check_pools(const char* what, const h3sa_pools* p) {
-  if (!p || p->count < 0 || p->heads <= 0 || p->pages <= 0 || p->row_bytes <= 0 || p->row_bytes % 16)
-    return set_error(H3SA_ERR_INVALID, "%s: invalid pools (row bytes must be a positive multiple of 16)", what);
+  if (!p || p->count < 0 || p->heads <= 0 || p->pages <= 0 || p->row_bytes <= 0 || p->row_bytes % 16 ||
+      static_cast<int64_t>(p->row_bytes) * kPage > INT32_MAX)
+    return set_error(H3SA_ERR_INVALID, "%s: invalid pools (row bytes must be a positive multiple of 16, below 2^24)",
+                     what);
   if (static_cast<int64_t>(p->pages) * kPage > INT32_MAX)
     return set_error(H3SA_ERR_INVALID, "%s: pool of %d pages too large", what, p->pages);
   for (int i = 0; i < p->count; ++i) {

@@ -50,6 +50,13 @@ def test_tables_and_counts_past_the_index_are_refused(call) -> None:
     assert "invalid sizes" in _refused(*call)
 
 
+@pytest.mark.parametrize("row_bytes", [1 << 24, (1 << 24) + 16, 1 << 28, (1 << 31) - 16])
+def test_rows_whose_page_passes_32_bits_are_refused(row_bytes) -> None:
+    for call in (_fork, _compact):
+        name, *args = call(_pools(row_bytes=row_bytes))
+        assert "row bytes" in _refused(name, *args)
+
+
 def test_the_struct_is_the_header_s() -> None:
     from h3sa import _lib
 
