@@ -143,8 +143,8 @@ def fork_pages(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, r
     if _bad(parents, device, _I32, (children,)):
         _refuse(what, "parents", device, _I32, (children,))
     error = _error_word(what, device, device_error)
-    if reserve_rows < 0:
-        raise ValueError(f"{what}: reserve_rows must not be negative")
+    if not 0 <= reserve_rows < 1 << 31:
+        raise ValueError(f"{what}: reserve_rows must not be negative or past 32 bits")
     p = _pools(what, pools, pages, device)
     with _on(stream):
         child_table = table.new_empty((children, width))
@@ -267,6 +267,9 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
         _refuse(what, "lengths", device, _I32, (batch,))
     if lse is not None and _bad(lse, device, _F32, (batch, rows, heads)):
         _refuse(what, "lse", device, _F32, (batch, rows, heads))
+    if not 0 <= shared_rows <= width * PAGE_ROWS:
+        raise RuntimeError(f"{what}: {shared_rows} shared rows are not whole pages of a table of {width} "
+                           "entries")
     error = _error_word(what, device, device_error)
     need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows))
     if out is not None and _bad(out, device, _BF16, query.shape):
