@@ -35,7 +35,7 @@ PoolTensors = Union[torch.Tensor, Sequence[torch.Tensor]]
 _FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_free_pages
 _ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
 _PAGES_WORK = LIB.h3sa_pages_workspace
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _I32, _F32, _BF16, _E4M3 = torch.int32, torch.float32, torch.bfloat16, torch.float8_e4m3fn
 _empty_like = torch.empty_like
 
@@ -66,6 +66,11 @@ def _on(stream: torch.cuda.Stream | None):
 
 
 def _handle(stream: torch.cuda.Stream | None, device: torch.device) -> int:
+    """The stream to launch on, which is the current device's, as the tensors must be."""
+
+    if device.index != _current_device() or (stream is not None and stream.device != device):
+        raise RuntimeError(f"h3sa kernels run on the current device (cuda:{_current_device()}): the tensors are on "
+                           f"{device}" + ("" if stream is None else f", the stream on {stream.device}"))
     return _raw_stream(device.index) if stream is None else stream.cuda_stream
 
 
