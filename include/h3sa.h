@@ -525,8 +525,9 @@ H3SA_API int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t wi
  * rows (whole pages) are the same pages in the table rows of all sequences at least that long;
  * shorter sequences see the first lengths[b] rows of them, which are then read for each of these by
  * itself. Rows that see nothing come out zero. Rows of a page past a sequence's end never reach its
- * outputs, whatever they hold, also where other sequences see them. Of its own rows, an infinity or NaN in
- * V reaches all its outputs in that column, also those of rows from which causal hides it. A length outside
+ * outputs, whatever they hold, also where other sequences see them. An infinity or NaN in V of its own
+ * rows makes all its outputs in that column infinite or NaN (weights of zero times infinity among the
+ * sums), also those of rows from which causal hides it. k_scale and v_scale may not be negative. A length outside
  * [0, width * 128] is clamped with H3SA_DEVERR_BAD_INDEX; a page outside the pool gives
  * H3SA_DEVERR_BAD_PAGE and invalid outputs. Results do not depend on timing. */
 H3SA_API int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
