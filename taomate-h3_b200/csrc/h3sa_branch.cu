@@ -1257,7 +1257,7 @@ int sm_count() {
 
 // Branches of up to this many rows have them on the warp line. 2 KV heads over 1024 shared keys, warp /
 // tensor (us): 8 branches, own lengths to 2000: 32 rows 16 / 24, 64 rows 19 / 25; 40 branches, to 1000: 25 /
-// 34, 39 / 40; over 8192 shared keys and up to 300 59 / 60, e4m3 69 / 67.
+// 34, 39 / 40; over 8192 shared keys and up to 300 59 / 60, e4m3 65 / 66.
 constexpr int kWarpOwnRows = 64;
 
 // The split form reads the shared blocks once for all branches and packs their rows into full tiles, but
@@ -1277,7 +1277,8 @@ bool joint_form(long long own, int batch, int kv_heads, int shared) {
 
 // Short tables on the warp line: a warp takes a branch's rows against all its keys, shared ones too, and
 // there is nothing to merge. 0.8 us a 32-key unit and warp (P in two terms) then stand against the merge,
-// its launch and the better spread. Whole / split (us), 1, 3 and 5 blocks a branch: 6 items 6.2 / 9.9, 12.5 / 10.5
+// its launch and the better spread. The limits count the launch, some 5 us of a call's host time; on the device alone, as
+// in a graph, the forms meet a block or two earlier. Whole / split (us on the device), 1, 3 and 5 blocks a branch: 6 items 6.2 / 9.9, 12.5 / 10.5
 // (the call 27.8 / 33, for its launch), 19 / 10.1; 96 items 6.3 / 10.7, 12.8 / 11.8, 19 / 12.2; 128 items 6.4 /
 // 14.0, 12.8 / 16.4, 19.2 / 17.3; 512 items 6.9 / 15.2, 13.5 / 21.3, 20.1 / 23.5; 1600 items 14 / 25, 34 / 36,
 // 54 / 39; e4m3 512 items 6.6 / 16.6, 12.4 / 23.7, 18.2 / 26.4.
@@ -1291,7 +1292,7 @@ bool whole_form(int width, int kv_heads, int batch, const Line& warp) {
 // Shared blocks under 8 KV heads, with merge and own parts (us, warp / tensor): bf16, 60 rows, 1024
 // keys 13 / 25, 4096 keys 20 / 27, 16384 keys 42 / 45, 65536 keys 153 / 83; 240 rows, 4096 keys 35 / 40, 16384
 // keys 100 / 50; 32 rows, 16384 keys 27 / 39, 65536 keys 94 / 78; 16 rows, 65536 keys 55 / 75. e4m3, 60 rows,
-// 16384 keys 39 / 49, 65536 keys 110 / 75; 32 rows, 65536 keys 66 / 66; 16 rows 44 / 61.
+// 16384 keys 39 / 50, 65536 keys 111 / 79; 32 rows, 65536 keys 66 / 71; 16 rows 42 / 66.
 // So: always up to one tile of rows, else up to the product where the two meet.
 constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 // The least part of a worker, in units: a piece costs the merge as much as some more keys cost the
@@ -1395,7 +1396,7 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   // Four warps share a row where rows are few, or not too many and in as many pieces as the tensor line
   // cuts a shared item into: its pieces are read one latency after another. One warp / four (us of the
   // whole call): 126 rows 13.8 / 12.8; 256 rows of 4096 shared keys (warp line) 19.8 / 17.1; 480 rows of
-  // 1024 (warp line) 14.6 / 18.0, of 98304 (tensor line) 105.6 / 103.6; 2400 rows 57.4 / 58.5.
+  // 1024 (warp line) 14.6 / 18.0, of 98304 (tensor line, e4m3) 99.2 / 98.9; 2400 rows 57.4 / 58.5.
   const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
   const bool team = !p.joint && stacked <= (p.tensor.shared_tiles > 0 ? 4ll : 2ll) * p.tensor.workers;
   const long long blocks =

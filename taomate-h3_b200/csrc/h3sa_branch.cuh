@@ -258,7 +258,7 @@ __device__ __forceinline__ float exp2_int(int k) { return __uint_as_float(static
 
 // A tile load that marks its lines as the first to go from L2. Keys that one worker alone reads would
 // push everything else out of it, the kernels' own code and queries among it, whose next reads then
-// queue behind them for memory: 85.9 -> 76 us for 60 rows over 98304 e4m3 keys of 8 heads.
+// queue behind them for memory: 109 -> 99 us for 60 rows over 98304 e4m3 keys of 8 heads.
 __device__ __forceinline__ void tma_load_3d_once(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1,
                                                  int c2, uint64_t policy) {
   asm volatile(

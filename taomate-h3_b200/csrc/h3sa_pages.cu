@@ -204,7 +204,7 @@ struct CompactArgs {
   int* to;      // [pages]
   int4* moves;
   int* n_moves;
-  int* slots;   // [3 * kCtas]
+  int* slots;   // [2 * kCtas]
   int* err;
 };
 

@@ -13,8 +13,13 @@ for all of them. The ledger lives in device memory and no call here waits for th
 
 Each operation returns the new ledger and leaves the one it was given as it was. Failures that
 only the device can see (too few free pages, an index out of range) are OR-ed into
-``device_error`` as the ``DEVERR_*`` bits of ``h3sa._lib``. The reference holds one history per
-stream and has no counterpart.
+``device_error`` as the ``DEVERR_*`` bits of ``h3sa._lib``; without one they go unreported. The
+reference holds one history per stream and has no counterpart.
+
+A ledger owns the pages that it describes. ``PagedLayerKV`` keeps its own lists of pages on the host
+and does not learn of forks or moves: once a ledger describes its pools, such a cache must not be
+written, grown or committed to, or both would hand out the same pages. e4m3 pools have one K and one
+V scale per KV head, so the e4m3 history of a streaming cache, with scales per commit, is none.
 """
 
 from __future__ import annotations
@@ -225,12 +230,13 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
 
     ``query``: bf16 ``[sequences, rows, heads, 128]`` (any strides with contiguous, 16-byte
     aligned rows). Pools ``[kv_heads, pages*128, 128]`` bf16, or e4m3 with fp32 per-head
-    ``k_scale`` / ``v_scale``; query head h reads KV head ``h // (heads // kv_heads)``. Row i of
+    ``k_scale`` / ``v_scale`` (not negative); query head h reads KV head ``h // (heads // kv_heads)``. Row i of
     sequence b sees its first ``lengths[b]`` keys, with ``causal`` only those up to itself, the
     query rows being the sequence's last ones (their K/V already written). The first
     ``shared_rows`` rows (a multiple of 128) are the same pages in the table rows of all
-    sequences that reach that far, as ``fork_pages`` leaves them. Rows that see nothing come out
-    zero. ``out``: optional contiguous bf16 result tensor; ``lse``: optional fp32
+    sequences that reach that far, as ``fork_pages`` leaves them; shorter sequences are read by
+    themselves. Rows that see nothing come out zero; an infinity or NaN in V of a sequence's own rows
+    makes its outputs in that column infinite or NaN, ``causal`` or not. ``out``: optional contiguous bf16 result tensor; ``lse``: optional fp32
     ``[sequences, rows, heads]`` that receives the log-sum-exp (-inf for such rows). Neither may
     overlap ``query``.
     """
