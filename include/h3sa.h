@@ -541,6 +541,93 @@ H3SA_API int h3sa_shared_prefix_attention(
     int32_t causal, float softmax_scale, void* workspace, int64_t workspace_bytes,
     int32_t* device_error, void* stream);
 
+/* ---- drafted trees: rows proposed behind a sequence, verified together, one path of them kept (no
+ * counterpart in the reference). Row i of a tree is a node; its drafted K/V rows lie in the sequence's
+ * pages behind its first lengths[b] rows, row lengths[b] + i, and are no part of lengths[b] until
+ * h3sa_keep_rows. counts int32 [batch], or NULL for all: how many of a sequence's rows are nodes. */
+
+/* Ancestor bits and positions of trees of up to 1024 nodes. parents int32 [batch, nodes]: a row in
+ * front of the node's own, or -1 for a root. masks int32 [batch, nodes, ceil(nodes / 32)]: bit n % 32 of
+ * word n / 32 says whether node n is the node itself or above it; positions int32 [batch, nodes]:
+ * lengths[b] plus the node's depth. Rows behind a sequence's nodes get zeros. A parent that is neither
+ * makes its node a root and sets H3SA_DEVERR_BAD_INDEX, as does a count outside [0, nodes], which is
+ * clamped. */
+H3SA_API int h3sa_draft_tree(const int32_t* parents, int32_t batch, int32_t nodes,
+                             const int32_t* lengths, const int32_t* counts, int32_t* masks,
+                             int32_t* positions, int32_t* device_error, void* stream);
+
+/* Rows of heads [batch, rows, heads, dim] with element strides; the last one is 1. */
+typedef struct h3sa_heads {
+  void* base;
+  int64_t stride_sequence, stride_row, stride_head;
+  int32_t heads, reserved;
+} h3sa_heads;
+
+enum { H3SA_BF16 = 0, H3SA_FP16 = 1, H3SA_FP32 = 2 };
+enum { H3SA_POS_ROW = 0, H3SA_POS_I32 = 1, H3SA_POS_I64 = 2, H3SA_POS_F64 = 3 };
+
+/* Rotary positions: pair k of the first 2 * pairs dimensions of a head turns by position *
+ * frequencies[k] (radians, fp64) and is multiplied by factor; the other dimensions stay as they are. Pairs are
+ * (k, k + pairs), or (2k, 2k + 1) if interleaved. positions [batch * rows, axes] of the given kind; pair
+ * k belongs to axis k / (pairs / axes). H3SA_POS_ROW (appended rows, one axis): a row's place in its
+ * sequence. Angles are taken in 64 bits, products in 32, results rounded once. */
+typedef struct h3sa_rotary {
+  const void* positions;
+  const double* frequencies;
+  int32_t position_kind, axes, pairs, interleaved;
+  float factor;
+  int32_t reserved;
+} h3sa_rotary;
+
+/* out = x rotated, both of `dtype`. dim: at most 1024. out may be x itself (same address and strides),
+ * else they may not overlap. Any strides and alignment of whole elements; 16 or 8 bytes are read at a time
+ * where pairs, dim, strides and addresses are multiples of them. */
+H3SA_API int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32_t batch,
+                         int32_t rows, int32_t dim, const h3sa_rotary* rotary, void* stream);
+
+/* Appends rows i < counts[b] of key and value (bf16, heads of 128) to the pages of their sequences, at
+ * rows lengths[b] + i through the table (int32 [batch, width]); lengths stay as they are. Keys are
+ * rotated on the way, and so is query into query_out (both NULL if there is none; query_out may be query
+ * itself); its rows behind counts[b] come out zero. rotary NULL: nothing is. Pools
+ * [kv_heads, pool_pages * 128, 128], 16-byte aligned, bf16, or e4m3 with positive k_scale / v_scale fp32
+ * [kv_heads], by which rows are divided (rounded once, limited to 448, NaN stays NaN). A row past the table's
+ * width, or of a sequence of negative length, sets H3SA_DEVERR_BAD_INDEX, a page outside the pool
+ * H3SA_DEVERR_BAD_PAGE; such rows are not written. No two sequences may write the same page. */
+H3SA_API int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value,
+                              const h3sa_heads* query, const h3sa_heads* query_out, int32_t batch,
+                              int32_t rows, void* key_pool, void* value_pool, int32_t pool_pages,
+                              int32_t e4m3, const float* k_scale, const float* v_scale,
+                              const int32_t* table, int32_t width, const int32_t* lengths,
+                              const int32_t* counts, const h3sa_rotary* rotary,
+                              int32_t* device_error, void* stream);
+
+/* Attention of the drafted rows of every sequence: row i of sequence b, i < counts[b], sees keys
+ * j < lengths[b] and lengths[b] + n for each n < counts[b] whose bit is set in masks [batch, rows, ceil(rows / 32)]
+ * (h3sa_draft_tree's, or any others). All else is h3sa_shared_prefix_attention's, its workspace size
+ * among it (shared_rows may not pass the lengths of the sequences that hold the shared pages; one
+ * whose length ends in front of them is read by itself). Rows behind counts[b], and rows that see
+ * nothing, come out zero. An infinity or NaN in K or V of a drafted row reaches only the rows that see it; one
+ * in V of a sequence's first lengths[b] rows makes all its outputs in that column infinite or NaN. A
+ * length or count outside its range, or both together past the table, is clamped with
+ * H3SA_DEVERR_BAD_INDEX. */
+H3SA_API int h3sa_tree_attention(
+    const void* query, int64_t stride_sequence, int64_t stride_row, int64_t stride_head, void* out,
+    float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool,
+    const void* value_pool, int32_t pool_pages, int32_t e4m3, const float* k_scale,
+    const float* v_scale, const int32_t* table, int32_t width, const int32_t* lengths,
+    const int32_t* masks, const int32_t* counts, int32_t shared_rows, float softmax_scale,
+    void* workspace, int64_t workspace_bytes, int32_t* device_error, void* stream);
+
+/* Keeps a path of every tree: row lengths[b] + path[b, k] goes to row lengths[b] + k in all pools, and
+ * lengths_out[b] = lengths[b] + the path's length. path int32 [sequences, steps] ascends and ends at the first
+ * negative entry or with the steps. A path that does not ascend or leaves the table (then
+ * H3SA_DEVERR_BAD_INDEX), or a page outside the pool (H3SA_DEVERR_BAD_PAGE), leaves its sequence as it
+ * was. The rows' pages belong to their sequences alone; lengths_out may not overlap lengths. */
+H3SA_API int h3sa_keep_rows(const h3sa_pools* pools, const int32_t* table, int32_t sequences,
+                            int32_t width, const int32_t* lengths, const int32_t* path,
+                            int32_t steps, int32_t* lengths_out, int32_t* device_error,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

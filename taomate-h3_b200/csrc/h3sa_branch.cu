@@ -80,6 +80,7 @@ struct Segment {
   int block0;    // first logical block
   int blocks;
   int kv_end;    // rows at or past it hold nothing
+  int clean;     // rows at or past it are nodes of a tree
   int direct;    // the segment is its rows' whole result
   long long slot_row[2];  // workspace row of each tile's partial
 };
@@ -109,7 +110,14 @@ struct alignas(1024) BrWide<true> {
   uint64_t full[2][kWide], empty[2][kWide];
 };
 
-template <bool kFp8>
+template <class P>
+struct BrTree {};
+template <>
+struct BrTree<TreeParams> {
+  int taken_out;  // whether a node's V held an infinity or NaN
+};
+
+template <bool kFp8, class P>
 struct alignas(1024) BrSmem {
   using Cfg = BrCfg<kFp8>;
   uint8_t q[2][kQBytes];  // also the epilogue's staging
@@ -123,12 +131,13 @@ struct alignas(1024) BrSmem {
   uint64_t m_sync, drain;
   uint32_t tmem_base;
   int abort_flag;
+  BrTree<P> tree;
 };
-template <bool kFp8>
+template <bool kFp8, class P>
 constexpr size_t br_smem_bytes() {
-  return sizeof(BrSmem<kFp8>) + 1024;
+  return sizeof(BrSmem<kFp8, P>) + 1024;
 }
-static_assert(br_smem_bytes<false>() <= 232448 && br_smem_bytes<true>() <= 232448,
+static_assert(br_smem_bytes<false, TreeParams>() <= 232448 && br_smem_bytes<true, TreeParams>() <= 232448,
               "branch attention needs more than 227 KB");
 
 __device__ __forceinline__ uint32_t e4m3x2_of(uint32_t h2) {
@@ -182,12 +191,12 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
 
 // Softmax of kCols score columns of this thread's row, its copy's share of one half of a block:
 // columns [col0, col0 + kCols) of the block, col0 = 64 half + copy * kCols, in TMEM at tS + col0.
-// P goes over the half's scores, zeros in the other copies' shares. m / l: running maximum (log2
-// units) and sum; `pv_done` waits until O holds all earlier halves, before O is rescaled because
+// P goes over the half's scores, zeros in the other copies' shares. key0: the block's first key, sight: of
+// this row. m / l: running maximum (log2 units) and sum; `pv_done` waits until O holds all earlier halves, before O is rescaled because
 // the maximum grew (lazily: only past the threshold).
-template <bool kFp8, int kCols, typename Wait>
-__device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half, int copy, int limit, float sl2,
-                                             bool first, float& m, float& l, Wait&& pv_done) {
+template <bool kFp8, int kCols, class S, typename Wait>
+__device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half, int copy, int key0, const S& sight,
+                                             float sl2, bool first, float& m, float& l, Wait&& pv_done) {
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
   const int col0 = 64 * half + copy * kCols;
   float s[kCols];
@@ -211,13 +220,24 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(r[j]);
   }
-  // columns at or past `limit` (relative to the block) are hidden from this row
+  // columns at or past `limit` (relative to the block) are hidden from this row, but for nodes that it sees
+  const int limit = sight.base - key0;
   int hide = __any_sync(0xffffffffu, limit < col0 + kCols) ? 1 : 0;
   asm volatile("" : "+r"(hide));  // keeps the compares below out of whole blocks
   if (hide) {
+    if constexpr (std::is_same_v<S, Sight>) {
 #pragma unroll
-    for (int j = 0; j < kCols; ++j)
-      if (col0 + j >= limit) s[j] = -INFINITY;
+      for (int c = 0; c < kCols; c += 32) {
+        const uint32_t seen = sight.seen32(key0 + col0 + c);
+#pragma unroll
+        for (int j = 0; j < min(32, kCols); ++j)
+          if (!(seen >> j & 1u)) s[c + j] = -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+        if (col0 + j >= limit) s[j] = -INFINITY;
+    }
   }
   float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
@@ -334,8 +354,10 @@ __device__ __forceinline__ float store_query_row(uint8_t* tile, int my, int copy
 // columns), by a warp; kTail: rows at or past `rows` become zeros. A lane takes a 16-byte chunk of a row at a
 // time, eight rows in two steps, and all its offsets but two are constants. Lanes of the second atom take
 // the halves of their chunk the other way round: the eight of a phase write eight different chunks.
-template <bool kTail>
-__device__ __forceinline__ void widen_block(uint32_t from, uint32_t to, int rows, int lane) {
+// kNodes: NaN in rows at or past `clean` become zeros too; returns whether this lane met one.
+template <bool kTail, bool kNodes>
+__device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows, int clean, int lane) {
+  uint32_t met = 0u;
   const int c = lane & 7, h = c >> 2, at = 2 * (c & 3);
   const int r = (lane >> 4) + ((lane >> 1) & 4);  // rows r and r ^ 2 of eight; those of a half warp differ by 4
 #pragma unroll
@@ -358,23 +380,62 @@ __device__ __forceinline__ void widen_block(uint32_t from, uint32_t to, int rows
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           if (kTail && (i0 + i) * 8 + row >= rows) x[i][k] = make_uint2(0u, 0u);
+          uint32_t w[4] = {f16x2_of_e4m3x2(x[i][k].x), f16x2_of_e4m3x2(x[i][k].x >> 16), f16x2_of_e4m3x2(x[i][k].y),
+                           f16x2_of_e4m3x2(x[i][k].y >> 16)};
+          if constexpr (kNodes) {
+            if ((i0 + i) * 8 + row >= clean) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t bad = non_finite<0x7c00u>(w[j]);
+                met |= bad;
+                w[j] &= ~bad;
+              }
+            }
+          }
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"((dst ^ (16 * k)) + (i0 + i) * 1024),
-                       "r"(f16x2_of_e4m3x2(x[i][k].x)), "r"(f16x2_of_e4m3x2(x[i][k].x >> 16)),
-                       "r"(f16x2_of_e4m3x2(x[i][k].y)), "r"(f16x2_of_e4m3x2(x[i][k].y >> 16))
+                       "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                        : "memory");
         }
     }
   }
+  return met != 0u;
 }
 
-template <bool kFp8>
+// Clears what must not be multiplied in V's block of a sequence's last rows: rows at or past `rows` of it may
+// hold anything, and nodes' infinities and NaN (rows from `clean` on) belong to those that see them. The block's
+// load has completed; both warps of a block of two tiles write the same. Returns whether this lane met one.
+template <bool kTree>
+__device__ __forceinline__ bool clear_block(uint8_t* base, int rows, int clean, int lane) {
+  uint32_t met = 0u;
+  if constexpr (kTree) {
+    const int from = max(0, clean);
+    for (int i = lane; i < (min(rows, kBlk) - from) * 16; i += 32) {
+      const int row = from + (i >> 4), a = (i >> 3) & 1;
+      uint4& v = reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7];
+      const uint4 bad = make_uint4(non_finite<0x7f80u>(v.x), non_finite<0x7f80u>(v.y), non_finite<0x7f80u>(v.z),
+                                   non_finite<0x7f80u>(v.w));
+      if (bad.x | bad.y | bad.z | bad.w) {
+        v = make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w);
+        met = 1u;
+      }
+    }
+  }
+  for (int i = lane; i < (kBlk - rows) * 16; i += 32) {
+    const int row = rows + (i >> 4), a = (i >> 3) & 1;
+    reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  return met != 0u;
+}
+
+template <bool kFp8, class P>
 __global__ void __launch_bounds__(kBrThreads, 1)
-    branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const BranchParams p) {
+    branch_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const P p) {
   using Cfg = BrCfg<kFp8>;
+  constexpr bool kTree = is_tree<P>;
   constexpr int kS = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
-  BrSmem<kFp8>& sm = *reinterpret_cast<BrSmem<kFp8>*>(
+  using Smem = BrSmem<kFp8, P>;
+  Smem& sm = *reinterpret_cast<Smem*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -417,6 +478,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     mbar_init(smem_u32(&sm.m_sync), 2);
     mbar_init(smem_u32(&sm.drain), 2);
     sm.abort_flag = 0;
+    if constexpr (kTree) sm.tree.taken_out = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -494,7 +556,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             g.row0 = at.t * kSpan;
             g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
             g.block0 = at.off;
-            g.kv_end = pl.shared_blocks * kBlk;
+            g.kv_end = g.clean = pl.shared_blocks * kBlk;
             item = at.head * ln.shared_tiles + at.t;
             row0 = 0;
             slot_rows = p.shared_slot_rows;
@@ -502,8 +564,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             seq = at.b;
             g.row0 = at.b * p.rows * p.group + at.t * kSpan;
             g.n_rows = min(kSpan, p.rows * p.group - at.t * kSpan);
-            g.kv_end = seq_length(p, at.b);
-            g.block0 = own_lo(p, g.kv_end) / kBlk + at.off;
+            const Extent x = extent_of(p, at.b);
+            g.kv_end = x.all;
+            g.clean = x.clean;
+            g.block0 = own_lo(p, x) / kBlk + at.off;
             item = (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
             row0 = p.own_row0;
             slot_rows = p.own_slot_rows;
@@ -625,22 +689,17 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     bool ok = true, was_solo = false;
     // the P V of this tile's last block, still to be issued
     bool pend = false, pend_acc = false;
-    int pend_slot = 0, pend_rows = 0;
+    int pend_slot = 0, pend_rows = 0, pend_clean = 0;
     uint32_t pend_bar = 0u, pend_ph = 0u;
     // Waits for P of one half of the pending block and issues its P V.
     auto finish = [&](int half) {
       const bool w = mbar_wait(p_bar + half * 8, p_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
-      if (!kFp8 && pend_rows < kBlk && half == 0) {
-        // rows past the sequence's end may hold anything, NaN among it, and the tensor core
-        // multiplies them with P's zeros: clear them (the tile's load has completed; both warps
-        // of a shared block write the same zeros; e4m3: done when widened)
-        uint8_t* base = sm.kv[pend_slot];
-        constexpr int kAtoms = Cfg::kTile / kAtom;
-        for (int i = lane; i < (kBlk - pend_rows) * kAtoms * 8; i += 32) {
-          const int row = pend_rows + (i >> 3) / kAtoms, a = (i >> 3) % kAtoms;
-          reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7] = make_uint4(0u, 0u, 0u, 0u);
+      if (!kFp8 && min(pend_rows, kTree ? pend_clean : kBlk) < kBlk && half == 0) {  // e4m3: done when widened
+        const bool met = clear_block<kTree>(sm.kv[pend_slot], min(pend_rows, kBlk), pend_clean, lane);
+        if constexpr (kTree) {
+          if (met) *static_cast<volatile int*>(&sm.tree.taken_out) = 1;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -737,6 +796,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             pend_ph = (phases >> vs) & 1u;
           }
           pend_rows = g.kv_end - (g.block0 + j) * kBlk;
+          pend_clean = g.clean - (g.block0 + j) * kBlk;
           first = false;
         }
         const uint32_t bits = (1u << ring) | (1u << vs);
@@ -831,12 +891,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if constexpr (kFp8) sl2 = score_factor(sl2 * __ldg(p.k_scale + it.head));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const int len = seq_length(p, it.at.b);
-      const int limit = it.shared && !takes_shared(p, len) ? 0 : len - (p.causal ? p.rows - 1 - it.at.i : 0);
+      const auto sight = sight_of(p, it.at, it.shared != 0);
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; ok && j < it.mine; ++j) {
-        const int left = limit - (it.block0 + j * it.step) * kBlk;
+        const int key0 = (it.block0 + j * it.step) * kBlk;
 #pragma unroll 1
         for (int h = 0; h < 2; ++h) {
           ok = mbar_wait(smem_u32(&sm.s_full[t][h]), s_ph, abort_flag, p.err);
@@ -847,9 +906,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             if (!first) ok = mbar_wait(smem_u32(&sm.pv_done[t]), h ^ 1, abort_flag, p.err);
           };
           if (!warp_live) pv_done();
-          else if (span == 128) softmax_half<kFp8, 64>(tS, tO, h, 0, left, sl2, first, m, l, pv_done);
-          else if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, left, sl2, first, m, l, pv_done);
-          else softmax_half<kFp8, 16>(tS, tO, h, copy, left, sl2, first, m, l, pv_done);
+          else if (span == 128) softmax_half<kFp8, 64>(tS, tO, h, 0, key0, sight, sl2, first, m, l, pv_done);
+          else if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+          else softmax_half<kFp8, 16>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
           tc_fence_before();
           mbar_arrive(smem_u32(&sm.p_full[t][h]));
         }
@@ -862,6 +921,23 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
       o_ph ^= 1u;
       tc_fence_after();
+      if constexpr (kTree) {  // what was taken out of V, to the rows that see it
+        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.tree.taken_out) != 0)) {
+          const NodeValues<kFp8> nodes(p, it.at.b, it.head);
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+            reg_fence32(o);
+            if (my < n_rows)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + nodes.non_finite_sum(p, sight, c * 32 + j));
+            tmem_st32(tO + c * 32, o);
+          }
+          tmem_wait_st();
+        }
+      }
       // ---- epilogue, through the query tile's buffer (every Q K^T of this item is complete)
       float* const stage = reinterpret_cast<float*>(sm.q[t]);
       float top = m, sum = l;
@@ -1023,8 +1099,18 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (side) phase1 ^= slot_bit;
           else phase0 ^= slot_bit;
           const int rows = g.kv_end - (g.block0 + j) * kBlk;  // that hold anything
-          if (rows >= kBlk) widen_block<false>(smem_u32(sm.kv[ring]), smem_u32(sm.wide.v[wide]), kBlk, lane);
-          else widen_block<true>(smem_u32(sm.kv[ring]), smem_u32(sm.wide.v[wide]), rows, lane);
+          const int clean = g.clean - (g.block0 + j) * kBlk;
+          const uint32_t from = smem_u32(sm.kv[ring]), to = smem_u32(sm.wide.v[wide]);
+          if (kTree && clean < kBlk) {
+            if constexpr (kTree) {
+              if (widen_block<true, true>(from, to, rows, clean, lane))
+                *static_cast<volatile int*>(&sm.tree.taken_out) = 1;
+            }
+          } else if (rows >= kBlk) {
+            widen_block<false, false>(from, to, kBlk, 0, lane);
+          } else {
+            widen_block<true, false>(from, to, rows, 0, lane);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (lane == 0) {
@@ -1125,8 +1211,8 @@ __device__ __forceinline__ void add_pieces(const BranchParams& p, const Pieces (
   }
 }
 
-template <bool kFp8, bool kJoint, int kTeam>
-__global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const BranchParams p) {
+template <bool kFp8, bool kJoint, int kTeam, class P>
+__global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P p) {
   constexpr int kTeams = kMergeWarps / kTeam;
   constexpr int kRows = kJoint ? kJointWarpRows : 1;
   __shared__ float4 sums[kTeam > 1 ? kMergeWarps : 1][32];
@@ -1165,10 +1251,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const Br
     r = t * kSpan + (static_cast<int>(blockIdx.x % kGroups) * kMergeWarps + warp) * kRows;
     if (r >= min(own_all, (t + 1) * kSpan)) return;
   }
-  const int len = seq_length(p, b);
+  const Extent ext = extent_of(p, b);
   int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * (kBlk / lo.unit)) + __ldcg(po + 3 + b);
-  for (int k = 0; k < t; ++k) u0 += weight_of(lo, own_units(p, lo, len, k));
-  const int units = own_units(p, lo, len, t);
+  for (int k = 0; k < t; ++k) u0 += weight_of(lo, own_units(p, lo, ext, k));
+  const int units = own_units(p, lo, ext, t);
   const int n_rows = min(lo.span, own_all - t * lo.span);
   if (shared_blocks == 0 && units > 0 && u0 / cut_o == (u0 + units - 1) / cut_o &&
       (own_by_warps || n_rows > kBlk || units == 1))
@@ -1332,7 +1418,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
   return s;
 }
 
-template <bool kFp8>
+template <bool kFp8, class P>
 int configure() {
   static std::mutex mu;
   static bool done[64] = {};
@@ -1340,9 +1426,9 @@ int configure() {
   cudaGetDevice(&dev);
   std::lock_guard<std::mutex> lk(mu);
   if (dev < 64 && done[dev]) return H3SA_OK;
-  const auto kernel = branch_attn_kernel<kFp8>;
+  const auto kernel = branch_attn_kernel<kFp8, P>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(br_smem_bytes<kFp8>()));
+                                       static_cast<int>(br_smem_bytes<kFp8, P>()));
   if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch attention)", e);
   cudaFuncAttributes attr;
   e = cudaFuncGetAttributes(&attr, kernel);
@@ -1357,23 +1443,23 @@ int configure() {
   return H3SA_OK;
 }
 
-template <bool kFp8>
-int launch_tensor(const BranchParams& p, cudaLaunchConfig_t cfg) {
-  int rc = configure<kFp8>();
+template <bool kFp8, class P>
+int launch_tensor(const P& p, cudaLaunchConfig_t cfg) {
+  int rc = configure<kFp8, P>();
   if (rc) return rc;
   CUtensorMap tmK, tmV;
   if ((rc = encode_pool(&tmK, p, p.key_pool, kFp8, kBlk))) return rc;
   if ((rc = encode_pool(&tmV, p, p.value_pool, kFp8, kBlk))) return rc;
   cfg.gridDim = dim3(p.tensor.workers);
   cfg.blockDim = dim3(kBrThreads);
-  cfg.dynamicSmemBytes = br_smem_bytes<kFp8>();
+  cfg.dynamicSmemBytes = br_smem_bytes<kFp8, P>();
   cfg.numAttrs = 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_attn_kernel<kFp8>, tmK, tmV, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_attn_kernel<kFp8, P>, tmK, tmV, p);
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_attn_kernel launch", e);
 }
 
-template <bool kFp8>
-int launch(const BranchParams& p, cudaStream_t stream) {
+template <bool kFp8, class P>
+int launch(const P& p, cudaStream_t stream) {
   cudaError_t e = cudaSuccess;
   cudaLaunchConfig_t cfg;
   memset(&cfg, 0, sizeof(cfg));
@@ -1385,7 +1471,7 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   cfg.attrs = &early;
   const bool tensor = p.tensor.own_tiles > 0 || p.tensor.shared_tiles > 0;
   if (tensor) {
-    const int rc = launch_tensor<kFp8>(p, cfg);
+    const int rc = launch_tensor<kFp8, P>(p, cfg);
     if (rc) return rc;
   }
   if (p.warp.own_tiles > 0) {  // takes the SMs that the other line is done with
@@ -1407,62 +1493,48 @@ int launch(const BranchParams& p, cudaStream_t stream) {
   cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  e = p.joint ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, true, 1>, p)
-      : team  ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, kMergeWarps>, p)
-              : cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, 1>, p);
+  e = p.joint ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, true, 1, P>, p)
+      : team  ? cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, kMergeWarps, P>, p)
+              : cudaLaunchKernelEx(&cfg, branch_merge_kernel<kFp8, false, 1, P>, p);
   if (e != cudaSuccess) return set_cuda_error("branch_merge_kernel launch", e);
   return H3SA_OK;
 }
 
 bool aligned(const void* q, size_t n) { return (reinterpret_cast<uintptr_t>(q) & (n - 1)) == 0; }
 
-}  // namespace
-}  // namespace h3sa
-
-using namespace h3sa;
-
-extern "C" {
-
-int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
-                                     int32_t shared_rows) {
-  if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
-    return 0;
-  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
-  return s.bytes;
-}
-
-int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int64_t stride_row,
-                                 int64_t stride_head, void* out, float* lse, int32_t batch,
-                                 int32_t rows, int32_t heads, int32_t kv_heads,
-                                 const void* key_pool, const void* value_pool, int32_t pool_pages,
-                                 int32_t e4m3, const float* k_scale, const float* v_scale,
-                                 const int32_t* table, int32_t width, const int32_t* lengths,
-                                 int32_t shared_rows, int32_t causal, float softmax_scale,
-                                 void* workspace, int64_t workspace_bytes, int32_t* device_error,
-                                 void* stream) {
+// Both attentions; `nodes`: the new rows are nodes of drafted trees, else they are a sequence's last rows.
+int attend(const char* what, const TreeParams* nodes, const void* query, int64_t stride_sequence, int64_t stride_row,
+           int64_t stride_head, void* out, float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+           const void* key_pool, const void* value_pool, int32_t pool_pages, int32_t e4m3, const float* k_scale,
+           const float* v_scale, const int32_t* table, int32_t width, const int32_t* lengths, int32_t shared_rows,
+           int32_t causal, float softmax_scale, void* workspace, int64_t workspace_bytes, int32_t* device_error,
+           void* stream) {
   if (batch < 0 || rows < 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: invalid sizes batch=%d rows=%d heads=%d "
-                     "kv_heads=%d (heads must be a multiple of kv_heads)", batch, rows, heads, kv_heads);
+    return set_error(H3SA_ERR_INVALID, "%s: invalid sizes batch=%d rows=%d heads=%d "
+                     "kv_heads=%d (heads must be a multiple of kv_heads)", what, batch, rows, heads, kv_heads);
   if (batch == 0 || rows == 0) return H3SA_OK;
   if (pool_pages <= 0 || width <= 0 || static_cast<int64_t>(pool_pages) * kBlk > INT32_MAX ||
       static_cast<int64_t>(width) * kBlk > INT32_MAX)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: invalid pool of %d pages or table of %d "
-                     "entries a sequence", pool_pages, width);
+    return set_error(H3SA_ERR_INVALID, "%s: invalid pool of %d pages or table of %d "
+                     "entries a sequence", what, pool_pages, width);
   if (shared_rows < 0 || shared_rows % kBlk || shared_rows / kBlk > width)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: %d shared rows are not whole pages of a "
-                     "table of %d entries", shared_rows, width);
+    return set_error(H3SA_ERR_INVALID, "%s: %d shared rows are not whole pages of a "
+                     "table of %d entries", what, shared_rows, width);
   if (!query || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
       (e4m3 && (!k_scale || !v_scale)))
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: null pointer argument");
+    return set_error(H3SA_ERR_INVALID, "%s: null pointer argument", what);
   if (!(softmax_scale > 0.f) || softmax_scale > 2.0e38f)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: the scale must be positive and finite");
+    return set_error(H3SA_ERR_INVALID, "%s: the scale must be positive and finite", what);
   if (!aligned(query, 16) || !aligned(out, 16) || !aligned(key_pool, 16) || !aligned(value_pool, 16) ||
       !aligned(workspace, 16) || stride_sequence % 8 || stride_row % 8 || stride_head % 8)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: tensors and query rows must be 16-byte aligned");
+    return set_error(H3SA_ERR_INVALID, "%s: tensors and query rows must be 16-byte aligned", what);
+  if (nodes && (!nodes->masks || static_cast<int64_t>(width) * kBlk + rows > INT32_MAX))
+    return set_error(H3SA_ERR_INVALID, "%s: masks are missing, or table of %d entries and %d rows too large", what, width,
+                     rows);
   const int group = heads / kv_heads;
   const int64_t stacked = static_cast<int64_t>(batch) * rows * group;
   if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
-    return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d is too large",
+    return set_error(H3SA_ERR_UNSUPPORTED, "%s: batch %d x rows %d x heads %d is too large", what,
                      batch, rows, heads);
   Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
   const auto line_units = [&](const Line& ln) {
@@ -1471,12 +1543,12 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
                        static_cast<int64_t>(batch) * ln.own_tiles * (width * blocks + ln.pad));
   };
   if (line_units(s.tensor) > INT32_MAX / 2 || line_units(s.warp) > INT32_MAX / 2)
-    return set_error(H3SA_ERR_UNSUPPORTED, "shared prefix attention: batch %d x rows %d x heads %d over %d "
-                     "pages exceeds the work index", batch, rows, heads, width);
+    return set_error(H3SA_ERR_UNSUPPORTED, "%s: batch %d x rows %d x heads %d over %d "
+                     "pages exceeds the work index", what, batch, rows, heads, width);
   if (workspace_bytes < s.bytes)
-    return set_error(H3SA_ERR_INVALID, "shared prefix attention: workspace of %lld bytes, %lld needed",
+    return set_error(H3SA_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                      static_cast<long long>(workspace_bytes), s.bytes);
-  BranchParams p;
+  TreeParams p;
   memset(&p, 0, sizeof(p));
   p.q = static_cast<const __nv_bfloat16*>(query);
   p.q_sb = stride_sequence;
@@ -1514,8 +1586,58 @@ int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int
   p.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + s.rows * kD);
   p.plan = reinterpret_cast<int*>(p.part_ml + s.rows);
   p.err = device_error;
-  return e4m3 ? launch<true>(p, static_cast<cudaStream_t>(stream))
-              : launch<false>(p, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s0 = static_cast<cudaStream_t>(stream);
+  if (nodes) {
+    p.masks = nodes->masks;
+    p.counts = nodes->counts;
+    p.words = (rows + 31) / 32;
+    return e4m3 ? launch<true, TreeParams>(p, s0) : launch<false, TreeParams>(p, s0);
+  }
+  return e4m3 ? launch<true, BranchParams>(p, s0) : launch<false, BranchParams>(p, s0);
+}
+
+}  // namespace
+}  // namespace h3sa
+
+using namespace h3sa;
+
+extern "C" {
+
+int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
+                                     int32_t shared_rows) {
+  if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
+    return 0;
+  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
+  return s.bytes;
+}
+
+int h3sa_shared_prefix_attention(const void* query, int64_t stride_sequence, int64_t stride_row,
+                                 int64_t stride_head, void* out, float* lse, int32_t batch,
+                                 int32_t rows, int32_t heads, int32_t kv_heads,
+                                 const void* key_pool, const void* value_pool, int32_t pool_pages,
+                                 int32_t e4m3, const float* k_scale, const float* v_scale,
+                                 const int32_t* table, int32_t width, const int32_t* lengths,
+                                 int32_t shared_rows, int32_t causal, float softmax_scale,
+                                 void* workspace, int64_t workspace_bytes, int32_t* device_error,
+                                 void* stream) {
+  return attend("shared prefix attention", nullptr, query, stride_sequence, stride_row, stride_head, out, lse, batch, rows,
+                heads, kv_heads, key_pool, value_pool, pool_pages, e4m3, k_scale, v_scale, table, width, lengths,
+                shared_rows, causal, softmax_scale, workspace, workspace_bytes, device_error, stream);
+}
+
+int h3sa_tree_attention(const void* query, int64_t stride_sequence, int64_t stride_row, int64_t stride_head, void* out,
+                        float* lse, int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, const void* key_pool,
+                        const void* value_pool, int32_t pool_pages, int32_t e4m3, const float* k_scale,
+                        const float* v_scale, const int32_t* table, int32_t width, const int32_t* lengths,
+                        const int32_t* masks, const int32_t* counts, int32_t shared_rows, float softmax_scale,
+                        void* workspace, int64_t workspace_bytes, int32_t* device_error, void* stream) {
+  TreeParams nodes;
+  memset(&nodes, 0, sizeof(nodes));
+  nodes.masks = reinterpret_cast<const uint32_t*>(masks);
+  nodes.counts = counts;
+  return attend("tree attention", &nodes, query, stride_sequence, stride_row, stride_head, out, lse, batch, rows, heads,
+                kv_heads, key_pool, value_pool, pool_pages, e4m3, k_scale, v_scale, table, width, lengths, shared_rows, 0,
+                softmax_scale, workspace, workspace_bytes, device_error, stream);
 }
 
 }  // extern "C"

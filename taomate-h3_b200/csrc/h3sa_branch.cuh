@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
@@ -63,31 +64,54 @@ struct BranchParams {
   int* err;
 };
 
-__device__ __forceinline__ int seq_length(const BranchParams& p, int b) {
+// New rows that are the nodes of a drafted tree: they lie behind the first lengths[b] rows, and row i sees
+// those and the nodes of its mask.
+struct TreeParams : BranchParams {
+  const uint32_t* masks;  // [batch, rows, words]: bit n of row i: node n is node i or above it
+  const int* counts;      // [batch] nodes, or null: `rows` of each
+  int words;
+};
+template <class P>
+constexpr bool is_tree = std::is_same_v<P, TreeParams>;
+
+// Rows of a sequence: all keys, and those that each of its new rows may see.
+struct Extent {
+  int all, clean;
+};
+__device__ __forceinline__ int clean_rows(const BranchParams& p, int b) {
   const int n = __ldg(p.lengths + b);
   return max(0, min(n, p.width * kBlk));
+}
+__device__ __forceinline__ Extent extent_of(const BranchParams& p, int b) {
+  const int n = clean_rows(p, b);
+  return Extent{n, n};
+}
+__device__ __forceinline__ Extent extent_of(const TreeParams& p, int b) {
+  const int n = clean_rows(p, b);
+  const int nodes = p.counts ? max(0, min(__ldg(p.counts + b), p.rows)) : p.rows;
+  return Extent{min(n + nodes, p.width * kBlk), n};
 }
 
 // A sequence that ends inside the shared blocks has no part in their items, where rows behind its end that
 // others see would meet its zeros of P, and NaN or infinities among them its output: its own items
 // have all its keys.
-__device__ __forceinline__ bool takes_shared(const BranchParams& p, int len) { return len >= p.shared_keys; }
+__device__ __forceinline__ bool takes_shared(const BranchParams& p, const Extent& x) { return x.clean >= p.shared_keys; }
 // The first key outside the shared items, and the units behind it of the rows of tile t of a
 // sequence of length `len`.
-__device__ __forceinline__ int own_lo(const BranchParams& p, int len) { return takes_shared(p, len) ? p.shared_keys : 0; }
-__device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, int len, int t) {
-  if (!p.causal) return len;
+__device__ __forceinline__ int own_lo(const BranchParams& p, const Extent& x) { return takes_shared(p, x) ? p.shared_keys : 0; }
+__device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, const Extent& x, int t) {
+  if (!p.causal) return x.all;
   const int last = min((t + 1) * ln.span, p.rows * p.group) - 1;
-  return len - (p.rows - 1 - last / p.group);
+  return x.all - (p.rows - 1 - last / p.group);
 }
-__device__ __forceinline__ int own_units(const BranchParams& p, const Line& ln, int len, int t) {
-  return max(0, own_limit(p, ln, len, t) - own_lo(p, len) + ln.unit - 1) / ln.unit;
+__device__ __forceinline__ int own_units(const BranchParams& p, const Line& ln, const Extent& x, int t) {
+  return max(0, own_limit(p, ln, x, t) - own_lo(p, x) + ln.unit - 1) / ln.unit;
 }
 __device__ __forceinline__ int weight_of(const Line& ln, int units) { return units > 0 ? units + ln.pad : 0; }
-__device__ __forceinline__ int own_weight_all(const BranchParams& p, const Line& ln, int len) {
-  if (!p.causal) return weight_of(ln, own_units(p, ln, len, 0)) * ln.own_tiles;
+__device__ __forceinline__ int own_weight_all(const BranchParams& p, const Line& ln, const Extent& x) {
+  if (!p.causal) return weight_of(ln, own_units(p, ln, x, 0)) * ln.own_tiles;
   int n = 0;
-  for (int t = 0; t < ln.own_tiles; ++t) n += weight_of(ln, own_units(p, ln, len, t));
+  for (int t = 0; t < ln.own_tiles; ++t) n += weight_of(ln, own_units(p, ln, x, t));
   return n;
 }
 
@@ -99,13 +123,14 @@ struct Plan {
   int longest;        // sequence whose table row gives the shared pages
 };
 
-__device__ __forceinline__ Plan make_plan(const BranchParams& p, const Line& ln, int lane) {
+template <class P>
+__device__ __forceinline__ Plan make_plan(const P& p, const Line& ln, int lane) {
   int own = 0, best = -1, at = 0;
   for (int b = lane; b < p.batch; b += 32) {
-    const int len = seq_length(p, b);
-    own += own_weight_all(p, ln, len);
-    if (len > best) {
-      best = len;
+    const Extent x = extent_of(p, b);
+    own += own_weight_all(p, ln, x);
+    if (x.clean > best) {
+      best = x.clean;
       at = b;
     }
   }
@@ -114,7 +139,7 @@ __device__ __forceinline__ Plan make_plan(const BranchParams& p, const Line& ln,
   at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
   Plan pl;
   pl.longest = at;
-  pl.shared_blocks = own_lo(p, top) / kBlk;
+  pl.shared_blocks = own_lo(p, Extent{top, top}) / kBlk;
   pl.shared_units = pl.shared_blocks * (kBlk / ln.unit);
   pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units) + own;
   const int all = pl.head_weight * p.kv_heads;
@@ -129,7 +154,8 @@ struct Place {
 };
 
 // The place of position `u` of the line (warp-collective).
-__device__ __forceinline__ Place locate(const BranchParams& p, const Line& ln, const Plan& pl, int u, int lane) {
+template <class P>
+__device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& pl, int u, int lane) {
   Place at;
   at.head = u / pl.head_weight;
   at.b = -1;
@@ -144,7 +170,7 @@ __device__ __forceinline__ Place locate(const BranchParams& p, const Line& ln, c
   x -= ln.shared_tiles * w;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < p.batch ? own_weight_all(p, ln, seq_length(p, b)) : 0;
+    const int n = b < p.batch ? own_weight_all(p, ln, extent_of(p, b)) : 0;
     int cum = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -160,14 +186,15 @@ __device__ __forceinline__ Place locate(const BranchParams& p, const Line& ln, c
     }
     x -= __shfl_sync(0xffffffffu, cum, 31);
   }
-  const int len = seq_length(p, at.b);
-  for (int v; x >= (v = weight_of(ln, own_units(p, ln, len, at.t))); ++at.t) x -= v;
+  const Extent ext = extent_of(p, at.b);
+  for (int v; x >= (v = weight_of(ln, own_units(p, ln, ext, at.t))); ++at.t) x -= v;
   at.off = x;
   return at;
 }
 
 // To the next item that has units; there must be one.
-__device__ __forceinline__ void step_item(const BranchParams& p, const Line& ln, const Plan& pl, Place& at) {
+template <class P>
+__device__ __forceinline__ void step_item(const P& p, const Line& ln, const Plan& pl, Place& at) {
   const bool shared = ln.shared_tiles > 0 && pl.shared_units > 0;
   at.off = 0;
   if (at.b < 0) {
@@ -184,16 +211,18 @@ __device__ __forceinline__ void step_item(const BranchParams& p, const Line& ln,
         if (shared) return;
       }
     }
-    if (ln.own_tiles > 0 && own_units(p, ln, seq_length(p, at.b), at.t) > 0) return;
+    if (ln.own_tiles > 0 && own_units(p, ln, extent_of(p, at.b), at.t) > 0) return;
   }
 }
-__device__ __forceinline__ int place_units(const BranchParams& p, const Line& ln, const Plan& pl, const Place& at) {
-  return at.b < 0 ? pl.shared_units : own_units(p, ln, seq_length(p, at.b), at.t);
+template <class P>
+__device__ __forceinline__ int place_units(const P& p, const Line& ln, const Plan& pl, const Place& at) {
+  return at.b < 0 ? pl.shared_units : own_units(p, ln, extent_of(p, at.b), at.t);
 }
 
 // Writes a line's schedule down for the merge: the shared units, a head's and a worker's part, and
 // what lies in front of each sequence's own items.
-__device__ __forceinline__ void write_plan(const BranchParams& p, const Line& ln, const Plan& pl, int* out, int lane) {
+template <class P>
+__device__ __forceinline__ void write_plan(const P& p, const Line& ln, const Plan& pl, int* out, int lane) {
   if (lane == 0) {
     out[0] = pl.shared_blocks;
     out[1] = pl.head_weight;
@@ -202,7 +231,7 @@ __device__ __forceinline__ void write_plan(const BranchParams& p, const Line& ln
   int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < p.batch ? own_weight_all(p, ln, seq_length(p, b)) : 0;
+    const int n = b < p.batch ? own_weight_all(p, ln, extent_of(p, b)) : 0;
     int cum = n;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -220,6 +249,13 @@ __device__ __forceinline__ void flag_lengths(const BranchParams& p, int lane) {
     if ((n < 0 || n > p.width * kBlk) && p.err) atomicOr(p.err, kErrBadIndex);
   }
 }
+__device__ __forceinline__ void flag_lengths(const TreeParams& p, int lane) {
+  for (int b = lane; b < p.batch; b += 32) {
+    const int n = __ldg(p.lengths + b), nodes = p.counts ? __ldg(p.counts + b) : p.rows;
+    const bool fits = n >= 0 && n <= p.width * kBlk && nodes >= 0 && nodes <= p.rows && n + nodes <= p.width * kBlk;
+    if (!fits && p.err) atomicOr(p.err, kErrBadIndex);
+  }
+}
 
 // A stacked row (branch, row, query head of the KV head's group).
 struct RowAt {
@@ -233,6 +269,79 @@ __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) 
   a.i = bi - a.b * p.rows;
   return a;
 }
+
+// What a node sees: all keys in front of `base`, and key base + n, n < count, if bit n of its mask says so.
+// A row that sees nothing of an item (one behind the nodes, one without the shared blocks) has 0 and 0.
+struct Sight {
+  int base, count;
+  const uint32_t* mask;
+  __device__ __forceinline__ uint32_t word(int w) const {
+    const int rest = count - 32 * w;
+    if (w < 0 || rest <= 0) return 0u;
+    const uint32_t bits = __ldg(mask + w);
+    return rest >= 32 ? bits : bits & ((1u << rest) - 1u);
+  }
+  // bit j: whether it sees key + j
+  __device__ __forceinline__ uint32_t seen32(int key) const {
+    const int x = key - base;
+    if (x <= -32) return 0xffffffffu;
+    if (x < 0) return (0xffffffffu >> (32 + x)) | (word(0) << -x);
+    return __funnelshift_r(word(x >> 5), word((x >> 5) + 1), x & 31);
+  }
+};
+__device__ __forceinline__ Sight sight_of(const TreeParams& p, const RowAt& ra, bool shared) {
+  const Extent x = extent_of(p, ra.b);
+  const int count = x.all - x.clean;
+  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{0, 0, nullptr};
+  return Sight{x.clean, count, p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words};
+}
+
+// Of a chain, only a limit.
+struct Limit {
+  int base;
+};
+__device__ __forceinline__ Limit sight_of(const BranchParams& p, const RowAt& ra, bool shared) {
+  const Extent x = extent_of(p, ra.b);
+  return Limit{shared && !takes_shared(p, x) ? 0 : x.all - (p.causal ? p.rows - 1 - ra.i : 0)};
+}
+
+// Infinities and NaN in V of a node must not reach rows that do not see it, whose P is zero there: they are
+// taken out of V's tile in shared memory, and a row that does see such a node gets them back in the end.
+// Two values of a word at a time; `top` are the exponent bits of one.
+template <uint32_t kTop>
+__device__ __forceinline__ uint32_t non_finite(uint32_t w) {  // 0xffff in each half that is an infinity or NaN
+  constexpr uint32_t kLow = kTop & (0u - kTop);               // the exponent's lowest bit: all ones and it carry out
+  const uint32_t carry = ((w & (kTop | kTop << 16)) + (kLow | kLow << 16)) & 0x80008000u;
+  return (carry >> 15) * 0xffffu;
+}
+
+// V of the nodes of sequence b in a KV head, read from the pool again.
+template <bool kFp8>
+struct NodeValues {
+  const uint8_t* pool;  // of the head
+  const int* table;
+  __device__ __forceinline__ NodeValues(const TreeParams& p, int b, int head)
+      : pool(static_cast<const uint8_t*>(p.value_pool) +
+             static_cast<size_t>(head) * p.pool_pages * kBlk * (kD * (kFp8 ? 1 : 2))),
+        table(p.table + static_cast<size_t>(b) * p.width) {}
+  // The infinities and NaN of column `col` in the nodes that a row sees, added up; 0 if there are none.
+  __device__ __forceinline__ float non_finite_sum(const TreeParams& p, const Sight& sight, int col) const {
+    float sum = 0.f;
+    for (int n = 0; n < sight.count; ++n) {
+      if (!(sight.word(n >> 5) >> (n & 31) & 1u)) continue;
+      const int key = sight.base + n, page = __ldg(table + key / kBlk);
+      if (page < 0 || page >= p.pool_pages) continue;
+      const size_t at = (static_cast<size_t>(page) * kBlk + key % kBlk) * kD + col;
+      if constexpr (kFp8) {
+        if ((pool[at] & 0x7fu) == 0x7fu) sum = __int_as_float(0x7fffffff);
+      } else {
+        const uint32_t v = reinterpret_cast<const uint16_t*>(pool)[at];
+        if ((v & 0x7f80u) == 0x7f80u) sum += __uint_as_float(v << 16);
+      }
+    }
+    return sum;
+  }
+};
 
 __device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
   uint32_t r;
@@ -271,6 +380,7 @@ __device__ __forceinline__ void tma_load_3d_once(uint32_t dst, const CUtensorMap
 // Launches the warp line's kernel (h3sa_branch_rows.cu); `after`: along with another kernel, whose end
 // the line then waits for as well. Returns an H3SA_* status.
 int launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg);
+int launch_branch_rows(const TreeParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg);
 
 // Tensor map of a pool with boxes of `rows` rows of 128 bytes, 128-byte swizzle.
 int encode_pool(CUtensorMap* map, const BranchParams& p, const void* pool, bool e4m3, int rows);

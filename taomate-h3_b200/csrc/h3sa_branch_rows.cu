@@ -85,18 +85,40 @@ __device__ __forceinline__ void split_bf16(const float (&p)[4], const float (&q)
   lo = make_uint4(rest(hi.x, p[0], p[1]), rest(hi.y, p[2], p[3]), rest(hi.z, q[0], q[1]), rest(hi.w, q[2], q[3]));
 }
 
+// Takes infinities and NaN out of 16 bytes of V; returns whether there were any.
+template <bool kFp8>
+__device__ __forceinline__ bool take_out(uint4& v) {
+  uint32_t* const w = &v.x;
+  uint32_t met = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t bad = kFp8 ? __vcmpeq4(w[i] & 0x7f7f7f7fu, 0x7f7f7f7fu) : non_finite<0x7f80u>(w[i]);
+    w[i] &= ~bad;
+    met |= bad;
+  }
+  return met != 0u;
+}
+
+// The column of o[j][e] and o[j][2 + e] in lane 4r + c: eight neighbouring columns are o[8h + i][e], i < 8, of one h and e.
+template <bool kFp8>
+__device__ __forceinline__ int column_of(int c, int j, int e) {
+  const int h = j >> 3, i = j & 7;
+  return kFp8 ? 32 * c + 8 * (2 * e + h) + i : 64 * h + 16 * c + 8 * e + i;
+}
+
 // What a warp knows of a segment: rows row0 .. of KV head `head` against `units` units of keys from key0.
 struct RowSegment {
-  int units, head, seq, shared, row0, n_rows, key0, kv_end, direct;
+  int units, head, seq, shared, row0, n_rows, key0, kv_end, clean, direct;
   long long slot;
 };
 
 // kWhole: no line; a warp takes whole items, a branch's rows against all its keys, and nothing is left
 // to merge. kFine: bf16 P in two terms.
-template <bool kFp8, bool kWhole, bool kFine>
+template <bool kFp8, bool kWhole, bool kFine, class P>
 __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     branch_rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const BranchParams p, const bool after) {
+                       const P p, const bool after) {
+  constexpr bool kTree = is_tree<P>;
   constexpr int kTileBytes = RowCfg<kFp8>::kTileBytes, kStageBytes = RowCfg<kFp8>::kStageBytes;
   constexpr int kRowStages = RowCfg<kFp8>::kStages;
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
@@ -152,10 +174,12 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.row0 = g.seq * own_all + t * kRowSpan;
         g.n_rows = min(kRowSpan, own_all - t * kRowSpan);
         g.key0 = 0;
-        g.kv_end = seq_length(p, g.seq);
+        const Extent x = extent_of(p, g.seq);
+        g.kv_end = x.all;
+        g.clean = x.clean;
         g.direct = 1;
         g.slot = 0;
-        g.units = own_units(p, ln, g.kv_end, t);
+        g.units = own_units(p, ln, x, t);
         if (g.units > 0) continue;
         for (int i = lane; !loader && i < g.n_rows * 16; i += 32) {  // rows that see nothing
           const RowAt ra = row_at(p, g.head, g.row0 + (i >> 4));
@@ -176,9 +200,10 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
         g.n_rows = min(kRowSpan, (g.shared ? p.batch * own_all : (at.b + 1) * own_all) - g.row0);
-        const int len = seq_length(p, g.seq);
-        g.key0 = (g.shared ? 0 : own_lo(p, len)) + at.off * kRowUnit;
-        g.kv_end = len;
+        const Extent x = extent_of(p, g.seq);
+        g.key0 = (g.shared ? 0 : own_lo(p, x)) + at.off * kRowUnit;
+        g.kv_end = x.all;
+        g.clean = x.clean;
         g.direct = pl.shared_blocks == 0 && n == units;
         const long long item = g.shared ? static_cast<long long>(at.head) * ln.shared_tiles + at.t
                                         : (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
@@ -271,11 +296,9 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         load16(b + from, qb + 4 * k);
       }
     }
-    const auto limit_of = [&](const RowAt& ra) {
-      const int len = seq_length(p, ra.b);
-      return g.shared && !takes_shared(p, len) ? 0 : len - (p.causal ? p.rows - 1 - ra.i : 0);
-    };
-    const int lim0 = limit_of(at0), lim1 = limit_of(at1);
+    const auto sight0 = sight_of(p, at0, g.shared != 0), sight1 = sight_of(p, at1, g.shared != 0);
+    const int lim0 = sight0.base, lim1 = sight1.base;
+    bool taken_out = false;  // whether a node's V held an infinity or NaN
     float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
@@ -342,6 +365,16 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       }
       // keys at or past a row's limit are hidden from it
       if (__any_sync(0xffffffffu, key + 32 > min(lim0, lim1))) {
+        if constexpr (kTree) {  // but for nodes that it sees
+          const uint32_t seen0 = sight0.seen32(key), seen1 = sight1.seen32(key);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if (!(seen0 >> (8 * j + 2 * c + k) & 1u)) s[j][k] = -INFINITY;
+              if (!(seen1 >> (8 * j + 2 * c + k) & 1u)) s[j][2 + k] = -INFINITY;
+            }
+        } else {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -350,6 +383,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
             if (at_key >= lim0) s[j][k] = -INFINITY;
             if (at_key >= lim1) s[j][2 + k] = -INFINITY;
           }
+        }
       }
       float t0 = fmaxf(fmax3(fmaxf(s[0][0], s[0][1]), s[1][0], s[1][1]), fmax3(fmaxf(s[2][0], s[2][1]), s[3][0], s[3][1]));
       float t1 = fmaxf(fmax3(fmaxf(s[0][2], s[0][3]), s[1][2], s[1][3]), fmax3(fmaxf(s[2][2], s[2][3]), s[3][2], s[3][3]));
@@ -399,6 +433,9 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
             v[k] = lds16(vt + atom * (kTileBytes / 2) + row * 128 + ((r ^ (row & 7)) << 4));
             // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
             if (tail && key + row >= g.kv_end) v[k] = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (kTree) {
+              if (key + row >= g.clean) taken_out |= take_out<kFp8>(v[k]);
+            }
           }
           const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, y[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
           const uint32_t z[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, t[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
@@ -430,6 +467,19 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       advance();
     }
     if (!ok) break;
+    if constexpr (kTree) {  // what was taken out of V, to the rows that see it
+      if (__any_sync(0xffffffffu, taken_out)) {
+        const NodeValues<kFp8> nodes(p, g.seq, g.head);
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = column_of<kFp8>(c, j, e);
+            o[j][e] += nodes.non_finite_sum(p, sight0, col);
+            o[j][2 + e] += nodes.non_finite_sum(p, sight1, col);
+          }
+      }
+    }
     l0 = quad_sum(l0);
     l1 = quad_sum(l1);
     // ---- this lane's columns: e4m3 32c .. + 31, bf16 16c .. + 15 and 64 + 16c .. + 15; eight at a time
@@ -472,8 +522,8 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
   if (after && blockIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-template <bool kFp8, bool kWhole, bool kFine>
-int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
+template <bool kFp8, bool kWhole, bool kFine, class P>
+int launch_rows(const P& p, bool after, cudaLaunchConfig_t cfg) {
   static std::mutex mu;
   static bool done[64] = {};
   int dev = 0;
@@ -481,7 +531,7 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   {
     std::lock_guard<std::mutex> lk(mu);
     if (dev >= 64 || !done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8, kWhole, kFine>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      const cudaError_t e = cudaFuncSetAttribute(branch_rows_kernel<kFp8, kWhole, kFine, P>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  static_cast<int>(kRowSmem));
       if (e != cudaSuccess) return set_cuda_error("cudaFuncSetAttribute(branch rows)", e);
       if (dev < 64) done[dev] = true;
@@ -495,18 +545,27 @@ int launch_rows(const BranchParams& p, bool after, cudaLaunchConfig_t cfg) {
   cfg.gridDim = dim3(kWhole ? min(sms, p.kv_heads * p.batch * p.warp.own_tiles) : sms);
   cfg.blockDim = dim3(2 * 32 * kRowWarps);
   cfg.dynamicSmemBytes = kRowSmem;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8, kWhole, kFine>, tmK, tmV, p, after);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, branch_rows_kernel<kFp8, kWhole, kFine, P>, tmK, tmV, p, after);
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("branch_rows_kernel launch", e);
+}
+
+template <class P>
+int launch_lines(const P& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
+  if (e4m3)
+    return p.whole ? launch_rows<true, true, false, P>(p, after, cfg) : launch_rows<true, false, false, P>(p, after, cfg);
+  if (p.whole) return launch_rows<false, true, true, P>(p, after, cfg);
+  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
+  return kRowWarps * stacked <= p.warp.workers ? launch_rows<false, false, true, P>(p, after, cfg)
+                                               : launch_rows<false, false, false, P>(p, after, cfg);
 }
 
 }  // namespace
 
 int launch_branch_rows(const BranchParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
-  if (e4m3) return p.whole ? launch_rows<true, true, false>(p, after, cfg) : launch_rows<true, false, false>(p, after, cfg);
-  if (p.whole) return launch_rows<false, true, true>(p, after, cfg);
-  const long long stacked = static_cast<long long>(p.batch) * p.rows * p.heads;
-  return kRowWarps * stacked <= p.warp.workers ? launch_rows<false, false, true>(p, after, cfg)
-                                               : launch_rows<false, false, false>(p, after, cfg);
+  return launch_lines(p, e4m3, after, cfg);
+}
+int launch_branch_rows(const TreeParams& p, bool e4m3, bool after, cudaLaunchConfig_t cfg) {
+  return launch_lines(p, e4m3, after, cfg);
 }
 
 int encode_pool(CUtensorMap* map, const BranchParams& p, const void* pool, bool e4m3, int rows) {

@@ -20,6 +20,10 @@ int set_cuda_error(const char* what, cudaError_t e);
 int encode_tiled_3d(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
                     const uint64_t dims[3], const uint64_t strides_bytes[2], const uint32_t box[3]);
 
+// What every call on a ledger checks of its pool tensors (an H3SA_* status) and of its tables' sizes.
+int check_pools(const char* what, const h3sa_pools* pools);
+bool ledger_sizes_ok(int32_t sequences, int32_t width);
+
 struct AttnLaunch {
   const void* query;  // [rows, heads, 128] bf16 or e4m3
   void* out;          // [rows, heads, 128] bf16

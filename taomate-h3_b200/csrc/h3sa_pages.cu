@@ -391,10 +391,12 @@ int copy_launch(const h3sa_pools* pools, const int4* moves, const int* n_moves, 
   return H3SA_OK;
 }
 
+}  // namespace
+
 // Loops run past the end of a table or a list by up to the threads of a cluster: what they count stays as
 // much below 2^31.
 constexpr int64_t kMaxEntries = INT32_MAX - 65536;
-bool sizes_ok(int32_t sequences, int32_t width) {
+bool ledger_sizes_ok(int32_t sequences, int32_t width) {
   return sequences >= 0 && width > 0 && static_cast<int64_t>(width) * kPage <= INT32_MAX &&
          static_cast<int64_t>(sequences) * width <= kMaxEntries;
 }
@@ -415,7 +417,6 @@ int check_pools(const char* what, const h3sa_pools* p) {
   return H3SA_OK;
 }
 
-}  // namespace
 }  // namespace h3sa
 
 using namespace h3sa;
@@ -436,7 +437,7 @@ int h3sa_fork_pages(const h3sa_pools* pools, const int32_t* table, int32_t seque
                     int32_t* device_error, void* stream) {
   int rc = check_pools("fork_pages", pools);
   if (rc) return rc;
-  if (!sizes_ok(sequences, width) || !sizes_ok(children, width) || reserve_rows < 0)
+  if (!ledger_sizes_ok(sequences, width) || !ledger_sizes_ok(children, width) || reserve_rows < 0)
     return set_error(H3SA_ERR_INVALID, "fork_pages: invalid sizes sequences=%d width=%d children=%d reserve=%d",
                      sequences, width, children, reserve_rows);
   if ((sequences > 0 && (!table || !lengths)) || !refs || !refs_out || !workspace ||
@@ -477,7 +478,7 @@ int h3sa_compact_pages(const h3sa_pools* pools, const int32_t* table, int32_t se
                        void* workspace, int32_t* device_error, void* stream) {
   int rc = check_pools("compact_pages", pools);
   if (rc) return rc;
-  if (!sizes_ok(sequences, width))
+  if (!ledger_sizes_ok(sequences, width))
     return set_error(H3SA_ERR_INVALID, "compact_pages: invalid sizes sequences=%d width=%d", sequences, width);
   if ((sequences > 0 && (!table || !table_out)) || !refs || !refs_out || !live || !workspace)
     return set_error(H3SA_ERR_INVALID, "compact_pages: null pointer argument");
@@ -506,7 +507,7 @@ int h3sa_compact_pages(const h3sa_pools* pools, const int32_t* table, int32_t se
 int h3sa_free_pages(const int32_t* table, int32_t sequences, int32_t width, const int32_t* lengths,
                     const int32_t* refs, int32_t pages, const uint8_t* release, int32_t* table_out,
                     int32_t* lengths_out, int32_t* refs_out, int32_t* device_error, void* stream) {
-  if (!sizes_ok(sequences, width) || pages <= 0 || static_cast<int64_t>(pages) * kPage > INT32_MAX)
+  if (!ledger_sizes_ok(sequences, width) || pages <= 0 || static_cast<int64_t>(pages) * kPage > INT32_MAX)
     return set_error(H3SA_ERR_INVALID, "free_pages: invalid sizes sequences=%d width=%d pages=%d", sequences,
                      width, pages);
   if ((sequences > 0 && (!table || !lengths || !release || !table_out || !lengths_out)) || !refs || !refs_out)

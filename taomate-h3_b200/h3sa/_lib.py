@@ -75,6 +75,30 @@ class Pools(ctypes.Structure):
     ]
 
 
+class Heads(ctypes.Structure):
+    _fields_ = [
+        ("base", ctypes.c_void_p),
+        ("stride_sequence", ctypes.c_int64),
+        ("stride_row", ctypes.c_int64),
+        ("stride_head", ctypes.c_int64),
+        ("heads", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class RotaryPositions(ctypes.Structure):
+    _fields_ = [
+        ("positions", ctypes.c_void_p),
+        ("frequencies", ctypes.c_void_p),
+        ("position_kind", ctypes.c_int32),
+        ("axes", ctypes.c_int32),
+        ("pairs", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("factor", ctypes.c_float),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
 _L = ctypes.c_int64
@@ -163,6 +187,18 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [_P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I, _I, _F,
          _P, _L, _P, _P]),
+    "h3sa_draft_tree": (ctypes.c_int, [_P, _I, _I, _P, _P, _P, _P, _P, _P]),
+    "h3sa_rotate": (
+        ctypes.c_int,
+        [ctypes.POINTER(Heads), ctypes.POINTER(Heads), _I, _I, _I, _I, ctypes.POINTER(RotaryPositions), _P]),
+    "h3sa_append_rows": (
+        ctypes.c_int,
+        [ctypes.POINTER(Heads), ctypes.POINTER(Heads), ctypes.POINTER(Heads), ctypes.POINTER(Heads), _I, _I, _P, _P, _I,
+         _I, _P, _P, _P, _I, _P, _P, ctypes.POINTER(RotaryPositions), _P, _P]),
+    "h3sa_tree_attention": (
+        ctypes.c_int,
+        [_P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _F, _P, _L, _P, _P]),
+    "h3sa_keep_rows": (ctypes.c_int, [ctypes.POINTER(Pools), _P, _I, _I, _P, _P, _I, _P, _P, _P]),
     "h3sa_permute_rows": (
         ctypes.c_int,
         [_P, _P, ctypes.POINTER(ctypes.c_int64), ctypes.POINTER(ctypes.c_int64),

@@ -39,6 +39,7 @@ PoolTensors = Union[torch.Tensor, Sequence[torch.Tensor]]
 # points are bound once, conditions are tested inline and messages built only on failure.
 _FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_free_pages
 _ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
+_ATTEND_TREE = LIB.h3sa_tree_attention
 _PAGES_WORK = LIB.h3sa_pages_workspace
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _I32, _F32, _BF16, _E4M3 = torch.int32, torch.float32, torch.bfloat16, torch.float8_e4m3fn
@@ -79,10 +80,10 @@ def _handle(stream: torch.cuda.Stream | None, device: torch.device) -> int:
     return _raw_stream(device.index) if stream is None else stream.cuda_stream
 
 
-def _pools(what: str, pools: PoolTensors, pages: int, device: torch.device) -> Pools:
+def _pools(what: str, pools: PoolTensors, pages: int | None, device: torch.device) -> Pools:
     """The pool tensors of a ledger: one tensor ``[count, heads, pages*128, d]`` or a sequence of
-    ``[heads, pages*128, d]``, all of one shape and dtype. The returned struct keeps its address
-    list alive."""
+    ``[heads, pages*128, d]``, all of one shape and dtype, of the ledger's pages where a call has them. The
+    returned struct keeps its address list alive."""
 
     p = Pools()
     if isinstance(pools, torch.Tensor):
@@ -108,6 +109,10 @@ def _pools(what: str, pools: PoolTensors, pages: int, device: torch.device) -> P
         address = (ctypes.c_void_p * len(pools))(*[t.data_ptr() for t in pools])
         p.list, p.count = ctypes.addressof(address), len(pools)
         p._address = address
+    if pages is None:
+        pages = rows // PAGE_ROWS
+        if heads == 0 or rows == 0 or rows % PAGE_ROWS:
+            raise RuntimeError(f"{what}: pool tensors must be [heads, pages*{PAGE_ROWS}, d]")
     if heads == 0 or rows != pages * PAGE_ROWS:
         raise RuntimeError(f"{what}: pool tensors must be [heads, {pages}*{PAGE_ROWS}, d] for {pages} "
                            "reference counts")
@@ -241,7 +246,17 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
     overlap ``query``.
     """
 
-    what = "shared_prefix_attention"
+    return _attend("shared_prefix_attention", None, None, query, key_pool, value_pool, table, lengths, shared_rows,
+                   softmax_scale, causal, k_scale, v_scale, out, lse, device_error, stream)
+
+
+def _attend(what: str, masks: torch.Tensor | None, counts: int | None, query: torch.Tensor, key_pool: torch.Tensor,
+            value_pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor, shared_rows: int, softmax_scale: float,
+            causal: bool, k_scale: torch.Tensor | None, v_scale: torch.Tensor | None, out: torch.Tensor | None,
+            lse: torch.Tensor | None, device_error: torch.Tensor | None,
+            stream: torch.cuda.Stream | None) -> torch.Tensor:
+    """``shared_prefix_attention``, and with ``masks`` ``h3sa.drafts.tree_attention`` (counts: an address)."""
+
     if not query.is_cuda:
         raise RuntimeError("h3sa kernels require CUDA tensors")
     device, shape, pool = query.device, query.shape, key_pool.shape
@@ -290,14 +305,19 @@ def shared_prefix_attention(query: torch.Tensor, key_pool: torch.Tensor, value_p
             out = (_empty_like(query) if query.is_contiguous() else
                    query.new_empty(shape))
         work = lengths.new_empty(need // 4)
-    code = _ATTEND(query.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(),
-                   None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
-                   key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
-                   k_scale.data_ptr() if e4m3 else None, v_scale.data_ptr() if e4m3 else None,
-                   table.data_ptr(), width, lengths.data_ptr(), shared_rows, 1 if causal else 0,
-                   softmax_scale, work.data_ptr(), need, error, _handle(stream, device))
+    args = (query.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(),
+            None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
+            key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
+            k_scale.data_ptr() if e4m3 else None, v_scale.data_ptr() if e4m3 else None,
+            table.data_ptr(), width, lengths.data_ptr())
+    if masks is None:
+        code = _ATTEND(*args, shared_rows, 1 if causal else 0, softmax_scale, work.data_ptr(), need, error,
+                       _handle(stream, device))
+    else:
+        code = _ATTEND_TREE(*args, masks.data_ptr(), counts, shared_rows, softmax_scale, work.data_ptr(), need, error,
+                            _handle(stream, device))
     if code:
-        check("h3sa_shared_prefix_attention", code)
+        check(f"h3sa_{what}", code)
     return out
 
 
