@@ -19,7 +19,9 @@
 #include <cuda_runtime.h>
 
 #include <cstring>
+#include <type_traits>
 
+#include "h3sa_fp8.cuh"
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
 
@@ -61,31 +63,41 @@ struct Angles {
 struct Heads {  // [batch, rows, heads, dim] by element strides; the last one is 1
   const void* src;
   void* dst;
-  long long sb, sn, sh, db, dn, dh;
+  long long sb, sn, db, dn;
+  int sh, dh;
   int heads;
+};
+
+// Rows of one tensor that go to one place: rotated to a tensor (the rows of h3sa_rotate, the queries of
+// h3sa_append_rows), or to a pool, keys rotated and values as they are.
+struct Part {
+  Heads h;
+  void* pool;          // [heads, pool_pages * 128, 128], or null
+  const float* scale;  // of e4m3 pools
+  int group;           // tokens of a block
+  // a head row's units: its pairs', then its other dimensions'
+  int pair_units, units;
+  int tasks, slots;    // tasks of a token: up to kBatch head rows each; slots: tasks that a block's threads cover
+  Divisor task_div;
+  int blocks;
 };
 
 struct RowsParams {
   Angles at;
-  Heads x;             // rotated to a tensor: the rows of h3sa_rotate, the queries of h3sa_append_rows
-  long long tokens;    // batch * rows
-  int rows, dim, group;  // group: tokens of a block
-  Divisor row_div;
-  // units of work of a token's x, k and v; a head's units are its pairs' and then its other dimensions'
-  int pair_units, head_units, x_units, k_units, units;
-  Divisor unit_div, head_div, value_div;
-  // ---- the cache
-  Heads k, v;
-  void* key_pool;
-  void* value_pool;
+  long long tokens;  // batch * rows, below 2^31
+  int rows, dim;
+  Divisor row_div, pair_div, axis_div;
+  Part part[3];  // x, keys, values
   int pool_pages, width;
   const int* table;
   const int* lengths;
   const int* counts;  // or null: all rows
-  const float* k_scale;
-  const float* v_scale;
   int* err;
 };
+
+// A token's row of the pool, as an element offset: kNoRow behind a sequence's count, kNoPlace for one that the table
+// has no page for.
+constexpr long long kNoRow = -1, kNoPlace = -2;
 
 __device__ __forceinline__ double position(const Angles& a, long long token, int axis) {
   const long long i = token * a.axes + axis;
@@ -121,226 +133,319 @@ template <typename T, int kN>
 __device__ __forceinline__ Vec<T, kN> load(const T* p) {
   return *reinterpret_cast<const Vec<T, kN>*>(p);
 }
+// A vector of kN values in 32 bits, two a register pair (a single one in the first half).
 template <typename T, int kN>
-__device__ __forceinline__ void store(T* p, const Vec<T, kN>& v) {
+struct Values {
+  uint64_t v[(kN + 1) / 2];
+};
+template <typename T, int kN>
+__device__ __forceinline__ Values<T, kN> widen(const Vec<T, kN>& x) {
+  Values<T, kN> r;
+  if constexpr (std::is_same_v<T, __nv_bfloat16> && kN >= 2) {
+    const uint32_t* const w = reinterpret_cast<const uint32_t*>(&x);
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j)
+      r.v[j] = f2_pack(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; j += 2) r.v[j / 2] = f2_pack(to_float(x.v[j]), kN > 1 ? to_float(x.v[j + 1]) : 0.f);
+  }
+  return r;
+}
+template <typename T, int kN>
+__device__ __forceinline__ void store_values(T* p, const Values<T, kN>& x) {
+  Vec<T, kN> v;
+  if constexpr (std::is_same_v<T, __nv_bfloat16> && kN >= 2) {
+    uint32_t* const w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int j = 0; j < kN / 2; ++j) {
+      float lo, hi;
+      f2_unpack(x.v[j], lo, hi);
+      w[j] = pack_bf16x2(lo, hi);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; j += 2) {
+      float lo, hi;
+      f2_unpack(x.v[j / 2], lo, hi);
+      v.v[j] = from_float<T>(lo);
+      if (kN > 1) v.v[j + 1] = from_float<T>(hi);
+    }
+  }
   *reinterpret_cast<Vec<T, kN>*>(p) = v;
 }
 
+// x / scale, rounded once, from inverse = 1 / scale: two corrections of the quotient (see h3sa_fp8.cuh); one that is
+// past the numbers or not a number needs none.
+__device__ __forceinline__ float quotient_of(float x, float scale, float inverse) {
+  const float q0 = x * inverse;
+  return fabsf(q0) < INFINITY ? div_by_scale(x, scale, inverse) : q0;
+}
 // Two values divided by their head's scale as e4m3: largest numbers for what is past them and for infinities,
 // NaN for NaN.
-__device__ __forceinline__ uint32_t e4m3_pair(float x, float y, float scale) {
+__device__ __forceinline__ uint32_t e4m3_pair(float x, float y) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(__fdiv_rn(y, scale)), "f"(__fdiv_rn(x, scale)));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(y), "f"(x));
   return r;
 }
-template <int kN>
-__device__ __forceinline__ void store_e4m3(uint8_t* dst, const float (&x)[kN], float scale) {
+template <typename T, int kN>
+__device__ __forceinline__ void store_e4m3(uint8_t* dst, const Values<T, kN>& v, float scale) {
+  const float inverse = 1.0f / scale;
+  float x[kN + kN % 2];
+#pragma unroll
+  for (int j = 0; j < kN; j += 2) f2_unpack(v.v[j / 2], x[j], x[j + 1]);
+  if (scale > 1e-30f && scale < 1e30f) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) x[j] = quotient_of(x[j], scale, inverse);
+  } else {  // whose inverse or residues would leave the normal numbers
+#pragma unroll
+    for (int j = 0; j < kN; ++j) x[j] = __fdiv_rn(x[j], scale);
+  }
   if constexpr (kN >= 4) {
     uint32_t w[kN / 4];
 #pragma unroll
-    for (int j = 0; j < kN; j += 4)
-      w[j / 4] = e4m3_pair(x[j], x[j + 1], scale) | (e4m3_pair(x[j + 2], x[j + 3], scale) << 16);
+    for (int j = 0; j < kN; j += 4) w[j / 4] = e4m3_pair(x[j], x[j + 1]) | (e4m3_pair(x[j + 2], x[j + 3]) << 16);
     if constexpr (kN == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
     else *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
   } else {
-    *dst = static_cast<uint8_t>(e4m3_pair(x[0], 0.f, scale));
+    *dst = static_cast<uint8_t>(e4m3_pair(x[0], 0.f));
   }
 }
 
-// A thread's unit of one token: kN pairs (two vectors), or kN other dimensions (one vector); of values,
-// 2 kN dimensions (two vectors).
-template <typename T, int kN, bool kInterleaved>
-struct Unit {
-  Vec<T, kN> a, b;
-  int c0, c1;  // their columns; c1 < 0: there is no second one
-  int pair;    // first pair, or -1
+// Cosines and sines of a unit's kN pairs, in the order of its values: two pairs a register pair, or (interleaved) each
+// pair's twice.
+template <int kN, bool kInterleaved>
+struct Turn {
+  static constexpr int kWords = kInterleaved ? kN : (kN + 1) / 2;
+  uint64_t c[kWords], s[kWords];
 };
-
-template <typename T, int kN, bool kInterleaved>
-__device__ __forceinline__ void locate(Unit<T, kN, kInterleaved>& u, int at, int pair_units, int pairs) {
-  if (at < pair_units) {
-    u.pair = at * kN;
-    u.c0 = kInterleaved ? 2 * u.pair : u.pair;
-    u.c1 = kInterleaved ? u.c0 + kN : u.c0 + pairs;
-  } else {
-    u.pair = -1;
-    u.c0 = 2 * pairs + (at - pair_units) * kN;
-    u.c1 = -1;
-  }
-}
-
-// The unit's values in 32 bits, turned: y0 at c0, y1 at c1. cs: cosines of the token, then its sines.
-template <typename T, int kN, bool kInterleaved>
-__device__ __forceinline__ void turn(const Unit<T, kN, kInterleaved>& u, const float* cs, int pairs, float (&y0)[kN],
-                                     float (&y1)[kN]) {
-#pragma unroll
-  for (int j = 0; j < kN; ++j) {
-    y0[j] = to_float(u.a.v[j]);
-    y1[j] = to_float(u.b.v[j]);
-  }
-  if (u.pair < 0) return;
+template <int kN, bool kInterleaved>
+__device__ __forceinline__ void load_turn(Turn<kN, kInterleaved>& t, const float* cosines, const float* sines) {
   float c[kN], s[kN];
   if constexpr (kN >= 4) {
 #pragma unroll
     for (int j = 0; j < kN; j += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(cs + u.pair + j);
-      const float4 y = *reinterpret_cast<const float4*>(cs + pairs + u.pair + j);
+      const float4 x = *reinterpret_cast<const float4*>(cosines + j);
+      const float4 y = *reinterpret_cast<const float4*>(sines + j);
       c[j] = x.x, c[j + 1] = x.y, c[j + 2] = x.z, c[j + 3] = x.w;
       s[j] = y.x, s[j + 1] = y.y, s[j + 2] = y.z, s[j + 3] = y.w;
     }
   } else {
+    c[0] = cosines[0];
+    s[0] = sines[0];
+  }
+  if constexpr (kInterleaved && kN > 1) {
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
-      c[j] = cs[u.pair + j];
-      s[j] = cs[pairs + u.pair + j];
-    }
-  }
-  if constexpr (kInterleaved && kN > 1) {  // pair j is (2j, 2j + 1) of the two vectors one after the other
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float(&y)[kN] = h ? y1 : y0;
-#pragma unroll
-      for (int j = 0; j < kN; j += 2) {
-        const int k = (h * kN + j) / 2;
-        const float p = y[j], q = y[j + 1];
-        y[j] = p * c[k] - q * s[k];
-        y[j + 1] = p * s[k] + q * c[k];
-      }
+      t.c[j] = f2_pack(c[j], c[j]);
+      t.s[j] = f2_pack(-s[j], s[j]);
     }
   } else {
 #pragma unroll
+    for (int j = 0; j < kN; j += 2) {
+      t.c[j / 2] = f2_pack(c[j], kN > 1 ? c[j + 1] : 0.f);
+      t.s[j / 2] = f2_pack(s[j], kN > 1 ? s[j + 1] : 0.f);
+    }
+  }
+}
+// (x, y) -> (x c - y s, x s + y c). y0 are the values at the pairs' first columns, y1 at the second ones; interleaved
+// the pairs themselves, one after the other.
+template <typename T, int kN, bool kInterleaved>
+__device__ __forceinline__ void turn(Values<T, kN>& y0, Values<T, kN>& y1, const Turn<kN, kInterleaved>& t) {
+  if constexpr (kInterleaved && kN > 1) {
+#pragma unroll
     for (int j = 0; j < kN; ++j) {
-      const float p = y0[j], q = y1[j];
-      y0[j] = p * c[j] - q * s[j];
-      y1[j] = p * s[j] + q * c[j];
+      uint64_t& y = j < kN / 2 ? y0.v[j] : y1.v[j - kN / 2];
+      float a, b;
+      f2_unpack(y, a, b);
+      y = f2_fma(f2_pack(b, a), t.s[j], f2_mul(y, t.c[j]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < (kN + 1) / 2; ++j) {
+      const uint64_t x = y0.v[j], y = y1.v[j], minus = f2_pack(-1.f, -1.f);
+      y0.v[j] = f2_fma(f2_mul(y, t.s[j]), minus, f2_mul(x, t.c[j]));
+      y1.v[j] = f2_fma(x, t.s[j], f2_mul(y, t.c[j]));
     }
   }
 }
 
-// kPaged: keys and values go to the pools too, keys rotated, as bf16 or (kFp8) divided by their head's
-// scale as e4m3. kN: values of a vector.
-template <typename T, int kN, bool kInterleaved, bool kPaged, bool kFp8>
-__global__ void __launch_bounds__(kThreads) rotate_rows_kernel(const RowsParams p) {
-  extern __shared__ float4 smem[];
-  float* const cs_all = reinterpret_cast<float*>(smem);  // [group][2][pairs]
-  __shared__ long long dst_rows[kPaged ? kThreads : 1];  // of a token: its row of the pool, -1 for none
-  const int pairs = p.at.pairs;
-  const long long first = static_cast<long long>(blockIdx.x) * p.group;
-  const int n_tokens = static_cast<int>(min(static_cast<long long>(p.group), p.tokens - first));
-  // a token of a sequence: (b, i); tokens stay below 2^31
-  const auto split = [&](long long token, int& b, int& i) {
-    b = static_cast<int>(quotient(static_cast<uint32_t>(token), p.row_div));
-    i = static_cast<int>(token) - b * p.rows;
+// A block's tokens in one part. A task is up to kBatch head rows of a token, `tasks` apart; a thread has one unit of each,
+// kN pairs or 2 kN other dimensions (two vectors, or one at an odd end), so it reads its cosines and sines once, and
+// has all rows on their way before it needs the first; those of its first task before the block works out its angles
+// and places.
+constexpr int kBatch = 4;
+enum Kind : int { kRotated = 0, kQueries = 1, kKeys = 2, kValues = 3 };
+template <typename T, int kN, bool kInterleaved, bool kFp8, int kKind>
+__device__ __forceinline__ void rows_block(const RowsParams& p, const Part& q, uint32_t block, float4* smem) {
+  constexpr bool kPaged = kKind != kRotated, kPool = kKind >= kKeys, kTurns = kKind != kValues;
+  const int pairs = kTurns ? p.at.pairs : 0;
+  const uint32_t first = block * static_cast<uint32_t>(q.group);
+  const int n_tokens = static_cast<int>(min(static_cast<uint32_t>(q.group), static_cast<uint32_t>(p.tokens) - first));
+  float* const cs_all = reinterpret_cast<float*>(smem);                                  // [group][2][pairs]
+  long long* const places = reinterpret_cast<long long*>(cs_all + q.group * 2 * pairs);  // [group]
+  const int slot = q.units <= kThreads ? static_cast<int>(threadIdx.x) / q.units : 0;
+  const int all = slot < q.slots ? n_tokens * q.tasks : 0, unit0 = static_cast<int>(threadIdx.x) - slot * q.units;
+  bool turns, two;  // of a unit, and its columns
+  int pair, c0, c1;
+  const auto take_unit = [&](int unit) {
+    turns = kTurns && unit < q.pair_units;
+    pair = unit * kN;
+    c0 = turns ? (kInterleaved ? 2 * pair : pair) : 2 * pairs + (unit - q.pair_units) * 2 * kN;
+    c1 = turns && !kInterleaved ? c0 + pairs : c0 + kN;
+    two = kPaged || c1 < p.dim;
   };
+  Vec<T, kN> va[kBatch], vb[kBatch];
+  // Loads of a task's rows, if they are not behind their sequence's count.
+  const auto fetch = [&](int task) {
+    const int t = static_cast<int>(quotient(static_cast<uint32_t>(task), q.task_div)), h0 = task - t * q.tasks;
+    const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
+    if (kPaged && p.counts && i >= __ldg(p.counts + b)) return;
+    const T* const src = static_cast<const T*>(q.h.src) + b * q.h.sb + i * q.h.sn;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int h = h0 + j * q.tasks;
+      if (h < q.h.heads) {
+        const T* const row = src + static_cast<long long>(h) * q.h.sh;
+        va[j] = load<T, kN>(row + c0);
+        if (two) vb[j] = load<T, kN>(row + c1);
+      }
+    }
+  };
+  take_unit(unit0);
+  if (slot < all) fetch(slot);
+  if constexpr (kPaged) {  // by the last warps, the first ones have angles
+    for (int t = kThreads - 1 - static_cast<int>(threadIdx.x); t < n_tokens; t += kThreads) {
+      const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
+      long long place = kNoRow;
+      if (!p.counts || i < __ldg(p.counts + b)) {
+        place = kNoPlace;
+        if constexpr (kPool) {
+          const int length = __ldg(p.lengths + b);
+          const long long row = length + i;
+          if (length < 0 || row >= static_cast<long long>(p.width) * kPage) {
+            if (p.err) atomicOr(p.err, kErrBadIndex);
+          } else {
+            const int page = __ldg(p.table + b * p.width + row / kPage);
+            if (page >= 0 && page < p.pool_pages) place = (static_cast<long long>(page) * kPage + row % kPage) * kDim;
+            else if (p.err) atomicOr(p.err, kErrBadPage);
+          }
+        }
+      }
+      places[t] = place;
+    }
+  }
   for (int k = threadIdx.x; k < n_tokens * pairs; k += kThreads) {
-    const int t = k / pairs, pair = k - t * pairs;
+    const int t = quotient(k, p.pair_div), at = k - t * pairs;
     double where;
     if (kPaged && p.at.kind == kPosNone) {
-      int b, i;
-      split(first + t, b, i);
-      where = static_cast<double>(__ldg(p.lengths + b)) + i;
+      const uint32_t b = quotient(first + t, p.row_div);
+      where = static_cast<double>(__ldg(p.lengths + b)) + (first + t - b * p.rows);
     } else {
-      where = position(p.at, first + t, pair / p.at.per_axis);
+      where = position(p.at, first + t, quotient(at, p.axis_div));
     }
-    const float2 v = cos_sin(where, __ldg(p.at.frequencies + pair), p.at.factor);
-    cs_all[t * 2 * pairs + pair] = v.x;
-    cs_all[t * 2 * pairs + pairs + pair] = v.y;
-  }
-  if constexpr (kPaged) {
-    for (int t = threadIdx.x; t < n_tokens; t += kThreads) {
-      int b, i;
-      split(first + t, b, i);
-      long long row = -1;
-      if (!p.counts || i < __ldg(p.counts + b)) {
-        const int len = __ldg(p.lengths + b);
-        const long long at = static_cast<long long>(len) + i;
-        if (len < 0 || at >= static_cast<long long>(p.width) * kPage) {
-          if (p.err) atomicOr(p.err, kErrBadIndex);
-        } else {
-          const int page = __ldg(p.table + static_cast<size_t>(b) * p.width + at / kPage);
-          if (page >= 0 && page < p.pool_pages) row = static_cast<long long>(page) * kPage + at % kPage;
-          else if (p.err) atomicOr(p.err, kErrBadPage);
-        }
-        if (row < 0) row = -2;  // a row that has no place, but is one
-      }
-      dst_rows[t] = row;
-    }
+    const float2 v = cos_sin(where, __ldg(p.at.frequencies + at), p.at.factor);
+    cs_all[t * 2 * pairs + at] = v.x;
+    cs_all[t * 2 * pairs + pairs + at] = v.y;
   }
   __syncthreads();
-  const uint32_t all = static_cast<uint32_t>(n_tokens) * static_cast<uint32_t>(p.units);
-  for (uint32_t n = threadIdx.x; n < all; n += kThreads) {
-    const int t = static_cast<int>(quotient(n, p.unit_div));
-    int at = static_cast<int>(n) - t * p.units;
-    int b, i;
-    split(first + t, b, i);
-    const float* const cs = cs_all + t * 2 * pairs;
-    Unit<T, kN, kInterleaved> u;
-    float y0[kN], y1[kN];
-    const bool is_x = !kPaged || at < p.x_units;
-    const bool is_k = kPaged && !is_x && at < p.x_units + p.k_units;
-    const Heads& h = is_x ? p.x : is_k ? p.k : p.v;
-    int head;
-    if (!kPaged || is_x || is_k) {
-      if (is_k) at -= p.x_units;
-      head = static_cast<int>(quotient(at, p.head_div));
-      locate(u, at - head * p.head_units, p.pair_units, pairs);
-    } else {
-      at -= p.x_units + p.k_units;
-      head = static_cast<int>(quotient(at, p.value_div));
-      u.pair = -1;
-      u.c0 = (at - head * static_cast<int>(p.value_div.d)) * 2 * kN;
-      u.c1 = u.c0 + kN;
-    }
-    const long long row = kPaged ? dst_rows[t] : 0;
-    const bool live = row != -1;  // rows of x behind a sequence's count come out zero
-    if (kPaged && !is_x && row < 0) continue;
-    const T* const src = static_cast<const T*>(h.src) + b * h.sb + i * h.sn + head * h.sh;
-    if (live) {
-      u.a = load<T, kN>(src + u.c0);
-      if (u.c1 >= 0) u.b = load<T, kN>(src + u.c1);
-    } else {
-      memset(&u.a, 0, sizeof(u.a));
-    }
-    if (u.c1 < 0 || !live) memset(&u.b, 0, sizeof(u.b));
-    turn(u, cs, pairs, y0, y1);
-    if (!live) {  // whatever the position was
+  const int unit_step = q.units <= kThreads ? q.units : kThreads;
+  for (int unit = unit0; unit < q.units; unit += unit_step) {
+    for (int task = slot; task < all; task += q.slots) {
+      if (unit != unit0 || task != slot) {
+        take_unit(unit);
+        fetch(task);
+      }
+      const int t = static_cast<int>(quotient(static_cast<uint32_t>(task), q.task_div)), h0 = task - t * q.tasks;
+      const long long place = kPaged ? places[t] : kNoPlace;
+      if (kPool && place < 0) continue;
+      T* out = nullptr;
+      if constexpr (!kPool) {
+        const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
+        out = static_cast<T*>(q.h.dst) + b * q.h.db + i * q.h.dn;
+      }
+      if (kPaged && place == kNoRow) {
+        for (int h = h0; h < q.h.heads; h += q.tasks) {
+          store_values(out + static_cast<long long>(h) * q.h.dh + c0, Values<T, kN>{});
+          store_values(out + static_cast<long long>(h) * q.h.dh + c1, Values<T, kN>{});
+        }
+        continue;
+      }
+      Turn<kN, kInterleaved> cs;
+      if (turns) load_turn(cs, cs_all + t * 2 * pairs + pair, cs_all + t * 2 * pairs + pairs + pair);
 #pragma unroll
-      for (int j = 0; j < kN; ++j) y0[j] = y1[j] = 0.f;
-    }
-    if (kFp8 && !is_x) {
-      const float scale = __ldg((is_k ? p.k_scale : p.v_scale) + head);
-      uint8_t* const dst = static_cast<uint8_t*>(is_k ? p.key_pool : p.value_pool) +
-                           (static_cast<long long>(head) * p.pool_pages * kPage + row) * kDim;
-      store_e4m3<kN>(dst + u.c0, y0, scale);
-      if (u.c1 >= 0) store_e4m3<kN>(dst + u.c1, y1, scale);
-      continue;
-    }
-    T* const dst = is_x ? static_cast<T*>(h.dst) + b * h.db + i * h.dn + head * h.dh
-                        : static_cast<T*>(is_k ? p.key_pool : p.value_pool) +
-                              (static_cast<long long>(head) * p.pool_pages * kPage + row) * kDim;
-    Vec<T, kN> r;
-#pragma unroll
-    for (int j = 0; j < kN; ++j) r.v[j] = from_float<T>(y0[j]);
-    store(dst + u.c0, r);
-    if (u.c1 >= 0) {
-#pragma unroll
-      for (int j = 0; j < kN; ++j) r.v[j] = from_float<T>(y1[j]);
-      store(dst + u.c1, r);
+      for (int j = 0; j < kBatch; ++j) {
+        const int h = h0 + j * q.tasks;
+        if (h < q.h.heads) {
+          Values<T, kN> y0 = widen(va[j]), y1 = widen(vb[j]);
+          if (turns) turn(y0, y1, cs);
+          if constexpr (!kPool) {
+            T* const dst = out + static_cast<long long>(h) * q.h.dh;
+            store_values(dst + c0, y0);
+            if (two) store_values(dst + c1, y1);
+          } else {
+            const long long to = static_cast<long long>(h) * p.pool_pages * (kPage * kDim) + place;
+            if constexpr (kFp8) {
+              const float scale = __ldg(q.scale + h);
+              store_e4m3(static_cast<uint8_t*>(q.pool) + to + c0, y0, scale);
+              store_e4m3(static_cast<uint8_t*>(q.pool) + to + c1, y1, scale);
+            } else {
+              store_values(static_cast<T*>(q.pool) + to + c0, y0);
+              store_values(static_cast<T*>(q.pool) + to + c1, y1);
+            }
+          }
+        }
+      }
     }
   }
 }
 
-template <typename T, int kN, bool kInterleaved, bool kPaged, bool kFp8>
-int launch(const RowsParams& p, cudaStream_t stream) {
-  const long long blocks = (p.tokens + p.group - 1) / p.group;
-  rotate_rows_kernel<T, kN, kInterleaved, kPaged, kFp8>
-      <<<static_cast<unsigned>(blocks), kThreads, static_cast<size_t>(p.group) * 8 * p.at.pairs, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? H3SA_OK : set_cuda_error("rotate_rows_kernel launch", e);
+template <typename T, int kN, bool kInterleaved>
+__global__ void __launch_bounds__(kThreads, kN == 8 ? 3 : 4) rotate_kernel(const __grid_constant__ RowsParams p) {
+  extern __shared__ float4 smem[];
+  rows_block<T, kN, kInterleaved, false, kRotated>(p, p.part[0], blockIdx.x, smem);
 }
-template <typename T, int kN, bool kPaged, bool kFp8>
-int launch(const RowsParams& p, bool interleaved, cudaStream_t stream) {
-  return interleaved ? launch<T, kN, true, kPaged, kFp8>(p, stream) : launch<T, kN, false, kPaged, kFp8>(p, stream);
+
+// Queries, keys and values have blocks of their own, in this order.
+template <int kN, bool kInterleaved, bool kFp8>
+__global__ void __launch_bounds__(kThreads, 3) append_rows_kernel(const __grid_constant__ RowsParams p) {
+  using T = __nv_bfloat16;
+  extern __shared__ float4 smem[];
+  uint32_t block = blockIdx.x;
+  if (block < p.part[0].blocks) {
+    rows_block<T, kN, kInterleaved, kFp8, kQueries>(p, p.part[0], block, smem);
+  } else if ((block -= p.part[0].blocks) < p.part[1].blocks) {
+    rows_block<T, kN, kInterleaved, kFp8, kKeys>(p, p.part[1], block, smem);
+  } else {
+    rows_block<T, kN, kInterleaved, kFp8, kValues>(p, p.part[2], block - p.part[1].blocks, smem);
+  }
+}
+
+size_t token_bytes(const Angles& a) { return 8 * static_cast<size_t>(a.pairs) + sizeof(long long); }
+
+template <typename T>
+int launch_rotate(const RowsParams& p, int n, bool interleaved, cudaStream_t stream) {
+  const auto kernel = n == 8   ? (interleaved ? rotate_kernel<T, sizeof(T) == 2 ? 8 : 4, true> : rotate_kernel<T, sizeof(T) == 2 ? 8 : 4, false>)
+                      : n == 4 ? (interleaved ? rotate_kernel<T, 4, true> : rotate_kernel<T, 4, false>)
+                               : (interleaved ? rotate_kernel<T, 1, true> : rotate_kernel<T, 1, false>);
+  kernel<<<p.part[0].blocks, kThreads, token_bytes(p.at) * p.part[0].group, stream>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? H3SA_OK : set_cuda_error("rotate_kernel launch", e);
+}
+template <bool kFp8>
+int launch_append(const RowsParams& p, int n, bool interleaved, cudaStream_t stream) {
+  const auto kernel = n == 8   ? (interleaved ? append_rows_kernel<8, true, kFp8> : append_rows_kernel<8, false, kFp8>)
+                      : n == 4 ? (interleaved ? append_rows_kernel<4, true, kFp8> : append_rows_kernel<4, false, kFp8>)
+                               : (interleaved ? append_rows_kernel<1, true, kFp8> : append_rows_kernel<1, false, kFp8>);
+  size_t group = 0;
+  unsigned blocks = 0;
+  for (const Part& q : p.part) {
+    if (q.blocks > 0 && static_cast<size_t>(q.group) > group) group = q.group;
+    blocks += static_cast<unsigned>(q.blocks);
+  }
+  kernel<<<blocks, kThreads, token_bytes(p.at) * group, stream>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? H3SA_OK : set_cuda_error("append_rows_kernel launch", e);
 }
 
 // The values of a vector: 16 bytes where columns, strides and addresses allow it, 8, or single values.
@@ -353,30 +458,41 @@ bool fits(const Heads& h, int size, int n) {
 }
 int vector_of(const RowsParams& p, int size) {
   for (int n = 16 / size; n >= 4; n /= 2)
-    if (p.at.pairs % n == 0 && p.dim % n == 0 && fits(p.x, size, n) && fits(p.k, size, n) && fits(p.v, size, n)) return n;
+    if (p.at.pairs % n == 0 && p.dim % n == 0 && fits(p.part[0].h, size, n) && fits(p.part[1].h, size, n) &&
+        fits(p.part[2].h, size, n))
+      return n;
   return 1;
 }
 
-// Blocks of a few tokens: enough units that a thread has four, as far as that leaves every SM some blocks.
+constexpr int kSms = 148;
+
+// A task is a head row while threads are few, kBatch of them from there on; a block has as many tokens as give
+// its threads a task each, as far as that leaves every SM some blocks.
 void lay_out(RowsParams& p, int n, int batch) {
   p.tokens = static_cast<long long>(batch) * p.rows;
-  p.pair_units = p.at.pairs / n;
-  p.head_units = p.pair_units + (p.dim - 2 * p.at.pairs) / n;
-  p.x_units = p.x.heads * p.head_units;
-  p.k_units = p.k.heads * p.head_units;
-  const int value_units = kDim / (2 * n);
-  p.units = p.x_units + p.k_units + p.v.heads * value_units;
   p.row_div = divisor(static_cast<uint32_t>(p.rows));
-  p.unit_div = divisor(static_cast<uint32_t>(p.units));
-  p.head_div = divisor(static_cast<uint32_t>(p.head_units));
-  p.value_div = divisor(static_cast<uint32_t>(value_units));
-  constexpr int kSms = 148;
-  int group = 4 * kThreads / p.units;
-  if (p.at.pairs > 0 && group > 32768 / (8 * p.at.pairs)) group = 32768 / (8 * p.at.pairs);
-  if (group > kThreads) group = kThreads;
-  const long long most = p.tokens / (4 * kSms);
-  if (group > most) group = static_cast<int>(most);
-  p.group = group < 1 ? 1 : group;
+  p.pair_div = divisor(static_cast<uint32_t>(p.at.pairs > 0 ? p.at.pairs : 1));
+  p.axis_div = divisor(static_cast<uint32_t>(p.at.per_axis > 0 ? p.at.per_axis : 1));
+  long long threads = 0;
+  for (Part& q : p.part) {
+    const int pairs = &q == p.part + 2 ? 0 : p.at.pairs;
+    q.pair_units = pairs / n;
+    q.units = q.pair_units + (p.dim - 2 * pairs + 2 * n - 1) / (2 * n);
+    threads += p.tokens * q.h.heads * q.units;
+  }
+  const int rows = threads >= static_cast<long long>(kSms) * kThreads * 3 * kBatch ? kBatch : 1;
+  for (Part& q : p.part) {
+    if (q.h.heads == 0) continue;
+    q.tasks = (q.h.heads + rows - 1) / rows;
+    q.slots = q.units <= kThreads ? kThreads / q.units : 1;
+    q.task_div = divisor(static_cast<uint32_t>(q.tasks));
+    long long group = q.slots / q.tasks;
+    const long long most = p.tokens / (4 * kSms), room = static_cast<long long>(32768 / token_bytes(p.at));
+    if (group > most) group = most;
+    if (group > room) group = room;
+    q.group = group < 1 ? 1 : static_cast<int>(group);
+    q.blocks = static_cast<int>((p.tokens + q.group - 1) / q.group);
+  }
 }
 
 int check_rotary(const char* what, const h3sa_rotary* r, int dim, bool rows_known, Angles& a) {
@@ -401,6 +517,9 @@ int check_rotary(const char* what, const h3sa_rotary* r, int dim, bool rows_know
   return H3SA_OK;
 }
 
+// Strides of heads are kept in 32 bits.
+bool head_stride_ok(const h3sa_heads* h) { return !h || (h->stride_head >= INT32_MIN && h->stride_head <= INT32_MAX); }
+
 Heads heads_of(const h3sa_heads* from, const h3sa_heads* to) {
   Heads h;
   memset(&h, 0, sizeof(h));
@@ -408,13 +527,13 @@ Heads heads_of(const h3sa_heads* from, const h3sa_heads* to) {
   h.src = from->base;
   h.sb = from->stride_sequence;
   h.sn = from->stride_row;
-  h.sh = from->stride_head;
+  h.sh = static_cast<int>(from->stride_head);
   h.heads = from->heads;
   if (to) {
     h.dst = to->base;
     h.db = to->stride_sequence;
     h.dn = to->stride_row;
-    h.dh = to->stride_head;
+    h.dh = static_cast<int>(to->stride_head);
   }
   return h;
 }
@@ -438,26 +557,22 @@ int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32
   if (const int rc = check_rotary("rotate", rotary, dim, false, p.at)) return rc;
   if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || static_cast<int64_t>(x->heads) * dim > INT32_MAX / 4096)
     return set_error(H3SA_ERR_UNSUPPORTED, "rotate: batch %d x rows %d x heads %d is too large", batch, rows, x->heads);
+  if (!head_stride_ok(x) || !head_stride_ok(out))
+    return set_error(H3SA_ERR_UNSUPPORTED, "rotate: strides of heads must fit 32 bits");
   const int size = dtype == H3SA_FP32 ? 4 : 2;
   if (!x->base || !out->base) return set_error(H3SA_ERR_INVALID, "rotate: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(x->base) | reinterpret_cast<uintptr_t>(out->base)) % size)
     return set_error(H3SA_ERR_INVALID, "rotate: tensors must be aligned to their type");
-  p.x = heads_of(x, out);
+  p.part[0].h = heads_of(x, out);
   p.rows = rows;
   p.dim = dim;
   const int n = vector_of(p, size);
   lay_out(p, n, batch);
   const bool inter = rotary && rotary->interleaved;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == H3SA_FP32)
-    return n == 4 ? launch<float, 4, false, false>(p, inter, s) : launch<float, 1, false, false>(p, inter, s);
-  if (dtype == H3SA_FP16)
-    return n == 8   ? launch<__half, 8, false, false>(p, inter, s)
-           : n == 4 ? launch<__half, 4, false, false>(p, inter, s)
-                    : launch<__half, 1, false, false>(p, inter, s);
-  return n == 8   ? launch<__nv_bfloat16, 8, false, false>(p, inter, s)
-         : n == 4 ? launch<__nv_bfloat16, 4, false, false>(p, inter, s)
-                  : launch<__nv_bfloat16, 1, false, false>(p, inter, s);
+  const cudaStream_t at = static_cast<cudaStream_t>(stream);
+  return dtype == H3SA_FP32   ? launch_rotate<float>(p, n, inter, at)
+         : dtype == H3SA_FP16 ? launch_rotate<__half>(p, n, inter, at)
+                              : launch_rotate<__nv_bfloat16>(p, n, inter, at);
 }
 
 int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_heads* query, const h3sa_heads* query_out,
@@ -482,40 +597,37 @@ int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_
   if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || heads > INT32_MAX / (4096 * kDim))
     return set_error(H3SA_ERR_UNSUPPORTED, "append rows: batch %d x rows %d x heads %lld is too large", batch, rows,
                      static_cast<long long>(heads));
+  if (!head_stride_ok(key) || !head_stride_ok(value) || !head_stride_ok(query) || !head_stride_ok(query_out))
+    return set_error(H3SA_ERR_UNSUPPORTED, "append rows: strides of heads must fit 32 bits");
   if (!key->base || !value->base || !key_pool || !value_pool || !table || !lengths ||
       (with_query && (!query->base || !query_out->base)) || (e4m3 && (!k_scale || !v_scale)))
     return set_error(H3SA_ERR_INVALID, "append rows: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(key_pool) | reinterpret_cast<uintptr_t>(value_pool)) & 15u)
     return set_error(H3SA_ERR_INVALID, "append rows: pools must be 16-byte aligned");
-  p.x = heads_of(with_query ? query : nullptr, query_out);
-  p.k = heads_of(key, nullptr);
-  p.v = heads_of(value, nullptr);
-  const uintptr_t odd = reinterpret_cast<uintptr_t>(p.x.src) | reinterpret_cast<uintptr_t>(p.x.dst) |
-                        reinterpret_cast<uintptr_t>(p.k.src) | reinterpret_cast<uintptr_t>(p.v.src);
+  Part &x = p.part[0], &k = p.part[1], &v = p.part[2];
+  x.h = heads_of(with_query ? query : nullptr, query_out);
+  k.h = heads_of(key, nullptr);
+  v.h = heads_of(value, nullptr);
+  const uintptr_t odd = reinterpret_cast<uintptr_t>(x.h.src) | reinterpret_cast<uintptr_t>(x.h.dst) |
+                        reinterpret_cast<uintptr_t>(k.h.src) | reinterpret_cast<uintptr_t>(v.h.src);
   if (odd & 1u) return set_error(H3SA_ERR_INVALID, "append rows: tensors must be aligned to their type");
   p.rows = rows;
   p.dim = kDim;
-  p.key_pool = key_pool;
-  p.value_pool = value_pool;
+  k.pool = key_pool;
+  k.scale = k_scale;
+  v.pool = value_pool;
+  v.scale = v_scale;
   p.pool_pages = pool_pages;
   p.width = width;
   p.table = table;
   p.lengths = lengths;
   p.counts = counts;
-  p.k_scale = k_scale;
-  p.v_scale = v_scale;
   p.err = device_error;
   const int n = vector_of(p, 2);
   lay_out(p, n, batch);
   const bool inter = rotary && rotary->interleaved;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (e4m3)
-    return n == 8   ? launch<__nv_bfloat16, 8, true, true>(p, inter, s)
-           : n == 4 ? launch<__nv_bfloat16, 4, true, true>(p, inter, s)
-                    : launch<__nv_bfloat16, 1, true, true>(p, inter, s);
-  return n == 8   ? launch<__nv_bfloat16, 8, true, false>(p, inter, s)
-         : n == 4 ? launch<__nv_bfloat16, 4, true, false>(p, inter, s)
-                  : launch<__nv_bfloat16, 1, true, false>(p, inter, s);
+  const cudaStream_t at = static_cast<cudaStream_t>(stream);
+  return e4m3 ? launch_append<true>(p, n, inter, at) : launch_append<false>(p, n, inter, at);
 }
 
 }  // extern "C"
