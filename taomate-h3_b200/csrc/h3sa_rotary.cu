@@ -10,10 +10,12 @@
 // then exact to 2^-25 of a turn for any position of 32 bits; cosine and sine of it are in 32 bits, as are
 // the products, and each result is rounded once.
 //
-// Both kernels are bound by memory: a value is read and written once, 6 flops stand against 8 bytes. All
-// heads of a token share its angles, so a block takes a few tokens, writes their cosines and
-// sines to shared memory once (some 60 instructions each) and then streams the heads past them, two
-// vectors of 16 bytes a thread and step.
+// Bound by memory: a value is read and written once. What has to be kept small is the instructions in
+// between, for which an SM has some 350 a warp and 2 KB: a thread keeps to one unit of a head row, 8 pairs in two
+// vectors of 16 bytes, with their frequencies in registers, works out its 8 angles once a token and turns up to eight heads by
+// them, all of which are on their way by then. There is nothing to share and nothing to wait for in a block.
+// (A table of the block's cosines and sines in shared memory took 57 us for 24605 tokens of 24 heads and 110 for 300001 of
+// one head.)
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -30,8 +32,9 @@ namespace {
 
 constexpr int kPage = 128;
 constexpr int kDim = 128;  // head dimension of a cache
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxDim = 1024;
+constexpr int kSms = 148;
 
 // x / d for x below 2^31 by one multiplication: m = ceil(2^(32 + s) / d) with 2^s >= d (Granlund and
 // Montgomery's division by invariant integers; m needs 33 bits, of which the first is a plain add).
@@ -74,11 +77,11 @@ struct Part {
   Heads h;
   void* pool;          // [heads, pool_pages * 128, 128], or null
   const float* scale;  // of e4m3 pools
-  int group;           // tokens of a block
   // a head row's units: its pairs', then its other dimensions'
   int pair_units, units;
   int tasks, slots;    // tasks of a token: up to kBatch head rows each; slots: tasks that a block's threads cover
   Divisor task_div;
+  long long all;       // tasks
   int blocks;
 };
 
@@ -86,7 +89,7 @@ struct RowsParams {
   Angles at;
   long long tokens;  // batch * rows, below 2^31
   int rows, dim;
-  Divisor row_div, pair_div, axis_div;
+  Divisor row_div;
   Part part[3];  // x, keys, values
   int pool_pages, width;
   const int* table;
@@ -95,25 +98,55 @@ struct RowsParams {
   int* err;
 };
 
-// A token's row of the pool, as an element offset: kNoRow behind a sequence's count, kNoPlace for one that the table
-// has no page for.
-constexpr long long kNoRow = -1, kNoPlace = -2;
-
-__device__ __forceinline__ double position(const Angles& a, long long token, int axis) {
-  const long long i = token * a.axes + axis;
-  if (a.kind == kPosI32) return static_cast<double>(__ldg(static_cast<const int*>(a.positions) + i));
-  if (a.kind == kPosI64) return static_cast<double>(__ldg(static_cast<const long long*>(a.positions) + i));
-  return __ldg(static_cast<const double*>(a.positions) + i);
+// f / 2 pi as a fraction of a turn in units of 2^-64. Whole turns a position do not matter, and p times this, cut to
+// 64 bits, is the fraction of p f / 2 pi, off by p 2^-65 (the quotient is taken in two terms). Numbers are brought
+// into an integer by adding 1.5 * 2^k, which leaves them in the sum's last bits: conversions of 64 bits are slow.
+__device__ __forceinline__ uint64_t turn_of(double f) {
+  const double hi = f * 0.15915494309189535;  // 1 / (2 pi), less 9.8e-18
+  const double lo = fma(f, 0.15915494309189535, -hi) + f * -9.839338337591243e-18;
+  const double r = hi - ((hi + 6755399441055744.0) - 6755399441055744.0);  // 1.5 * 2^52
+  const double top = r + 1572864.0;                                        // 1.5 * 2^20: last bit 2^-32
+  const double rest = r - (top - 1572864.0) + lo;
+  return (static_cast<uint64_t>(static_cast<uint32_t>(__double2loint(top))) << 32) +
+         static_cast<uint64_t>(static_cast<long long>(__double2loint(rest + 0.0003662109375)));  // 1.5 * 2^-12: 2^-64
 }
-
-__device__ __forceinline__ float2 cos_sin(double p, double frequency, float factor) {
-  const double turn = frequency * 0.15915494309189535;
-  const double t = p * turn;
-  // the fraction by one rounding: whole turns are exact in 64 bits
-  const float f = static_cast<float>(fma(p, turn, -rint(t)));
-  float s, c;
-  sincospif(2.0f * f, &s, &c);
-  return make_float2(c * factor, s * factor);
+// What a pair needs of its frequency: turn_of it, or for positions between whole numbers the bits of f / 2 pi.
+__device__ __forceinline__ uint64_t frequency_word(const Angles& a, int pair) {
+  const double f = __ldg(a.frequencies + pair);
+  return a.kind == kPosF64 ? static_cast<uint64_t>(__double_as_longlong(f * 0.15915494309189535)) : turn_of(f);
+}
+// A token's position on one axis, as 64 bits.
+__device__ __forceinline__ uint64_t position_word(const Angles& a, long long token, int axis) {
+  const long long at = token * a.axes + axis;
+  if (a.kind == kPosI32) return static_cast<uint64_t>(static_cast<long long>(__ldg(static_cast<const int*>(a.positions) + at)));
+  return __ldg(static_cast<const unsigned long long*>(a.positions) + at);
+}
+// The fraction of a turn, in [-1/2, 1/2).
+__device__ __forceinline__ float fraction(bool between, uint64_t position, uint64_t frequency) {
+  uint32_t hi;
+  if (!between) {
+    hi = static_cast<uint32_t>((position * frequency) >> 32);
+  } else {  // in 64-bit arithmetic, whole turns taken off by one rounding
+    const double p = __longlong_as_double(static_cast<long long>(position));
+    const double unit = __longlong_as_double(static_cast<long long>(frequency)), t = p * unit;
+    const double whole = (t + 6755399441055744.0) - 6755399441055744.0;
+    hi = static_cast<uint32_t>(__double2loint(fma(p, unit, -whole) + 1572864.0));
+  }
+  return static_cast<float>(static_cast<int>(hi)) * 2.3283064365386963e-10f;  // 2^-32
+}
+// Cosine and sine of a fraction of a turn. For 16-bit values the approximate functions, off by up to 2^-21, which is
+// 2^-10 of their rounding.
+template <typename T>
+__device__ __forceinline__ void cos_sin(float fraction, float factor, float& c, float& s) {
+  if constexpr (sizeof(T) == 2) {
+    const float a = fraction * 6.2831853071795865f;
+    s = __sinf(a);
+    c = __cosf(a);
+  } else {
+    sincospif(2.0f * fraction, &s, &c);
+  }
+  c *= factor;
+  s *= factor;
 }
 
 template <typename T> __device__ __forceinline__ float to_float(T x);
@@ -219,21 +252,13 @@ struct Turn {
   static constexpr int kWords = kInterleaved ? kN : (kN + 1) / 2;
   uint64_t c[kWords], s[kWords];
 };
-template <int kN, bool kInterleaved>
-__device__ __forceinline__ void load_turn(Turn<kN, kInterleaved>& t, const float* cosines, const float* sines) {
-  float c[kN], s[kN];
-  if constexpr (kN >= 4) {
+template <typename T, int kN, bool kInterleaved>
+__device__ __forceinline__ void make_turn(Turn<kN, kInterleaved>& t, bool between, uint64_t position, const uint64_t (&frequency)[kN],
+                                          float factor) {
+  float c[kN + kN % 2], s[kN + kN % 2];
+  c[kN - 1 + kN % 2] = s[kN - 1 + kN % 2] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kN; j += 4) {
-      const float4 x = *reinterpret_cast<const float4*>(cosines + j);
-      const float4 y = *reinterpret_cast<const float4*>(sines + j);
-      c[j] = x.x, c[j + 1] = x.y, c[j + 2] = x.z, c[j + 3] = x.w;
-      s[j] = y.x, s[j + 1] = y.y, s[j + 2] = y.z, s[j + 3] = y.w;
-    }
-  } else {
-    c[0] = cosines[0];
-    s[0] = sines[0];
-  }
+  for (int j = 0; j < kN; ++j) cos_sin<T>(fraction(between, position, frequency[j]), factor, c[j], s[j]);
   if constexpr (kInterleaved && kN > 1) {
 #pragma unroll
     for (int j = 0; j < kN; ++j) {
@@ -243,8 +268,8 @@ __device__ __forceinline__ void load_turn(Turn<kN, kInterleaved>& t, const float
   } else {
 #pragma unroll
     for (int j = 0; j < kN; j += 2) {
-      t.c[j / 2] = f2_pack(c[j], kN > 1 ? c[j + 1] : 0.f);
-      t.s[j / 2] = f2_pack(s[j], kN > 1 ? s[j + 1] : 0.f);
+      t.c[j / 2] = f2_pack(c[j], c[j + 1]);
+      t.s[j / 2] = f2_pack(s[j], s[j + 1]);
     }
   }
 }
@@ -270,101 +295,63 @@ __device__ __forceinline__ void turn(Values<T, kN>& y0, Values<T, kN>& y1, const
   }
 }
 
-// A block's tokens in one part. A task is up to kBatch head rows of a token, `tasks` apart; a thread has one unit of each,
-// kN pairs or 2 kN other dimensions (two vectors, or one at an odd end), so it reads its cosines and sines once, and
-// has all rows on their way before it needs the first; those of its first task before the block works out its angles
-// and places.
-constexpr int kBatch = 4;
+// A block's share of one part. A task is up to kBatch head rows of a token, `tasks` apart; a thread has one unit of each,
+// kN pairs or 2 kN other dimensions (two vectors, or one at an odd end), and takes every `stride`-th task.
+constexpr int kFew = 2, kMany = 6, kAppended = 4;  // kBatch
 enum Kind : int { kRotated = 0, kQueries = 1, kKeys = 2, kValues = 3 };
-template <typename T, int kN, bool kInterleaved, bool kFp8, int kKind>
-__device__ __forceinline__ void rows_block(const RowsParams& p, const Part& q, uint32_t block, float4* smem) {
+template <typename T, int kN, bool kInterleaved, bool kFp8, int kKind, int kBatch>
+__device__ __forceinline__ void rows_block(const RowsParams& p, const Part& q, uint32_t block) {
   constexpr bool kPaged = kKind != kRotated, kPool = kKind >= kKeys, kTurns = kKind != kValues;
   const int pairs = kTurns ? p.at.pairs : 0;
-  const uint32_t first = block * static_cast<uint32_t>(q.group);
-  const int n_tokens = static_cast<int>(min(static_cast<uint32_t>(q.group), static_cast<uint32_t>(p.tokens) - first));
-  float* const cs_all = reinterpret_cast<float*>(smem);                                  // [group][2][pairs]
-  long long* const places = reinterpret_cast<long long*>(cs_all + q.group * 2 * pairs);  // [group]
   const int slot = q.units <= kThreads ? static_cast<int>(threadIdx.x) / q.units : 0;
-  const int all = slot < q.slots ? n_tokens * q.tasks : 0, unit0 = static_cast<int>(threadIdx.x) - slot * q.units;
-  bool turns, two;  // of a unit, and its columns
-  int pair, c0, c1;
-  const auto take_unit = [&](int unit) {
-    turns = kTurns && unit < q.pair_units;
-    pair = unit * kN;
-    c0 = turns ? (kInterleaved ? 2 * pair : pair) : 2 * pairs + (unit - q.pair_units) * 2 * kN;
-    c1 = turns && !kInterleaved ? c0 + pairs : c0 + kN;
-    two = kPaged || c1 < p.dim;
-  };
-  Vec<T, kN> va[kBatch], vb[kBatch];
-  // Loads of a task's rows, if they are not behind their sequence's count.
-  const auto fetch = [&](int task) {
-    const int t = static_cast<int>(quotient(static_cast<uint32_t>(task), q.task_div)), h0 = task - t * q.tasks;
-    const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
-    if (kPaged && p.counts && i >= __ldg(p.counts + b)) return;
-    const T* const src = static_cast<const T*>(q.h.src) + b * q.h.sb + i * q.h.sn;
+  if (slot >= q.slots) return;
+  const bool between = p.at.kind == kPosF64;
+  const uint32_t stride = static_cast<uint32_t>(q.blocks) * q.slots;
+  for (int unit = static_cast<int>(threadIdx.x) - slot * q.units; unit < q.units; unit += kThreads) {
+    const bool turns = kTurns && unit < q.pair_units;
+    const int pair = unit * kN;
+    const int c0 = turns ? (kInterleaved ? 2 * pair : pair) : 2 * pairs + (unit - q.pair_units) * 2 * kN;
+    const int c1 = turns && !kInterleaved ? c0 + pairs : c0 + kN;
+    const bool two = kPaged || c1 < p.dim;
+    const int axis = turns ? pair / p.at.per_axis : 0;  // of all its pairs
+    uint64_t frequency[kN];
+    if (turns) {
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
-      const int h = h0 + j * q.tasks;
-      if (h < q.h.heads) {
-        const T* const row = src + static_cast<long long>(h) * q.h.sh;
-        va[j] = load<T, kN>(row + c0);
-        if (two) vb[j] = load<T, kN>(row + c1);
-      }
+      for (int j = 0; j < kN; ++j) frequency[j] = frequency_word(p.at, pair + j);
     }
-  };
-  take_unit(unit0);
-  if (slot < all) fetch(slot);
-  if constexpr (kPaged) {  // by the last warps, the first ones have angles
-    for (int t = kThreads - 1 - static_cast<int>(threadIdx.x); t < n_tokens; t += kThreads) {
-      const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
-      long long place = kNoRow;
-      if (!p.counts || i < __ldg(p.counts + b)) {
-        place = kNoPlace;
-        if constexpr (kPool) {
-          const int length = __ldg(p.lengths + b);
-          const long long row = length + i;
-          if (length < 0 || row >= static_cast<long long>(p.width) * kPage) {
-            if (p.err) atomicOr(p.err, kErrBadIndex);
-          } else {
-            const int page = __ldg(p.table + b * p.width + row / kPage);
-            if (page >= 0 && page < p.pool_pages) place = (static_cast<long long>(page) * kPage + row % kPage) * kDim;
-            else if (p.err) atomicOr(p.err, kErrBadPage);
+    for (uint32_t task = block * q.slots + slot; task < q.all; task += stride) {
+      const uint32_t token = quotient(task, q.task_div);
+      const int h0 = static_cast<int>(task - token * q.tasks);
+      const long long b = quotient(token, p.row_div), i = token - b * p.rows;
+      const bool live = !kPaged || !p.counts || i < __ldg(p.counts + b);
+      if (kPool && !live) continue;
+      Vec<T, kN> va[kBatch], vb[kBatch];
+      if (live) {
+        const T* const src = static_cast<const T*>(q.h.src) + b * q.h.sb + i * q.h.sn;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int h = h0 + j * q.tasks;
+          if (h < q.h.heads) {
+            const T* const row = src + static_cast<long long>(h) * q.h.sh;
+            va[j] = load<T, kN>(row + c0);
+            if (two) vb[j] = load<T, kN>(row + c1);
           }
         }
       }
-      places[t] = place;
-    }
-  }
-  for (int k = threadIdx.x; k < n_tokens * pairs; k += kThreads) {
-    const int t = quotient(k, p.pair_div), at = k - t * pairs;
-    double where;
-    if (kPaged && p.at.kind == kPosNone) {
-      const uint32_t b = quotient(first + t, p.row_div);
-      where = static_cast<double>(__ldg(p.lengths + b)) + (first + t - b * p.rows);
-    } else {
-      where = position(p.at, first + t, quotient(at, p.axis_div));
-    }
-    const float2 v = cos_sin(where, __ldg(p.at.frequencies + at), p.at.factor);
-    cs_all[t * 2 * pairs + at] = v.x;
-    cs_all[t * 2 * pairs + pairs + at] = v.y;
-  }
-  __syncthreads();
-  const int unit_step = q.units <= kThreads ? q.units : kThreads;
-  for (int unit = unit0; unit < q.units; unit += unit_step) {
-    for (int task = slot; task < all; task += q.slots) {
-      if (unit != unit0 || task != slot) {
-        take_unit(unit);
-        fetch(task);
+      long long place = 0;  // the row of the pool
+      if constexpr (kPool) {
+        const int length = __ldg(p.lengths + b);
+        const long long row = length + i;
+        const bool inside = length >= 0 && row < static_cast<long long>(p.width) * kPage;
+        const int page = inside ? __ldg(p.table + b * p.width + row / kPage) : 0;
+        if (!inside || page < 0 || page >= p.pool_pages) {
+          if (p.err && unit == 0 && h0 == 0) atomicOr(p.err, inside ? kErrBadPage : kErrBadIndex);
+          continue;
+        }
+        place = (static_cast<long long>(page) * kPage + row % kPage) * kDim;
       }
-      const int t = static_cast<int>(quotient(static_cast<uint32_t>(task), q.task_div)), h0 = task - t * q.tasks;
-      const long long place = kPaged ? places[t] : kNoPlace;
-      if (kPool && place < 0) continue;
-      T* out = nullptr;
-      if constexpr (!kPool) {
-        const long long b = quotient(first + t, p.row_div), i = first + t - b * p.rows;
-        out = static_cast<T*>(q.h.dst) + b * q.h.db + i * q.h.dn;
-      }
-      if (kPaged && place == kNoRow) {
+      T* const out = kPool ? nullptr : static_cast<T*>(q.h.dst) + b * q.h.db + i * q.h.dn;
+      if (!live) {  // queries behind a count
         for (int h = h0; h < q.h.heads; h += q.tasks) {
           store_values(out + static_cast<long long>(h) * q.h.dh + c0, Values<T, kN>{});
           store_values(out + static_cast<long long>(h) * q.h.dh + c1, Values<T, kN>{});
@@ -372,7 +359,12 @@ __device__ __forceinline__ void rows_block(const RowsParams& p, const Part& q, u
         continue;
       }
       Turn<kN, kInterleaved> cs;
-      if (turns) load_turn(cs, cs_all + t * 2 * pairs + pair, cs_all + t * 2 * pairs + pairs + pair);
+      if (turns) {
+        const uint64_t where = kPaged && p.at.kind == kPosNone
+                                   ? static_cast<uint64_t>(static_cast<long long>(__ldg(p.lengths + b)) + i)
+                                   : position_word(p.at, token, axis);
+        make_turn<T>(cs, between, where, frequency, p.at.factor);
+      }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int h = h0 + j * q.tasks;
@@ -400,50 +392,48 @@ __device__ __forceinline__ void rows_block(const RowsParams& p, const Part& q, u
   }
 }
 
-template <typename T, int kN, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads, kN == 8 ? 3 : 4) rotate_kernel(const __grid_constant__ RowsParams p) {
-  extern __shared__ float4 smem[];
-  rows_block<T, kN, kInterleaved, false, kRotated>(p, p.part[0], blockIdx.x, smem);
+template <typename T, int kN, bool kInterleaved, int kBatch>
+__global__ void __launch_bounds__(kThreads, kBatch == kFew ? 8 : kN == 8 ? 4 : 5) rotate_kernel(const __grid_constant__ RowsParams p) {
+  rows_block<T, kN, kInterleaved, false, kRotated, kBatch>(p, p.part[0], blockIdx.x);
 }
 
 // Queries, keys and values have blocks of their own, in this order.
 template <int kN, bool kInterleaved, bool kFp8>
-__global__ void __launch_bounds__(kThreads, 3) append_rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(kThreads, 5) append_rows_kernel(const __grid_constant__ RowsParams p) {
   using T = __nv_bfloat16;
-  extern __shared__ float4 smem[];
   uint32_t block = blockIdx.x;
   if (block < p.part[0].blocks) {
-    rows_block<T, kN, kInterleaved, kFp8, kQueries>(p, p.part[0], block, smem);
+    rows_block<T, kN, kInterleaved, kFp8, kQueries, kAppended>(p, p.part[0], block);
   } else if ((block -= p.part[0].blocks) < p.part[1].blocks) {
-    rows_block<T, kN, kInterleaved, kFp8, kKeys>(p, p.part[1], block, smem);
+    rows_block<T, kN, kInterleaved, kFp8, kKeys, kAppended>(p, p.part[1], block);
   } else {
-    rows_block<T, kN, kInterleaved, kFp8, kValues>(p, p.part[2], block - p.part[1].blocks, smem);
+    rows_block<T, kN, kInterleaved, kFp8, kValues, kAppended>(p, p.part[2], block - p.part[1].blocks);
   }
 }
 
-size_t token_bytes(const Angles& a) { return 8 * static_cast<size_t>(a.pairs) + sizeof(long long); }
-
-template <typename T>
-int launch_rotate(const RowsParams& p, int n, bool interleaved, cudaStream_t stream) {
-  const auto kernel = n == 8   ? (interleaved ? rotate_kernel<T, sizeof(T) == 2 ? 8 : 4, true> : rotate_kernel<T, sizeof(T) == 2 ? 8 : 4, false>)
-                      : n == 4 ? (interleaved ? rotate_kernel<T, 4, true> : rotate_kernel<T, 4, false>)
-                               : (interleaved ? rotate_kernel<T, 1, true> : rotate_kernel<T, 1, false>);
-  kernel<<<p.part[0].blocks, kThreads, token_bytes(p.at) * p.part[0].group, stream>>>(p);
+template <typename T, int kN, int kBatch>
+int launch_rotate(const RowsParams& p, bool interleaved, cudaStream_t stream) {
+  const auto kernel = interleaved ? rotate_kernel<T, kN, true, kBatch> : rotate_kernel<T, kN, false, kBatch>;
+  kernel<<<p.part[0].blocks, kThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("rotate_kernel launch", e);
+}
+template <typename T>
+int launch_rotate(const RowsParams& p, int n, bool few, bool interleaved, cudaStream_t stream) {
+  constexpr int kWide = 16 / sizeof(T);
+  if (n == kWide)
+    return few ? launch_rotate<T, kWide, kFew>(p, interleaved, stream) : launch_rotate<T, kWide, kMany>(p, interleaved, stream);
+  if (n == 4) return few ? launch_rotate<T, 4, kFew>(p, interleaved, stream) : launch_rotate<T, 4, kMany>(p, interleaved, stream);
+  return few ? launch_rotate<T, 1, kFew>(p, interleaved, stream) : launch_rotate<T, 1, kMany>(p, interleaved, stream);
 }
 template <bool kFp8>
 int launch_append(const RowsParams& p, int n, bool interleaved, cudaStream_t stream) {
   const auto kernel = n == 8   ? (interleaved ? append_rows_kernel<8, true, kFp8> : append_rows_kernel<8, false, kFp8>)
                       : n == 4 ? (interleaved ? append_rows_kernel<4, true, kFp8> : append_rows_kernel<4, false, kFp8>)
                                : (interleaved ? append_rows_kernel<1, true, kFp8> : append_rows_kernel<1, false, kFp8>);
-  size_t group = 0;
   unsigned blocks = 0;
-  for (const Part& q : p.part) {
-    if (q.blocks > 0 && static_cast<size_t>(q.group) > group) group = q.group;
-    blocks += static_cast<unsigned>(q.blocks);
-  }
-  kernel<<<blocks, kThreads, token_bytes(p.at) * group, stream>>>(p);
+  for (const Part& q : p.part) blocks += static_cast<unsigned>(q.blocks);
+  kernel<<<blocks, kThreads, 0, stream>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? H3SA_OK : set_cuda_error("append_rows_kernel launch", e);
 }
@@ -458,21 +448,17 @@ bool fits(const Heads& h, int size, int n) {
 }
 int vector_of(const RowsParams& p, int size) {
   for (int n = 16 / size; n >= 4; n /= 2)
-    if (p.at.pairs % n == 0 && p.dim % n == 0 && fits(p.part[0].h, size, n) && fits(p.part[1].h, size, n) &&
-        fits(p.part[2].h, size, n))
+    if (p.at.per_axis % n == 0 && p.at.pairs % n == 0 && p.dim % n == 0 && fits(p.part[0].h, size, n) &&
+        fits(p.part[1].h, size, n) && fits(p.part[2].h, size, n))
       return n;
   return 1;
 }
 
-constexpr int kSms = 148;
-
-// A task is a head row while threads are few, kBatch of them from there on; a block has as many tokens as give
-// its threads a task each, as far as that leaves every SM some blocks.
-void lay_out(RowsParams& p, int n, int batch) {
+// A task is a head row while threads are few, `most_rows` of them from there on, of which a thread takes up to
+// four: that pays for its frequencies.
+void lay_out(RowsParams& p, int n, int batch, int most_rows) {
   p.tokens = static_cast<long long>(batch) * p.rows;
   p.row_div = divisor(static_cast<uint32_t>(p.rows));
-  p.pair_div = divisor(static_cast<uint32_t>(p.at.pairs > 0 ? p.at.pairs : 1));
-  p.axis_div = divisor(static_cast<uint32_t>(p.at.per_axis > 0 ? p.at.per_axis : 1));
   long long threads = 0;
   for (Part& q : p.part) {
     const int pairs = &q == p.part + 2 ? 0 : p.at.pairs;
@@ -480,24 +466,21 @@ void lay_out(RowsParams& p, int n, int batch) {
     q.units = q.pair_units + (p.dim - 2 * pairs + 2 * n - 1) / (2 * n);
     threads += p.tokens * q.h.heads * q.units;
   }
-  const int rows = threads >= static_cast<long long>(kSms) * kThreads * 3 * kBatch ? kBatch : 1;
+  const int rows = threads >= 768ll * kSms * most_rows ? most_rows : 1;
   for (Part& q : p.part) {
     if (q.h.heads == 0) continue;
     q.tasks = (q.h.heads + rows - 1) / rows;
     q.slots = q.units <= kThreads ? kThreads / q.units : 1;
     q.task_div = divisor(static_cast<uint32_t>(q.tasks));
-    long long group = q.slots / q.tasks;
-    const long long most = p.tokens / (4 * kSms), room = static_cast<long long>(32768 / token_bytes(p.at));
-    if (group > most) group = most;
-    if (group > room) group = room;
-    q.group = group < 1 ? 1 : static_cast<int>(group);
-    q.blocks = static_cast<int>((p.tokens + q.group - 1) / q.group);
+    q.all = p.tokens * q.tasks;
+    const long long once = (q.all + q.slots - 1) / q.slots, some = 8 * kSms;
+    q.blocks = static_cast<int>(once <= some ? once : once <= 4 * some ? some : (once + 3) / 4);
   }
 }
 
 int check_rotary(const char* what, const h3sa_rotary* r, int dim, bool rows_known, Angles& a) {
   memset(&a, 0, sizeof(a));
-  a.axes = a.per_axis = 1;
+  a.axes = 1;
   if (!r || r->pairs == 0) return H3SA_OK;
   if (r->pairs < 0 || r->pairs > dim / 2 || r->axes <= 0 || r->pairs % r->axes)
     return set_error(H3SA_ERR_INVALID, "%s: %d pairs over %d axes do not fit a head of %d", what, r->pairs, r->axes, dim);
@@ -555,7 +538,7 @@ int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32
   memset(&p, 0, sizeof(p));
   if (batch == 0 || rows == 0 || x->heads == 0) return H3SA_OK;
   if (const int rc = check_rotary("rotate", rotary, dim, false, p.at)) return rc;
-  if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || static_cast<int64_t>(x->heads) * dim > INT32_MAX / 4096)
+  if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * x->heads > INT32_MAX / 2)
     return set_error(H3SA_ERR_UNSUPPORTED, "rotate: batch %d x rows %d x heads %d is too large", batch, rows, x->heads);
   if (!head_stride_ok(x) || !head_stride_ok(out))
     return set_error(H3SA_ERR_UNSUPPORTED, "rotate: strides of heads must fit 32 bits");
@@ -567,12 +550,13 @@ int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32
   p.rows = rows;
   p.dim = dim;
   const int n = vector_of(p, size);
-  lay_out(p, n, batch);
+  const bool few = x->heads <= kFew;
+  lay_out(p, n, batch, few ? kFew : kMany);
   const bool inter = rotary && rotary->interleaved;
   const cudaStream_t at = static_cast<cudaStream_t>(stream);
-  return dtype == H3SA_FP32   ? launch_rotate<float>(p, n, inter, at)
-         : dtype == H3SA_FP16 ? launch_rotate<__half>(p, n, inter, at)
-                              : launch_rotate<__nv_bfloat16>(p, n, inter, at);
+  return dtype == H3SA_FP32   ? launch_rotate<float>(p, n, few, inter, at)
+         : dtype == H3SA_FP16 ? launch_rotate<__half>(p, n, few, inter, at)
+                              : launch_rotate<__nv_bfloat16>(p, n, few, inter, at);
 }
 
 int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_heads* query, const h3sa_heads* query_out,
@@ -594,7 +578,7 @@ int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_
                      pool_pages, width);
   const bool with_query = query && query->heads > 0;
   const int64_t heads = 2ll * key->heads + (with_query ? query->heads : 0);
-  if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || heads > INT32_MAX / (4096 * kDim))
+  if (static_cast<int64_t>(batch) * rows > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX / 2)
     return set_error(H3SA_ERR_UNSUPPORTED, "append rows: batch %d x rows %d x heads %lld is too large", batch, rows,
                      static_cast<long long>(heads));
   if (!head_stride_ok(key) || !head_stride_ok(value) || !head_stride_ok(query) || !head_stride_ok(query_out))
@@ -624,7 +608,7 @@ int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_
   p.counts = counts;
   p.err = device_error;
   const int n = vector_of(p, 2);
-  lay_out(p, n, batch);
+  lay_out(p, n, batch, kAppended);
   const bool inter = rotary && rotary->interleaved;
   const cudaStream_t at = static_cast<cudaStream_t>(stream);
   return e4m3 ? launch_append<true>(p, n, inter, at) : launch_append<false>(p, n, inter, at);
