@@ -563,8 +563,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           } else {
             seq = at.b;
             g.row0 = at.b * p.rows * p.group + at.t * kSpan;
-            g.n_rows = min(kSpan, p.rows * p.group - at.t * kSpan);
             const Extent x = extent_of(p, at.b);
+            g.n_rows = min(kSpan, x.rows - at.t * kSpan);
             g.kv_end = x.all;
             g.clean = x.clean;
             g.block0 = own_lo(p, x) / kBlk + at.off;
@@ -916,6 +916,12 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      if constexpr (kTree) {
+        if (sight.hidden) {
+          m = -INFINITY;
+          l = 0.f;
+        }
+      }
       more = take(next);  // its query rows arrive while this item's O is written
       ok = mbar_wait(smem_u32(&sm.o_full[t]), o_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, ok))) break;
@@ -1252,18 +1258,31 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
     if (r >= min(own_all, (t + 1) * kSpan)) return;
   }
   const Extent ext = extent_of(p, b);
+  const auto write_row = [&](int row, const float4& acc, float m, float sum) {
+    float scale = sum == 0.f ? 0.f : 1.0f / sum;
+    if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
+    const int i = row / p.group;
+    const long long id = (static_cast<long long>(b) * p.rows + i) * p.heads + head * p.group + row - i * p.group;
+    reinterpret_cast<uint2*>(p.out + id * kD)[lane] =
+        make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
+    if (p.lse && lane == 0) p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
+  };
   int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * (kBlk / lo.unit)) + __ldcg(po + 3 + b);
   for (int k = 0; k < t; ++k) u0 += weight_of(lo, own_units(p, lo, ext, k));
   const int units = own_units(p, lo, ext, t);
-  const int n_rows = min(lo.span, own_all - t * lo.span);
+  const int n_rows = min(lo.span, ext.rows - t * lo.span), last = min(own_all, (t + 1) * lo.span);
   if (shared_blocks == 0 && units > 0 && u0 / cut_o == (u0 + units - 1) / cut_o &&
-      (own_by_warps || n_rows > kBlk || units == 1))
-    return;  // written by the segment itself
+      (own_by_warps || n_rows > kBlk || units == 1)) {  // written by the segment itself
+    if constexpr (is_tree<P>) {  // but for rows behind the nodes
+      for (int k = max(0, ext.rows - r); k < kRows && r + k < last; ++k) write_row(r + k, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+    }
+    return;
+  }
   Pieces sh[kRows], own[kRows];
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    // rows past the item read its last row again and write nothing
-    const int rk = min(r + k, t * lo.span + n_rows - 1);
+    // rows past the item (and behind the nodes) read its last row again, and what they read is not written
+    const int rk = min(r + k, t * lo.span + max(n_rows, 1) - 1);
     const int row = b * own_all + rk, t_sh = row / ls.span;
     sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, shared_units,
                       min(ls.span, p.batch * own_all - t_sh * ls.span), row % ls.span,
@@ -1311,14 +1330,9 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   }
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    if (r + k >= t * lo.span + n_rows) break;
-    float scale = sum[k] == 0.f ? 0.f : 1.0f / sum[k];
-    if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
-    const int i = (r + k) / p.group;
-    const long long id = (static_cast<long long>(b) * p.rows + i) * p.heads + head * p.group + r + k - i * p.group;
-    reinterpret_cast<uint2*>(p.out + id * kD)[lane] = make_uint2(
-        pack_bf16x2(acc[k].x * scale, acc[k].y * scale), pack_bf16x2(acc[k].z * scale, acc[k].w * scale));
-    if (p.lse && lane == 0) p.lse[id] = sum[k] == 0.f ? -INFINITY : (m[k] + log2f(sum[k])) * 0.6931471805599453f;
+    if (r + k >= last) break;
+    if (is_tree<P> && r + k >= ext.rows) write_row(r + k, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+    else write_row(r + k, acc[k], m[k], sum[k]);
   }
 }
 

@@ -74,9 +74,10 @@ struct TreeParams : BranchParams {
 template <class P>
 constexpr bool is_tree = std::is_same_v<P, TreeParams>;
 
-// Rows of a sequence: all keys, and those that each of its new rows may see.
+// Rows of a sequence: all keys, and those that each of its new rows may see; `rows`: of its stacked query rows, those
+// that there are (of a tree the nodes', the rest of its rows come out zero).
 struct Extent {
-  int all, clean;
+  int all, clean, rows;
 };
 __device__ __forceinline__ int clean_rows(const BranchParams& p, int b) {
   const int n = __ldg(p.lengths + b);
@@ -84,12 +85,13 @@ __device__ __forceinline__ int clean_rows(const BranchParams& p, int b) {
 }
 __device__ __forceinline__ Extent extent_of(const BranchParams& p, int b) {
   const int n = clean_rows(p, b);
-  return Extent{n, n};
+  return Extent{n, n, p.rows * p.group};
 }
 __device__ __forceinline__ Extent extent_of(const TreeParams& p, int b) {
   const int n = clean_rows(p, b);
   const int nodes = p.counts ? max(0, min(__ldg(p.counts + b), p.rows)) : p.rows;
-  return Extent{min(n + nodes, p.width * kBlk), n};
+  const int all = min(n + nodes, p.width * kBlk);
+  return Extent{all, n, (all - n) * p.group};
 }
 
 // A sequence that ends inside the shared blocks has no part in their items, where rows behind its end that
@@ -104,11 +106,15 @@ __device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, 
   const int last = min((t + 1) * ln.span, p.rows * p.group) - 1;
   return x.all - (p.rows - 1 - last / p.group);
 }
-__device__ __forceinline__ int own_units(const BranchParams& p, const Line& ln, const Extent& x, int t) {
+template <class P>
+__device__ __forceinline__ int own_units(const P& p, const Line& ln, const Extent& x, int t) {
+  if (is_tree<P> && t * ln.span >= x.rows) return 0;
   return max(0, own_limit(p, ln, x, t) - own_lo(p, x) + ln.unit - 1) / ln.unit;
 }
 __device__ __forceinline__ int weight_of(const Line& ln, int units) { return units > 0 ? units + ln.pad : 0; }
-__device__ __forceinline__ int own_weight_all(const BranchParams& p, const Line& ln, const Extent& x) {
+template <class P>
+__device__ __forceinline__ int own_weight_all(const P& p, const Line& ln, const Extent& x) {
+  if constexpr (is_tree<P>) return weight_of(ln, own_units(p, ln, x, 0)) * min(ln.own_tiles, (x.rows + ln.span - 1) / ln.span);
   if (!p.causal) return weight_of(ln, own_units(p, ln, x, 0)) * ln.own_tiles;
   int n = 0;
   for (int t = 0; t < ln.own_tiles; ++t) n += weight_of(ln, own_units(p, ln, x, t));
@@ -139,7 +145,7 @@ __device__ __forceinline__ Plan make_plan(const P& p, const Line& ln, int lane) 
   at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
   Plan pl;
   pl.longest = at;
-  pl.shared_blocks = own_lo(p, Extent{top, top}) / kBlk;
+  pl.shared_blocks = own_lo(p, Extent{top, top, 0}) / kBlk;
   pl.shared_units = pl.shared_blocks * (kBlk / ln.unit);
   pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units) + own;
   const int all = pl.head_weight * p.kv_heads;
@@ -270,11 +276,14 @@ __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) 
   return a;
 }
 
-// What a node sees: all keys in front of `base`, and key base + n, n < count, if bit n of its mask says so.
-// A row that sees nothing of an item (one behind the nodes, one without the shared blocks) has 0 and 0.
+// What a node sees: all keys in front of `base`, and key base + n, n < count, if bit n of its mask says so. A row that
+// has no part in an item (one behind the nodes, one without the shared blocks) is `hidden`: it goes through the item as if it
+// saw everything, which costs least (hiding keys of such rows one by one took 111 us for 94), and what it
+// has then is dropped.
 struct Sight {
   int base, count;
   const uint32_t* mask;
+  bool hidden;
   __device__ __forceinline__ uint32_t word(int w) const {
     const int rest = count - 32 * w;
     if (w < 0 || rest <= 0) return 0u;
@@ -292,8 +301,8 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const TreeParams& p, const RowAt& ra, bool shared) {
   const Extent x = extent_of(p, ra.b);
   const int count = x.all - x.clean;
-  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{0, 0, nullptr};
-  return Sight{x.clean, count, p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words};
+  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, nullptr, true};
+  return Sight{x.clean, count, p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words, false};
 }
 
 // Of a chain, only a limit.

@@ -172,16 +172,18 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.seq = bh - g.head * p.batch;
         g.shared = 0;
         g.row0 = g.seq * own_all + t * kRowSpan;
-        g.n_rows = min(kRowSpan, own_all - t * kRowSpan);
         g.key0 = 0;
         const Extent x = extent_of(p, g.seq);
+        g.n_rows = min(kRowSpan, x.rows - t * kRowSpan);
         g.kv_end = x.all;
         g.clean = x.clean;
         g.direct = 1;
         g.slot = 0;
         g.units = own_units(p, ln, x, t);
-        if (g.units > 0) continue;
-        for (int i = lane; !loader && i < g.n_rows * 16; i += 32) {  // rows that see nothing
+        if (!kTree && g.units > 0) continue;
+        // rows that see nothing, or come behind the nodes
+        const int none = g.units > 0 ? g.n_rows : 0, all = min(kRowSpan, own_all - t * kRowSpan);
+        for (int i = none * 16 + lane; !loader && i < all * 16; i += 32) {
           const RowAt ra = row_at(p, g.head, g.row0 + (i >> 4));
           const long long id = (static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h;
           reinterpret_cast<uint4*>(p.out + id * kD)[i & 15] = make_uint4(0u, 0u, 0u, 0u);
@@ -199,8 +201,8 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.shared = at.b < 0;
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
-        g.n_rows = min(kRowSpan, (g.shared ? p.batch * own_all : (at.b + 1) * own_all) - g.row0);
         const Extent x = extent_of(p, g.seq);
+        g.n_rows = min(kRowSpan, g.shared ? p.batch * own_all - g.row0 : x.rows - at.t * kRowSpan);
         g.key0 = (g.shared ? 0 : own_lo(p, x)) + at.off * kRowUnit;
         g.kv_end = x.all;
         g.clean = x.clean;
@@ -467,7 +469,20 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       advance();
     }
     if (!ok) break;
-    if constexpr (kTree) {  // what was taken out of V, to the rows that see it
+    if constexpr (kTree) {
+      if (sight0.hidden) {
+        m0 = -INFINITY;
+        l0 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = 0.f;
+      }
+      if (sight1.hidden) {
+        m1 = -INFINITY;
+        l1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j][2] = o[j][3] = 0.f;
+      }
+      // what was taken out of V, to the rows that see it
       if (__any_sync(0xffffffffu, taken_out)) {
         const NodeValues<kFp8> nodes(p, g.seq, g.head);
 #pragma unroll

@@ -24,7 +24,7 @@ from .kernels import HEAD_DIM, PAGE_ROWS
 from .rotary import _rotary
 
 _TREE, _APPEND, _KEEP = LIB.h3sa_draft_tree, LIB.h3sa_append_rows, LIB.h3sa_keep_rows
-_empty_like, _empty = torch.empty_like, torch.empty
+_empty_like = torch.empty_like
 
 
 def _counts(what: str, counts: torch.Tensor | None, device: torch.device, batch: int) -> int | None:
@@ -131,7 +131,7 @@ def append_rows(key: torch.Tensor, value: torch.Tensor, key_pool: torch.Tensor, 
             raise RuntimeError(f"{what}: query must be bf16 [{batch}, {rows}, heads, {HEAD_DIM}] on {device}")
         if query_out is None:
             with _on(stream):
-                query_out = _empty(wide, dtype=_BF16, device=device)
+                query_out = _empty_like(query) if query.is_contiguous() else query.new_empty(wide)
         elif query_out.shape != wide or query_out.dtype is not _BF16 or query_out.device != device:
             raise RuntimeError(f"{what}: query_out must be bf16 {list(wide)} on {device}")
         (qb, qn, qh, q1), (ob, on, oh, o1) = query.stride(), query_out.stride()

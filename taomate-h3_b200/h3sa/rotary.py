@@ -24,7 +24,7 @@ _ROTATE = LIB.h3sa_rotate
 _F64 = torch.float64
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _POSITIONS = {torch.int32: 1, torch.int64: 2, torch.float64: 3}
-_empty = torch.empty
+_empty_like = torch.empty_like
 
 
 def rotary_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none", scale: float = 1.0,
@@ -111,20 +111,22 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     device, shape, kind = x.device, x.shape, _DTYPES.get(x.dtype)
     if kind is None or len(shape) not in (3, 4):
         raise RuntimeError(f"{what}: x must be bf16, fp16 or fp32 [tokens, heads, dim] or [sequences, rows, heads, dim]")
-    *batch, rows, heads, dim = shape
+    if len(shape) == 3:
+        batch, (rows, heads, dim), sb, (sn, sh, last) = 1, shape, 0, x.stride()
+    else:
+        (batch, rows, heads, dim), (sb, sn, sh, last) = shape, x.stride()
     rotary = _rotary(what, frequencies, positions, shape[:-2], dim, interleaved, factor, device)
-    *sb, sn, sh, last = x.stride()
     if last != 1:
         raise RuntimeError(f"{what}: rows of x must be contiguous")
     handle = _handle(stream, device)
     if out is None:
         with _on(stream):
-            out = _empty(shape, dtype=x.dtype, device=device)
+            out = _empty_like(x) if x.is_contiguous() else x.new_empty(shape)
     elif out.dtype is not x.dtype or out.shape != shape or out.device != device or out.stride(-1) != 1:
         raise RuntimeError(f"{what}: out must be {x.dtype} {list(shape)} on {device} with contiguous rows")
-    *db, dn, dh, _ = out.stride()
-    code = _ROTATE(Heads(x.data_ptr(), sb[0] if sb else 0, sn, sh, heads, 0),
-                   Heads(out.data_ptr(), db[0] if db else 0, dn, dh, heads, 0), kind, batch[0] if batch else 1, rows, dim,
+    dn, dh, _ = out.stride()[-3:]
+    code = _ROTATE(Heads(x.data_ptr(), sb, sn, sh, heads, 0),
+                   Heads(out.data_ptr(), out.stride(0) if batch > 1 else 0, dn, dh, heads, 0), kind, batch, rows, dim,
                    rotary, handle)
     if code:
         check("h3sa_rotate", code)
