@@ -521,7 +521,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     int later = 0;
     Place later_at = at;
     if (u < u_end && at.off > 0) {
-      const int rest = weight_of(ln, place_units(p, ln, pl, at)) - at.off;
+      const PlaceUnits it = place_units(p, ln, pl, at);
+      const int rest = weight_of(ln, it.units, it.cost) - at.off;
       if (rest < u_end - u) {
         later = rest;
         u += rest;
@@ -546,8 +547,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       memset(&g, 0, sizeof(g));
       int seq = 0;
       while (u < u_end && !g.live) {
-        const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
-        const int blocks = min(units, at.off + part) - at.off;
+        const PlaceUnits it = place_units(p, ln, pl, at);
+        const UnitRange in = units_in(ln, it, at.off, u_end - u);
+        const int blocks = in.count;
         if (blocks > 0) {
           long long item, row0;
           int slot_rows;
@@ -555,7 +557,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             seq = pl.longest;
             g.row0 = at.t * kSpan;
             g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
-            g.block0 = at.off;
+            g.block0 = in.first;
             g.kv_end = g.clean = pl.shared_blocks * kBlk;
             item = at.head * ln.shared_tiles + at.t;
             row0 = 0;
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             g.n_rows = min(kSpan, x.rows - at.t * kSpan);
             g.kv_end = x.all;
             g.clean = x.clean;
-            g.block0 = own_lo(p, x) / kBlk + at.off;
+            g.block0 = own_lo(p, x) / kBlk + in.first;
             item = (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
             row0 = p.own_row0;
             slot_rows = p.own_slot_rows;
@@ -576,9 +578,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           g.live = at.b < 0 ? 2 : 1;
           g.head = at.head;
           g.blocks = blocks;
-          g.direct = pl.shared_blocks == 0 && blocks == units && (g.n_rows > kBlk || blocks == 1);
+          g.direct = pl.shared_blocks == 0 && blocks == it.units && (g.n_rows > kBlk || blocks == 1);
         }
-        u += part;
+        u += in.part;
         if (u < u_end) {
           step_item(p, ln, pl, at);
         } else if (later > 0) {
@@ -1154,10 +1156,10 @@ struct Pieces {  // of one row in one item: workspace rows first + j * stride, j
   int n, stride;
   long long first;
 };
-__device__ __forceinline__ Pieces pieces_of(int cut, int u0, int units, int n_rows, int r, long long item,
+__device__ __forceinline__ Pieces pieces_of(int cut, int u0, int units, int cost, int n_rows, int r, long long item,
                                             long long row0, int slot_rows, bool warps) {
   if (units == 0) return Pieces{0, 0, 0};
-  const int c_lo = u0 / cut, n_cta = (u0 + units - 1) / cut - c_lo + 1;
+  const int c_lo = u0 / cut, n_cta = (u0 + (units - 1) * cost) / cut - c_lo + 1;
   if (warps) return Pieces{n_cta, slot_rows, row0 + (item + c_lo) * slot_rows + r};
   const long long first = row0 + (item + c_lo) * 2 * slot_rows;
   // items of both tiles: the slot of the row's tile in each CTA; else the slots of both
@@ -1234,20 +1236,21 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   const int* const po = p.plan + (own_by_warps ? 3 + p.batch : 0);
   const int shared_blocks = kJoint ? 0 : __ldcg(po);
   const int cut_s = __ldcg(ps + 2), cut_o = __ldcg(po + 2);
-  const int shared_units = shared_blocks * (kBlk / ls.unit), shared_weight = weight_of(ls, shared_units);
+  const int shared_units = shared_blocks * over_pow2(kBlk, ls.unit), cost_s = shared_cost(p, ls);
+  const int shared_weight = weight_of(ls, shared_units, cost_s);
   const int own_all = p.rows * p.group;
   // split form: stacked rows of all branches, one a team, head by head; joint form: kRows rows of
   // an item a warp
   int head, b, t, r;
   if (!kJoint) {
     const int stacked = p.batch * own_all;
-    const long long id = static_cast<long long>(blockIdx.x) * kTeams + team;
-    if (id >= static_cast<long long>(stacked) * p.kv_heads) return;  // a whole block if kTeam > 1
-    head = static_cast<int>(id / stacked);
-    const int row = static_cast<int>(id - static_cast<long long>(head) * stacked);
-    b = row / own_all;
+    const uint32_t id = blockIdx.x * kTeams + team;  // rows of all heads are below 2^31
+    if (id >= static_cast<uint32_t>(stacked) * p.kv_heads) return;  // a whole block if kTeam > 1
+    head = quotient(id, p.stacked_div);
+    const int row = id - head * stacked;
+    b = quotient(row, p.own_div);
     r = row - b * own_all;
-    t = r / lo.span;
+    t = over_pow2(r, lo.span);
   } else {
     constexpr int kGroups = kSpan / (kRows * kMergeWarps);
     const int item = blockIdx.x / kGroups;
@@ -1261,17 +1264,18 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   const auto write_row = [&](int row, const float4& acc, float m, float sum) {
     float scale = sum == 0.f ? 0.f : 1.0f / sum;
     if constexpr (kFp8) scale *= __ldg(p.v_scale + head);
-    const int i = row / p.group;
+    const int i = quotient(row, p.group_div);
     const long long id = (static_cast<long long>(b) * p.rows + i) * p.heads + head * p.group + row - i * p.group;
     reinterpret_cast<uint2*>(p.out + id * kD)[lane] =
         make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
     if (p.lse && lane == 0) p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
   };
-  int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * (kBlk / lo.unit)) + __ldcg(po + 3 + b);
-  for (int k = 0; k < t; ++k) u0 += weight_of(lo, own_units(p, lo, ext, k));
-  const int units = own_units(p, lo, ext, t);
+  int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * over_pow2(kBlk, lo.unit), shared_cost(p, lo)) +
+           __ldcg(po + 3 + b);
+  for (int k = 0; k < t; ++k) u0 += own_weight(p, lo, ext, k);
+  const int units = own_units(p, lo, ext, t), cost_o = own_cost(p, lo, ext, t);
   const int n_rows = min(lo.span, ext.rows - t * lo.span), last = min(own_all, (t + 1) * lo.span);
-  if (shared_blocks == 0 && units > 0 && u0 / cut_o == (u0 + units - 1) / cut_o &&
+  if (shared_blocks == 0 && units > 0 && u0 / cut_o == (u0 + (units - 1) * cost_o) / cut_o &&
       (own_by_warps || n_rows > kBlk || units == 1)) {  // written by the segment itself
     if constexpr (is_tree<P>) {  // but for rows behind the nodes
       for (int k = max(0, ext.rows - r); k < kRows && r + k < last; ++k) write_row(r + k, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
@@ -1283,11 +1287,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   for (int k = 0; k < kRows; ++k) {
     // rows past the item (and behind the nodes) read its last row again, and what they read is not written
     const int rk = min(r + k, t * lo.span + max(n_rows, 1) - 1);
-    const int row = b * own_all + rk, t_sh = row / ls.span;
-    sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, shared_units,
-                      min(ls.span, p.batch * own_all - t_sh * ls.span), row % ls.span,
+    const int row = b * own_all + rk, t_sh = over_pow2(row, ls.span);
+    sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, shared_units, cost_s,
+                      min(ls.span, p.batch * own_all - t_sh * ls.span), row & (ls.span - 1),
                       head * ls.shared_tiles + t_sh, 0, p.shared_slot_rows, shared_by_warps);
-    own[k] = pieces_of(cut_o, u0, units, n_rows, rk - t * lo.span,
+    own[k] = pieces_of(cut_o, u0, units, cost_o, n_rows, rk - t * lo.span,
                        (static_cast<long long>(head) * p.batch + b) * lo.own_tiles + t, p.own_row0,
                        p.own_slot_rows, own_by_warps);
   }
@@ -1401,16 +1405,45 @@ constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 // heads over 1024 keys: 2 units 11.3, 4 units 12.2, 6 units 13.2.
 constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 
-Shape shape_of(int batch, int rows, int kv_heads, int group, int shared) {
+// Trees of more than 16 stacked rows. The warp line reads a tree's keys once for every 16 rows and the tensor line
+// starts some 8 us later (17 in e4m3, which it widens), so what decides is the keys, of which the host knows the
+// tables' width. us a million keys and KV heads: warps 50 for each 16 rows (e4m3 40), tensor cores 81 (88) an item. 8 KV
+// heads, warp / tensor (us): 64 rows, 24 trees of up to 300 keys 33 / 39, 1000 59 / 48, 16000 424 / 186; 48 rows,
+// 1000 47 / 43; 32 rows, 1000 35 / 42, 4000 72 / 70, 16000 232 / 178; one tree of 48 rows over 60000 130 / 76; e4m3: 64
+// rows, 1000 53 / 63, 4000 114 / 104; 48 rows, 4000 85 / 102, 16000 229 / 213; 32 rows, 16000 179 / 199. With shared keys (20 trees of 52 rows over
+// 1024 and up to 700 of their own 73 / 50) both parts are in one kernel.
+bool tree_on_tensor(int batch, int own, int kv_heads, int shared, int width, bool e4m3) {
+  if (own <= kRowSpan) return false;
+  const auto tiles = [](long long n, int span) { return (n + span - 1) / span; };
+  const long long keys = static_cast<long long>(batch) * (width - shared) * kBlk, all = static_cast<long long>(batch) * own;
+  const double warps = static_cast<double>(kv_heads) * (keys * tiles(own, kRowSpan) + 1.0 * shared * kBlk * tiles(all, kRowSpan));
+  const double tensor = static_cast<double>(kv_heads) * (keys + 1.4 * shared * kBlk * tiles(all, kSpan));
+  return e4m3 ? warps - 2.2 * tensor > 680000.0 : warps - 1.62 * tensor > 256000.0;
+}
+
+// The shape of a tree's call has the tables' width, a chain's 0.
+Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, int width = 0, bool e4m3 = false) {
   Shape s;
   memset(&s, 0, sizeof(s));
   const long long own = static_cast<long long>(rows) * group;
   const long long all = own * batch;
   const auto tiles = [](long long n, int span) { return static_cast<int>((n + span - 1) / span); };
   s.joint = joint_form(own, batch, kv_heads, shared) ? 1 : 0;
-  s.tensor = Line{kSpan, kBlk, 2, 0, 0, sm_count(), 1};
-  s.warp = Line{kRowSpan, kRowUnit, 2, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
-  Line& lo = own <= kWarpOwnRows ? s.warp : s.tensor;
+  s.tensor = Line{kSpan, kBlk, 2, 1, 1, 0, 0, sm_count(), 1};
+  s.warp = Line{kRowSpan, kRowUnit, 2, 1, 1, 0, 0, sm_count() * kRowWarpsPerBlock, kWarpLeast};
+  if (width > 0) {
+    s.tensor.few = kFewCost;
+    s.tensor.many = s.tensor.least = kManyCost;
+    s.tensor.pad = kTreePad;
+  }
+  bool on_tensor = own > kWarpOwnRows;
+  if (width > 0 && !on_tensor) {
+    Line whole = s.warp;
+    whole.own_tiles = tiles(own, kRowSpan);
+    on_tensor = !whole_form(width, kv_heads, batch, whole) &&
+                tree_on_tensor(batch, static_cast<int>(own), kv_heads, shared, width, e4m3);
+  }
+  Line& lo = on_tensor ? s.tensor : s.warp;
   lo.own_tiles = tiles(own, lo.span);
   s.own_slot_rows = static_cast<int>(own < lo.span ? own : lo.span);
   if (&lo == &s.tensor && own > kBlk) s.own_slot_rows = kBlk;
@@ -1550,11 +1583,12 @@ int attend(const char* what, const TreeParams* nodes, const void* query, int64_t
   if (stacked > INT32_MAX / 2 || static_cast<int64_t>(batch) * rows * heads > INT32_MAX)
     return set_error(H3SA_ERR_UNSUPPORTED, "%s: batch %d x rows %d x heads %d is too large", what,
                      batch, rows, heads);
-  Shape s = shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
+  Shape s = nodes ? shape_of(batch, rows, kv_heads, group, shared_rows / kBlk, width, e4m3 != 0)
+                  : shape_of(batch, rows, kv_heads, group, shared_rows / kBlk);
   const auto line_units = [&](const Line& ln) {
     const int64_t blocks = kBlk / ln.unit;
-    return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks + ln.pad) +
-                       static_cast<int64_t>(batch) * ln.own_tiles * (width * blocks + ln.pad));
+    return kv_heads * (ln.shared_tiles * (shared_rows / kBlk * blocks * ln.many + ln.pad) +
+                       static_cast<int64_t>(batch) * ln.own_tiles * (width * blocks * ln.many + ln.pad));
   };
   if (line_units(s.tensor) > INT32_MAX / 2 || line_units(s.warp) > INT32_MAX / 2)
     return set_error(H3SA_ERR_UNSUPPORTED, "%s: batch %d x rows %d x heads %d over %d "
@@ -1578,6 +1612,10 @@ int attend(const char* what, const TreeParams* nodes, const void* query, int64_t
   p.heads = heads;
   p.kv_heads = kv_heads;
   p.group = group;
+  p.rows_div = divisor(static_cast<uint32_t>(rows));
+  p.group_div = divisor(static_cast<uint32_t>(group));
+  p.own_div = divisor(static_cast<uint32_t>(rows) * group);
+  p.stacked_div = divisor(static_cast<uint32_t>(stacked));
   p.causal = causal ? 1 : 0;
   p.joint = s.joint;
   if (whole_form(width, kv_heads, batch, s.warp)) {
@@ -1622,6 +1660,15 @@ int64_t h3sa_shared_prefix_workspace(int32_t batch, int32_t rows, int32_t heads,
   if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0)
     return 0;
   const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk);
+  return s.bytes;
+}
+
+int64_t h3sa_tree_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads, int32_t shared_rows,
+                            int32_t width, int32_t e4m3) {
+  if (batch <= 0 || rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || shared_rows < 0 || width <= 0 ||
+      shared_rows / kBlk > width || static_cast<int64_t>(rows) * (heads / kv_heads) > INT32_MAX / 2)
+    return 0;
+  const Shape s = shape_of(batch, rows, kv_heads, heads / kv_heads, shared_rows / kBlk, width, e4m3 != 0);
   return s.bytes;
 }
 

@@ -9,6 +9,7 @@
 #include <climits>
 #include <type_traits>
 
+#include "h3sa_div.cuh"
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
 
@@ -28,10 +29,11 @@ constexpr float kGrowth = 8.0f;
 constexpr float kBoostF8 = 7.0f;
 
 // A line: items of up to `span` query rows, first those against the shared blocks and then those
-// of each branch against its own, KV head by KV head; an item has a unit for every `unit` keys and
-// weighs `pad` more, which is about what starting and ending it costs.
+// of each branch against its own, KV head by KV head; an item has a unit for every `unit` keys, each
+// weighs `few` or, in an item of more than 128 rows, `many`, and the item `pad` more, which is about what starting and
+// ending it costs.
 struct Line {
-  int span, unit, pad;
+  int span, unit, pad, few, many;
   int shared_tiles;  // items per KV head against the shared blocks (0: the other line has them)
   int own_tiles;     // items per KV head and branch against its own (0: the other line has them)
   int workers;
@@ -46,6 +48,7 @@ struct BranchParams {
   const int* table;            // [batch, width]
   const int* lengths;          // [batch]
   int width, batch, rows, heads, kv_heads, group;
+  Divisor rows_div, group_div, own_div, stacked_div;  // of rows, group, rows * group, batch * rows * group
   int shared_keys;             // leading keys of the shared items (0: there are none), whole blocks
   int causal, joint;
   int whole;                   // the warp line takes whole items
@@ -104,20 +107,39 @@ __device__ __forceinline__ int own_lo(const BranchParams& p, const Extent& x) { 
 __device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, const Extent& x, int t) {
   if (!p.causal) return x.all;
   const int last = min((t + 1) * ln.span, p.rows * p.group) - 1;
-  return x.all - (p.rows - 1 - last / p.group);
+  return x.all - (p.rows - 1 - static_cast<int>(quotient(last, p.group_div)));
 }
 template <class P>
 __device__ __forceinline__ int own_units(const P& p, const Line& ln, const Extent& x, int t) {
   if (is_tree<P> && t * ln.span >= x.rows) return 0;
-  return max(0, own_limit(p, ln, x, t) - own_lo(p, x) + ln.unit - 1) / ln.unit;
+  return over_pow2(max(0, own_limit(p, ln, x, t) - own_lo(p, x) + ln.unit - 1), ln.unit);
 }
-__device__ __forceinline__ int weight_of(const Line& ln, int units) { return units > 0 ? units + ln.pad : 0; }
+// What a unit of an item of `rows` rows weighs: 1, or of the tensor line in a tree's call one of the two below (of
+// chains all weigh the same). Blocks of up to 128 and of more rows take a CTA 1.6 and 2.6 us (e4m3 1.5 and 2.2), and an item 6 to 8 us
+// (10) from its end to the next one's first scores.
+constexpr int kFewCost = 5, kManyCost = 8, kTreePad = 24;
+template <class P>
+__device__ __forceinline__ int cost_of(const P&, const Line& ln, int rows) {
+  return is_tree<P> ? (rows > kBlk ? ln.many : ln.few) : 1;
+}
+template <class P>
+__device__ __forceinline__ int shared_cost(const P& p, const Line& ln) { return cost_of(p, ln, p.batch * p.rows * p.group); }
+template <class P>
+__device__ __forceinline__ int own_cost(const P& p, const Line& ln, const Extent& x, int t) { return cost_of(p, ln, x.rows - t * ln.span); }
+__device__ __forceinline__ int weight_of(const Line& ln, int units, int cost) { return units > 0 ? units * cost + ln.pad : 0; }
+template <class P>
+__device__ __forceinline__ int own_weight(const P& p, const Line& ln, const Extent& x, int t) {
+  return weight_of(ln, own_units(p, ln, x, t), own_cost(p, ln, x, t));
+}
 template <class P>
 __device__ __forceinline__ int own_weight_all(const P& p, const Line& ln, const Extent& x) {
-  if constexpr (is_tree<P>) return weight_of(ln, own_units(p, ln, x, 0)) * min(ln.own_tiles, (x.rows + ln.span - 1) / ln.span);
-  if (!p.causal) return weight_of(ln, own_units(p, ln, x, 0)) * ln.own_tiles;
+  if constexpr (is_tree<P>) {  // all live tiles but the last are full
+    const int tiles = min(ln.own_tiles, over_pow2(x.rows + ln.span - 1, ln.span));
+    return tiles == 0 ? 0 : own_weight(p, ln, x, 0) * (tiles - 1) + own_weight(p, ln, x, tiles - 1);
+  }
+  if (!p.causal) return own_weight(p, ln, x, 0) * ln.own_tiles;
   int n = 0;
-  for (int t = 0; t < ln.own_tiles; ++t) n += weight_of(ln, own_units(p, ln, x, t));
+  for (int t = 0; t < ln.own_tiles; ++t) n += own_weight(p, ln, x, t);
   return n;
 }
 
@@ -146,8 +168,8 @@ __device__ __forceinline__ Plan make_plan(const P& p, const Line& ln, int lane) 
   Plan pl;
   pl.longest = at;
   pl.shared_blocks = own_lo(p, Extent{top, top, 0}) / kBlk;
-  pl.shared_units = pl.shared_blocks * (kBlk / ln.unit);
-  pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units) + own;
+  pl.shared_units = pl.shared_blocks * over_pow2(kBlk, ln.unit);
+  pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units, shared_cost(p, ln)) + own;
   const int all = pl.head_weight * p.kv_heads;
   pl.cut = max(ln.least, (all + ln.workers - 1) / ln.workers);
   return pl;
@@ -167,7 +189,7 @@ __device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& 
   at.b = -1;
   at.t = 0;
   int x = u - at.head * pl.head_weight;
-  const int w = weight_of(ln, pl.shared_units);
+  const int w = weight_of(ln, pl.shared_units, shared_cost(p, ln));
   if (x < ln.shared_tiles * w) {
     at.t = x / w;
     at.off = x - at.t * w;
@@ -193,7 +215,7 @@ __device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& 
     x -= __shfl_sync(0xffffffffu, cum, 31);
   }
   const Extent ext = extent_of(p, at.b);
-  for (int v; x >= (v = weight_of(ln, own_units(p, ln, ext, at.t))); ++at.t) x -= v;
+  for (int v; x >= (v = own_weight(p, ln, ext, at.t)); ++at.t) x -= v;
   at.off = x;
   return at;
 }
@@ -220,9 +242,27 @@ __device__ __forceinline__ void step_item(const P& p, const Line& ln, const Plan
     if (ln.own_tiles > 0 && own_units(p, ln, extent_of(p, at.b), at.t) > 0) return;
   }
 }
+// The item at a place: its units, and what each weighs.
+struct PlaceUnits {
+  int units, cost;
+};
 template <class P>
-__device__ __forceinline__ int place_units(const P& p, const Line& ln, const Plan& pl, const Place& at) {
-  return at.b < 0 ? pl.shared_units : own_units(p, ln, extent_of(p, at.b), at.t);
+__device__ __forceinline__ PlaceUnits place_units(const P& p, const Line& ln, const Plan& pl, const Place& at) {
+  if (at.b < 0) return PlaceUnits{pl.shared_units, shared_cost(p, ln)};
+  const Extent x = extent_of(p, at.b);
+  return PlaceUnits{own_units(p, ln, x, at.t), own_cost(p, ln, x, at.t)};
+}
+// Its units that begin in [off, off + part) of it; part: what is left of the item or of the worker's own part.
+struct UnitRange {
+  int part, first, count;
+};
+__device__ __forceinline__ UnitRange units_in(const Line& ln, const PlaceUnits& it, int off, int left) {
+  UnitRange r;
+  r.part = min(weight_of(ln, it.units, it.cost) - off, left);
+  const auto up = [&](int x) { return it.cost == 1 ? x : it.cost == kManyCost ? (x + kManyCost - 1) / kManyCost : (x + kFewCost - 1) / kFewCost; };
+  r.first = up(off);
+  r.count = min(it.units, up(off + r.part)) - r.first;
+  return r;
 }
 
 // Writes a line's schedule down for the merge: the shared units, a head's and a worker's part, and
@@ -268,10 +308,10 @@ struct RowAt {
   int b, i, h;
 };
 __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) {
-  const int bi = r / p.group;
+  const int bi = quotient(r, p.group_div);
   RowAt a;
   a.h = head * p.group + (r - bi * p.group);
-  a.b = bi / p.rows;
+  a.b = quotient(bi, p.rows_div);
   a.i = bi - a.b * p.rows;
   return a;
 }
@@ -284,10 +324,11 @@ struct Sight {
   int base, count;
   const uint32_t* mask;
   bool hidden;
+  uint32_t word0;  // the mask's first word, as the bits after it mostly are none
   __device__ __forceinline__ uint32_t word(int w) const {
     const int rest = count - 32 * w;
     if (w < 0 || rest <= 0) return 0u;
-    const uint32_t bits = __ldg(mask + w);
+    const uint32_t bits = w == 0 ? word0 : __ldg(mask + w);
     return rest >= 32 ? bits : bits & ((1u << rest) - 1u);
   }
   // bit j: whether it sees key + j
@@ -301,8 +342,9 @@ struct Sight {
 __device__ __forceinline__ Sight sight_of(const TreeParams& p, const RowAt& ra, bool shared) {
   const Extent x = extent_of(p, ra.b);
   const int count = x.all - x.clean;
-  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, nullptr, true};
-  return Sight{x.clean, count, p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words, false};
+  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, nullptr, true, 0u};
+  const uint32_t* const mask = p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words;
+  return Sight{x.clean, count, mask, false, __ldg(mask)};
 }
 
 // Of a chain, only a limit.

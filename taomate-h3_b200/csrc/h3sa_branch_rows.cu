@@ -193,25 +193,25 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       return g;
     }
     while (u < u_end && g.units == 0) {
-      const int units = place_units(p, ln, pl, at), part = min(weight_of(ln, units) - at.off, u_end - u);
-      const int n = min(units, at.off + part) - at.off;
-      if (n > 0) {
-        g.units = n;
+      const PlaceUnits it = place_units(p, ln, pl, at);
+      const UnitRange in = units_in(ln, it, at.off, u_end - u);
+      if (in.count > 0) {
+        g.units = in.count;
         g.head = at.head;
         g.shared = at.b < 0;
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
         const Extent x = extent_of(p, g.seq);
         g.n_rows = min(kRowSpan, g.shared ? p.batch * own_all - g.row0 : x.rows - at.t * kRowSpan);
-        g.key0 = (g.shared ? 0 : own_lo(p, x)) + at.off * kRowUnit;
+        g.key0 = (g.shared ? 0 : own_lo(p, x)) + in.first * kRowUnit;
         g.kv_end = x.all;
         g.clean = x.clean;
-        g.direct = pl.shared_blocks == 0 && n == units;
+        g.direct = pl.shared_blocks == 0 && in.count == it.units;
         const long long item = g.shared ? static_cast<long long>(at.head) * ln.shared_tiles + at.t
                                         : (static_cast<long long>(at.head) * p.batch + at.b) * ln.own_tiles + at.t;
         g.slot = (g.shared ? 0 : p.own_row0) + (item + worker) * (g.shared ? p.shared_slot_rows : p.own_slot_rows);
       }
-      u += part;
+      u += in.part;
       if (u < u_end) step_item(p, ln, pl, at);
     }
     return g;

@@ -23,6 +23,7 @@
 #include <cstring>
 #include <type_traits>
 
+#include "h3sa_div.cuh"
 #include "h3sa_fp8.cuh"
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
@@ -35,24 +36,6 @@ constexpr int kDim = 128;  // head dimension of a cache
 constexpr int kThreads = 128;
 constexpr int kMaxDim = 1024;
 constexpr int kSms = 148;
-
-// x / d for x below 2^31 by one multiplication: m = ceil(2^(32 + s) / d) with 2^s >= d (Granlund and
-// Montgomery's division by invariant integers; m needs 33 bits, of which the first is a plain add).
-struct Divisor {
-  uint32_t d, m, s;
-};
-Divisor divisor(uint32_t d) {
-  Divisor v;
-  v.d = d;
-  v.s = 0;
-  while ((1ull << v.s) < d) ++v.s;
-  v.m = static_cast<uint32_t>(((((1ull << v.s) - d) << 32) / d) + 1);
-  return v;
-}
-__device__ __forceinline__ uint32_t quotient(uint32_t x, const Divisor& v) {
-  const uint32_t hi = __umulhi(x, v.m);
-  return (hi + x) >> v.s;  // x below 2^31: the sum stays below 2^32
-}
 
 enum PositionKind : int { kPosNone = 0, kPosI32 = 1, kPosI64 = 2, kPosF64 = 3 };
 

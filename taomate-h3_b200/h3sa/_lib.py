@@ -195,6 +195,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         ctypes.c_int,
         [ctypes.POINTER(Heads), ctypes.POINTER(Heads), ctypes.POINTER(Heads), ctypes.POINTER(Heads), _I, _I, _P, _P, _I,
          _I, _P, _P, _P, _I, _P, _P, ctypes.POINTER(RotaryPositions), _P, _P]),
+    "h3sa_tree_workspace": (_L, [_I, _I, _I, _I, _I, _I, _I]),
     "h3sa_tree_attention": (
         ctypes.c_int,
         [_P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _F, _P, _L, _P, _P]),

@@ -39,7 +39,7 @@ PoolTensors = Union[torch.Tensor, Sequence[torch.Tensor]]
 # points are bound once, conditions are tested inline and messages built only on failure.
 _FORK, _COMPACT, _FREE = LIB.h3sa_fork_pages, LIB.h3sa_compact_pages, LIB.h3sa_free_pages
 _ATTEND, _ATTEND_WORK = LIB.h3sa_shared_prefix_attention, LIB.h3sa_shared_prefix_workspace
-_ATTEND_TREE = LIB.h3sa_tree_attention
+_ATTEND_TREE, _TREE_WORK = LIB.h3sa_tree_attention, LIB.h3sa_tree_workspace
 _PAGES_WORK = LIB.h3sa_pages_workspace
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _I32, _F32, _BF16, _E4M3 = torch.int32, torch.float32, torch.bfloat16, torch.float8_e4m3fn
@@ -297,7 +297,8 @@ def _attend(what: str, masks: torch.Tensor | None, counts: int | None, query: to
         raise RuntimeError(f"{what}: {shared_rows} shared rows are not whole pages of a table of {width} "
                            "entries")
     error = _error_word(what, device, device_error)
-    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows))
+    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows) if masks is None else
+               _TREE_WORK(batch, rows, heads, kv_heads, shared_rows, width, 1 if e4m3 else 0))
     if out is not None and _bad(out, device, _BF16, query.shape):
         _refuse(what, "out", device, _BF16, query.shape)
     with _on(stream):
