@@ -56,6 +56,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstddef>
 #include <cstring>
 #include <mutex>
 
@@ -105,7 +106,7 @@ constexpr int kWideTile = 2 * kAtom;
 template <bool kFp8>
 struct BrWide {};
 template <>
-struct alignas(1024) BrWide<true> {
+struct BrWide<true> {  // begins at a multiple of 1024 bytes, as the tiles in front of it are multiples
   uint8_t v[kWide][kWideTile];
   uint64_t full[2][kWide], empty[2][kWide];
 };
@@ -114,7 +115,8 @@ template <class P>
 struct BrTree {};
 template <>
 struct BrTree<TreeParams> {
-  int taken_out;  // whether a node's V held an infinity or NaN
+  int taken_out;          // whether a node's V held an infinity or NaN
+  int before[kMaxStack];  // see live_row_at
 };
 
 template <bool kFp8, class P>
@@ -137,6 +139,8 @@ template <bool kFp8, class P>
 constexpr size_t br_smem_bytes() {
   return sizeof(BrSmem<kFp8, P>) + 1024;
 }
+using BrSmemTreeF8 = BrSmem<true, TreeParams>;
+static_assert(offsetof(BrSmemTreeF8, wide) % 1024 == 0, "widened V must be aligned to its swizzle");
 static_assert(br_smem_bytes<false, TreeParams>() <= 232448 && br_smem_bytes<true, TreeParams>() <= 232448,
               "branch attention needs more than 227 KB");
 
@@ -444,7 +448,12 @@ __global__ void __launch_bounds__(kBrThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Plan pl;
   const Line& ln = p.tensor;
-  if (warp == 0) pl = make_plan(p, ln, lane);  // under way while the others set up
+  if (warp == 0) {  // under way while the others set up
+    pl = make_plan(p, ln, lane);
+    if constexpr (kTree) {
+      if (p.compact && ln.shared_tiles > 0) stack_rows(p, sm.tree.before, lane);
+    }
+  }
   if (threadIdx.x == 64) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
@@ -556,7 +565,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (at.b < 0) {
             seq = pl.longest;
             g.row0 = at.t * kSpan;
-            g.n_rows = min(kSpan, p.batch * p.rows * p.group - g.row0);
+            g.n_rows = min(kSpan, pl.live - g.row0);
             g.block0 = in.first;
             g.kv_end = g.clean = pl.shared_blocks * kBlk;
             item = at.head * ln.shared_tiles + at.t;
@@ -874,7 +883,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         it.direct = g.direct;
         it.shared = g.live == 2;
         const int my = lr & (it.span - 1);
-        it.at = row_at(p, g.head, it.row0 + min(my, it.n_rows - 1));
+        const int row = it.row0 + min(my, it.n_rows - 1);
+        if constexpr (kTree) it.at = it.shared && p.compact ? live_row_at(p, sm.tree.before, g.head, row) : row_at(p, g.head, row);
+        else it.at = row_at(p, g.head, row);
         const uint4* src = reinterpret_cast<const uint4*>(p.q + it.at.b * p.q_sb + it.at.i * p.q_sn + it.at.h * p.q_sh);
 #pragma unroll
         for (int c = 0; c < 16; ++c) qv[c] = my < it.n_rows ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
@@ -1232,12 +1243,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   const bool shared_by_warps = p.warp.shared_tiles > 0, own_by_warps = !kJoint && p.warp.own_tiles > 0;
   const Line& ls = shared_by_warps ? p.warp : p.tensor;
   const Line& lo = own_by_warps ? p.warp : p.tensor;
-  const int* const ps = p.plan + (shared_by_warps ? 3 + p.batch : 0);
-  const int* const po = p.plan + (own_by_warps ? 3 + p.batch : 0);
+  const int line = kPlanHead + 2 * p.batch;
+  const int* const ps = p.plan + (shared_by_warps ? line : 0);
+  const int* const po = p.plan + (own_by_warps ? line : 0);
   const int shared_blocks = kJoint ? 0 : __ldcg(po);
-  const int cut_s = __ldcg(ps + 2), cut_o = __ldcg(po + 2);
-  const int shared_units = shared_blocks * over_pow2(kBlk, ls.unit), cost_s = shared_cost(p, ls);
+  const int cut_s = __ldcg(ps + 2), cut_o = __ldcg(po + 2), live = __ldcg(ps + 3);
+  const int shared_units = shared_blocks * over_pow2(kBlk, ls.unit), cost_s = cost_of(p, ls, live);
   const int shared_weight = weight_of(ls, shared_units, cost_s);
+  bool compact = false;
+  if constexpr (is_tree<P>) compact = p.compact != 0;
   const int own_all = p.rows * p.group;
   // split form: stacked rows of all branches, one a team, head by head; joint form: kRows rows of
   // an item a warp
@@ -1270,8 +1284,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
         make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
     if (p.lse && lane == 0) p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
   };
-  int u0 = head * __ldcg(po + 1) + lo.shared_tiles * weight_of(lo, shared_blocks * over_pow2(kBlk, lo.unit), shared_cost(p, lo)) +
-           __ldcg(po + 3 + b);
+  int u0 = head * __ldcg(po + 1) + (ps == po ? live_tiles(p, ls, live) * shared_weight : 0) + __ldcg(po + kPlanHead + b);
   for (int k = 0; k < t; ++k) u0 += own_weight(p, lo, ext, k);
   const int units = own_units(p, lo, ext, t), cost_o = own_cost(p, lo, ext, t);
   const int n_rows = min(lo.span, ext.rows - t * lo.span), last = min(own_all, (t + 1) * lo.span);
@@ -1287,9 +1300,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   for (int k = 0; k < kRows; ++k) {
     // rows past the item (and behind the nodes) read its last row again, and what they read is not written
     const int rk = min(r + k, t * lo.span + max(n_rows, 1) - 1);
-    const int row = b * own_all + rk, t_sh = over_pow2(row, ls.span);
-    sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, shared_units, cost_s,
-                      min(ls.span, p.batch * own_all - t_sh * ls.span), row & (ls.span - 1),
+    const int row = (compact ? __ldcg(ps + kPlanHead + p.batch + b) : b * own_all) + rk, t_sh = over_pow2(row, ls.span);
+    sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, compact && (rk >= ext.rows || !takes_shared(p, ext)) ? 0 : shared_units,
+                      cost_s,
+                      min(ls.span, live - t_sh * ls.span), row & (ls.span - 1),
                       head * ls.shared_tiles + t_sh, 0, p.shared_slot_rows, shared_by_warps);
     own[k] = pieces_of(cut_o, u0, units, cost_o, n_rows, rk - t * lo.span,
                        (static_cast<long long>(head) * p.batch + b) * lo.own_tiles + t, p.own_row0,
@@ -1461,7 +1475,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, int wid
   }
   s.rows = s.own_row0 +
            (static_cast<long long>(kv_heads) * batch * lo.own_tiles + lo.workers) * own_slots * s.own_slot_rows;
-  s.bytes = s.rows * (kD * 4 + 8) + 2 * (3ll + batch) * 4;
+  s.bytes = s.rows * (kD * 4 + 8) + 2 * (kPlanHead + 2ll * batch) * 4;
   return s;
 }
 
@@ -1643,6 +1657,7 @@ int attend(const char* what, const TreeParams* nodes, const void* query, int64_t
     p.masks = nodes->masks;
     p.counts = nodes->counts;
     p.words = (rows + 31) / 32;
+    p.compact = p.shared_keys > 0 && batch <= kMaxStack ? 1 : 0;
     return e4m3 ? launch<true, TreeParams>(p, s0) : launch<false, TreeParams>(p, s0);
   }
   return e4m3 ? launch<true, BranchParams>(p, s0) : launch<false, BranchParams>(p, s0);

@@ -73,7 +73,12 @@ struct TreeParams : BranchParams {
   const uint32_t* masks;  // [batch, rows, words]: bit n of row i: node n is node i or above it
   const int* counts;      // [batch] nodes, or null: `rows` of each
   int words;
+  int compact;            // shared items are stacked of rows that there are (up to kMaxStack sequences)
 };
+constexpr int kMaxStack = 256;
+// Header of a line's schedule as the merge reads it; own offsets [batch] and, of the line with the shared items, the
+// stacked rows in front of each sequence [batch] follow.
+constexpr int kPlanHead = 4;
 template <class P>
 constexpr bool is_tree = std::is_same_v<P, TreeParams>;
 
@@ -123,8 +128,6 @@ __device__ __forceinline__ int cost_of(const P&, const Line& ln, int rows) {
   return is_tree<P> ? (rows > kBlk ? ln.many : ln.few) : 1;
 }
 template <class P>
-__device__ __forceinline__ int shared_cost(const P& p, const Line& ln) { return cost_of(p, ln, p.batch * p.rows * p.group); }
-template <class P>
 __device__ __forceinline__ int own_cost(const P& p, const Line& ln, const Extent& x, int t) { return cost_of(p, ln, x.rows - t * ln.span); }
 __device__ __forceinline__ int weight_of(const Line& ln, int units, int cost) { return units > 0 ? units * cost + ln.pad : 0; }
 template <class P>
@@ -143,9 +146,24 @@ __device__ __forceinline__ int own_weight_all(const P& p, const Line& ln, const 
   return n;
 }
 
+// Rows of a sequence among those stacked for the shared items.
+template <class P>
+__device__ __forceinline__ int stacked_of(const P& p, const Extent& x) {
+  if constexpr (is_tree<P>) return p.compact ? (takes_shared(p, x) ? x.rows : 0) : p.rows * p.group;
+  return p.rows * p.group;
+}
+template <class P>
+__device__ __forceinline__ int live_tiles(const P&, const Line& ln, int live) {
+  if constexpr (is_tree<P>) return min(ln.shared_tiles, over_pow2(live + ln.span - 1, ln.span));
+  return ln.shared_tiles;
+}
+
 struct Plan {
   int shared_blocks;  // of the shared items: 0 if no sequence has all of them
   int shared_units;   // units of one shared item
+  int live;           // stacked rows
+  int shared_tiles;   // shared items a KV head
+  int shared_weight;  // of one of them
   int head_weight;    // one KV head's part of the line
   int cut;            // one worker's part
   int longest;        // sequence whose table row gives the shared pages
@@ -153,23 +171,29 @@ struct Plan {
 
 template <class P>
 __device__ __forceinline__ Plan make_plan(const P& p, const Line& ln, int lane) {
-  int own = 0, best = -1, at = 0;
+  int own = 0, best = -1, at = 0, live = 0;
   for (int b = lane; b < p.batch; b += 32) {
     const Extent x = extent_of(p, b);
     own += own_weight_all(p, ln, x);
+    live += stacked_of(p, x);
     if (x.clean > best) {
       best = x.clean;
       at = b;
     }
   }
   own = __reduce_add_sync(0xffffffffu, own);
+  if constexpr (is_tree<P>) live = __reduce_add_sync(0xffffffffu, live);
+  else live = p.batch * p.rows * p.group;
   const int top = __reduce_max_sync(0xffffffffu, best);
   at = __reduce_min_sync(0xffffffffu, best == top ? at : INT_MAX);
   Plan pl;
   pl.longest = at;
   pl.shared_blocks = own_lo(p, Extent{top, top, 0}) / kBlk;
   pl.shared_units = pl.shared_blocks * over_pow2(kBlk, ln.unit);
-  pl.head_weight = ln.shared_tiles * weight_of(ln, pl.shared_units, shared_cost(p, ln)) + own;
+  pl.live = live;
+  pl.shared_tiles = live_tiles(p, ln, live);
+  pl.shared_weight = weight_of(ln, pl.shared_units, cost_of(p, ln, live));
+  pl.head_weight = pl.shared_tiles * pl.shared_weight + own;
   const int all = pl.head_weight * p.kv_heads;
   pl.cut = max(ln.least, (all + ln.workers - 1) / ln.workers);
   return pl;
@@ -189,13 +213,13 @@ __device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& 
   at.b = -1;
   at.t = 0;
   int x = u - at.head * pl.head_weight;
-  const int w = weight_of(ln, pl.shared_units, shared_cost(p, ln));
-  if (x < ln.shared_tiles * w) {
+  const int w = pl.shared_weight;
+  if (x < pl.shared_tiles * w) {
     at.t = x / w;
     at.off = x - at.t * w;
     return at;
   }
-  x -= ln.shared_tiles * w;
+  x -= pl.shared_tiles * w;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
     const int n = b < p.batch ? own_weight_all(p, ln, extent_of(p, b)) : 0;
@@ -223,10 +247,10 @@ __device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& 
 // To the next item that has units; there must be one.
 template <class P>
 __device__ __forceinline__ void step_item(const P& p, const Line& ln, const Plan& pl, Place& at) {
-  const bool shared = ln.shared_tiles > 0 && pl.shared_units > 0;
+  const bool shared = pl.shared_tiles > 0 && pl.shared_units > 0;
   at.off = 0;
   if (at.b < 0) {
-    if (++at.t < ln.shared_tiles) return;
+    if (++at.t < pl.shared_tiles) return;
     at.b = 0;
     at.t = -1;
   }
@@ -248,7 +272,7 @@ struct PlaceUnits {
 };
 template <class P>
 __device__ __forceinline__ PlaceUnits place_units(const P& p, const Line& ln, const Plan& pl, const Place& at) {
-  if (at.b < 0) return PlaceUnits{pl.shared_units, shared_cost(p, ln)};
+  if (at.b < 0) return PlaceUnits{pl.shared_units, cost_of(p, ln, pl.live)};
   const Extent x = extent_of(p, at.b);
   return PlaceUnits{own_units(p, ln, x, at.t), own_cost(p, ln, x, at.t)};
 }
@@ -265,7 +289,23 @@ __device__ __forceinline__ UnitRange units_in(const Line& ln, const PlaceUnits& 
   return r;
 }
 
-// Writes a line's schedule down for the merge: the shared units, a head's and a worker's part, and
+// Stacked rows in front of each sequence's (warp-collective).
+__device__ __forceinline__ void stack_rows(const TreeParams& p, int* before, int lane) {
+  int sum = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const int b = b0 + lane, n = b < p.batch ? stacked_of(p, extent_of(p, b)) : 0;
+    int cum = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, cum, d);
+      if (lane >= d) cum += v;
+    }
+    if (b < p.batch) before[b] = sum + cum - n;
+    sum += __shfl_sync(0xffffffffu, cum, 31);
+  }
+}
+
+// Writes a line's schedule down for the merge: the shared units, a head's and a worker's part, the stacked rows, and
 // what lies in front of each sequence's own items.
 template <class P>
 __device__ __forceinline__ void write_plan(const P& p, const Line& ln, const Plan& pl, int* out, int lane) {
@@ -273,6 +313,10 @@ __device__ __forceinline__ void write_plan(const P& p, const Line& ln, const Pla
     out[0] = pl.shared_blocks;
     out[1] = pl.head_weight;
     out[2] = pl.cut;
+    out[3] = pl.live;
+  }
+  if constexpr (is_tree<P>) {
+    if (p.compact && ln.shared_tiles > 0) stack_rows(p, out + kPlanHead + p.batch, lane);
   }
   int before = 0;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
@@ -284,7 +328,7 @@ __device__ __forceinline__ void write_plan(const P& p, const Line& ln, const Pla
       const int v = __shfl_up_sync(0xffffffffu, cum, d);
       if (lane >= d) cum += v;
     }
-    if (b < p.batch) out[3 + b] = before + cum - n;
+    if (b < p.batch) out[kPlanHead + b] = before + cum - n;
     before += __shfl_sync(0xffffffffu, cum, 31);
   }
 }
@@ -345,6 +389,23 @@ __device__ __forceinline__ Sight sight_of(const TreeParams& p, const RowAt& ra, 
   if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, nullptr, true, 0u};
   const uint32_t* const mask = p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words;
   return Sight{x.clean, count, mask, false, __ldg(mask)};
+}
+
+// The r-th of the rows that there are, from what lies in front of each sequence's: it is in the last one that
+// begins at or before it.
+__device__ __forceinline__ RowAt live_row_at(const TreeParams& p, const int* before, int head, int r) {
+  int lo = 0, hi = p.batch;  // before[lo] <= r < before[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (before[mid] <= r) lo = mid;
+    else hi = mid;
+  }
+  r -= before[lo];
+  RowAt a;
+  a.b = lo;
+  a.i = quotient(r, p.group_div);
+  a.h = head * p.group + r - a.i * p.group;
+  return a;
 }
 
 // Of a chain, only a limit.

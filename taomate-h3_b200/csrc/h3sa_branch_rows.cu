@@ -125,6 +125,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[kRowWarps][kMaxRowStages], empty[kRowWarps][kMaxRowStages];
   __shared__ int abort_word;
+  __shared__ int before[kTree ? kMaxStack : 1];  // see live_row_at
   volatile int* abort_flag = &abort_word;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = (threadIdx.x >> 5) & (kRowWarps - 1), lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -154,6 +155,9 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     u_end = p.kv_heads * p.batch * ln.own_tiles;
   } else {
     pl = make_plan(p, ln, lane);
+    if constexpr (kTree) {
+      if (p.compact && ln.shared_tiles > 0 && threadIdx.x < 32) stack_rows(p, before, lane);
+    }
     const int all = pl.head_weight * p.kv_heads;
     u = min(all, worker * pl.cut);
     u_end = min(all, u + pl.cut);
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         g.seq = g.shared ? pl.longest : at.b;
         g.row0 = (g.shared ? 0 : at.b * own_all) + at.t * kRowSpan;
         const Extent x = extent_of(p, g.seq);
-        g.n_rows = min(kRowSpan, g.shared ? p.batch * own_all - g.row0 : x.rows - at.t * kRowSpan);
+        g.n_rows = min(kRowSpan, g.shared ? pl.live - g.row0 : x.rows - at.t * kRowSpan);
         g.key0 = (g.shared ? 0 : own_lo(p, x)) + in.first * kRowUnit;
         g.kv_end = x.all;
         g.clean = x.clean;
@@ -284,8 +288,14 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
   // ================================================================ products and softmax
   for (RowSegment g = next_segment(); g.units > 0; g = next_segment()) {
     // this lane's rows, r and r + 8 of the item
-    const RowAt at0 = row_at(p, g.head, g.row0 + min(r, g.n_rows - 1));
-    const RowAt at1 = row_at(p, g.head, g.row0 + min(r + 8, g.n_rows - 1));
+    const auto at_row = [&](int k) {
+      const int row = g.row0 + min(k, g.n_rows - 1);
+      if constexpr (kTree) {
+        if (g.shared && p.compact) return live_row_at(p, before, g.head, row);
+      }
+      return row_at(p, g.head, row);
+    };
+    const RowAt at0 = at_row(r), at1 = at_row(r + 8);
     uint32_t qa[16], qb[16];
     {
       const __nv_bfloat16* a = p.q + at0.b * p.q_sb + at0.i * p.q_sn + at0.h * p.q_sh;
@@ -530,7 +540,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
   }
   if (worker == 0) {
     flag_lengths(p, lane);
-    if constexpr (!kWhole) write_plan(p, ln, pl, p.plan + 3 + p.batch, lane);
+    if constexpr (!kWhole) write_plan(p, ln, pl, p.plan + kPlanHead + 2 * p.batch, lane);
   }
   // what follows this kernel needs the other line's too; one block's wait holds it, and the others make
   // room for it
