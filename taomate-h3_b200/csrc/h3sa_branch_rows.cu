@@ -428,6 +428,27 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
         l1 += s[j][2] + s[j][3];
       }
       const bool tail = key + 32 > g.kv_end;
+      if constexpr (kTree) {
+        if (key + 32 > g.clean) {  // the unit has nodes
+          bool met = false;
+          for (int i = lane; i < kTileBytes / 16; i += 32) {  // 16 bytes of a row
+            const int row = (i >> 3) & 31;
+            if (key + row < g.clean || key + row >= g.kv_end) continue;
+            const uint32_t at = vt + (i >> 8) * (kTileBytes / 2) + row * 128 + (i & 7) * 16;
+            uint4 v = lds16(at);
+            if (take_out<kFp8>(v)) {
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                           : "memory");
+              met = true;
+            }
+          }
+          if (__any_sync(0xffffffffu, met)) {
+            taken_out = true;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the stage is filled again by TMA
+          }
+          __syncwarp();
+        }
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // sixteen keys
         uint4 a, rest;
@@ -445,9 +466,6 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
             v[k] = lds16(vt + atom * (kTileBytes / 2) + row * 128 + ((r ^ (row & 7)) << 4));
             // values past the sequence's end may be anything, NaN too, and P's zeros do not undo that
             if (tail && key + row >= g.kv_end) v[k] = make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (kTree) {
-              if (key + row >= g.clean) taken_out |= take_out<kFp8>(v[k]);
-            }
           }
           const uint32_t x[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, y[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
           const uint32_t z[4] = {v[2].x, v[2].y, v[2].z, v[2].w}, t[4] = {v[3].x, v[3].y, v[3].z, v[3].w};
