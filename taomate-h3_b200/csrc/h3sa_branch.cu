@@ -1419,20 +1419,19 @@ constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 // heads over 1024 keys: 2 units 11.3, 4 units 12.2, 6 units 13.2.
 constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 
-// Trees of more than 16 stacked rows. The warp line reads a tree's keys once for every 16 rows and the tensor line
-// starts some 8 us later (17 in e4m3, which it widens), so what decides is the keys, of which the host knows the
-// tables' width. us a million keys and KV heads: warps 50 for each 16 rows (e4m3 40), tensor cores 81 (88) an item. 8 KV
-// heads, warp / tensor (us): 64 rows, 24 trees of up to 300 keys 33 / 39, 1000 59 / 48, 16000 424 / 186; 48 rows,
-// 1000 47 / 43; 32 rows, 1000 35 / 42, 4000 72 / 70, 16000 232 / 178; one tree of 48 rows over 60000 130 / 76; e4m3: 64
-// rows, 1000 53 / 63, 4000 114 / 104; 48 rows, 4000 85 / 102, 16000 229 / 213; 32 rows, 16000 179 / 199. With shared keys (20 trees of 52 rows over
-// 1024 and up to 700 of their own 73 / 50) both parts are in one kernel.
+// Trees of 17 to 64 stacked rows. The warp line reads a tree's keys once for every 16 rows, the tensor line once, but starts
+// some 12 us later (17 in e4m3, which it widens), so what decides is the keys, of which the host knows the tables'
+// width. us a million keys and KV heads: warps 44 for each 16 rows (e4m3 35), tensor cores 89 (95) an item. 8 KV
+// heads, bf16, warp / tensor (us): 64 rows, 24 trees of up to 1000 keys 52 / 60, 4000 112 / 88, 16000 373 / 203; 48 rows,
+// 1000 41 / 54, 16000 268 / 178; one tree of 64 rows over up to 60000 144 / 75; e4m3: 64 rows, 4000 100 / 124, 16000 295 / 242. With shared
+// keys (20 trees of 52 rows over 1024 and up to 700 of their own 73 / 55) both parts are in one kernel.
 bool tree_on_tensor(int batch, int own, int kv_heads, int shared, int width, bool e4m3) {
   if (own <= kRowSpan) return false;
   const auto tiles = [](long long n, int span) { return (n + span - 1) / span; };
   const long long keys = static_cast<long long>(batch) * (width - shared) * kBlk, all = static_cast<long long>(batch) * own;
   const double warps = static_cast<double>(kv_heads) * (keys * tiles(own, kRowSpan) + 1.0 * shared * kBlk * tiles(all, kRowSpan));
   const double tensor = static_cast<double>(kv_heads) * (keys + 1.4 * shared * kBlk * tiles(all, kSpan));
-  return e4m3 ? warps - 2.2 * tensor > 680000.0 : warps - 1.62 * tensor > 256000.0;
+  return e4m3 ? warps - 2.6 * tensor > 1150000.0 : warps - 1.7 * tensor > 570000.0;
 }
 
 // The shape of a tree's call has the tables' width, a chain's 0.

@@ -542,3 +542,190 @@ def test_keep_refuses_bad_paths_on_the_device() -> None:
         only[0] = -1  # the other sequence's path is kept
         want = od.keep(pools, np.array(table), np.array([0, 200]), only)
         assert torch.equal(dev.cpu(), want[0]) and kept.tolist() == [lengths[0], 202]
+
+
+# ------------------------------------------------------------------------------------ more of each
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("lengths,counts,heads,kv,shared,nodes", [
+    ([200] * 300, [1, 2, 0] * 100, 2, 1, 1, 2),                     # more sequences than are stacked by live rows
+    ([400] * 90, [0, 1, 0, 2, 0, 0] * 15, 4, 2, 3, 2),              # most of them without a node
+    ([700] * 9, [0] * 9, 4, 2, 5, 3),                               # none has a node
+    ([1300] * 12, [30, 0, 7, 31, 1, 30, 2, 0, 0, 29, 31, 0], 4, 1, 10, 31),  # tiles that end inside sequences
+    ([640, 639, 641, 0, 650], [20, 20, 1, 0, 20], 4, 1, 5, 20),     # one that ends a row in front of the shared pages' end
+])
+def test_stacked_rows_are_those_that_there_are(lengths, counts, heads, kv, shared, nodes, kind) -> None:
+    _attend(lengths, counts, heads, kv, shared=shared, kind=kind, nodes=nodes, seed=3)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("counts,heads", [([8, 5, 8, 3], 4), ([16, 9, 1, 16], 4), ([50, 64, 3, 33], 4)])
+def test_long_tables_take_the_tensor_cores(counts, heads, kind) -> None:
+    """Tables wide enough that trees of more than 16 rows leave the warp line, with little in them."""
+
+    from h3sa.drafts import tree_attention
+
+    rng, gen = np.random.default_rng(8), torch.Generator().manual_seed(8)
+    lengths, counts, nodes = np.array([300, 1000, 0, 1]), np.array(counts), max(counts)
+    table, pages = _table(rng, lengths + counts)
+    wide = np.full((4, 8000), -1)
+    wide[:, :table.shape[1]] = table
+    (k, ks), (v, vs) = _pool(gen, 2, pages, kind), _pool(gen, 2, pages, kind)
+    sees = od.ancestors(_trees(rng, 4, nodes), counts)
+    q = torch.randn(4, nodes, 2 * heads, 128, generator=gen).bfloat16()
+    want, _, spread, peak = od.attention(q, k, v, table, lengths, counts, sees, SCALE, ks, vs)
+    scales = {} if ks is None else dict(k_scale=ks.cuda(), v_scale=vs.cuda())
+    err = _error()
+    out = tree_attention(q.cuda(), k.cuda(), v.cuda(), _dev(wide), _dev(lengths), _dev(od.words(sees)), SCALE, counts=_dev(counts),
+                         device_error=err, **scales)
+    tol = (2.0 ** -7 + 2.0 ** -12) * spread if kind == "bf16" else (2.0 ** -8 + 2.0 ** -9) * spread + 2.0 ** -30 * peak
+    assert int(err) == 0 and ((out.double().cpu() - want).abs() <= tol).all()
+
+
+def test_garbage_in_unused_rows_of_the_query_stays_there() -> None:
+    """Queries behind the counts may hold anything."""
+
+    from h3sa.drafts import tree_attention
+
+    rng, gen = np.random.default_rng(9), torch.Generator().manual_seed(9)
+    for nodes, shared in ((9, 0), (20, 0), (70, 0), (20, 2)):
+        lengths, counts = np.array([400, 300, 0]), np.array([nodes - 3, nodes, 0])
+        table, pages = _table(rng, lengths + counts, shared)
+        k, v = _pool(gen, 2, pages, "bf16")[0].cuda(), _pool(gen, 2, pages, "bf16")[0].cuda()
+        masks = _dev(od.words(od.ancestors(_trees(rng, 3, nodes), counts)))
+        q = torch.randn(3, nodes, 4, 128, generator=gen).bfloat16().cuda()
+        run = lambda q: tree_attention(q, k, v, _dev(table), _dev(lengths), masks, SCALE, counts=_dev(counts), shared_rows=128 * shared)  # noqa: E731
+        want = run(q)
+        for b, n in enumerate(counts):
+            q[b, n:] = torch.tensor([float("nan"), float("inf"), -3.0e38, -float("inf")]).bfloat16().repeat(32).cuda()
+        assert torch.equal(run(q), want)
+
+
+def test_offsets_past_32_bits() -> None:
+    """Pools of more than 2^31 elements: rows of the last page are appended, attended to and kept."""
+
+    from h3sa.drafts import append_rows, keep_rows, tree_attention
+
+    gen = torch.Generator().manual_seed(10)
+    pages = 66000
+    pools = torch.empty(2, 2, pages * 128, 128, dtype=torch.bfloat16, device="cuda")
+    small = torch.empty(2, 2, 2 * 128, 128, dtype=torch.bfloat16, device="cuda")
+    lengths, counts = _dev([120]), _dev([20])
+    key, value, query = (torch.randn(1, 20, 2, 128, generator=gen).bfloat16().cuda() for _ in range(3))
+    base = torch.randn(2, 2, 128, 128, generator=gen).bfloat16().cuda()
+    masks = _dev(od.words(np.tri(20, dtype=bool)[None]))
+    outs = []
+    for p, table in ((pools, [[pages - 1, pages - 2]]), (small, [[1, 0]])):
+        p[:, :, table[0][0] * 128:table[0][0] * 128 + 128] = base
+        err = _error()
+        append_rows(key, value, p[0], p[1], _dev(table), lengths, counts=counts, device_error=err)
+        out = tree_attention(query, p[0], p[1], _dev(table), lengths, masks, SCALE, counts=counts, device_error=err)
+        kept = keep_rows(p, _dev(table), lengths, _dev([[2, 7, 19]]), device_error=err)
+        assert int(err) == 0 and kept.tolist() == [123]
+        outs.append((out, p[:, :, table[0][0] * 128:table[0][0] * 128 + 128].clone(), p[:, :, table[0][1] * 128:table[0][1] * 128 + 12].clone()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_appends_in_two_graphs_and_on_another_stream() -> None:
+    from h3sa.drafts import append_rows, keep_rows
+    from h3sa.rotary import rotary_frequencies
+
+    gen = torch.Generator().manual_seed(11)
+    f = rotary_frequencies(128)[0].cuda()
+    key, query = (torch.randn(2, 7, 2, 128, generator=gen).bfloat16().cuda() for _ in range(2))
+    table, lengths, counts = _dev([[0, 1], [2, 3]]), _dev([100, 124]), _dev([7, 5])
+    path = _dev([[0, 3, 6], [1, -1, -1]])
+    pools = [torch.zeros(2, 2, 4 * 128, 128, device="cuda").bfloat16() for _ in range(3)]
+    outs = [torch.empty_like(query) for _ in range(2)]
+    kept = [None, None]
+
+    def step(p, out):
+        append_rows(key, key, p[0], p[1], table, lengths, counts=counts, frequencies=f, query=query, query_out=out)
+        return keep_rows(p, table, lengths, path)
+
+    step(pools[2], outs[0])
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            kept[i] = step(pools[i], outs[i])
+    lengths.copy_(_dev([3, 125]))
+    counts.copy_(_dev([7, 2]))
+    for p in pools:
+        p.zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs[0].replay()
+    with torch.cuda.stream(side):
+        graphs[1].replay()
+    out = append_rows(key, key, pools[2][0], pools[2][1], table, lengths, counts=counts, frequencies=f, query=query, stream=side)
+    last = keep_rows(pools[2], table, lengths, path, stream=side)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(pools[i], pools[2]) and torch.equal(outs[i], out) and torch.equal(kept[i], last)
+
+
+def test_wrappers_refuse() -> None:
+    from h3sa import drafts
+    from h3sa.rotary import rotary_frequencies, rotate
+
+    f = rotary_frequencies(128)[0].cuda()
+    key = torch.zeros(2, 3, 2, 128, device="cuda").bfloat16()
+    pool = torch.zeros(2, 2 * 128, 128, device="cuda").bfloat16()
+    table, lengths, masks = _dev([[0], [1]]), _dev([0, 0]), _dev(np.zeros((2, 3, 1)))
+
+    def append(match, *change, **kw):
+        args = dict(key=key, value=key, key_pool=pool, value_pool=pool, table=table, lengths=lengths)
+        args.update(dict(change), **kw)
+        with pytest.raises(RuntimeError, match=match):
+            drafts.append_rows(**args)
+
+    append("key must be bf16", key=key.float())
+    append("key must be bf16", key=key[0])
+    append("value must be", value=key[:, :2])
+    append("KV pools", key_pool=pool[:1])
+    append("KV pools", value_pool=pool.float())
+    append("bf16 or e4m3", key_pool=pool.float(), value_pool=pool.float())
+    append("take no scales", k_scale=lengths.float(), v_scale=lengths.float())
+    append("need k_scale", key_pool=pool.to(torch.float8_e4m3fn), value_pool=pool.to(torch.float8_e4m3fn))
+    append("table", table=table[0])
+    append("lengths", lengths=lengths.long())
+    append("counts", counts=lengths[:1])
+    append("frequencies", frequencies=f.float())
+    append("do not fit", frequencies=torch.cat((f, f)))
+    append("axes need positions", frequencies=f.view(2, 32))
+    append("positions must be", frequencies=f, positions=lengths)
+    append("positions must be contiguous", frequencies=f, positions=key[..., 0, 0].float())
+    append("query must be", query=key[:, :2])
+    append("query_out", query=key, query_out=key[:, :2])
+    append("without a query", query_out=key)
+    append("rows of key", key=key.transpose(2, 3).contiguous().transpose(2, 3))
+    append("int32 tensor", device_error=lengths.long())
+    append("require CUDA", key=key.cpu())
+    query = torch.zeros(2, 3, 4, 128, device="cuda").bfloat16()
+    for match, change in (("masks", dict(masks=masks[:, :, 0])), ("masks", dict(masks=masks.long())), ("query", dict(query=query[0])),
+                          ("counts", dict(counts=lengths[:1])), ("shared rows", dict(shared_rows=256)), ("shared rows", dict(shared_rows=64)),
+                          ("scale", dict(softmax_scale=0.0)), ("require CUDA", dict(query=query.cpu(), masks=masks.cpu()))):
+        args = dict(query=query, key_pool=pool, value_pool=pool, table=table, lengths=lengths, masks=masks, softmax_scale=0.1)
+        args.update(change)
+        with pytest.raises(RuntimeError, match=match):
+            drafts.tree_attention(**args)
+    for match, args in (("parents", (lengths, lengths)), ("parents", (masks[..., 0].long(), lengths)), ("lengths", (masks[..., 0], lengths[:1])),
+                        ("at most 1024", (_dev(np.zeros((1, 1025))), lengths[:1])), ("require CUDA", (masks[..., 0].cpu(), lengths.cpu()))):
+        with pytest.raises(RuntimeError, match=match):
+            drafts.draft_tree(*args)
+    for match, args in (("pool tensors", ([pool[0]], table, lengths, masks[..., 0])), ("no pool tensors", ([], table, lengths, masks[..., 0])),
+                        ("pool tensors", ([pool[:, :100]], table, lengths, masks[..., 0])), ("path", ([pool], table, lengths, lengths)),
+                        ("path", ([pool], table, lengths, masks[:1, :, 0])), ("lengths", ([pool], table, lengths.long(), masks[..., 0])),
+                        ("row bytes", (torch.zeros(1, 1, 128, 3, device="cuda"), table, lengths, masks[..., 0].contiguous()))):
+        with pytest.raises(RuntimeError, match=match):
+            drafts.keep_rows(*args)
+    x, at = torch.zeros(5, 2, 128, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    for match, args, kw in (("bf16, fp16 or fp32", (x.double(), at, f), {}), ("bf16, fp16 or fp32", (x[0], at, f), {}),
+                            ("positions", (x, at[:4], f), {}), ("positions", (x, at.float(), f), {}), ("do not fit", (x[..., :64], at, f), {}),
+                            ("positions", (x, at, f.view(2, 32)), {}), ("float64", (x, at, f.float()), {}), ("out must be", (x, at, f), dict(out=x.half())),
+                            ("contiguous", (x.transpose(1, 2).contiguous().transpose(1, 2), at, f), {}), ("finite", (x, at, f), dict(factor=float("inf"))),
+                            ("at most 1024", (torch.zeros(5, 1, 1026, device="cuda"), at, f), {}), ("require CUDA", (x.cpu(), at, f), {})):
+        with pytest.raises(RuntimeError, match=match):
+            rotate(*args, **kw)
