@@ -26,10 +26,13 @@
 //   warp 3      e4m3: widens V to f16.
 //   warps 4-7, 8-11: softmax and epilogue of query tile 0 and 1, one thread per TMEM lane.
 // An item of more than 128 rows takes both tiles, each block being used by both; smaller items
-// take one tile per block in turn, so two blocks are in flight. Items of up to 32 (64) rows are
-// held 4 (2) times, once per 32-lane (64-lane) part of the tile: each copy takes the exponentials
+// take one tile per block in turn, so two blocks are in flight. Items of up to 32 (64) rows of
+// chains are held 4 (2) times, once per 32-lane (64-lane) part of the tile: each copy takes the exponentials
 // of its own quarter (half) of the block's columns and writes zeros elsewhere, which spreads the
-// softmax of few rows over all four warps; the copies are joined in the epilogue.
+// softmax of few rows over all four warps; the copies are joined in the epilogue. Trees' rows are held once:
+// what bounds the kernel beside the softmax is its own code, streaming past the instruction caches, and the two other
+// forms in between cost trees more than they bring (wide e4m3 trees 237 -> 206 us without them, 64 rows over 16000
+// keys 203 -> 199, e4m3 239 -> 214).
 // TMEM columns: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P of a tile overwrites the
 // first half of its S. A tile's MMAs are issued in order by one warp, so the barrier of a QK^T also
 // says that the tile's previous P V is complete.
@@ -876,7 +879,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (!g.direct && lr < it.n_rows) p.part_ml[it.ws_row + lr] = make_float2(-INFINITY, 0.f);
           continue;
         }
-        it.span = g.n_rows > 64 ? 128 : it.n_rows <= 32 ? 32 : 64;
+        it.span = kTree || g.n_rows > 64 ? 128 : it.n_rows <= 32 ? 32 : 64;
         it.block0 = g.block0 + it.begin;
         it.head = g.head;
         it.row0 = g.row0 + r0;
@@ -897,7 +900,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     bool more = take(next);
     while (more) {
       const Item it = next;
-      const int span = it.span, n_rows = it.n_rows, copies = kBlk / span;
+      const int span = kTree ? kBlk : it.span, n_rows = it.n_rows, copies = kBlk / span;
       const int my = lr & (span - 1);  // this thread's row of the tile
       const int copy = lr / span;      // and which copy of it
       float sl2 = p.scale_log2 * store_query_row<kFp8>(sm.q[t], my, copy, copies, span, qv);
