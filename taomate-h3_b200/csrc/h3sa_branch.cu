@@ -206,6 +206,29 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
                                              float sl2, bool first, float& m, float& l, Wait&& pv_done) {
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
   const int col0 = 64 * half + copy * kCols;
+  // Columns at or past `limit` (relative to the block) are hidden from this row, but for nodes that it sees: -inf, of
+  // trees in TMEM before the scores are read, which keeps the tests out of the code of whole blocks.
+  const int limit = sight.base - key0;
+  int hide = __any_sync(0xffffffffu, limit < col0 + kCols) ? 1 : 0;
+  asm volatile("" : "+r"(hide));
+  if constexpr (std::is_same_v<S, Sight>) {
+    static_assert(kCols == 64, "rows of trees are held once");
+    if (hide) {
+#pragma unroll 1
+      for (int c = 0; c < 64; c += 32) {
+        uint32_t r[32];
+        tmem_ld32(tS + col0 + c, r);
+        const uint32_t seen = sight.seen32(key0 + col0 + c);
+        tmem_wait_ld();
+        reg_fence32(r);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (!(seen >> j & 1u)) r[j] = 0xff800000u;
+        tmem_st32(tS + col0 + c, r);
+      }
+      tmem_wait_st();
+    }
+  }
   float s[kCols];
   if constexpr (kCols >= 32) {
     uint32_t r[kCols / 32][32];
@@ -227,24 +250,10 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
 #pragma unroll
     for (int j = 0; j < 16; ++j) s[j] = __uint_as_float(r[j]);
   }
-  // columns at or past `limit` (relative to the block) are hidden from this row, but for nodes that it sees
-  const int limit = sight.base - key0;
-  int hide = __any_sync(0xffffffffu, limit < col0 + kCols) ? 1 : 0;
-  asm volatile("" : "+r"(hide));  // keeps the compares below out of whole blocks
-  if (hide) {
-    if constexpr (std::is_same_v<S, Sight>) {
+  if (!std::is_same_v<S, Sight> && hide) {
 #pragma unroll
-      for (int c = 0; c < kCols; c += 32) {
-        const uint32_t seen = sight.seen32(key0 + col0 + c);
-#pragma unroll
-        for (int j = 0; j < min(32, kCols); ++j)
-          if (!(seen >> j & 1u)) s[c + j] = -INFINITY;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < kCols; ++j)
-        if (col0 + j >= limit) s[j] = -INFINITY;
-    }
+    for (int j = 0; j < kCols; ++j)
+      if (col0 + j >= limit) s[j] = -INFINITY;
   }
   float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
 #pragma unroll
@@ -921,10 +930,14 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           const auto pv_done = [&]() {
             if (!first) ok = mbar_wait(smem_u32(&sm.pv_done[t]), h ^ 1, abort_flag, p.err);
           };
-          if (!warp_live) pv_done();
-          else if (span == 128) softmax_half<kFp8, 64>(tS, tO, h, 0, key0, sight, sl2, first, m, l, pv_done);
-          else if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
-          else softmax_half<kFp8, 16>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+          if (!warp_live) {
+            pv_done();
+          } else if (span == 128) {
+            softmax_half<kFp8, 64>(tS, tO, h, 0, key0, sight, sl2, first, m, l, pv_done);
+          } else if constexpr (!kTree) {
+            if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+            else softmax_half<kFp8, 16>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+          }
           tc_fence_before();
           mbar_arrive(smem_u32(&sm.p_full[t][h]));
         }
@@ -1128,7 +1141,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
               if (widen_block<true, true>(from, to, rows, clean, lane))
                 *static_cast<volatile int*>(&sm.tree.taken_out) = 1;
             }
-          } else if (rows >= kBlk) {
+          } else if (kTree || rows >= kBlk) {  // a tree's last rows are nodes
             widen_block<false, false>(from, to, kBlk, 0, lane);
           } else {
             widen_block<true, false>(from, to, rows, 0, lane);
