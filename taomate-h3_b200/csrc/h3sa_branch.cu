@@ -201,8 +201,8 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x2) {
 // P goes over the half's scores, zeros in the other copies' shares. key0: the block's first key, sight: of
 // this row. m / l: running maximum (log2 units) and sum; `pv_done` waits until O holds all earlier halves, before O is rescaled because
 // the maximum grew (lazily: only past the threshold).
-template <bool kFp8, int kCols, class S, typename Wait>
-__device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half, int copy, int key0, const S& sight,
+template <bool kFp8, int kCols, class P, class S, typename Wait>
+__device__ __forceinline__ void softmax_half(const P& p, uint32_t tS, uint32_t tO, int half, int copy, int key0, const S& sight,
                                              float sl2, bool first, float& m, float& l, Wait&& pv_done) {
   constexpr float kBoost = kFp8 ? kBoostF8 : 0.0f;
   const int col0 = 64 * half + copy * kCols;
@@ -218,7 +218,7 @@ __device__ __forceinline__ void softmax_half(uint32_t tS, uint32_t tO, int half,
       for (int c = 0; c < 64; c += 32) {
         uint32_t r[32];
         tmem_ld32(tS + col0 + c, r);
-        const uint32_t seen = sight.seen32(key0 + col0 + c);
+        const uint32_t seen = sight.seen32(p, key0 + col0 + c);
         tmem_wait_ld();
         reg_fence32(r);
 #pragma unroll
@@ -376,7 +376,7 @@ __device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows
   uint32_t met = 0u;
   const int c = lane & 7, h = c >> 2, at = 2 * (c & 3);
   const int r = (lane >> 4) + ((lane >> 1) & 4);  // rows r and r ^ 2 of eight; those of a half warp differ by 4
-#pragma unroll
+#pragma unroll 1  // for its code: 224 us instead of 156 for 24 trees of 64 rows over 16000 keys, 234 for 228 (chains)
   for (int step = 0; step < 2; ++step) {
     const int row = r ^ (2 * step);
     const uint32_t src = from + row * 128 + ((c ^ row) << 4) + 8 * h;
@@ -933,10 +933,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (!warp_live) {
             pv_done();
           } else if (span == 128) {
-            softmax_half<kFp8, 64>(tS, tO, h, 0, key0, sight, sl2, first, m, l, pv_done);
+            softmax_half<kFp8, 64>(p, tS, tO, h, 0, key0, sight, sl2, first, m, l, pv_done);
           } else if constexpr (!kTree) {
-            if (span == 64) softmax_half<kFp8, 32>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
-            else softmax_half<kFp8, 16>(tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+            if (span == 64) softmax_half<kFp8, 32>(p, tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
+            else softmax_half<kFp8, 16>(p, tS, tO, h, copy, key0, sight, sl2, first, m, l, pv_done);
           }
           tc_fence_before();
           mbar_arrive(smem_u32(&sm.p_full[t][h]));
@@ -946,7 +946,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       if constexpr (kTree) {
-        if (sight.hidden) {
+        if (sight.hidden()) {
           m = -INFINITY;
           l = 0.f;
         }
@@ -1436,18 +1436,18 @@ constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 
 // Trees of 17 to 64 stacked rows. The warp line reads a tree's keys once for every 16 rows, the tensor line once, but starts
-// some 12 us later (17 in e4m3, which it widens), so what decides is the keys, of which the host knows the tables'
-// width. us a million keys and KV heads: warps 44 for each 16 rows (e4m3 35), tensor cores 89 (95) an item. 8 KV
-// heads, bf16, warp / tensor (us): 64 rows, 24 trees of up to 1000 keys 52 / 60, 4000 112 / 88, 16000 373 / 203; 48 rows,
-// 1000 41 / 54, 16000 268 / 178; one tree of 64 rows over up to 60000 144 / 75; e4m3: 64 rows, 4000 100 / 124, 16000 295 / 242. With shared
-// keys (20 trees of 52 rows over 1024 and up to 700 of their own 73 / 55) both parts are in one kernel.
+// some 13 us later, so what decides is the keys, of which the host knows the tables' width. us a million keys and KV
+// heads: warps 44 for each 16 rows (e4m3 35), tensor cores 89 (66) an item. 8 KV heads, bf16, warp / tensor (us): 64 rows, 24
+// trees of up to 1000 keys 48 / 60, 4000 112 / 85, 16000 373 / 200; 48 rows, 1000 39 / 54, 16000 268 / 175; 32 rows, 16000 227 / 189;
+// one tree of 64 rows over up to 60000 144 / 71; e4m3: 64 rows, 1000 47 / 58, 4000 100 / 86, 16000 295 / 156; 48 rows, 4000 76 / 82. With
+// shared keys (20 trees of 52 rows over 1024 and up to 700 of their own 73 / 52) both parts are in one kernel.
 bool tree_on_tensor(int batch, int own, int kv_heads, int shared, int width, bool e4m3) {
   if (own <= kRowSpan) return false;
   const auto tiles = [](long long n, int span) { return (n + span - 1) / span; };
   const long long keys = static_cast<long long>(batch) * (width - shared) * kBlk, all = static_cast<long long>(batch) * own;
   const double warps = static_cast<double>(kv_heads) * (keys * tiles(own, kRowSpan) + 1.0 * shared * kBlk * tiles(all, kRowSpan));
   const double tensor = static_cast<double>(kv_heads) * (keys + 1.4 * shared * kBlk * tiles(all, kSpan));
-  return e4m3 ? warps - 2.6 * tensor > 1150000.0 : warps - 1.7 * tensor > 570000.0;
+  return e4m3 ? warps - 1.9 * tensor > 640000.0 : warps - 1.7 * tensor > 570000.0;
 }
 
 // The shape of a tree's call has the tables' width, a chain's 0.

@@ -365,30 +365,27 @@ __device__ __forceinline__ RowAt row_at(const BranchParams& p, int head, int r) 
 // saw everything, which costs least (hiding keys of such rows one by one took 111 us for 94), and what it
 // has then is dropped.
 struct Sight {
-  int base, count;
-  const uint32_t* mask;
-  bool hidden;
-  uint32_t word0;  // the mask's first word, as the bits after it mostly are none
-  __device__ __forceinline__ uint32_t word(int w) const {
+  int base, count, row;  // row of the masks
+  __device__ __forceinline__ bool hidden() const { return base == INT_MAX; }
+  __device__ __forceinline__ uint32_t word(const TreeParams& p, int w) const {
     const int rest = count - 32 * w;
     if (w < 0 || rest <= 0) return 0u;
-    const uint32_t bits = w == 0 ? word0 : __ldg(mask + w);
+    const uint32_t bits = __ldg(p.masks + static_cast<size_t>(row) * p.words + w);
     return rest >= 32 ? bits : bits & ((1u << rest) - 1u);
   }
   // bit j: whether it sees key + j
-  __device__ __forceinline__ uint32_t seen32(int key) const {
+  __device__ __forceinline__ uint32_t seen32(const TreeParams& p, int key) const {
     const int x = key - base;
     if (x <= -32) return 0xffffffffu;
-    if (x < 0) return (0xffffffffu >> (32 + x)) | (word(0) << -x);
-    return __funnelshift_r(word(x >> 5), word((x >> 5) + 1), x & 31);
+    if (x < 0) return (0xffffffffu >> (32 + x)) | (word(p, 0) << -x);
+    return __funnelshift_r(word(p, x >> 5), word(p, (x >> 5) + 1), x & 31);
   }
 };
 __device__ __forceinline__ Sight sight_of(const TreeParams& p, const RowAt& ra, bool shared) {
   const Extent x = extent_of(p, ra.b);
   const int count = x.all - x.clean;
-  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, nullptr, true, 0u};
-  const uint32_t* const mask = p.masks + (static_cast<size_t>(ra.b) * p.rows + ra.i) * p.words;
-  return Sight{x.clean, count, mask, false, __ldg(mask)};
+  if (ra.i >= count || (shared && !takes_shared(p, x))) return Sight{INT_MAX, 0, 0};
+  return Sight{x.clean, count, ra.b * p.rows + ra.i};
 }
 
 // The r-th of the rows that there are, from what lies in front of each sequence's: it is in the last one that
@@ -440,7 +437,7 @@ struct NodeValues {
   __device__ __forceinline__ float non_finite_sum(const TreeParams& p, const Sight& sight, int col) const {
     float sum = 0.f;
     for (int n = 0; n < sight.count; ++n) {
-      if (!(sight.word(n >> 5) >> (n & 31) & 1u)) continue;
+      if (!(sight.word(p, n >> 5) >> (n & 31) & 1u)) continue;
       const int key = sight.base + n, page = __ldg(table + key / kBlk);
       if (page < 0 || page >= p.pool_pages) continue;
       const size_t at = (static_cast<size_t>(page) * kBlk + key % kBlk) * kD + col;

@@ -310,6 +310,10 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     }
     const auto sight0 = sight_of(p, at0, g.shared != 0), sight1 = sight_of(p, at1, g.shared != 0);
     const int lim0 = sight0.base, lim1 = sight1.base;
+    if constexpr (kTree) {  // read at the end of the item, mostly the first words
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.masks + static_cast<size_t>(sight0.row) * p.words));
+      asm volatile("prefetch.global.L1 [%0];" ::"l"(p.masks + static_cast<size_t>(sight1.row) * p.words));
+    }
     bool taken_out = false;  // whether a node's V held an infinity or NaN
     float sl2 = p.scale_log2, sl2b = p.scale_log2;  // of row r and row r + 8
 #pragma unroll
@@ -378,7 +382,7 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       // keys at or past a row's limit are hidden from it
       if (__any_sync(0xffffffffu, key + 32 > min(lim0, lim1))) {
         if constexpr (kTree) {  // but for nodes that it sees
-          const uint32_t seen0 = sight0.seen32(key), seen1 = sight1.seen32(key);
+          const uint32_t seen0 = sight0.seen32(p, key), seen1 = sight1.seen32(p, key);
 #pragma unroll
           for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -498,13 +502,13 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
     }
     if (!ok) break;
     if constexpr (kTree) {
-      if (sight0.hidden) {
+      if (sight0.hidden()) {
         m0 = -INFINITY;
         l0 = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[j][0] = o[j][1] = 0.f;
       }
-      if (sight1.hidden) {
+      if (sight1.hidden()) {
         m1 = -INFINITY;
         l1 = 0.f;
 #pragma unroll
