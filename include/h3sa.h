@@ -608,7 +608,7 @@ H3SA_API int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value,
  * nothing, come out zero. An infinity or NaN in K or V of a drafted row reaches only the rows that see it; one
  * in V of a sequence's first lengths[b] rows makes all its outputs in that column infinite or NaN. A
  * length or count outside its range, or both together past the table, is clamped with
- * H3SA_DEVERR_BAD_INDEX. */
+ * H3SA_DEVERR_BAD_INDEX. workspace may be NULL where h3sa_tree_workspace is 0. */
 H3SA_API int64_t h3sa_tree_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
                                      int32_t shared_rows, int32_t width, int32_t e4m3);
 H3SA_API int h3sa_tree_attention(

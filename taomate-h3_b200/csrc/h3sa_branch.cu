@@ -1491,6 +1491,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, int wid
   s.rows = s.own_row0 +
            (static_cast<long long>(kv_heads) * batch * lo.own_tiles + lo.workers) * own_slots * s.own_slot_rows;
   s.bytes = s.rows * (kD * 4 + 8) + 2 * (kPlanHead + 2ll * batch) * 4;
+  if (width > 0 && whole_form(width, kv_heads, batch, s.warp)) s.bytes = 0;  // nothing to merge
   return s;
 }
 
@@ -1596,7 +1597,7 @@ int attend(const char* what, const TreeParams* nodes, const void* query, int64_t
   if (shared_rows < 0 || shared_rows % kBlk || shared_rows / kBlk > width)
     return set_error(H3SA_ERR_INVALID, "%s: %d shared rows are not whole pages of a "
                      "table of %d entries", what, shared_rows, width);
-  if (!query || !out || !key_pool || !value_pool || !table || !lengths || !workspace ||
+  if (!query || !out || !key_pool || !value_pool || !table || !lengths ||
       (e4m3 && (!k_scale || !v_scale)))
     return set_error(H3SA_ERR_INVALID, "%s: null pointer argument", what);
   if (!(softmax_scale > 0.f) || softmax_scale > 2.0e38f)
@@ -1622,6 +1623,7 @@ int attend(const char* what, const TreeParams* nodes, const void* query, int64_t
   if (line_units(s.tensor) > INT32_MAX / 2 || line_units(s.warp) > INT32_MAX / 2)
     return set_error(H3SA_ERR_UNSUPPORTED, "%s: batch %d x rows %d x heads %d over %d "
                      "pages exceeds the work index", what, batch, rows, heads, width);
+  if (s.bytes > 0 && !workspace) return set_error(H3SA_ERR_INVALID, "%s: null pointer argument", what);
   if (workspace_bytes < s.bytes)
     return set_error(H3SA_ERR_INVALID, "%s: workspace of %lld bytes, %lld needed", what,
                      static_cast<long long>(workspace_bytes), s.bytes);

@@ -297,15 +297,15 @@ def _attend(what: str, masks: torch.Tensor | None, counts: int | None, query: to
         raise RuntimeError(f"{what}: {shared_rows} shared rows are not whole pages of a table of {width} "
                            "entries")
     error = _error_word(what, device, device_error)
-    need = max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows) if masks is None else
-               _TREE_WORK(batch, rows, heads, kv_heads, shared_rows, width, 1 if e4m3 else 0))
+    need = (max(16, _ATTEND_WORK(batch, rows, heads, kv_heads, shared_rows)) if masks is None else
+            _TREE_WORK(batch, rows, heads, kv_heads, shared_rows, width, 1 if e4m3 else 0))
     if out is not None and _bad(out, device, _BF16, query.shape):
         _refuse(what, "out", device, _BF16, query.shape)
     with _on(stream):
         if out is None:
             out = (_empty_like(query) if query.is_contiguous() else
                    query.new_empty(shape))
-        work = lengths.new_empty(need // 4)
+        work = lengths.new_empty(need // 4) if need else None
     args = (query.data_ptr(), strides[0], strides[1], strides[2], out.data_ptr(),
             None if lse is None else lse.data_ptr(), batch, rows, heads, kv_heads,
             key_pool.data_ptr(), value_pool.data_ptr(), pool_rows // PAGE_ROWS, 1 if e4m3 else 0,
@@ -315,8 +315,8 @@ def _attend(what: str, masks: torch.Tensor | None, counts: int | None, query: to
         code = _ATTEND(*args, shared_rows, 1 if causal else 0, softmax_scale, work.data_ptr(), need, error,
                        _handle(stream, device))
     else:
-        code = _ATTEND_TREE(*args, masks.data_ptr(), counts, shared_rows, softmax_scale, work.data_ptr(), need, error,
-                            _handle(stream, device))
+        code = _ATTEND_TREE(*args, masks.data_ptr(), counts, shared_rows, softmax_scale,
+                            None if work is None else work.data_ptr(), need, error, _handle(stream, device))
     if code:
         check(f"h3sa_{what}", code)
     return out
