@@ -570,7 +570,8 @@ enum { H3SA_POS_ROW = 0, H3SA_POS_I32 = 1, H3SA_POS_I64 = 2, H3SA_POS_F64 = 3 };
  * frequencies[k] (radians, fp64) and is multiplied by factor; the other dimensions stay as they are. Pairs are
  * (k, k + pairs), or (2k, 2k + 1) if interleaved. positions [batch * rows, axes] of the given kind; pair
  * k belongs to axis k / (pairs / axes). H3SA_POS_ROW (appended rows, one axis): a row's place in its
- * sequence. Angles are taken in 64 bits, products in 32, results rounded once. */
+ * sequence. Angles are taken in 64 bits, products in 32, results rounded once. Positions and frequencies are
+ * finite, and |position| * |frequency| below 2^50 where positions are H3SA_POS_F64, |frequency| where not. */
 typedef struct h3sa_rotary {
   const void* positions;
   const double* frequencies;
@@ -580,7 +581,7 @@ typedef struct h3sa_rotary {
 } h3sa_rotary;
 
 /* out = x rotated, both of `dtype`. dim: at most 1024. out may be x itself (same address and strides),
- * else they may not overlap. Any strides and alignment of whole elements; 16 or 8 bytes are read at a time
+ * else they may not overlap; rows of out may not overlap each other. Any strides and alignment of whole elements; 16 or 8 bytes are read at a time
  * where pairs, dim, strides and addresses are multiples of them. */
 H3SA_API int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32_t batch,
                          int32_t rows, int32_t dim, const h3sa_rotary* rotary, void* stream);
@@ -588,7 +589,7 @@ H3SA_API int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dty
 /* Appends rows i < counts[b] of key and value (bf16, heads of 128) to the pages of their sequences, at
  * rows lengths[b] + i through the table (int32 [batch, width]); lengths stay as they are. Keys are
  * rotated on the way, and so is query into query_out (both NULL if there is none; query_out may be query
- * itself); its rows behind counts[b] come out zero. rotary NULL: nothing is. Pools
+ * itself, else it overlaps no other argument, and its rows not each other); its rows behind counts[b] come out zero. rotary NULL: nothing is. Pools
  * [kv_heads, pool_pages * 128, 128], 16-byte aligned, bf16, or e4m3 with positive k_scale / v_scale fp32
  * [kv_heads], by which rows are divided (rounded once, limited to 448, NaN stays NaN). A row past the table's
  * width, or of a sequence of negative length, sets H3SA_DEVERR_BAD_INDEX, a page outside the pool
@@ -623,7 +624,8 @@ H3SA_API int h3sa_tree_attention(
  * lengths_out[b] = lengths[b] + the path's length. path int32 [sequences, steps] ascends and ends at the first
  * negative entry or with the steps. A path that does not ascend or leaves the table (then
  * H3SA_DEVERR_BAD_INDEX), or a page outside the pool (H3SA_DEVERR_BAD_PAGE), leaves its sequence as it
- * was. The rows' pages belong to their sequences alone; lengths_out may not overlap lengths. */
+ * was. The rows' pages belong to their sequences alone; lengths_out may not overlap lengths, nor one pool tensor
+ * another. */
 H3SA_API int h3sa_keep_rows(const h3sa_pools* pools, const int32_t* table, int32_t sequences,
                             int32_t width, const int32_t* lengths, const int32_t* path,
                             int32_t steps, int32_t* lengths_out, int32_t* device_error,

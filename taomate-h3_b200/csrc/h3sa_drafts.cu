@@ -2,7 +2,11 @@
 // behind the history in every pool tensor.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstring>
+#include <functional>
+#include <memory>
+#include <new>
 
 #include "h3sa_host.h"
 #include "h3sa_ptx.cuh"
@@ -158,6 +162,22 @@ __global__ void __launch_bounds__(32 * kKeepWarps) keep_rows_kernel(const KeepAr
   }
 }
 
+// Whether pool tensors are apart: rows move in place, and a tensor given twice would see them move twice.
+int check_apart(const h3sa_pools* p) {
+  const int64_t bytes = static_cast<int64_t>(p->heads) * p->pages * kPage * p->row_bytes;
+  bool apart = true;
+  if (!p->list) {
+    apart = p->count < 2 || p->stride >= bytes || p->stride <= -bytes;
+  } else if (p->count > 1) {
+    const std::unique_ptr<const char*[]> at(new (std::nothrow) const char*[p->count]);
+    if (!at) return set_error(H3SA_ERR_INVALID, "keep_rows: no host memory for %d addresses", p->count);
+    for (int i = 0; i < p->count; ++i) at[i] = static_cast<const char*>(p->list[i]);
+    std::sort(at.get(), at.get() + p->count, std::less<const char*>());
+    for (int i = 1; i < p->count; ++i) apart = apart && at[i] - at[i - 1] >= bytes;
+  }
+  return apart ? H3SA_OK : set_error(H3SA_ERR_INVALID, "keep_rows: pool tensors overlap");
+}
+
 }  // namespace
 }  // namespace h3sa
 
@@ -196,6 +216,7 @@ int h3sa_keep_rows(const h3sa_pools* pools, const int32_t* table, int32_t sequen
   if (pools->count == 0 || items > static_cast<long long>(INT32_MAX))
     return set_error(H3SA_ERR_INVALID, "keep_rows: %d pool tensors of %d heads and %d sequences are none or too many",
                      pools->count, pools->heads, sequences);
+  if (const int rc = check_apart(pools)) return rc;
   for (int first = 0; first < pools->count; first += kMaxPools) {
     KeepArgs a;
     memset(&a, 0, sizeof(a));

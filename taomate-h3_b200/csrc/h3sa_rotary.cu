@@ -486,6 +486,13 @@ int check_rotary(const char* what, const h3sa_rotary* r, int dim, bool rows_know
 // Strides of heads are kept in 32 bits.
 bool head_stride_ok(const h3sa_heads* h) { return !h || (h->stride_head >= INT32_MIN && h->stride_head <= INT32_MAX); }
 
+// Rows that are written lie apart: those of a tensor that repeats some by a stride of zero would be written from
+// several places, and read and written at once in place.
+bool rows_apart(const h3sa_heads* h, int batch, int rows, int dim) {
+  const auto apart = [&](long long n, long long stride) { return n < 2 || stride >= dim || stride <= -dim; };
+  return apart(batch, h->stride_sequence) && apart(rows, h->stride_row) && apart(h->heads, h->stride_head);
+}
+
 Heads heads_of(const h3sa_heads* from, const h3sa_heads* to) {
   Heads h;
   memset(&h, 0, sizeof(h));
@@ -525,6 +532,7 @@ int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32
     return set_error(H3SA_ERR_UNSUPPORTED, "rotate: batch %d x rows %d x heads %d is too large", batch, rows, x->heads);
   if (!head_stride_ok(x) || !head_stride_ok(out))
     return set_error(H3SA_ERR_UNSUPPORTED, "rotate: strides of heads must fit 32 bits");
+  if (!rows_apart(out, batch, rows, dim)) return set_error(H3SA_ERR_INVALID, "rotate: rows of out overlap");
   const int size = dtype == H3SA_FP32 ? 4 : 2;
   if (!x->base || !out->base) return set_error(H3SA_ERR_INVALID, "rotate: null pointer argument");
   if ((reinterpret_cast<uintptr_t>(x->base) | reinterpret_cast<uintptr_t>(out->base)) % size)
@@ -566,6 +574,8 @@ int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value, const h3sa_
                      static_cast<long long>(heads));
   if (!head_stride_ok(key) || !head_stride_ok(value) || !head_stride_ok(query) || !head_stride_ok(query_out))
     return set_error(H3SA_ERR_UNSUPPORTED, "append rows: strides of heads must fit 32 bits");
+  if (with_query && !rows_apart(query_out, batch, rows, kDim))
+    return set_error(H3SA_ERR_INVALID, "append rows: rows of query_out overlap");
   if (!key->base || !value->base || !key_pool || !value_pool || !table || !lengths ||
       (with_query && (!query->base || !query_out->base)) || (e4m3 && (!k_scale || !v_scale)))
     return set_error(H3SA_ERR_INVALID, "append rows: null pointer argument");

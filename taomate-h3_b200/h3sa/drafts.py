@@ -182,7 +182,7 @@ def keep_rows(pools: PoolTensors, table: torch.Tensor, lengths: torch.Tensor, pa
     """The accepted rows become history: row ``lengths[b] + path[b, k]`` moves to row ``lengths[b] + k`` in every pool
     tensor, and the new lengths are returned. ``path`` int32 ``[sequences, steps]``: drafted rows in ascending
     order, negative after the last one. A path that does not ascend or leaves the table, or a page that is none of
-    the pool, leaves its sequence as it was (``device_error``)."""
+    the pool, leaves its sequence as it was (``device_error``). Pool tensors may not overlap."""
 
     what = "keep_rows"
     if not table.is_cuda:

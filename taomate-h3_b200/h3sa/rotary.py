@@ -101,8 +101,8 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     strides with contiguous rows (16 bytes are read at a time where pairs, ``dim``, strides and addresses
     are multiples of that). ``positions``: int32, int64 or float64, one a row, or ``[..., axes]``.
     ``frequencies``: fp64 ``[pairs]``, or ``[axes, pairs of an axis]``, where the pairs of the first axis come
-    first. ``out``: a tensor like ``x`` for the result, ``x`` itself for a rotation in place; it may not overlap
-    ``x`` otherwise.
+    first. Both are finite, and an angle (int positions: a frequency) is below 2^50. ``out``: a tensor like ``x`` for
+    the result, ``x`` itself for a rotation in place; it may not overlap ``x`` otherwise, nor its rows each other.
     """
 
     what = "rotate"

@@ -65,6 +65,7 @@ def test_tree_refuses(change, match) -> None:
     ({}, {}, {}, dict(position_kind=0), "positions must be"), ({}, {}, {}, dict(positions=None), "null pointer"), ({}, {}, {}, dict(frequencies=None), "null pointer"),
     ({}, {}, {}, dict(factor=math.inf), "finite"), ({}, {}, {}, dict(factor=math.nan), "finite"), (dict(base=None), {}, {}, {}, "null pointer"),
     ({}, dict(base=None), {}, {}, "null pointer"), (dict(base=P + 1), {}, {}, {}, "aligned"), ({}, dict(base=P + 2), dict(dtype=2), {}, "aligned"),
+    ({}, dict(stride_head=0), {}, {}, "overlap"), ({}, dict(stride_row=127), {}, {}, "overlap"), ({}, dict(stride_sequence=-100), {}, {}, "overlap"),
     (dict(stride_head=1 << 31), {}, {}, {}, "32 bits"), ({}, dict(stride_head=-(1 << 31) - 1), {}, {}, "32 bits"),
     ({}, {}, dict(batch=1 << 20, rows=1 << 11), {}, "too large"), (dict(heads=1 << 12), dict(heads=1 << 12), dict(batch=1 << 10, rows=1 << 9), {}, "too large"),
 ])
@@ -85,6 +86,7 @@ APPEND = dict(key=None, value=None, query=None, query_out=None, batch=2, rows=4,
     (dict(query=dict(base=None), query_out={}), "null pointer"), (dict(e4m3=1, ks=P), "null pointer"), (dict(k=P + 8), "16-byte aligned"),
     (dict(key=dict(base=P + 1)), "aligned"), (dict(query={}, query_out=dict(base=P + 1)), "aligned"), (dict(value=dict(stride_head=1 << 31)), "32 bits"),
     (dict(batch=1 << 20, rows=1 << 11), "too large"), (dict(batch=1 << 14, rows=1 << 14), "too large"),
+    (dict(query={}, query_out=dict(stride_row=0)), "overlap"), (dict(query={}, query_out=dict(stride_head=64)), "overlap"),
     (dict(rotary=dict(pairs=65)), "do not fit"), (dict(rotary=dict(position_kind=0, axes=2)), "positions must be"), (dict(rotary=dict(factor=-math.inf)), "finite"),
 ])
 def test_append_refuses(change, match) -> None:
@@ -133,6 +135,24 @@ def test_keep_refuses(pools, change, match) -> None:
     for name, value in {**dict(base=P, stride=4096, count=2, heads=1, pages=8, row_bytes=32), **pools}.items():
         setattr(p, name, value)
     _call("h3sa_keep_rows", {**KEEP, "pools": p}, change, match)
+
+
+@pytest.mark.parametrize("at", [(P, 2 * P, P), (2 * P, 3 * P, P, 3 * P + 32752), (P + 16, P)])
+def test_keep_refuses_pools_that_overlap(at) -> None:
+    """Rows of a tensor that is given twice would move twice."""
+
+    p, listed = _lib().Pools(), (ctypes.c_void_p * len(at))(*at)
+    for name, value in dict(list=ctypes.addressof(listed), count=len(at), heads=1, pages=8, row_bytes=32).items():
+        setattr(p, name, value)
+    _call("h3sa_keep_rows", {**KEEP, "pools": p}, {}, "overlap")
+
+
+@pytest.mark.parametrize("stride", [0, 32752, -32752])
+def test_keep_refuses_strides_that_overlap(stride) -> None:
+    p = _lib().Pools()
+    for name, value in dict(base=P, stride=stride, count=2, heads=1, pages=8, row_bytes=32).items():
+        setattr(p, name, value)
+    _call("h3sa_keep_rows", {**KEEP, "pools": p}, {}, "overlap")
 
 
 def test_the_structs_are_the_header_s() -> None:
