@@ -960,15 +960,12 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.tree.taken_out) != 0)) {
           const NodeValues<kFp8> nodes(p, it.at.b, it.head);
 #pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
+          for (int c = 0; c < kD; ++c) {  // column by column, for its code: it is seldom needed
+            const float lost = my < n_rows ? nodes.non_finite_sum(p, sight, c) : 0.f;
+            __syncwarp();
+            const uint32_t o = tmem_ld1(tO + c);
             tmem_wait_ld();
-            reg_fence32(o);
-            if (my < n_rows)
-#pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) + nodes.non_finite_sum(p, sight, c * 32 + j));
-            tmem_st32(tO + c * 32, o);
+            tmem_st1(tO + c, __float_as_uint(__uint_as_float(o) + lost));
           }
           tmem_wait_st();
         }
@@ -1463,7 +1460,7 @@ Shape shape_of(int batch, int rows, int kv_heads, int group, int shared, int wid
   if (width > 0) {
     s.tensor.few = kFewCost;
     s.tensor.many = s.tensor.least = kManyCost;
-    s.tensor.pad = kTreePad;
+    s.tensor.pad = e4m3 ? kTreePadF8 : kTreePad;
   }
   bool on_tensor = own > kWarpOwnRows;
   if (width > 0 && !on_tensor) {

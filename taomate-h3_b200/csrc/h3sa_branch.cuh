@@ -107,7 +107,7 @@ __device__ __forceinline__ Extent extent_of(const TreeParams& p, int b) {
 // have all its keys.
 __device__ __forceinline__ bool takes_shared(const BranchParams& p, const Extent& x) { return x.clean >= p.shared_keys; }
 // The first key outside the shared items, and the units behind it of the rows of tile t of a
-// sequence of length `len`.
+// sequence.
 __device__ __forceinline__ int own_lo(const BranchParams& p, const Extent& x) { return takes_shared(p, x) ? p.shared_keys : 0; }
 __device__ __forceinline__ int own_limit(const BranchParams& p, const Line& ln, const Extent& x, int t) {
   if (!p.causal) return x.all;
@@ -120,9 +120,11 @@ __device__ __forceinline__ int own_units(const P& p, const Line& ln, const Exten
   return over_pow2(max(0, own_limit(p, ln, x, t) - own_lo(p, x) + ln.unit - 1), ln.unit);
 }
 // What a unit of an item of `rows` rows weighs: 1, or of the tensor line in a tree's call one of the two below (of
-// chains all weigh the same). Blocks of up to 128 and of more rows take a CTA 1.6 and 2.6 us (e4m3 1.5 and 2.2), and an item 6 to 8 us
-// (10) from its end to the next one's first scores.
-constexpr int kFewCost = 5, kManyCost = 8, kTreePad = 24;
+// chains all weigh the same). Blocks of up to 128 and of more rows take a CTA 1.5 to 1.75 and 2.6 us (e4m3 1.1 and 2.1), and
+// an item 4 to 6 us (8 to 12) from its last scores to the next one's first. Weight of an item, 8 / 16 / 24 (us): 24 trees of 96
+// rows over 9000 keys 130.5 / 130 / 133.5, 20 small trees over 8192 shared keys 73 / 70.5 / 71; e4m3, 16 / 24 / 40: wide trees
+// 188.7 / 188 / 186, 24 trees of 64 rows over 16000 keys 163 / 160 / 158.
+constexpr int kFewCost = 5, kManyCost = 8, kTreePad = 16, kTreePadF8 = 40;
 template <class P>
 __device__ __forceinline__ int cost_of(const P&, const Line& ln, int rows) {
   return is_tree<P> ? (rows > kBlk ? ln.many : ln.few) : 1;

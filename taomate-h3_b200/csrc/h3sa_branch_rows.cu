@@ -517,14 +517,19 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
       // what was taken out of V, to the rows that see it
       if (__any_sync(0xffffffffu, taken_out)) {
         const NodeValues<kFp8> nodes(p, g.seq, g.head);
+#pragma unroll 1
+        for (int k = 0; k < 32; ++k) {  // one column's code: it is seldom needed
+          const int col = column_of<kFp8>(c, k >> 1, k & 1);
+          const float lost0 = nodes.non_finite_sum(p, sight0, col), lost1 = nodes.non_finite_sum(p, sight1, col);
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+          for (int j = 0; j < 16; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = column_of<kFp8>(c, j, e);
-            o[j][e] += nodes.non_finite_sum(p, sight0, col);
-            o[j][2 + e] += nodes.non_finite_sum(p, sight1, col);
-          }
+            for (int e = 0; e < 2; ++e)
+              if (k == 2 * j + e) {
+                o[j][e] += lost0;
+                o[j][2 + e] += lost1;
+              }
+        }
       }
     }
     l0 = quad_sum(l0);

@@ -14,8 +14,9 @@
 // between, for which an SM has some 350 a warp and 2 KB: a thread keeps to one unit of a head row, 8 pairs in two
 // vectors of 16 bytes, with their frequencies in registers, works out its 8 angles once a token and turns up to eight heads by
 // them, all of which are on their way by then. There is nothing to share and nothing to wait for in a block.
-// (A table of the block's cosines and sines in shared memory took 57 us for 24605 tokens of 24 heads and 110 for 300001 of
-// one head.)
+// Measured: 24605 tokens of 24 heads, bf16, three axes: 51 us, 5.9 TB/s of the 302 MB read and written; 300001 of one head 45 us
+// (a table of the block's cosines and sines in shared memory took 57 and 110); appends of 16-bit prompts into e4m3 pools
+// 75 us for 373 MB, 5.0 TB/s, the divisions and conversions beside the loads; a few rows 4.2 us, launch and two dependent loads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
