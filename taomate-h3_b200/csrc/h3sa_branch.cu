@@ -20,7 +20,7 @@
 //
 // Warp roles of branch_attn_kernel (one persistent CTA per SM, 384 threads):
 //   warp 0      walks the CTA's units: publishes each item segment in a small descriptor ring and
-//               loads its K and V blocks by TMA into one ring of tiles (K0 V0 K1 V1 ...).
+//               loads its K and V blocks by TMA into one ring of tiles.
 //   warp 1, 2   issue the MMAs of query tile 0 and 1: S_t = Q_t K^T, then O_t += P_t V, one elected
 //               lane per tcgen05 instruction (warp 1 also owns TMEM).
 //   warp 3      e4m3: widens V to f16.
@@ -95,6 +95,9 @@ struct BrCfg {
   static constexpr int kTile = kBlk * kD * kElem;
   static constexpr int kStages = kFp8 ? 6 : 5;  // even for e4m3: K in the even slots, V in the odd ones
   static constexpr int kSteps = kFp8 ? 4 : 8;   // MMA K steps of S
+  // Order of a segment's loads: K0 K1 V0 K2 V1 ..., each V behind the next K, which is wanted first (V waits for a
+  // softmax); e4m3: K0 V0 K1 V1 ..., as V is widened on its way.
+  static constexpr bool kSkew = !kFp8;
   static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
   static constexpr uint32_t kIdescPV = kFp8 ? idesc_f16(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
 };
@@ -623,20 +626,29 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (!g.live) break;
       // ---- its blocks
       const bool pair = g.n_rows > kBlk;
-      for (int j0 = 0; ok && j0 < g.blocks; j0 += 32) {
-        const int n = min(32, g.blocks - j0);
-        int page = 0;
-        if (lane < n) page = __ldg(p.table + static_cast<size_t>(seq) * p.width + g.block0 + j0 + lane);
-        if (__any_sync(0xffffffffu, page < 0 || page >= p.pool_pages)) {
-          if (lane == 0) {
-            if (p.err) atomicOr(p.err, kErrBadPage);
-            *abort_flag = 1;
+      const int first_tile = last_tile ^ 1;
+      int pages = 0, page = 0, page_before = 0;  // 32 blocks', and those of the last two K
+      for (int i = 0, k = 0; ok && i < 2 * g.blocks; ++i) {
+        const bool is_k = Cfg::kSkew ? i == 0 || ((i & 1) && k < g.blocks) : (i & 1) == 0;
+        if (is_k) {
+          if ((k & 31) == 0) {
+            pages = k + lane < g.blocks ? __ldg(p.table + static_cast<size_t>(seq) * p.width + g.block0 + k + lane) : 0;
+            if (__any_sync(0xffffffffu, pages < 0 || pages >= p.pool_pages)) {
+              if (lane == 0) {
+                if (p.err) atomicOr(p.err, kErrBadPage);
+                *abort_flag = 1;
+              }
+              ok = false;
+              break;
+            }
           }
-          ok = false;
-          break;
+          page_before = page;
+          page = __shfl_sync(0xffffffffu, pages, k & 31);
+          ++k;
         }
-        for (int j = 0; ok && j < 2 * n; ++j) {
-          const int pg = __shfl_sync(0xffffffffu, page, j >> 1);
+        {
+          const int j = is_k || !Cfg::kSkew || i == 2 * g.blocks - 1 ? k - 1 : k - 2;  // the block
+          const int pg = j == k - 1 ? page : page_before;
           const uint32_t bit = 1u << ring;
           if (used0 & bit) {
             ok = mbar_wait(smem_u32(&sm.empty[0][ring]), (free0 >> ring) & 1u, abort_flag, p.err);
@@ -648,9 +660,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           }
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           // a block of one tile signals that tile's barrier, a shared one tile 0's
-          if ((j & 1) == 0) last_tile = pair ? 1 : last_tile ^ 1;
-          const int side = pair ? 0 : last_tile;
-          const bool widened = kFp8 && (j & 1);  // warp 3 alone reads it, and releases it on tile 0's
+          const int side = pair ? 0 : first_tile ^ (j & 1);
+          const bool widened = kFp8 && !is_k;  // warp 3 alone reads it, and releases it on tile 0's
           used0 = pair || side == 0 || widened ? used0 | bit : used0 & ~bit;
           used1 = (pair || side == 1) && !widened ? used1 | bit : used1 & ~bit;
           on_tile1 = side ? on_tile1 | bit : on_tile1 & ~bit;
@@ -659,7 +670,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (lane == 0) {
             const uint32_t bar = smem_u32(&sm.full[side][ring]);
             mbar_expect_tx(bar, Cfg::kTile);
-            const CUtensorMap* map = (j & 1) ? &tmV : &tmK;
+            const CUtensorMap* map = is_k ? &tmK : &tmV;
             for (int a = 0; a < Cfg::kTile / kAtom; ++a) {
               const uint32_t dst = smem_u32(sm.kv[ring]) + a * kAtom;
               if (once) tma_load_3d_once(dst, map, bar, a * (128 / Cfg::kElem), pg * kBlk, g.head, policy);
@@ -670,6 +681,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (++ring == kS) ring = 0;
         }
       }
+      last_tile = pair ? 1 : first_tile ^ ((g.blocks - 1) & 1);
     }
     if (!ok) {
       // leaving early: no copy may still be in flight when the CTA ends
@@ -700,7 +712,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     const uint32_t q_bar = smem_u32(&sm.q_full[mt]), s_bar = smem_u32(&sm.s_full[mt]);
     const uint32_t p_bar = smem_u32(&sm.p_full[mt]), o_bar = smem_u32(&sm.o_full[mt]);
     const uint32_t pv_bar = smem_u32(&sm.pv_done[mt]);
-    int ring = 0;  // K tile of the next unit; V follows it
+    int ring = 0;  // K tile of the next unit
     int wide = 0;  // e4m3: the next widened block
     // The next phase of each slot's two full barriers, a bit per slot: a tile's own blocks land
     // on its barrier, blocks of both tiles on that of tile 0. So a warp never waits on a phase
@@ -766,6 +778,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       tc_commit(o_bar);
       free_v();
     };
+    const auto wrap = [](int slot) { return slot >= kS ? slot - kS : slot; };
     Segment g;
     while (ok && next_segment(g)) {
       const bool pair = g.n_rows > kBlk;
@@ -781,7 +794,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       bool first = true;
       for (int j = 0; ok && j < g.blocks; ++j) {
         const int owner = pair ? mt : last_tile ^ 1;
-        const int vs = ring + 1 == kS ? 0 : ring + 1;
+        const bool last = j == g.blocks - 1;
+        const int vs = wrap(ring + (Cfg::kSkew ? (j == 0 ? 2 : 3) - last : 1));  // its V
         const bool second = !pair && owner == 1;
         if (owner == mt) {
           const uint32_t phases = second ? phase1 : phase0;
@@ -831,7 +845,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           if (++wide == kWide) wide = 0;
         }
         last_tile = pair ? 1 : owner;
-        ring = vs + 1 == kS ? 0 : vs + 1;
+        ring = wrap(last ? vs + 1 : ring + (Cfg::kSkew && j == 0 ? 1 : 2));
       }
       if (ok && pend) finish_item();
     }
