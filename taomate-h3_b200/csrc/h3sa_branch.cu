@@ -1225,18 +1225,18 @@ __device__ __forceinline__ void add_pieces(const BranchParams& p, const Pieces (
     for (int k = 0; k < kRows; ++k)
 #pragma unroll
       for (int j = 0; j < kB; ++j) {
-        const long long at = static_cast<long long>(min(i0 + j, n - 1)) * q[k].stride;
-        ml[k][j] = __ldcg(ml_at[k] + at);
-        v[k][j] = __ldcg(o_at[k] + at * (kD / 4));
+        ml[k][j] = make_float2(-INFINITY, 0.f);
+        if (i0 + j < n) {
+          const long long at = static_cast<long long>(i0 + j) * q[k].stride;
+          ml[k][j] = __ldcg(ml_at[k] + at);
+          v[k][j] = __ldcg(o_at[k] + at * (kD / 4));
+        }
       }
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
       float top = m[k];
 #pragma unroll
-      for (int j = 0; j < kB; ++j) {
-        if (i0 + j >= n) ml[k][j] = make_float2(-INFINITY, 0.f);
-        top = fmaxf(top, ml[k][j].x);
-      }
+      for (int j = 0; j < kB; ++j) top = fmaxf(top, ml[k][j].x);
       // a sum of 0: the piece saw nothing and its O was not written. Sums that are NaN stay so.
       const float keep = sum[k] != 0.f ? fast_exp2(m[k] - top) : 0.f;
       sum[k] = sum[k] != 0.f ? sum[k] * keep : 0.f;
@@ -1275,8 +1275,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
   const int* const po = p.plan + (own_by_warps ? line : 0);
   const int shared_blocks = kJoint ? 0 : __ldcg(po);
   const int cut_s = __ldcg(ps + 2), cut_o = __ldcg(po + 2), live = __ldcg(ps + 3);
-  const int shared_units = shared_blocks * over_pow2(kBlk, ls.unit), cost_s = cost_of(p, ls, live);
-  const int shared_weight = weight_of(ls, shared_units, cost_s);
+  const int shared_units = shared_blocks * over_pow2(kBlk, ls.unit);
+  const int shared_weight = weight_of(ls, shared_units, shared_cost(p, ls, live, 0));
   bool compact = false;
   if constexpr (is_tree<P>) compact = p.compact != 0;
   const int own_all = p.rows * p.group;
@@ -1311,7 +1311,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
         make_uint2(pack_bf16x2(acc.x * scale, acc.y * scale), pack_bf16x2(acc.z * scale, acc.w * scale));
     if (p.lse && lane == 0) p.lse[id] = sum == 0.f ? -INFINITY : (m + log2f(sum)) * 0.6931471805599453f;
   };
-  int u0 = head * __ldcg(po + 1) + (ps == po ? live_tiles(p, ls, live) * shared_weight : 0) + __ldcg(po + kPlanHead + b);
+  if constexpr (is_tree<P>) {
+    if (r >= ext.rows) {  // rows behind the nodes
+      for (int k = part; k < kRows && r + k < min(own_all, (t + 1) * lo.span); k += kTeam)
+        write_row(r + k, make_float4(0.f, 0.f, 0.f, 0.f), 0.f, 0.f);
+      return;
+    }
+  }
+  int u0 = head * __ldcg(po + 1) + (ps == po ? shared_weight_all(p, ls, shared_units, live, live_tiles(p, ls, live)) : 0) + __ldcg(po + kPlanHead + b);
   for (int k = 0; k < t; ++k) u0 += own_weight(p, lo, ext, k);
   const int units = own_units(p, lo, ext, t), cost_o = own_cost(p, lo, ext, t);
   const int n_rows = min(lo.span, ext.rows - t * lo.span), last = min(own_all, (t + 1) * lo.span);
@@ -1329,7 +1336,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) branch_merge_kernel(const P 
     const int rk = min(r + k, t * lo.span + max(n_rows, 1) - 1);
     const int row = (compact ? __ldcg(ps + kPlanHead + p.batch + b) : b * own_all) + rk, t_sh = over_pow2(row, ls.span);
     sh[k] = pieces_of(cut_s, head * __ldcg(ps + 1) + t_sh * shared_weight, compact && (rk >= ext.rows || !takes_shared(p, ext)) ? 0 : shared_units,
-                      cost_s,
+                      shared_cost(p, ls, live, t_sh),
                       min(ls.span, live - t_sh * ls.span), row & (ls.span - 1),
                       head * ls.shared_tiles + t_sh, 0, p.shared_slot_rows, shared_by_warps);
     own[k] = pieces_of(cut_o, u0, units, cost_o, n_rows, rk - t * lo.span,

@@ -160,12 +160,22 @@ __device__ __forceinline__ int live_tiles(const P&, const Line& ln, int live) {
   return ln.shared_tiles;
 }
 
+// What a KV head's shared items weigh, from the units of one; all but the last one of a tree's call weigh the same.
+template <class P>
+__device__ __forceinline__ int shared_cost(const P& p, const Line& ln, int live, int t) { return cost_of(p, ln, live - t * ln.span); }
+template <class P>
+__device__ __forceinline__ int shared_weight_all(const P& p, const Line& ln, int units, int live, int tiles) {
+  return tiles == 0 ? 0 : weight_of(ln, units, shared_cost(p, ln, live, 0)) * (tiles - 1) +
+                              weight_of(ln, units, shared_cost(p, ln, live, tiles - 1));
+}
+
 struct Plan {
   int shared_blocks;  // of the shared items: 0 if no sequence has all of them
   int shared_units;   // units of one shared item
   int live;           // stacked rows
   int shared_tiles;   // shared items a KV head
-  int shared_weight;  // of one of them
+  int shared_weight;  // of one of them, but perhaps the last
+  int shared_all;     // of all of them
   int head_weight;    // one KV head's part of the line
   int cut;            // one worker's part
   int longest;        // sequence whose table row gives the shared pages
@@ -194,8 +204,9 @@ __device__ __forceinline__ Plan make_plan(const P& p, const Line& ln, int lane) 
   pl.shared_units = pl.shared_blocks * over_pow2(kBlk, ln.unit);
   pl.live = live;
   pl.shared_tiles = live_tiles(p, ln, live);
-  pl.shared_weight = weight_of(ln, pl.shared_units, cost_of(p, ln, live));
-  pl.head_weight = pl.shared_tiles * pl.shared_weight + own;
+  pl.shared_weight = weight_of(ln, pl.shared_units, shared_cost(p, ln, live, 0));
+  pl.shared_all = shared_weight_all(p, ln, pl.shared_units, live, pl.shared_tiles);
+  pl.head_weight = pl.shared_all + own;
   const int all = pl.head_weight * p.kv_heads;
   pl.cut = max(ln.least, (all + ln.workers - 1) / ln.workers);
   return pl;
@@ -216,12 +227,12 @@ __device__ __forceinline__ Place locate(const P& p, const Line& ln, const Plan& 
   at.t = 0;
   int x = u - at.head * pl.head_weight;
   const int w = pl.shared_weight;
-  if (x < pl.shared_tiles * w) {
+  if (x < pl.shared_all) {
     at.t = x / w;
     at.off = x - at.t * w;
     return at;
   }
-  x -= pl.shared_tiles * w;
+  x -= pl.shared_all;
   for (int b0 = 0; b0 < p.batch; b0 += 32) {
     const int b = b0 + lane;
     const int n = b < p.batch ? own_weight_all(p, ln, extent_of(p, b)) : 0;
@@ -274,7 +285,7 @@ struct PlaceUnits {
 };
 template <class P>
 __device__ __forceinline__ PlaceUnits place_units(const P& p, const Line& ln, const Plan& pl, const Place& at) {
-  if (at.b < 0) return PlaceUnits{pl.shared_units, cost_of(p, ln, pl.live)};
+  if (at.b < 0) return PlaceUnits{pl.shared_units, shared_cost(p, ln, pl.live, at.t)};
   const Extent x = extent_of(p, at.b);
   return PlaceUnits{own_units(p, ln, x, at.t), own_cost(p, ln, x, at.t)};
 }
