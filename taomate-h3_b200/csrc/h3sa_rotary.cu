@@ -14,7 +14,7 @@
 // between, for which an SM has some 350 a warp and 2 KB: a thread keeps to one unit of a head row, 8 pairs in two
 // vectors of 16 bytes, with their frequencies in registers, works out its 8 angles once a token and turns up to eight heads by
 // them, all of which are on their way by then. There is nothing to share and nothing to wait for in a block.
-// Measured: 24605 tokens of 24 heads, bf16, three axes: 51 us, 5.9 TB/s of the 302 MB read and written; 300001 of one head 45 us
+// Measured: 24605 tokens of 24 heads, bf16, three axes: 50 us, 6.05 TB/s of the 302 MB read and written; 300001 of one head 45 us
 // (a table of the block's cosines and sines in shared memory took 57 and 110); appends of 16-bit prompts into e4m3 pools
 // 75 us for 373 MB, 5.0 TB/s, the divisions and conversions beside the loads; a few rows 4.2 us, launch and two dependent loads.
 #include <cuda_bf16.h>
@@ -439,7 +439,8 @@ int vector_of(const RowsParams& p, int size) {
 }
 
 // A task is a head row while threads are few, `most_rows` of them from there on, of which a thread takes up to
-// four: that pays for its frequencies.
+// four: that pays for its frequencies. Tasks of kMany rows pay sooner, and a thread takes two (two / four: 24605 tokens of 24 heads 50.1 /
+// 51.3 us, 30000 of 16 in fp32 78.5 / 83.9, 60000 of 8 heads of 64 26.8 / 26.3; but one head of 300001 49.5 / 44.9, e4m3 prompts 74.9 / 74.3).
 void lay_out(RowsParams& p, int n, int batch, int most_rows) {
   p.tokens = static_cast<long long>(batch) * p.rows;
   p.row_div = divisor(static_cast<uint32_t>(p.rows));
@@ -458,7 +459,8 @@ void lay_out(RowsParams& p, int n, int batch, int most_rows) {
     q.task_div = divisor(static_cast<uint32_t>(q.tasks));
     q.all = p.tokens * q.tasks;
     const long long once = (q.all + q.slots - 1) / q.slots, some = 8 * kSms;
-    q.blocks = static_cast<int>(once <= some ? once : once <= 4 * some ? some : (once + 3) / 4);
+    const int each = most_rows == kMany ? 2 : 4;
+    q.blocks = static_cast<int>(once <= some ? once : once <= each * some ? some : (once + each - 1) / each);
   }
 }
 
