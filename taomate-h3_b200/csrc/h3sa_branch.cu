@@ -32,7 +32,8 @@
 // softmax of few rows over all four warps; the copies are joined in the epilogue. Trees' rows are held once:
 // what bounds the kernel beside the softmax is its own code, streaming past the instruction caches, and the two other
 // forms in between cost trees more than they bring (wide e4m3 trees 237 -> 206 us without them, 64 rows over 16000
-// keys 203 -> 199, e4m3 239 -> 214).
+// keys 203 -> 199, e4m3 239 -> 214). Measured, trees: 24 of 96 rows over up to 9000 keys each 111 us (4.3 TB/s of 472 MB; 5.9 while
+// blocks stream), 20 small ones over 8192 shared keys 66 us, e4m3, four of 635 rows over up to 24001 keys 187 us (620 TFLOP/s).
 // TMEM columns: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P of a tile overwrites the
 // first half of its S. A tile's MMAs are issued in order by one warp, so the barrier of a QK^T also
 // says that the tile's previous P V is complete.
@@ -96,7 +97,8 @@ struct BrCfg {
   static constexpr int kStages = kFp8 ? 6 : 5;  // even for e4m3: K in the even slots, V in the odd ones
   static constexpr int kSteps = kFp8 ? 4 : 8;   // MMA K steps of S
   // Order of a segment's loads: K0 K1 V0 K2 V1 ..., each V behind the next K, which is wanted first (V waits for a
-  // softmax); e4m3: K0 V0 K1 V1 ..., as V is widened on its way.
+  // softmax, in a slot of the ring: 24 trees of 96 rows over 9000 keys 130 -> 111 us, 24 chains of 4 x 32 rows over 8192 shared
+  // keys 50.7 -> 49.8); e4m3: K0 V0 K1 V1 ..., as V is widened on its way.
   static constexpr bool kSkew = !kFp8;
   static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
   static constexpr uint32_t kIdescPV = kFp8 ? idesc_f16(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
@@ -1454,18 +1456,19 @@ constexpr long long kWarpSharedWork = 600000;  // KV heads x keys x 16-row tiles
 constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 
 // Trees of 17 to 64 stacked rows. The warp line reads a tree's keys once for every 16 rows, the tensor line once, but starts
-// some 13 us later, so what decides is the keys, of which the host knows the tables' width. us a million keys and KV
-// heads: warps 44 for each 16 rows (e4m3 35), tensor cores 89 (66) an item. 8 KV heads, bf16, warp / tensor (us): 64 rows, 24
-// trees of up to 1000 keys 48 / 60, 4000 112 / 85, 16000 373 / 200; 48 rows, 1000 39 / 54, 16000 268 / 175; 32 rows, 16000 227 / 189;
-// one tree of 64 rows over up to 60000 144 / 71; e4m3: 64 rows, 1000 47 / 58, 4000 100 / 86, 16000 295 / 156; 48 rows, 4000 76 / 82. With
-// shared keys (20 trees of 52 rows over 1024 and up to 700 of their own 73 / 52) both parts are in one kernel.
+// some 6 us later (e4m3 10), so what decides is the keys, of which the host knows the tables' width. 8 KV heads, bf16, tensor / warp
+// (us): 64 rows, 24 trees of up to 1000 keys 48.5 / 46.4, 4000 72 / 112, 16000 164 / 413; 48 rows, 1000 44 / 37, 4000 64 / 77; 32 rows,
+// 2000 48 / 42, 4000 59 / 62, 16000 153 / 228; 24 rows, 2000 46 / 36, 8000 91 / 111; one tree of 64 rows over up to 8000 29 / 27, 16000
+// 35 / 39, 40000 49 / 82; e4m3: 64 rows, 24 trees of 2000 73 / 64, 4000 90 / 96, 16000 157 / 281; 48 rows, 4000 84 / 74, 8000 114 / 136; 32
+// rows, 16000 148 / 153. Shared keys (20 trees of 48 rows over 4096 and up to 700 of their own: 55 / 63, e4m3 64 / 62) count by
+// the tiles of all trees' rows.
 bool tree_on_tensor(int batch, int own, int kv_heads, int shared, int width, bool e4m3) {
   if (own <= kRowSpan) return false;
   const auto tiles = [](long long n, int span) { return (n + span - 1) / span; };
   const long long keys = static_cast<long long>(batch) * (width - shared) * kBlk, all = static_cast<long long>(batch) * own;
   const double warps = static_cast<double>(kv_heads) * (keys * tiles(own, kRowSpan) + 1.0 * shared * kBlk * tiles(all, kRowSpan));
   const double tensor = static_cast<double>(kv_heads) * (keys + 1.4 * shared * kBlk * tiles(all, kSpan));
-  return e4m3 ? warps - 1.9 * tensor > 640000.0 : warps - 1.7 * tensor > 570000.0;
+  return e4m3 ? warps - 2.0 * tensor > 420000.0 : warps - 1.3 * tensor > 340000.0;
 }
 
 // The shape of a tree's call has the tables' width, a chain's 0.

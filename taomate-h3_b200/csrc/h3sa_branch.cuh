@@ -121,9 +121,9 @@ __device__ __forceinline__ int own_units(const P& p, const Line& ln, const Exten
 }
 // What a unit of an item of `rows` rows weighs: 1, or of the tensor line in a tree's call one of the two below (of
 // chains all weigh the same). Blocks of up to 128 and of more rows take a CTA 1.5 to 1.75 and 2.6 us (e4m3 1.1 and 2.1), and
-// an item 4 to 6 us (8 to 12) from its last scores to the next one's first. Weight of an item, 8 / 16 / 24 (us): 24 trees of 96
-// rows over 9000 keys 130.5 / 130 / 133.5, 20 small trees over 8192 shared keys 73 / 70.5 / 71; e4m3, 16 / 24 / 40: wide trees
-// 188.7 / 188 / 186, 24 trees of 64 rows over 16000 keys 163 / 160 / 158.
+// an item 4 to 6 us (8 to 12) from its last scores to the next one's first. Weight of an item, 12 / 16 / 20 (us): 24 trees of 96
+// rows over 9000 keys 113.4 / 111.5 / 112.1, 12 trees of up to 240 over shared and own keys 74.2 / 72.6 / 73.6; e4m3, 16 / 24 / 40: wide
+// trees 188.7 / 188 / 186, 24 trees of 64 rows over 16000 keys 163 / 160 / 158.
 constexpr int kFewCost = 5, kManyCost = 8, kTreePad = 16, kTreePadF8 = 40;
 template <class P>
 __device__ __forceinline__ int cost_of(const P&, const Line& ln, int rows) {
