@@ -603,12 +603,13 @@ H3SA_API int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value,
                               int32_t* device_error, void* stream);
 
 /* Attention of the drafted rows of every sequence: row i of sequence b, i < counts[b], sees keys
- * j < lengths[b] and lengths[b] + n for each n < counts[b] whose bit is set in masks [batch, rows, ceil(rows / 32)]
- * (h3sa_draft_tree's, or any others). All else is h3sa_shared_prefix_attention's (shared_rows may not pass the lengths of the sequences that hold the shared pages; one
- * whose length ends in front of them is read by itself). Rows behind counts[b], and rows that see
- * nothing, come out zero. An infinity or NaN in K or V of a drafted row reaches only the rows that see it; one
- * in V of a sequence's first lengths[b] rows makes all its outputs in that column infinite or NaN. A
- * length or count outside its range, or both together past the table, is clamped with
+ * j < lengths[b] and lengths[b] + n for each n < counts[b] whose bit is set in masks
+ * [batch, rows, ceil(rows / 32)] (h3sa_draft_tree's, or any others). All else is
+ * h3sa_shared_prefix_attention's (shared_rows may not pass the lengths of the sequences that hold the
+ * shared pages; one whose length ends in front of them is read by itself). Rows behind counts[b], and
+ * rows that see nothing, come out zero. An infinity or NaN in K or V of a drafted row reaches only the
+ * rows that see it; one in V of a sequence's first lengths[b] rows makes all its outputs in that column
+ * infinite or NaN. A length or count outside its range, or both together past the table, is clamped with
  * H3SA_DEVERR_BAD_INDEX. workspace may be NULL where h3sa_tree_workspace is 0. */
 H3SA_API int64_t h3sa_tree_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
                                      int32_t shared_rows, int32_t width, int32_t e4m3);
