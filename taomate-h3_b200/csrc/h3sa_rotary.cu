@@ -91,8 +91,9 @@ __device__ __forceinline__ uint64_t turn_of(double f) {
   const double r = hi - ((hi + 6755399441055744.0) - 6755399441055744.0);  // 1.5 * 2^52
   const double top = r + 1572864.0;                                        // 1.5 * 2^20: last bit 2^-32
   const double rest = r - (top - 1572864.0) + lo;
-  return (static_cast<uint64_t>(static_cast<uint32_t>(__double2loint(top))) << 32) +
-         static_cast<uint64_t>(static_cast<long long>(__double2loint(rest + 0.0003662109375)));  // 1.5 * 2^-12: 2^-64
+  // 1.5 * 2^-12: last bit 2^-64. As a difference of all 64 bits: where top was a tie, rest may be 2^-33 and have 33 bits.
+  const long long low = __double_as_longlong(rest + 0.0003662109375) - __double_as_longlong(0.0003662109375);
+  return (static_cast<uint64_t>(static_cast<uint32_t>(__double2loint(top))) << 32) + static_cast<uint64_t>(low);
 }
 // What a pair needs of its frequency: turn_of it, or for positions between whole numbers the bits of f / 2 pi.
 __device__ __forceinline__ uint64_t frequency_word(const Angles& a, int pair) {
