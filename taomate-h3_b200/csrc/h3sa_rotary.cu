@@ -89,8 +89,9 @@ __device__ __forceinline__ uint64_t turn_of(double f) {
   const double hi = f * 0.15915494309189535;  // 1 / (2 pi), less 9.8e-18
   const double lo = fma(f, 0.15915494309189535, -hi) + f * -9.839338337591243e-18;
   const double r = hi - ((hi + 6755399441055744.0) - 6755399441055744.0);  // 1.5 * 2^52
-  const double top = r + 1572864.0;                                        // 1.5 * 2^20: last bit 2^-32
-  const double rest = r - (top - 1572864.0) + lo;
+  const double t = r + lo, off = (r - t) + lo;  // of a large f, lo too has bits in front of 2^-32
+  const double top = t + 1572864.0;             // 1.5 * 2^20: last bit 2^-32
+  const double rest = t - (top - 1572864.0) + off;
   // 1.5 * 2^-12: last bit 2^-64. As a difference of all 64 bits: where top was a tie, rest may be 2^-33 and have 33 bits.
   const long long low = __double_as_longlong(rest + 0.0003662109375) - __double_as_longlong(0.0003662109375);
   return (static_cast<uint64_t>(static_cast<uint32_t>(__double2loint(top))) << 32) + static_cast<uint64_t>(low);

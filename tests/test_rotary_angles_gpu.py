@@ -60,3 +60,12 @@ def test_frequencies_at_a_tie_at_rows_own_places() -> None:
         row = pools[0][0, (length + i) % 128].double().cpu()
         for have, want in ((row[:len(TIES)], cos[i]), (row[len(TIES):2 * len(TIES)], sin[i])):
             assert (have - torch.from_numpy(want)).abs().max() <= 2.0 ** -9 + 2.0 ** -20
+
+
+def test_large_frequencies() -> None:
+    """Up to 2^48 radians a position, where the product with 1 / (2 pi) takes more than the 32 bits behind those of a turn."""
+
+    rng = np.random.default_rng(0)
+    frequencies = rng.choice([-1.0, 1.0], 64) * rng.uniform(1.0, 2.0, 64) * 2.0 ** rng.integers(10, 48, 64)
+    _check([0, 1, -3, 1000], torch.int32, frequencies, 2.0 ** -21)
+    _check([1, 77777, -(1 << 31)], torch.int64, frequencies[np.abs(frequencies) < 2.0 ** 40], 2.0 ** -21)
