@@ -107,29 +107,32 @@ __device__ __forceinline__ uint64_t position_word(const Angles& a, long long tok
   if (a.kind == kPosI32) return static_cast<uint64_t>(static_cast<long long>(__ldg(static_cast<const int*>(a.positions) + at)));
   return __ldg(static_cast<const unsigned long long*>(a.positions) + at);
 }
-// The fraction of a turn, in [-1/2, 1/2).
-__device__ __forceinline__ float fraction(bool between, uint64_t position, uint64_t frequency) {
-  uint32_t hi;
-  if (!between) {
-    hi = static_cast<uint32_t>((position * frequency) >> 32);
-  } else {  // in 64-bit arithmetic, whole turns taken off by one rounding
-    const double p = __longlong_as_double(static_cast<long long>(position));
-    const double unit = __longlong_as_double(static_cast<long long>(frequency)), t = p * unit;
-    const double whole = (t + 6755399441055744.0) - 6755399441055744.0;
-    hi = static_cast<uint32_t>(__double2loint(fma(p, unit, -whole) + 1572864.0));
-  }
-  return static_cast<float>(static_cast<int>(hi)) * 2.3283064365386963e-10f;  // 2^-32
+// The fraction of a turn, in [-1/2, 1/2), in units of 2^-32.
+__device__ __forceinline__ int fraction(bool between, uint64_t position, uint64_t frequency) {
+  if (!between) return static_cast<int>(static_cast<uint32_t>((position * frequency) >> 32));
+  // in 64-bit arithmetic, whole turns taken off by one rounding
+  const double p = __longlong_as_double(static_cast<long long>(position));
+  const double unit = __longlong_as_double(static_cast<long long>(frequency)), t = p * unit;
+  const double whole = (t + 6755399441055744.0) - 6755399441055744.0;
+  return __double2loint(fma(p, unit, -whole) + 1572864.0);
 }
 // Cosine and sine of a fraction of a turn. For 16-bit values the approximate functions, off by up to 2^-21, which is
-// 2^-10 of their rounding.
+// 2^-10 of their rounding. For 32 bits the fraction's first 24 bits, which a float holds, by the function, and the other 8,
+// an angle below 2^-21, by the first term of the sums' formulas: all 32 in one float are off by up to 2^-26 of a turn, more
+// than the results' own rounding (rotations at positions to 2^31 off by 4.5e-8 of their length, with one float 5.7e-8; with
+// cosines and sines taken in 64 bits 4.2e-8. 300001 tokens of one head 64.6 us, with one float 62.6, others the same).
 template <typename T>
-__device__ __forceinline__ void cos_sin(float fraction, float factor, float& c, float& s) {
+__device__ __forceinline__ void cos_sin(int fraction, float factor, float& c, float& s) {
   if constexpr (sizeof(T) == 2) {
-    const float a = fraction * 6.2831853071795865f;
+    const float a = static_cast<float>(fraction) * 2.3283064365386963e-10f * 6.2831853071795865f;  // 2^-32
     s = __sinf(a);
     c = __cosf(a);
   } else {
-    sincospif(2.0f * fraction, &s, &c);
+    const float rest = static_cast<float>(fraction & 0xff) * 1.4629180792671596e-9f;  // 2 pi 2^-32
+    float c0, s0;
+    sincospif(static_cast<float>(fraction & ~0xff) * 4.6566128730773926e-10f, &s0, &c0);  // 2^-31
+    c = fmaf(-s0, rest, c0);
+    s = fmaf(c0, rest, s0);
   }
   c *= factor;
   s *= factor;
