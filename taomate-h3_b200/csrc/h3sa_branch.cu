@@ -979,9 +979,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           for (int c = 0; c < kD; ++c) {  // column by column, for its code: it is seldom needed
             const float lost = my < n_rows ? nodes.non_finite_sum(p, sight, c) : 0.f;
             __syncwarp();
-            const uint32_t o = tmem_ld1(tO + c);
-            tmem_wait_ld();
-            tmem_st1(tO + c, __float_as_uint(__uint_as_float(o) + lost));
+            tmem_st1(tO + c, __float_as_uint(__uint_as_float(tmem_ld1(tO + c)) + lost));
           }
           tmem_wait_st();
         }

@@ -207,10 +207,15 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
       H3SA_W8(0), H3SA_W8(8)
       : "memory");
 }
-// One column.
+// One column, read and waited for in one statement: what it returns may be used at once.
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   uint32_t r;
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r)
+      : "r"(taddr)
+      : "memory");
   return r;
 }
 __device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
