@@ -424,28 +424,31 @@ __device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows
 
 // Clears what must not be multiplied in V's block of a sequence's last rows: rows at or past `rows` of it may
 // hold anything, and nodes' infinities and NaN (rows from `clean` on) belong to those that see them. The block's
-// load has completed; both warps of a block of two tiles write the same. Returns whether this lane met one.
+// load has completed. Both MMA warps clear a block of two tiles, each what the other has left, so the one that comes second
+// may find nothing: `taken_out` is set before the value goes, and whoever finds it gone passes both on by its own barriers.
 template <bool kTree>
-__device__ __forceinline__ bool clear_block(uint8_t* base, int rows, int clean, int lane) {
-  uint32_t met = 0u;
+__device__ __forceinline__ void clear_block(uint32_t base, int rows, int clean, int lane, volatile int* taken_out) {
+  const auto store = [](uint32_t at, const uint4& v) {
+    asm volatile("st.volatile.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+  };
   if constexpr (kTree) {
     const int from = max(0, clean);
     for (int i = lane; i < (min(rows, kBlk) - from) * 16; i += 32) {
-      const int row = from + (i >> 4), a = (i >> 3) & 1;
-      uint4& v = reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7];
+      const uint32_t at = base + (i >> 3 & 1) * kAtom + (from + (i >> 4)) * 128 + (i & 7) * 16;
+      uint4 v;
+      asm volatile("ld.volatile.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
       const uint4 bad = make_uint4(non_finite<0x7f80u>(v.x), non_finite<0x7f80u>(v.y), non_finite<0x7f80u>(v.z),
                                    non_finite<0x7f80u>(v.w));
       if (bad.x | bad.y | bad.z | bad.w) {
-        v = make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w);
-        met = 1u;
+        *taken_out = 1;
+        __threadfence_block();
+        store(at, make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w));
       }
     }
+    __threadfence_block();
   }
-  for (int i = lane; i < (kBlk - rows) * 16; i += 32) {
-    const int row = rows + (i >> 4), a = (i >> 3) & 1;
-    reinterpret_cast<uint4*>(base + a * kAtom + row * 128)[i & 7] = make_uint4(0u, 0u, 0u, 0u);
-  }
-  return met != 0u;
+  for (int i = lane; i < (kBlk - rows) * 16; i += 32)
+    store(base + (i >> 3 & 1) * kAtom + (rows + (i >> 4)) * 128 + (i & 7) * 16, make_uint4(0u, 0u, 0u, 0u));
 }
 
 template <bool kFp8, class P>
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         mbar_init(smem_u32(&sm.p_full[t][h]), 128);
       }
       mbar_init(smem_u32(&sm.pv_done[t]), 1);
-      mbar_init(smem_u32(&sm.o_full[t]), 1);
+      mbar_init(smem_u32(&sm.o_full[t]), kTree ? 2 : 1);
       mbar_init(smem_u32(&sm.wg[t]), 128);
     }
     if constexpr (kFp8) {
@@ -734,10 +737,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
       if (!kFp8 && min(pend_rows, kTree ? pend_clean : kBlk) < kBlk && half == 0) {  // e4m3: done when widened
-        const bool met = clear_block<kTree>(sm.kv[pend_slot], min(pend_rows, kBlk), pend_clean, lane);
-        if constexpr (kTree) {
-          if (met) *static_cast<volatile int*>(&sm.tree.taken_out) = 1;
-        }
+        volatile int* taken_out = nullptr;
+        if constexpr (kTree) taken_out = &sm.tree.taken_out;
+        clear_block<kTree>(smem_u32(sm.kv[pend_slot]), min(pend_rows, kBlk), pend_clean, lane, taken_out);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
@@ -778,6 +780,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if (ok) finish(1);
       if (!ok) return;
       tc_commit(o_bar);
+      if constexpr (kTree) {  // and what this warp knows of taken_out
+        __syncwarp();
+        if (lane == 0) mbar_arrive(o_bar);
+      }
       free_v();
     };
     const auto wrap = [](int slot) { return slot >= kS ? slot - kS : slot; };
