@@ -79,6 +79,7 @@ constexpr int kAtom = kBlk * 128;  // 128 rows of one 128-byte swizzle atom
 // One item segment of a CTA, as warp 0 publishes it.
 struct Segment {
   int live;      // 0: the CTA's last descriptor; 2: against the shared blocks
+  int number;    // of the CTA's segments, from 1
   int head;      // KV head
   int row0;      // first stacked query row of the item
   int n_rows;    // rows of the item (1..256)
@@ -119,13 +120,24 @@ struct BrWide<true> {  // begins at a multiple of 1024 bytes, as the tiles in fr
   uint64_t full[2][kWide], empty[2][kWide];
 };
 
+// By tile, the numbers of the segments in whose V a node had an infinity or NaN. A tile's epilogue reads the one of its segment when
+// its warps have taken one of the next two, and no warp can be more than the descriptors' ring in front of that: places of
+// twice the ring are not taken again before they are read.
+constexpr int kTakenOut = 2 * kDescRing;
 template <class P>
 struct BrTree {};
 template <>
 struct BrTree<TreeParams> {
-  int taken_out;          // whether a node's V held an infinity or NaN
+  int taken_out[2][kTakenOut];
   int before[kMaxStack];  // see live_row_at
 };
+
+// Of tile `t`, or both where they share the segment's blocks.
+__device__ __forceinline__ void mark_taken_out(BrTree<TreeParams>& tree, const Segment& g, int t) {
+  const int at = g.number % kTakenOut;
+  *static_cast<volatile int*>(&tree.taken_out[t][at]) = g.number;
+  if (g.n_rows > kBlk) *static_cast<volatile int*>(&tree.taken_out[t ^ 1][at]) = g.number;
+}
 
 template <bool kFp8, class P>
 struct alignas(1024) BrSmem {
@@ -425,9 +437,10 @@ __device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows
 // Clears what must not be multiplied in V's block of a sequence's last rows: rows at or past `rows` of it may
 // hold anything, and nodes' infinities and NaN (rows from `clean` on) belong to those that see them. The block's
 // load has completed. Both MMA warps clear a block of two tiles, each what the other has left, so the one that comes second
-// may find nothing: `taken_out` is set before the value goes, and whoever finds it gone passes both on by its own barriers.
-template <bool kTree>
-__device__ __forceinline__ void clear_block(uint32_t base, int rows, int clean, int lane, volatile int* taken_out) {
+// may find nothing: it is marked (for both tiles) before the value goes, and whoever finds it gone passes that on by its
+// own barriers.
+template <bool kTree, typename Mark>
+__device__ __forceinline__ void clear_block(uint32_t base, int rows, int clean, int lane, Mark&& mark) {
   const auto store = [](uint32_t at, const uint4& v) {
     asm volatile("st.volatile.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
   };
@@ -440,7 +453,7 @@ __device__ __forceinline__ void clear_block(uint32_t base, int rows, int clean, 
       const uint4 bad = make_uint4(non_finite<0x7f80u>(v.x), non_finite<0x7f80u>(v.y), non_finite<0x7f80u>(v.z),
                                    non_finite<0x7f80u>(v.w));
       if (bad.x | bad.y | bad.z | bad.w) {
-        *taken_out = 1;
+        mark();
         __threadfence_block();
         store(at, make_uint4(v.x & ~bad.x, v.y & ~bad.y, v.z & ~bad.z, v.w & ~bad.w));
       }
@@ -507,7 +520,9 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     mbar_init(smem_u32(&sm.m_sync), 2);
     mbar_init(smem_u32(&sm.drain), 2);
     sm.abort_flag = 0;
-    if constexpr (kTree) sm.tree.taken_out = 0;
+    if constexpr (kTree) {
+      for (int n = 0; n < kTakenOut; ++n) sm.tree.taken_out[0][n] = sm.tree.taken_out[1][n] = 0;
+    }
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -570,10 +585,11 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     uint32_t used0 = 0u, used1 = 0u, free0 = 0u, free1 = 0u, on_tile1 = 0u, full0 = 0u, full1 = 0u;
     int ds = 0, ds_phase = 0;
     bool ok = true;
-    while (ok) {
+    for (int number = 1; ok; ++number) {
       // ---- the next segment: what is left of the current item within the CTA's range
       Segment g;
       memset(&g, 0, sizeof(g));
+      g.number = number;
       int seq = 0;
       while (u < u_end && !g.live) {
         const PlaceUnits it = place_units(p, ln, pl, at);
@@ -731,15 +747,16 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     bool pend = false, pend_acc = false;
     int pend_slot = 0, pend_rows = 0, pend_clean = 0;
     uint32_t pend_bar = 0u, pend_ph = 0u;
+    Segment g;  // which holds the pending block
     // Waits for P of one half of the pending block and issues its P V.
     auto finish = [&](int half) {
       const bool w = mbar_wait(p_bar + half * 8, p_ph, abort_flag, p.err);
       if (!(ok = __all_sync(0xffffffffu, w))) return;
       tc_fence_after();
       if (!kFp8 && min(pend_rows, kTree ? pend_clean : kBlk) < kBlk && half == 0) {  // e4m3: done when widened
-        volatile int* taken_out = nullptr;
-        if constexpr (kTree) taken_out = &sm.tree.taken_out;
-        clear_block<kTree>(smem_u32(sm.kv[pend_slot]), min(pend_rows, kBlk), pend_clean, lane, taken_out);
+        clear_block<kTree>(smem_u32(sm.kv[pend_slot]), min(pend_rows, kBlk), pend_clean, lane, [&]() {
+          if constexpr (kTree) mark_taken_out(sm.tree, g, mt);
+        });
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
@@ -787,7 +804,6 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       free_v();
     };
     const auto wrap = [](int slot) { return slot >= kS ? slot - kS : slot; };
-    Segment g;
     while (ok && next_segment(g)) {
       const bool pair = g.n_rows > kBlk;
       if (pair && was_solo) {
@@ -889,7 +905,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     struct Item {
       int mine, begin, step;  // blocks of this tile: how many, the first, every step-th
       int block0, head, row0, n_rows, span;  // of this tile; span: rows a copy has room for
-      int direct, shared;
+      int marks;  // four times the segment's number, 2 if against the shared blocks, 1 if direct (in one register)
       long long ws_row;
       RowAt at;  // this thread's row
     };
@@ -914,11 +930,10 @@ __global__ void __launch_bounds__(kBrThreads, 1)
         it.block0 = g.block0 + it.begin;
         it.head = g.head;
         it.row0 = g.row0 + r0;
-        it.direct = g.direct;
-        it.shared = g.live == 2;
+        it.marks = 4 * g.number + (g.live == 2 ? 2 : 0) + g.direct;
         const int my = lr & (it.span - 1);
         const int row = it.row0 + min(my, it.n_rows - 1);
-        if constexpr (kTree) it.at = it.shared && p.compact ? live_row_at(p, sm.tree.before, g.head, row) : row_at(p, g.head, row);
+        if constexpr (kTree) it.at = (it.marks & 2) && p.compact ? live_row_at(p, sm.tree.before, g.head, row) : row_at(p, g.head, row);
         else it.at = row_at(p, g.head, row);
         const uint4* src = reinterpret_cast<const uint4*>(p.q + it.at.b * p.q_sb + it.at.i * p.q_sn + it.at.h * p.q_sh);
 #pragma unroll
@@ -931,6 +946,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     bool more = take(next);
     while (more) {
       const Item it = next;
+      const bool direct = it.marks & 1;
       const int span = kTree ? kBlk : it.span, n_rows = it.n_rows, copies = kBlk / span;
       const int my = lr & (span - 1);  // this thread's row of the tile
       const int copy = lr / span;      // and which copy of it
@@ -938,7 +954,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       if constexpr (kFp8) sl2 = score_factor(sl2 * __ldg(p.k_scale + it.head));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&sm.q_full[t]));
-      const auto sight = sight_of(p, it.at, it.shared != 0);
+      const auto sight = sight_of(p, it.at, (it.marks & 2) != 0);
       const bool warp_live = quad * 32 % span < n_rows;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; ok && j < it.mine; ++j) {
@@ -979,11 +995,13 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       o_ph ^= 1u;
       tc_fence_after();
       if constexpr (kTree) {  // what was taken out of V, to the rows that see it
-        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&sm.tree.taken_out) != 0)) {
+        const volatile int& taken_out = sm.tree.taken_out[t][it.marks / 4 % kTakenOut];
+        if (__any_sync(0xffffffffu, taken_out == it.marks / 4)) {
           const NodeValues<kFp8> nodes(p, it.at.b, it.head);
+          const int key_end = (it.block0 + (it.mine - 1) * it.step + 1) * kBlk;
 #pragma unroll 1
           for (int c = 0; c < kD; ++c) {  // column by column, for its code: it is seldom needed
-            const float lost = my < n_rows ? nodes.non_finite_sum(p, sight, c) : 0.f;
+            const float lost = my < n_rows ? nodes.non_finite_sum(p, sight, c, it.block0 * kBlk, key_end, it.step) : 0.f;
             __syncwarp();
             tmem_st1(tO + c, __float_as_uint(__uint_as_float(tmem_ld1(tO + c)) + lost));
           }
@@ -1009,13 +1027,13 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       }
       // A copy that saw nothing weighs nothing; sums that are NaN stay so.
       float weight = l == 0.f ? 0.f : fast_exp2(m - top);
-      if (it.direct) {
+      if (direct) {
         weight = sum == 0.f ? 0.f : weight / sum;
         if constexpr (kFp8) weight *= __ldg(p.v_scale + it.head);
       }
       if (my < n_rows && copy == 0) {
         const float base = top - (kFp8 ? kBoostF8 : 0.f);
-        if (!it.direct) p.part_ml[it.ws_row + my] = make_float2(base, sum);
+        if (!direct) p.part_ml[it.ws_row + my] = make_float2(base, sum);
         else if (p.lse)
           p.lse[(static_cast<long long>(it.at.b) * p.rows + it.at.i) * p.heads + it.at.h] =
               sum == 0.f ? -INFINITY : (base + log2f(sum)) * 0.6931471805599453f;
@@ -1055,7 +1073,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
             const int lo = __shfl_sync(0xffffffffu, static_cast<int>(own_dst), r);
             const int hi = __shfl_sync(0xffffffffu, static_cast<int>(own_dst >> 32), r);
             if (quad * 32 + r >= n_rows) continue;
-            if (it.direct) {
+            if (direct) {
               const long long dst = static_cast<long long>(static_cast<uint32_t>(lo)) | (static_cast<long long>(hi) << 32);
               *reinterpret_cast<uint2*>(p.out + dst + half * 64 + c4 * 4) =
                   make_uint2(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w));
@@ -1102,7 +1120,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
               a.z += v.z;
               a.w += v.w;
             }
-            if (it.direct) {
+            if (direct) {
               const RowAt ra = row_at(p, it.head, it.row0 + r);
               __nv_bfloat16* dst =
                 p.out + ((static_cast<long long>(ra.b) * p.rows + ra.i) * p.heads + ra.h) * kD;
@@ -1155,8 +1173,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           const uint32_t from = smem_u32(sm.kv[ring]), to = smem_u32(sm.wide.v[wide]);
           if (kTree && clean < kBlk) {
             if constexpr (kTree) {
-              if (widen_block<true, true>(from, to, rows, clean, lane))
-                *static_cast<volatile int*>(&sm.tree.taken_out) = 1;
+              if (widen_block<true, true>(from, to, rows, clean, lane)) mark_taken_out(sm.tree, g, side);
             }
           } else if (kTree || rows >= kBlk) {  // a tree's last rows are nodes
             widen_block<false, false>(from, to, kBlk, 0, lane);

@@ -446,11 +446,14 @@ struct NodeValues {
       : pool(static_cast<const uint8_t*>(p.value_pool) +
              static_cast<size_t>(head) * p.pool_pages * kBlk * (kD * (kFp8 ? 1 : 2))),
         table(p.table + static_cast<size_t>(b) * p.width) {}
-  // The infinities and NaN of column `col` in the nodes that a row sees, added up; 0 if there are none.
-  __device__ __forceinline__ float non_finite_sum(const TreeParams& p, const Sight& sight, int col) const {
+  // The infinities and NaN of column `col` in the nodes that a row sees, added up; 0 if there are none. Only of keys in
+  // [from, to), and of every step-th (1 or 2) block there: those of other pieces are added to them, and here, where
+  // this piece's weight may vanish, they would make NaN.
+  __device__ __forceinline__ float non_finite_sum(const TreeParams& p, const Sight& sight, int col, int from, int to, int step) const {
     float sum = 0.f;
-    for (int n = 0; n < sight.count; ++n) {
-      if (!(sight.word(p, n >> 5) >> (n & 31) & 1u)) continue;
+    if (sight.hidden()) return sum;
+    for (int n = max(0, from - sight.base), end = min(sight.count, to - sight.base); n < end; ++n) {
+      if (!(sight.word(p, n >> 5) >> (n & 31) & 1u) || (((sight.base + n - from) / kBlk) & (step - 1))) continue;
       const int key = sight.base + n, page = __ldg(table + key / kBlk);
       if (page < 0 || page >= p.pool_pages) continue;
       const size_t at = (static_cast<size_t>(page) * kBlk + key % kBlk) * kD + col;

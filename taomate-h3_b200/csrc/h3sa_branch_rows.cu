@@ -520,7 +520,9 @@ __global__ void __launch_bounds__(2 * 32 * kRowWarps, 1)
 #pragma unroll 1
         for (int k = 0; k < 32; ++k) {  // one column's code: it is seldom needed
           const int col = column_of<kFp8>(c, k >> 1, k & 1);
-          const float lost0 = nodes.non_finite_sum(p, sight0, col), lost1 = nodes.non_finite_sum(p, sight1, col);
+          const int end = g.key0 + g.units * kRowUnit;
+          const float lost0 = nodes.non_finite_sum(p, sight0, col, g.key0, end, 1);
+          const float lost1 = nodes.non_finite_sum(p, sight1, col, g.key0, end, 1);
 #pragma unroll
           for (int j = 0; j < 16; ++j)
 #pragma unroll

@@ -64,3 +64,43 @@ def test_values_that_one_tile_alone_sees(seen_by, kind) -> None:
     got = call(call.k, v, times=50)
     assert torch.equal(torch.isnan(got), torch.isnan(want))
     assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
+
+
+@pytest.mark.parametrize("nodes", [24, 48])  # 96 rows: one tile; 192: both
+def test_an_infinity_stays_in_its_item(nodes) -> None:
+    """CTAs go on from an item whose node holds an infinity to the first blocks of the next, all of whose weight is in
+    later blocks: nodes score far above the history, whose part in the output vanishes. What the node adds is infinite and
+    not infinity times a vanished weight."""
+
+    lengths, counts = [1100 + 13 * i for i in range(24)], [nodes] * 24
+    sees = np.tri(nodes, dtype=bool)[None].repeat(24, 0)
+    call = _Call(lengths, counts, 32, 8, sees)
+    call.q = torch.full_like(call.q, 1.5)
+    k, v = call.k.clone(), call.v.clone()
+    for b in range(24):
+        for n in range(nodes):
+            k[:, call.node(b, n)] = 40.0
+        v[:, call.node(b, 0), 7] = float("inf")
+    want = call(k, call.v)
+    want[..., 7] = float("inf")
+    assert torch.equal(call(k, v), want)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("lengths,nodes,heads,kv", [([128 * 30 + 100] * 2, 60, 8, 1), ([128 * 70 + 127, 900, 20], 24, 4, 1), ([700, 40], 9, 4, 2)])
+def test_nodes_of_several_blocks_and_pieces(lengths, nodes, heads, kv, kind) -> None:
+    """Bad values in nodes on both sides of a page's end, seen by some rows each."""
+
+    counts = [nodes - i for i in range(len(lengths))]
+    rng = np.random.default_rng(3)
+    sees = rng.random((len(lengths), nodes, nodes)) < 0.3
+    sees &= (np.arange(nodes) < np.array(counts)[:, None])[:, None, :]
+    call = _Call(lengths, counts, heads, kv, sees, kind=kind)
+    want, v = call(call.k, call.v), call.v.clone()
+    for b, count in enumerate(counts):
+        for n, column in ((0, 3), (count // 2, 64), (count - 1, 127), (count - 1, 3)):
+            v[:, call.node(b, n), column] = torch.tensor(float("nan")).to(v.dtype)
+            want[b, :count, :, column][torch.from_numpy(sees[b, :count, n])] = float("nan")
+    got = call(call.k, v, times=3)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(nan=0.0), want.nan_to_num(nan=0.0))
