@@ -581,15 +581,17 @@ typedef struct h3sa_rotary {
 } h3sa_rotary;
 
 /* out = x rotated, both of `dtype`. dim: at most 1024. out may be x itself (same address and strides),
- * else they may not overlap; rows of out may not overlap each other. Any strides and alignment of whole elements; 16 or 8 bytes are read at a time
- * where pairs, dim, strides and addresses are multiples of them. */
+ * else they may not overlap. Rows of out may not overlap each other: an axis of out steps over all that those of smaller
+ * steps reach, as in slices and transposed views. Any other strides and alignment of whole elements; 16 or 8 bytes are
+ * read at a time where pairs, dim, strides and addresses are multiples of them. */
 H3SA_API int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32_t batch,
                          int32_t rows, int32_t dim, const h3sa_rotary* rotary, void* stream);
 
 /* Appends rows i < counts[b] of key and value (bf16, heads of 128) to the pages of their sequences, at
  * rows lengths[b] + i through the table (int32 [batch, width]); lengths stay as they are. Keys are
  * rotated on the way, and so is query into query_out (both NULL if there is none; query_out may be query
- * itself, else it overlaps no other argument, and its rows not each other); its rows behind counts[b] come out zero. rotary NULL: nothing is. Pools
+ * itself, else it overlaps no other argument, and its rows not each other, see h3sa_rotate); its rows behind counts[b] come
+ * out zero. rotary NULL: nothing is. Pools
  * [kv_heads, pool_pages * 128, 128], 16-byte aligned, bf16, or e4m3 with positive k_scale / v_scale fp32
  * [kv_heads], by which rows are divided (rounded once, limited to 448, NaN stays NaN). A row past the table's
  * width, or of a sequence of negative length, sets H3SA_DEVERR_BAD_INDEX, a page outside the pool

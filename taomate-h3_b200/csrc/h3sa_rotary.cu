@@ -21,6 +21,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstring>
 #include <type_traits>
 
@@ -494,11 +495,26 @@ int check_rotary(const char* what, const h3sa_rotary* r, int dim, bool rows_know
 // Strides of heads are kept in 32 bits.
 bool head_stride_ok(const h3sa_heads* h) { return !h || (h->stride_head >= INT32_MIN && h->stride_head <= INT32_MAX); }
 
-// Rows that are written lie apart: those of a tensor that repeats some by a stride of zero would be written from
-// several places, and read and written at once in place.
+// Rows that are written lie apart: those of a tensor that repeats some by a stride of zero, or by one axis' steps into
+// another's, would be written from several places, and read and written at once in place. Every axis steps over all that
+// the ones of smaller steps reach, as the axes of any slice or transposed view do.
 bool rows_apart(const h3sa_heads* h, int batch, int rows, int dim) {
-  const auto apart = [&](long long n, long long stride) { return n < 2 || stride >= dim || stride <= -dim; };
-  return apart(batch, h->stride_sequence) && apart(rows, h->stride_row) && apart(h->heads, h->stride_head);
+  struct Axis {
+    long long n;
+    unsigned long long step;
+  };
+  const auto axis = [](long long n, int64_t stride) {
+    return Axis{n, n < 2 ? 0 : stride < 0 ? 0ull - static_cast<uint64_t>(stride) : static_cast<uint64_t>(stride)};
+  };
+  Axis axes[3] = {axis(batch, h->stride_sequence), axis(rows, h->stride_row), axis(h->heads, h->stride_head)};
+  std::sort(axes, axes + 3, [](const Axis& a, const Axis& b) { return a.step < b.step; });
+  unsigned __int128 reach = static_cast<unsigned>(dim);
+  for (const Axis& a : axes) {
+    if (a.n < 2) continue;
+    if (a.step < reach) return false;
+    reach += static_cast<unsigned __int128>(a.n - 1) * a.step;
+  }
+  return true;
 }
 
 Heads heads_of(const h3sa_heads* from, const h3sa_heads* to) {

@@ -102,7 +102,8 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, frequencies: torch.Tensor, 
     are multiples of that). ``positions``: int32, int64 or float64, one a row, or ``[..., axes]``.
     ``frequencies``: fp64 ``[pairs]``, or ``[axes, pairs of an axis]``, where the pairs of the first axis come
     first. Both are finite, and an angle (int positions: a frequency) is below 2^50. ``out``: a tensor like ``x`` for
-    the result, ``x`` itself for a rotation in place; it may not overlap ``x`` otherwise, nor its rows each other.
+    the result, ``x`` itself for a rotation in place; it may not overlap ``x`` otherwise, nor its rows each other (an axis of
+    ``out`` steps over all that those of smaller steps reach, as in slices and transposed views).
     """
 
     what = "rotate"
