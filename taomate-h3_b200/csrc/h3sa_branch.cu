@@ -120,7 +120,7 @@ struct BrWide<true> {  // begins at a multiple of 1024 bytes, as the tiles in fr
   uint64_t full[2][kWide], empty[2][kWide];
 };
 
-// By tile, the numbers of the segments in whose V a node had an infinity or NaN. A tile's epilogue reads the one of its segment when
+// The numbers of the segments in whose V a node had an infinity or NaN. A tile's epilogue reads the one of its segment when
 // its warps have taken one of the next two, and no warp can be more than the descriptors' ring in front of that: places of
 // twice the ring are not taken again before they are read.
 constexpr int kTakenOut = 2 * kDescRing;
@@ -128,15 +128,12 @@ template <class P>
 struct BrTree {};
 template <>
 struct BrTree<TreeParams> {
-  int taken_out[2][kTakenOut];
+  int taken_out[kTakenOut];
   int before[kMaxStack];  // see live_row_at
 };
 
-// Of tile `t`, or both where they share the segment's blocks.
-__device__ __forceinline__ void mark_taken_out(BrTree<TreeParams>& tree, const Segment& g, int t) {
-  const int at = g.number % kTakenOut;
-  *static_cast<volatile int*>(&tree.taken_out[t][at]) = g.number;
-  if (g.n_rows > kBlk) *static_cast<volatile int*>(&tree.taken_out[t ^ 1][at]) = g.number;
+__device__ __forceinline__ void mark_taken_out(BrTree<TreeParams>& tree, int number) {
+  *static_cast<volatile int*>(tree.taken_out + number % kTakenOut) = number;
 }
 
 template <bool kFp8, class P>
@@ -437,7 +434,7 @@ __device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows
 // Clears what must not be multiplied in V's block of a sequence's last rows: rows at or past `rows` of it may
 // hold anything, and nodes' infinities and NaN (rows from `clean` on) belong to those that see them. The block's
 // load has completed. Both MMA warps clear a block of two tiles, each what the other has left, so the one that comes second
-// may find nothing: it is marked (for both tiles) before the value goes, and whoever finds it gone passes that on by its
+// may find nothing: the segment is marked before the value goes, and whoever finds it gone passes that on by its
 // own barriers.
 template <bool kTree, typename Mark>
 __device__ __forceinline__ void clear_block(uint32_t base, int rows, int clean, int lane, Mark&& mark) {
@@ -521,7 +518,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
     mbar_init(smem_u32(&sm.drain), 2);
     sm.abort_flag = 0;
     if constexpr (kTree) {
-      for (int n = 0; n < kTakenOut; ++n) sm.tree.taken_out[0][n] = sm.tree.taken_out[1][n] = 0;
+      for (int n = 0; n < kTakenOut; ++n) sm.tree.taken_out[n] = 0;
     }
     fence_mbar_init();
   }
@@ -755,7 +752,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       tc_fence_after();
       if (!kFp8 && min(pend_rows, kTree ? pend_clean : kBlk) < kBlk && half == 0) {  // e4m3: done when widened
         clear_block<kTree>(smem_u32(sm.kv[pend_slot]), min(pend_rows, kBlk), pend_clean, lane, [&]() {
-          if constexpr (kTree) mark_taken_out(sm.tree, g, mt);
+          if constexpr (kTree) mark_taken_out(sm.tree, g.number);
         });
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
@@ -995,7 +992,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
       o_ph ^= 1u;
       tc_fence_after();
       if constexpr (kTree) {  // what was taken out of V, to the rows that see it
-        const volatile int& taken_out = sm.tree.taken_out[t][it.marks / 4 % kTakenOut];
+        const volatile int& taken_out = sm.tree.taken_out[it.marks / 4 % kTakenOut];
         if (__any_sync(0xffffffffu, taken_out == it.marks / 4)) {
           const NodeValues<kFp8> nodes(p, it.at.b, it.head);
           const int key_end = (it.block0 + (it.mine - 1) * it.step + 1) * kBlk;
@@ -1003,7 +1000,8 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           for (int c = 0; c < kD; ++c) {  // column by column, for its code: it is seldom needed
             const float lost = my < n_rows ? nodes.non_finite_sum(p, sight, c, it.block0 * kBlk, key_end, it.step) : 0.f;
             __syncwarp();
-            tmem_st1(tO + c, __float_as_uint(__uint_as_float(tmem_ld1(tO + c)) + lost));
+            const float o = __uint_as_float(tmem_ld1(tO + c));
+            tmem_st1(tO + c, __float_as_uint(lost == 0.f ? o : o + lost));  // none: perhaps the other tile's, which may come late
           }
           tmem_wait_st();
         }
@@ -1173,7 +1171,7 @@ __global__ void __launch_bounds__(kBrThreads, 1)
           const uint32_t from = smem_u32(sm.kv[ring]), to = smem_u32(sm.wide.v[wide]);
           if (kTree && clean < kBlk) {
             if constexpr (kTree) {
-              if (widen_block<true, true>(from, to, rows, clean, lane)) mark_taken_out(sm.tree, g, side);
+              if (widen_block<true, true>(from, to, rows, clean, lane)) mark_taken_out(sm.tree, g.number);
             }
           } else if (kTree || rows >= kBlk) {  // a tree's last rows are nodes
             widen_block<false, false>(from, to, kBlk, 0, lane);
