@@ -546,8 +546,8 @@ H3SA_API int h3sa_shared_prefix_attention(
  * pages behind its first lengths[b] rows, row lengths[b] + i, and are no part of lengths[b] until
  * h3sa_keep_rows. counts int32 [batch], or NULL for all: how many of a sequence's rows are nodes. */
 
-/* Ancestor bits and positions of trees of up to 1024 nodes. parents int32 [batch, nodes]: a row in
- * front of the node's own, or -1 for a root. masks int32 [batch, nodes, ceil(nodes / 32)]: bit n % 32 of
+/* Ancestor bits and positions of up to 65535 trees of up to 1024 nodes. parents int32 [batch, nodes]: a row
+ * in front of the node's own, or -1 for a root. masks int32 [batch, nodes, ceil(nodes / 32)]: bit n % 32 of
  * word n / 32 says whether node n is the node itself or above it; positions int32 [batch, nodes]:
  * lengths[b] plus the node's depth. Rows behind a sequence's nodes get zeros. A parent that is neither
  * makes its node a root and sets H3SA_DEVERR_BAD_INDEX, as does a count outside [0, nodes], which is
@@ -570,7 +570,8 @@ enum { H3SA_POS_ROW = 0, H3SA_POS_I32 = 1, H3SA_POS_I64 = 2, H3SA_POS_F64 = 3 };
  * frequencies[k] (radians, fp64) and is multiplied by factor; the other dimensions stay as they are. Pairs are
  * (k, k + pairs), or (2k, 2k + 1) if interleaved. positions [batch * rows, axes] of the given kind; pair
  * k belongs to axis k / (pairs / axes). H3SA_POS_ROW (appended rows, one axis): a row's place in its
- * sequence. Angles are taken in 64 bits, products in 32, results rounded once. Positions and frequencies are
+ * sequence. Angles are taken in 64 bits, cosines, sines and products in 32 (fp32 rows: off by some steps of 2^-24 of the
+ * pair's length; 16-bit rows: by 2^-20 of it), results rounded once. Positions and frequencies are
  * finite, and |position| * |frequency| below 2^50 where positions are H3SA_POS_F64, |frequency| where not. */
 typedef struct h3sa_rotary {
   const void* positions;
@@ -583,7 +584,8 @@ typedef struct h3sa_rotary {
 /* out = x rotated, both of `dtype`. dim: at most 1024. out may be x itself (same address and strides),
  * else they may not overlap. Rows of out may not overlap each other: an axis of out steps over all that those of smaller
  * steps reach, as in slices and transposed views. Any other strides and alignment of whole elements; 16 or 8 bytes are
- * read at a time where pairs, dim, strides and addresses are multiples of them. */
+ * read at a time where pairs, dim, strides and addresses are multiples of them. batch * rows * heads: below 2^30
+ * (h3sa_append_rows: heads of query, keys and values together). */
 H3SA_API int h3sa_rotate(const h3sa_heads* x, const h3sa_heads* out, int32_t dtype, int32_t batch,
                          int32_t rows, int32_t dim, const h3sa_rotary* rotary, void* stream);
 
@@ -612,7 +614,8 @@ H3SA_API int h3sa_append_rows(const h3sa_heads* key, const h3sa_heads* value,
  * rows that see nothing, come out zero. An infinity or NaN in K or V of a drafted row reaches only the
  * rows that see it; one in V of a sequence's first lengths[b] rows makes all its outputs in that column
  * infinite or NaN. A length or count outside its range, or both together past the table, is clamped with
- * H3SA_DEVERR_BAD_INDEX. workspace may be NULL where h3sa_tree_workspace is 0. */
+ * H3SA_DEVERR_BAD_INDEX. workspace may be NULL where h3sa_tree_workspace is 0. The kernels are chosen by the
+ * table's width, as the lengths are on the device: a table no wider than the longest sequence needs is the fastest. */
 H3SA_API int64_t h3sa_tree_workspace(int32_t batch, int32_t rows, int32_t heads, int32_t kv_heads,
                                      int32_t shared_rows, int32_t width, int32_t e4m3);
 H3SA_API int h3sa_tree_attention(

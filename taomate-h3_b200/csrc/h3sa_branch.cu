@@ -32,8 +32,9 @@
 // softmax of few rows over all four warps; the copies are joined in the epilogue. Trees' rows are held once:
 // what bounds the kernel beside the softmax is its own code, streaming past the instruction caches, and the two other
 // forms in between cost trees more than they bring (wide e4m3 trees 237 -> 206 us without them, 64 rows over 16000
-// keys 203 -> 199, e4m3 239 -> 214). Measured, trees: 24 of 96 rows over up to 9000 keys each 111 us (4.3 TB/s of 472 MB; 5.9 while
-// blocks stream), 20 small ones over 8192 shared keys 66 us, e4m3, four of 635 rows over up to 24001 keys 187 us (620 TFLOP/s).
+// keys 203 -> 199, e4m3 239 -> 214). Measured, trees, with the merge: 24 of 96 rows over up to 9000 keys each 98 to 102 us
+// (4.7 TB/s of 472 MB; 5.9 while blocks stream), 20 small ones over 8192 shared keys 61 to 63, e4m3, four of 635 rows over up to
+// 24001 keys 179 to 193 (600 to 650 TFLOP/s, by power).
 // TMEM columns: S0 [0,128), S1 [128,256), O0 [256,384), O1 [384,512); P of a tile overwrites the
 // first half of its S. A tile's MMAs are issued in order by one warp, so the barrier of a QK^T also
 // says that the tile's previous P V is complete.
@@ -46,14 +47,14 @@
 // is f16 (11 bits down to 2^-21 of a fresh maximum, steps of 2^-31 of it below), and warp 3 widens each
 // V block to f16 in shared memory, where kind::f16 takes it: one f16 product costs what two of e4m3 do, and
 // the softmax has no terms to split. Against two e4m3 terms (us): 3 x 1211 rows of 24 heads to 15.7 K keys 721 /
-// 821, 60 stacked rows of 8 KV heads over 98304 keys 97.6 / 92.2: a block's 1850 cycles in warp 3 take issue
-// slots from the softmax warps beside it.
+// 821, 60 stacked rows of 8 KV heads over 98304 keys 97.6 / 92.2 (91 since the widening loop is half as long): a block's 1850
+// cycles in warp 3 take issue slots from the softmax warps beside it.
 // P of bf16 caches is bf16, 8 bits of each weight however small, as the output has.
 //
 // Measured: 3 branches of 1211 rows, 24 heads, to 15.7 K keys, bf16, joint: 640 to 750 us (0.86 to
 // 1.0 PFLOP/s, by power), the tensor pipe 53 % active; what bounds it is the softmax's latency, 2000 cycles
-// a half block of both tiles in step, 1024 of them 2^x. 60 stacked rows of 8 KV heads over 98304 e4m3 keys:
-// 87 us (2.3 TB/s), bound by the round trips of half blocks; 9 us go by before the first scores (all
+// a half block of both tiles in step, 1024 of them 2^x. 60 stacked rows of 8 KV heads over 98304 e4m3 keys, with own rows and
+// merge: 91 us (2.5 TB/s of 227 MB), bound by the round trips of half blocks; 9 us go by before the first scores (all
 // CTAs' first loads and queries at once) and 5 in the epilogue.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -98,8 +99,9 @@ struct BrCfg {
   static constexpr int kStages = kFp8 ? 6 : 5;  // even for e4m3: K in the even slots, V in the odd ones
   static constexpr int kSteps = kFp8 ? 4 : 8;   // MMA K steps of S
   // Order of a segment's loads: K0 K1 V0 K2 V1 ..., each V behind the next K, which is wanted first (V waits for a
-  // softmax, in a slot of the ring: 24 trees of 96 rows over 9000 keys 130 -> 111 us, 24 chains of 4 x 32 rows over 8192 shared
-  // keys 50.7 -> 49.8); e4m3: K0 V0 K1 V1 ..., as V is widened on its way.
+  // softmax, in a slot of the ring). In turn / as it is, us: 24 trees of 96 rows over 9000 keys 118.6 / 101.8, of 64 over 16000
+  // 179 / 150; 24 chains of 96 rows over 9000 keys 101.3 / 89.7, of 4 x 32 over 8192 shared keys 46.8 / 46.1; e4m3: K0 V0 K1
+  // V1 ..., as V is widened on its way.
   static constexpr bool kSkew = !kFp8;
   static constexpr uint32_t kIdescQK = kFp8 ? idesc_e4m3(kBlk, kBlk / 2, false) : idesc_bf16(kBlk, kBlk / 2, false);
   static constexpr uint32_t kIdescPV = kFp8 ? idesc_f16(kBlk, kD, true) : idesc_bf16(kBlk, kD, true);
@@ -390,7 +392,9 @@ __device__ __forceinline__ bool widen_block(uint32_t from, uint32_t to, int rows
   uint32_t met = 0u;
   const int c = lane & 7, h = c >> 2, at = 2 * (c & 3);
   const int r = (lane >> 4) + ((lane >> 1) & 4);  // rows r and r ^ 2 of eight; those of a half warp differ by 4
-#pragma unroll 1  // for its code: 224 us instead of 156 for 24 trees of 64 rows over 16000 keys, 234 for 228 (chains)
+  // Not unrolled, for its code. Unrolled / as it is, us: 24 trees of 64 rows over 16000 keys 198 / 159, four of 635 rows over up to
+  // 24001 207 / 179; chains: 24 of 96 rows over 9000 keys 118 / 108, 60 stacked rows over 98304 shared keys 97.4 / 90.7.
+#pragma unroll 1
   for (int step = 0; step < 2; ++step) {
     const int row = r ^ (2 * step);
     const uint32_t src = from + row * 128 + ((c ^ row) << 4) + 8 * h;
@@ -1480,7 +1484,9 @@ constexpr int kWarpLeast = 2, kWarpLeastBeside = 8;
 // 2000 48 / 42, 4000 59 / 62, 16000 153 / 228; 24 rows, 2000 46 / 36, 8000 91 / 111; one tree of 64 rows over up to 8000 29 / 27, 16000
 // 35 / 39, 40000 49 / 82; e4m3: 64 rows, 24 trees of 2000 73 / 64, 4000 90 / 96, 16000 157 / 281; 48 rows, 4000 84 / 74, 8000 114 / 136; 32
 // rows, 16000 148 / 153. Shared keys (20 trees of 48 rows over 4096 and up to 700 of their own: 55 / 63, e4m3 64 / 62) count by
-// the tiles of all trees' rows.
+// the tiles of all trees' rows. A table wider than its longest sequence stands for keys that are not there. Tables of 8 / 256
+// pages, up to 1000 keys (us): 24 trees of 24 rows 23.5 / 34.4 (e4m3 24.6 / 24.6), of 64 rows 45.7 / 46.1 (44.4 / 57.0), 4 trees of 64
+// rows 18.3 / 22.9 (19.0 / 25.9); two of 9 rows and 311 keys, 3 / 256 pages, 13.6 / 12.6, but a launch more a call.
 bool tree_on_tensor(int batch, int own, int kv_heads, int shared, int width, bool e4m3) {
   if (own <= kRowSpan) return false;
   const auto tiles = [](long long n, int span) { return (n + span - 1) / span; };

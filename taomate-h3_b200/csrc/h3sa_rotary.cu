@@ -6,17 +6,23 @@
 //
 // Pairs are (k, k + pairs) in the half layout and (2k, 2k + 1) interleaved; dimensions behind the last
 // pair stay as they are. Positions may have several axes (time, height, width); pair k then belongs to
-// axis k / per_axis. Angles are taken in whole turns: t = p * (f_k / 2 pi) in 64 bits, whose fraction is
-// then exact to 2^-25 of a turn for any position of 32 bits; cosine and sine of it are in 32 bits, as are
-// the products, and each result is rounded once.
+// axis k / per_axis. Angles are taken in whole turns: of f_k / 2 pi only the fraction of a turn matters, as an integer in
+// units of 2^-64 off by half of one, and p times that, cut to 64 bits, is the angle: positions of 32 bits leave it
+// exact to 2^-33 of a turn, of which the upper 32 bits are used. Positions between whole numbers take a product of
+// doubles instead, off by 2^-52 of itself. Cosine and sine of it are in 32 bits, as are the products, and each result is
+// rounded once.
 //
 // Bound by memory: a value is read and written once. What has to be kept small is the instructions in
 // between, for which an SM has some 350 a warp and 2 KB: a thread keeps to one unit of a head row, 8 pairs in two
-// vectors of 16 bytes, with their frequencies in registers, works out its 8 angles once a token and turns up to eight heads by
-// them, all of which are on their way by then. There is nothing to share and nothing to wait for in a block.
-// Measured: 24605 tokens of 24 heads, bf16, three axes: 50 us, 6.05 TB/s of the 302 MB read and written; 300001 of one head 45 us
-// (a table of the block's cosines and sines in shared memory took 57 and 110); appends of 16-bit prompts into e4m3 pools
-// 75 us for 373 MB, 5.0 TB/s, the divisions and conversions beside the loads; a few rows 4.2 us, launch and two dependent loads.
+// vectors of 16 bytes, with their frequencies in registers, works out its 8 angles once a task and turns up to six heads by
+// them (appends four, tensors of up to two heads two), all of which are on their way by then. There is nothing to share and
+// nothing to wait for in a block.
+// Measured: 24605 tokens of 24 heads, bf16, three axes: 48 to 50 us, 6.05 TB/s and more of the 302 MB read and written; 7 prompts of up
+// to 3001 rows, 32 / 8 heads, into bf16 pools 66 us of 61 to 63 at the copy rate, into e4m3 pools 69 to 75 us of 57, 5.0 TB/s,
+// the divisions and conversions beside the loads; a few rows 2.7 us in a row of launches, 4.2 with the start of a graph.
+// 300001 tokens of one head take 42.5 us of 23.6: 8 angles are worked out for 16 values, and the 64 registers of eight blocks an
+// SM, which keep enough rows on their way, spill 84 to 120 bytes. (A table of the block's cosines and sines in shared memory took
+// 57 and 110.) Appends keep 96 registers and spill up to 80 bytes, most in the half layout into e4m3 pools.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -117,11 +123,12 @@ __device__ __forceinline__ int fraction(bool between, uint64_t position, uint64_
   const double whole = (t + 6755399441055744.0) - 6755399441055744.0;
   return __double2loint(fma(p, unit, -whole) + 1572864.0);
 }
-// Cosine and sine of a fraction of a turn. For 16-bit values the approximate functions, off by up to 2^-21, which is
-// 2^-10 of their rounding. For 32 bits the fraction's first 24 bits, which a float holds, by the function, and the other 8,
-// an angle below 2^-21, by the first term of the sums' formulas: all 32 in one float are off by up to 2^-26 of a turn, more
-// than the results' own rounding (rotations at positions to 2^31 off by 4.5e-8 of their length, with one float 5.7e-8; with
-// cosines and sines taken in 64 bits 4.2e-8. 300001 tokens of one head 64.6 us, with one float 62.6, others the same).
+// Cosine and sine of a fraction of a turn. For 16-bit values the approximate functions, which with the roundings of the angle
+// are off by under 2^-20: 2^-9 of what rounding a value of 1 to fp16 leaves. For 32 bits the fraction's first 24 bits, which
+// a float holds, by the function, and the other 8, an angle below 2^-21, by the first term of the sums' formulas: all 32 in
+// one float are off by up to 2^-26 of a turn, more than the results' own rounding (rotations at positions to 2^31 off by
+// 4.5e-8 of their length, with one float 5.7e-8; with cosines and sines taken in 64 bits 4.2e-8. 300001 tokens of one head
+// 64.6 us, with one float 62.6, others the same).
 template <typename T>
 __device__ __forceinline__ void cos_sin(int fraction, float factor, float& c, float& s) {
   if constexpr (sizeof(T) == 2) {
@@ -444,9 +451,10 @@ int vector_of(const RowsParams& p, int size) {
   return 1;
 }
 
-// A task is a head row while threads are few, `most_rows` of them from there on, of which a thread takes up to
-// four: that pays for its frequencies. Tasks of kMany rows pay sooner, and a thread takes two (two / four: 24605 tokens of 24 heads 50.1 /
-// 51.3 us, 30000 of 16 in fp32 78.5 / 83.9, 60000 of 8 heads of 64 26.8 / 26.3; but one head of 300001 49.5 / 44.9, e4m3 prompts 74.9 / 74.3).
+// A task is a head row while threads are few, `most_rows` of them from there on, of which a thread takes up to four, or two
+// where most_rows is kMany (whose tasks pay for a thread's frequencies sooner). Two / four, us: 24605 tokens of 24 heads 50.1 /
+// 51.3, 30000 of 16 in fp32 78.5 / 83.9, 60000 of 8 heads of 64 26.8 / 26.3; but one head of 300001 49.5 / 44.9, e4m3 prompts
+// 74.9 / 74.3.
 void lay_out(RowsParams& p, int n, int batch, int most_rows) {
   p.tokens = static_cast<long long>(batch) * p.rows;
   p.row_div = divisor(static_cast<uint32_t>(p.rows));

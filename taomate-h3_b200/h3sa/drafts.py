@@ -38,7 +38,7 @@ def _counts(what: str, counts: torch.Tensor | None, device: torch.device, batch:
 def draft_tree(parents: torch.Tensor, lengths: torch.Tensor, *, counts: torch.Tensor | None = None,
                device_error: torch.Tensor | None = None, stream: torch.cuda.Stream | None = None,
                ) -> tuple[torch.Tensor, torch.Tensor]:
-    """Ancestor bits and positions of trees: ``parents`` int32 ``[sequences, nodes]`` (up to 1024 nodes), each a
+    """Ancestor bits and positions of trees: ``parents`` int32 ``[sequences, nodes]`` (up to 65535 and 1024), each a
     row in front of its own, or -1 for a root. Returns ``masks`` int32 ``[sequences, nodes, ceil(nodes / 32)]``, whose
     bit n % 32 of word n // 32 says whether node n is the row itself or above it, and ``positions`` int32
     ``[sequences, nodes]``, ``lengths`` plus the row's depth. Rows behind ``counts`` get zeros. A parent that is
@@ -163,7 +163,8 @@ def tree_attention(query: torch.Tensor, key_pool: torch.Tensor, value_pool: torc
     All other arguments are those of ``shared_prefix_attention``; the first ``shared_rows`` rows are the same pages
     in the table rows of all sequences whose ``lengths`` reach that far. Rows behind ``counts``, and rows that see
     nothing, come out zero with a log-sum-exp of -inf. An infinity or NaN in K or V of a drafted row reaches only the rows that
-    see it; one in V of a sequence's history makes all its outputs in that column infinite or NaN.
+    see it; one in V of a sequence's history makes all its outputs in that column infinite or NaN. The lengths stay on the
+    device, so the kernels are chosen by the width of ``table``: one no wider than the longest sequence needs is the fastest.
     """
 
     what = "tree_attention"

@@ -69,3 +69,28 @@ def test_large_frequencies() -> None:
     frequencies = rng.choice([-1.0, 1.0], 64) * rng.uniform(1.0, 2.0, 64) * 2.0 ** rng.integers(10, 48, 64)
     _check([0, 1, -3, 1000], torch.int32, frequencies, 2.0 ** -21)
     _check([1, 77777, -(1 << 31)], torch.int64, frequencies[np.abs(frequencies) < 2.0 ** 40], 2.0 ** -21)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_16_bit_rows(kind, interleaved) -> None:
+    """The angle as a float of up to pi: 2^-26 of a turn, the float 2 pi and a product, together 2^-21.7; the approximate
+    functions 2^-21.2: under 2^-20.3 of |x| + |y|. A factor, a product and the sum in 32 bits, 2^-24 each, leave it below
+    2^-20; then half a step of the result."""
+
+    from h3sa.rotary import rotary_frequencies, rotate
+
+    rng, gen, factor = np.random.default_rng(3), torch.Generator().manual_seed(3), 1.25
+    frequencies = rotary_frequencies(96, base=1e6)[0].numpy()
+    positions = rng.integers(-(1 << 31), 1 << 31, 300).astype(np.int32)
+    pairs = torch.randn(300, 5, 2, 48, generator=gen).to(kind)
+    rows = (pairs.transpose(-1, -2) if interleaved else pairs).reshape(300, 5, 96)
+    out = rotate(rows.cuda(), torch.from_numpy(positions).cuda(), torch.from_numpy(frequencies).cuda(), interleaved=interleaved, factor=factor)
+    got = out.double().cpu().view(300, 5, 48, 2).transpose(-1, -2) if interleaved else out.double().cpu().view(300, 5, 2, 48)
+    x, y = pairs.double().unbind(2)
+    c, s = (torch.from_numpy(t)[:, None] * factor for t in angles.cos_sin(positions, frequencies))
+    half = torch.finfo(kind).eps / 2
+    for have, want in zip(got.unbind(2), (x * c - y * s, x * s + y * c)):
+        slack = 2.0 ** -20 * factor * (x.abs() + y.abs())
+        tol = slack + half * (want.abs() + slack) + half * torch.finfo(kind).smallest_normal
+        assert ((have - want).abs() <= tol).all(), float(((have - want).abs() / tol).max())
